@@ -389,6 +389,73 @@ MI_API int mi_copy_blocks(void *key_pool, void *value_pool, int32_t num_layers,
                    int64_t num_pairs, int32_t *dev_status, void *stream);
 
 /*
+ * 4-bit paged KV cache.  K and V are held in microscaled 4-bit floating point
+ * (MXFP4: e2m1 codes, one power-of-two scale for every 32 along head_dim), 4.25
+ * bits per element.  key_pages / value_pages are bytes
+ *   [num_blocks][num_kv_heads][mi_mxfp4_page_bytes(block_size, head_dim)];
+ * a page holds, for every 16 tokens, a group of head_dim / 32 * 272 bytes:
+ *   codes   [head_dim / 32][16 tokens][16 bytes], element 2j in the low nibble of byte j
+ *   scales  [16 tokens][head_dim / 32]: byte e stands for 2^(e - 127), 0 for zero, 255 for NaN.
+ * block_size must be a multiple of 16, head_dim a multiple of 32 up to 256
+ * (MI_ERR_UNSUPPORTED otherwise); pages are 16-byte aligned.  Zero-filled pages hold
+ * zeros.  mi_copy_blocks copies them as it copies others (block_bytes =
+ * num_kv_heads * mi_mxfp4_page_bytes).  The reference has no quantised cache.
+ */
+
+/* Bytes of one kv head of one page, or a negative status. */
+MI_API int64_t mi_mxfp4_page_bytes(int32_t block_size, int32_t head_dim);
+
+/*
+ * Quantising store: token t's rows (any token stride, in elements; each
+ * [num_kv_heads, head_dim] row contiguous; f32/f16/bf16) to slot
+ * slots[t] = block * block_size + offset, -1 writes nothing.  A block of 32 with
+ * largest magnitude a > 0 gets the scale 2^e, e = max(floor(log2 a) - 2, -126),
+ * and codes rounded to the nearest value, ties to even, saturating at 6; one with
+ * an infinity or a NaN reads as NaN.  Slots must be unique within a call;
+ * those outside the pool are skipped (MI_DEV_BAD_SLOT).
+ */
+MI_API int mi_store_kv_mxfp4(void *key_pages, void *value_pages, int64_t num_blocks,
+                      int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                      const void *slots, int32_t index_dtype, const void *keys,
+                      const void *values, int32_t dtype, int64_t key_token_stride,
+                      int64_t value_token_stride, int64_t num_tokens,
+                      int32_t *dev_status, void *stream);
+
+/*
+ * Dequantising block-table gather: rows of logical position t of sequence s to
+ * out[cu_seqlens_k[s] + t] in `dtype`, for t < context_s.  `max_context`
+ * bounds the launch shape, `out_rows` is the row capacity of the outputs (never
+ * written past).  Outputs are contiguous and 16-byte aligned.
+ */
+MI_API int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void *key_pages,
+                             const void *value_pages, int64_t num_blocks,
+                             int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t dtype, const int32_t *block_tables,
+                             int64_t block_table_stride, const int32_t *cu_seqlens_k,
+                             int64_t num_seqs, int64_t out_rows, int64_t max_context,
+                             int32_t *dev_status, void *stream);
+
+/*
+ * Paged decode over the 4-bit cache: out[s, h] = softmax(scale * K_s q[s, h]) V_s
+ * over context_lens[s] positions, GQA with any group; a sequence without
+ * keys gives zeros.  query / out are contiguous [num_seqs, num_q_heads, head_dim]
+ * in `dtype`, 16-byte aligned.  The workspace holds partial states for the
+ * duration of the call and needs no initial value; calls that can run at the
+ * same time need one each.  `max_context` of the size query is
+ * block_table_stride * block_size.
+ */
+MI_API size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int32_t num_q_heads,
+                                             int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t dtype, int64_t max_context, int device);
+MI_API int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages,
+                          const void *value_pages, int64_t num_blocks, int32_t block_size,
+                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t dtype, const int32_t *block_tables,
+                          int64_t block_table_stride, const int32_t *context_lens,
+                          int64_t num_seqs, float scale, void *workspace,
+                          size_t workspace_bytes, int32_t *dev_status, void *stream);
+
+/*
  * Bounded-wait self test: one thread spins on `flag` (device int32) until it
  * becomes non-zero or `timeout_ns` passes, then ORs MI_DEV_TIMEOUT into
  * dev_status if it ran out.  Exercises the same bounded-wait helper every

@@ -125,6 +125,7 @@ constexpr float kLog2eHost = 1.4426950408889634f;
 namespace mi {
 int capi_fail(int code, const char *msg) { return fail(code, msg); }
 int capi_select_device(const void *p) { return select_device(p); }
+int capi_cuda_status(cudaError_t e) { return cuda_status(e); }
 }  // namespace mi
 
 extern "C" {

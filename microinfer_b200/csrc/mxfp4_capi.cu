@@ -1,0 +1,185 @@
+// extern "C" entry points of the 4-bit paged cache: argument validation and
+// launch.  Nothing here allocates or synchronises.
+#include <cstdio>
+
+#include "common.cuh"
+#include "launch.cuh"
+#include "mxfp4.cuh"
+#include "params.cuh"
+
+namespace mi {
+
+int capi_fail(int code, const char *msg);
+int capi_select_device(const void *p);
+int capi_cuda_status(cudaError_t e);
+
+cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtype, bool vec,
+                               cudaStream_t stream);
+cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
+                                cudaStream_t stream);
+cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream);
+size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
+                              int64_t capacity, int sms);
+
+}  // namespace mi
+
+using namespace mi;
+
+namespace {
+
+constexpr float kLog2eHost = 1.4426950408889634f;
+
+bool known_dtype(int32_t dtype) {
+  return dtype == MI_DTYPE_FLOAT32 || dtype == MI_DTYPE_FLOAT16 || dtype == MI_DTYPE_BFLOAT16;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What every entry point asks of a 4-bit cache.
+int check_cache(int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim) {
+  if (num_blocks <= 0 || block_size <= 0 || num_kv_heads <= 0 || head_dim <= 0)
+    return capi_fail(MI_ERR_INVALID, "cache dimensions must be positive");
+  if (block_size % kMxGroup != 0)
+    return capi_fail(MI_ERR_UNSUPPORTED, "a 4-bit cache needs a block_size that is a multiple of 16");
+  if (head_dim % kMxBlock != 0 || head_dim > 256)
+    return capi_fail(MI_ERR_UNSUPPORTED, "a 4-bit cache needs a head_dim that is a multiple of 32, at most 256");
+  return MI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mi_mxfp4_page_bytes(int32_t block_size, int32_t head_dim) {
+  if (const int s = check_cache(1, block_size, 1, head_dim)) return s;
+  return static_cast<int64_t>(block_size / kMxGroup) * mx_group_bytes(head_dim);
+}
+
+int mi_store_kv_mxfp4(void *key_pages, void *value_pages, int64_t num_blocks, int32_t block_size,
+                      int32_t num_kv_heads, int32_t head_dim, const void *slots, int32_t index_dtype,
+                      const void *keys, const void *values, int32_t dtype, int64_t key_token_stride,
+                      int64_t value_token_stride, int64_t num_tokens, int32_t *dev_status, void *stream) {
+  if (!known_dtype(dtype)) return capi_fail(MI_ERR_INVALID, "unknown dtype");
+  if (index_dtype != MI_INDEX_INT32 && index_dtype != MI_INDEX_INT64)
+    return capi_fail(MI_ERR_INVALID, "index dtype must be int32 or int64");
+  if (const int s = check_cache(num_blocks, block_size, num_kv_heads, head_dim)) return s;
+  if (num_tokens < 0) return capi_fail(MI_ERR_INVALID, "num_tokens must be >= 0");
+  if (key_token_stride < 0 || value_token_stride < 0)
+    return capi_fail(MI_ERR_INVALID, "token strides must be >= 0");
+  if (num_tokens == 0) return MI_OK;
+  if (!key_pages || !value_pages || !keys || !values || !slots) return capi_fail(MI_ERR_INVALID, "null pointer");
+  if (!aligned16(key_pages) || !aligned16(value_pages))
+    return capi_fail(MI_ERR_ALIGNMENT, "pages must be 16-byte aligned");
+  if (const int s = capi_select_device(key_pages)) return s;
+  const int e = dtype == MI_DTYPE_FLOAT32 ? 4 : 2;
+  MxStoreParams p = {};
+  p.key_pages = static_cast<uint8_t *>(key_pages);
+  p.value_pages = static_cast<uint8_t *>(value_pages);
+  p.slots = slots;
+  p.keys = keys;
+  p.values = values;
+  p.key_stride = key_token_stride;
+  p.value_stride = value_token_stride;
+  p.num_slots = num_blocks * block_size;
+  p.num_tokens = num_tokens;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.status = dev_status;
+  const bool vec = aligned16(keys) && aligned16(values) && key_token_stride * e % 16 == 0 &&
+                   value_token_stride * e % 16 == 0;
+  return capi_cuda_status(launch_mxfp4_store(p, dtype, index_dtype, vec, static_cast<cudaStream_t>(stream)));
+}
+
+int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void *key_pages, const void *value_pages,
+                             int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t dtype, const int32_t *block_tables, int64_t block_table_stride,
+                             const int32_t *cu_seqlens_k, int64_t num_seqs, int64_t out_rows,
+                             int64_t max_context, int32_t *dev_status, void *stream) {
+  if (!known_dtype(dtype)) return capi_fail(MI_ERR_INVALID, "unknown dtype");
+  if (const int s = check_cache(num_blocks, block_size, num_kv_heads, head_dim)) return s;
+  if (num_seqs < 0 || max_context < 0 || block_table_stride < 0 || out_rows < 0)
+    return capi_fail(MI_ERR_INVALID, "negative sizes");
+  if (num_seqs > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences in one call");
+  if (num_seqs == 0 || max_context == 0 || out_rows == 0) return MI_OK;
+  if (max_context / kMxGroup > (int64_t{1} << 33) / num_kv_heads)
+    return capi_fail(MI_ERR_UNSUPPORTED, "max_context too large for one call");
+  if (!out_keys || !out_values || !key_pages || !value_pages || !block_tables || !cu_seqlens_k)
+    return capi_fail(MI_ERR_INVALID, "null pointer");
+  if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(out_keys) || !aligned16(out_values))
+    return capi_fail(MI_ERR_ALIGNMENT, "pages and outputs must be 16-byte aligned");
+  if (const int s = capi_select_device(key_pages)) return s;
+  MxGatherParams p = {};
+  p.out_keys = out_keys;
+  p.out_values = out_values;
+  p.key_pages = static_cast<const uint8_t *>(key_pages);
+  p.value_pages = static_cast<const uint8_t *>(value_pages);
+  p.block_tables = block_tables;
+  p.cu_seqlens_k = cu_seqlens_k;
+  p.block_table_stride = block_table_stride;
+  p.num_blocks = num_blocks;
+  p.out_rows = out_rows;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.status = dev_status;
+  return capi_cuda_status(
+      launch_mxfp4_gather(p, dtype, num_seqs, max_context, static_cast<cudaStream_t>(stream)));
+}
+
+size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                             int32_t head_dim, int32_t dtype, int64_t max_context, int device) {
+  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context <= 0 ||
+      num_q_heads % num_kv_heads != 0)
+    return 0;
+  return mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, max_context,
+                                sm_count_of(device < 0 ? 0 : device));
+}
+
+int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, const void *value_pages,
+                          int64_t num_blocks, int32_t block_size, int32_t num_q_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t dtype, const int32_t *block_tables,
+                          int64_t block_table_stride, const int32_t *context_lens, int64_t num_seqs,
+                          float scale, void *workspace, size_t workspace_bytes, int32_t *dev_status,
+                          void *stream) {
+  if (!known_dtype(dtype)) return capi_fail(MI_ERR_INVALID, "unknown dtype");
+  if (const int s = check_cache(num_blocks, block_size, num_kv_heads, head_dim)) return s;
+  if (num_seqs < 0) return capi_fail(MI_ERR_INVALID, "num_seqs must be >= 0");
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0)
+    return capi_fail(MI_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads");
+  if (block_table_stride < 0 || block_table_stride > INT32_MAX)
+    return capi_fail(MI_ERR_INVALID, "block_table_stride out of range");
+  if (num_seqs > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences in one call");
+  if (num_q_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 query heads");
+  if (num_seqs == 0) return MI_OK;
+  if (!out || !query || !key_pages || !value_pages || !block_tables || !context_lens)
+    return capi_fail(MI_ERR_INVALID, "null pointer");
+  if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
+    return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
+  if (const int s = capi_select_device(key_pages)) return s;
+  const size_t need = mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype,
+                                             block_table_stride * block_size, sm_count_current());
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_decode_mxfp4_workspace_bytes)");
+  if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  MxDecodeParams p = {};
+  p.out = out;
+  p.query = query;
+  p.key_pages = static_cast<const uint8_t *>(key_pages);
+  p.value_pages = static_cast<const uint8_t *>(value_pages);
+  p.block_tables = block_tables;
+  p.context_lens = context_lens;
+  p.workspace = static_cast<float *>(workspace);
+  p.bt_stride = block_table_stride;
+  p.num_blocks = num_blocks;
+  p.num_seqs = num_seqs;
+  p.block_size = block_size;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.scale_log2 = scale * kLog2eHost;
+  p.status = dev_status;
+  return capi_cuda_status(launch_mxfp4_decode(p, dtype, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

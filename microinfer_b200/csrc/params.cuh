@@ -137,6 +137,56 @@ struct QkPrologueParams {
   int32_t *status;
 };
 
+// 4-bit paged cache (mxfp4.cuh): quantising store, dequantising gather, decode.
+struct MxStoreParams {
+  uint8_t *key_pages;
+  uint8_t *value_pages;
+  const void *slots;
+  const void *keys;  // [T, Hkv, D] rows key_stride elements apart
+  const void *values;
+  int64_t key_stride;
+  int64_t value_stride;
+  int64_t num_slots;
+  int64_t num_tokens;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t *status;
+};
+struct MxGatherParams {
+  void *out_keys;
+  void *out_values;
+  const uint8_t *key_pages;
+  const uint8_t *value_pages;
+  const int32_t *block_tables;
+  const int32_t *cu_seqlens_k;
+  int64_t block_table_stride;
+  int64_t num_blocks;
+  int64_t out_rows;  // rows of out_keys / out_values; never written past
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t *status;
+};
+struct MxDecodeParams {
+  void *out;
+  const void *query;
+  const uint8_t *key_pages;
+  const uint8_t *value_pages;
+  const int32_t *block_tables;
+  const int32_t *context_lens;
+  float *workspace;  // partial states, see decode_mxfp4.cu
+  int64_t bt_stride;
+  int64_t num_blocks;
+  int64_t num_seqs;
+  int32_t block_size;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  float scale_log2;
+  int32_t *status;
+};
+
 // Per-step runner metadata from the device page table (runner_meta.cu).
 struct RunnerMetaParams {
   int32_t *page_table;  // [max_rows, max_pages]

@@ -5,6 +5,10 @@ the step's K/V are written into the paged pool first, then the queries
 attend.  Prefill without a block table ("direct", no cached prefix) attends
 to this step's contiguous K/V with the dense varlen kernel, which replaces the
 reference's FlashAttention varlen / per-request SDPA paths (:17-55).
+
+A layer of the 4-bit pool (``LayerMXFP4Cache``) binds like any other: its store
+quantises, and paged attention reads the codes; direct prefill attends to this
+step's K/V as they are.
 """
 
 from __future__ import annotations
@@ -12,20 +16,22 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from microinfer_b200.layer.mxfp4_attention import paged_attention_mxfp4_meta
 from microinfer_b200.layer.paged_attention import (
     paged_attention_meta,
     paged_decode_store,
     varlen_prefill,
 )
 from microinfer_b200.worker.kv_cache import LayerKVCache
+from microinfer_b200.worker.mxfp4_cache import LayerMXFP4Cache
 
 
 class CachedAttention(nn.Module):
     def __init__(self):
         super().__init__()
-        self.cache: LayerKVCache | None = None
+        self.cache: LayerKVCache | LayerMXFP4Cache | None = None
 
-    def bind_cache(self, cache: LayerKVCache):
+    def bind_cache(self, cache: LayerKVCache | LayerMXFP4Cache):
         self.cache = cache
 
     def forward(self, q, k, v, metadata):
@@ -37,7 +43,7 @@ class CachedAttention(nn.Module):
         if cache is not None:
             if metadata.slot_mapping is None:
                 raise ValueError("bound cache requires slot_mapping")
-            if (metadata.is_decode and not metadata.validate_cache_write
+            if (not isinstance(cache, LayerMXFP4Cache) and metadata.is_decode and not metadata.validate_cache_write
                     and metadata.context_lens is not None):
                 # One launch: store this step's K/V, then decode over the cache.
                 return paged_decode_store(q, cache.keys, cache.values, metadata.block_tables,
@@ -46,6 +52,8 @@ class CachedAttention(nn.Module):
                 cache.write_checked(metadata.slot_mapping, k, v)
             else:
                 cache.write_slots(metadata.slot_mapping, k, v)
+        if not direct and isinstance(cache, LayerMXFP4Cache):
+            return paged_attention_mxfp4_meta(q, cache.keys, cache.values, metadata)
         if not direct:
             return paged_attention_meta(q, cache.keys, cache.values, metadata)
         if q.shape[1] % k.shape[1]:

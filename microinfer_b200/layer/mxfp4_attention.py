@@ -1,0 +1,219 @@
+"""Attention over the 4-bit paged cache (``worker.mxfp4_cache``).
+
+* ``paged_decode_mxfp4``        one query token per request, as ``paged_decode``
+* ``paged_prefill_mxfp4``       causal chunked prefill on a cached prefix, as ``paged_prefill``
+* ``gather_paged_kv_mxfp4``     rows in logical order, as ``gather_paged_kv``
+* ``paged_attention_mxfp4_meta``  dispatch on the step's metadata, as ``paged_attention_meta``
+
+Decode reads the codes and decodes them in registers.  Prefill decodes each
+context once into a workspace of the query's type and attends to that with the
+dense tensor-core kernel: a chunk of n tokens does 4 * n * Hq flops for each of the
+Hkv elements decoded, so the extra pass is a few percent of a chunk of ordinary size.
+Workspaces come from torch's allocator for the length of the call, so that calls on several
+streams, and captured graphs, each have their own.
+"""
+
+from __future__ import annotations
+
+import math
+from functools import lru_cache
+
+import torch
+
+from microinfer_b200 import _lib
+from microinfer_b200.layer.paged_attention import _idx, varlen_prefill
+from microinfer_b200.worker.mxfp4_cache import page_dims
+
+
+def _check_query(query, hkv, d, out):
+    if query.ndim != 3:
+        raise ValueError("query must have shape [tokens, Hq, D]")
+    if query.shape[2] != d:
+        raise ValueError("query and cache head dimensions differ")
+    if query.shape[1] == 0 or query.shape[1] % hkv:
+        raise ValueError("Hq must be divisible by Hkv")
+    if out is not None:
+        if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+            raise ValueError("out must be contiguous, of the query's shape and dtype")
+        if out.device != query.device:
+            raise ValueError("out must be on the query's device")
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@lru_cache(maxsize=4096)
+def _decode_workspace_bytes(n, hq, hkv, d, dtype, capacity, device):
+    return _lib.load().mi_paged_decode_mxfp4_workspace_bytes(n, hq, hkv, d, dtype, capacity, device)
+
+
+def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens, *,
+                       scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One query token per request over its 4-bit pages; a request without keys gives zeros.
+
+    ``query`` [requests, Hq, D] in fp32, fp16 or bf16, any group Hq / Hkv.
+    """
+    if torch.compiler.is_compiling():  # an opaque node for torch.compile
+        res = torch.ops.microinfer_b200.paged_decode_mxfp4(query, key_pages, value_pages,
+                                                           block_tables, context_lens, scale)
+        return res if out is None else out.copy_(res)
+    nb, bs, hkv, d = page_dims(key_pages, value_pages)
+    _check_query(query, hkv, d, out)
+    n, hq, _ = query.shape
+    dtype = _lib.dtype_code(query.dtype)
+    if block_tables.ndim != 2 or block_tables.shape[0] != n:
+        raise ValueError("block_tables must have one row per request")
+    if context_lens.shape != (n,):
+        raise ValueError("context_lens must have one entry per request")
+    if n == 0:
+        return torch.empty_like(query) if out is None else out
+    device = _lib.require_cuda(query, key_pages, value_pages, block_tables, context_lens)
+    width = block_tables.shape[1]
+    if width == 0:  # no request can have a key
+        return torch.zeros_like(query) if out is None else out.zero_()
+    query, block_tables, context_lens = _aligned(query), _idx(block_tables), _idx(context_lens)
+    if out is None:
+        out = torch.empty_like(query)
+    need = _decode_workspace_bytes(n, hq, hkv, d, dtype, width * bs, device.index or 0)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _lib.call(
+        "mi_paged_decode_mxfp4", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),
+        value_pages.data_ptr(), nb, bs, hq, hkv, d, dtype, block_tables.data_ptr(), width,
+        context_lens.data_ptr(), n, 1.0 / math.sqrt(d) if scale is None else float(scale),
+        _lib.ptr(workspace), need, _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
+    )
+    return out
+
+
+def _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most):
+    nb, bs, hkv, d = dims
+    device = key_pages.device
+    _lib.call(
+        "mi_gather_paged_kv_mxfp4", keys.data_ptr(), values.data_ptr(), key_pages.data_ptr(),
+        value_pages.data_ptr(), nb, bs, hkv, d, _lib.dtype_code(keys.dtype),
+        block_tables.data_ptr(), block_tables.shape[1], cu_seqlens_k.data_ptr(),
+        block_tables.shape[0], rows, most, _lib.status_buffer(device).data_ptr(),
+        _lib.stream_of(device),
+    )
+
+
+def gather_paged_kv_mxfp4(key_pages, value_pages, block_tables, contexts, *,
+                          dtype: torch.dtype = torch.bfloat16,
+                          cu_seqlens_k: torch.Tensor | None = None, out=None):
+    """Rows of each request in logical order, request-major, as ``dtype``.
+
+    ``contexts`` is a host sequence of context lengths; ``cu_seqlens_k`` (device,
+    cumulative) skips the host prefix sum and its copy; ``out=(keys, values)``
+    (contiguous ``[sum(contexts), Hkv, D]``) writes into existing tensors of any of the types.
+    """
+    dims = page_dims(key_pages, value_pages)
+    _, bs, hkv, d = dims
+    device = _lib.require_cuda(key_pages, value_pages, block_tables)
+    contexts = [int(c) for c in contexts]
+    if any(c < 0 for c in contexts):
+        raise ValueError("contexts must be non-negative")
+    if block_tables.ndim != 2 or len(contexts) != block_tables.shape[0]:
+        raise ValueError("one context per block-table row")
+    total = sum(contexts)
+    if out is None:
+        _lib.dtype_code(dtype)
+        keys = torch.empty((total, hkv, d), dtype=dtype, device=device)
+        values = torch.empty_like(keys)
+    else:
+        keys, values = out
+        want = (total, hkv, d)
+        if (tuple(keys.shape) != want or tuple(values.shape) != want or keys.dtype != values.dtype
+                or not (keys.is_contiguous() and values.is_contiguous())):
+            raise ValueError("out must be two contiguous [sum(contexts), Hkv, D] tensors of one dtype")
+        _lib.dtype_code(keys.dtype)
+        _lib.require_cuda(key_pages, keys, values)
+    if total == 0:
+        return keys, values
+    if max(contexts) > block_tables.shape[1] * bs:
+        raise ValueError("a context is longer than its block-table row")
+    if cu_seqlens_k is None:
+        cu = [0]
+        for c in contexts:
+            cu.append(cu[-1] + c)
+        cu_seqlens_k = torch.tensor(cu, dtype=torch.int32).to(device, non_blocking=True)
+    elif cu_seqlens_k.shape != (len(contexts) + 1,):
+        raise ValueError("cu_seqlens_k must have num_requests + 1 entries")
+    _lib.require_cuda(key_pages, cu_seqlens_k)
+    _gather(keys, values, key_pages, value_pages, dims, _idx(block_tables), _idx(cu_seqlens_k),
+            total, max(contexts))
+    return keys, values
+
+
+def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, *,
+                        max_seqlen_q: int, total_k: int | None = None, scale: float | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal chunked prefill from the 4-bit cache; also mixed batches.
+
+    As ``paged_prefill``: request r's rows sit at the end of its context
+    (``cu_seqlens_k`` is cumulative over contexts, the chunk included, which is
+    already stored).  ``total_k`` is the sum of the contexts (or a bound on
+    it) and sizes the workspace; without it the block table's capacity does.
+    """
+    if torch.compiler.is_compiling():  # an opaque node for torch.compile
+        res = torch.ops.microinfer_b200.paged_prefill_mxfp4(
+            query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables,
+            int(max_seqlen_q), total_k, scale)
+        return res if out is None else out.copy_(res)
+    dims = page_dims(key_pages, value_pages)
+    _, bs, hkv, d = dims
+    _check_query(query, hkv, d, out)
+    _lib.dtype_code(query.dtype)
+    if block_tables.ndim != 2:
+        raise ValueError("block_tables must have one row per request")
+    requests, width = block_tables.shape
+    if cu_seqlens_q.shape != (requests + 1,) or cu_seqlens_k.shape != (requests + 1,):
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have num_requests + 1 entries")
+    if query.shape[0] == 0 or requests == 0:
+        return torch.empty_like(query) if out is None else out
+    if max_seqlen_q <= 0:
+        raise ValueError("max_seqlen_q must be positive")
+    if total_k is not None and total_k < 0:
+        raise ValueError("total_k must be non-negative")
+    device = _lib.require_cuda(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables)
+    rows = requests * width * bs
+    if total_k is not None:
+        rows = min(rows, int(total_k))
+    if rows == 0:  # no request can have a key
+        return torch.zeros_like(query) if out is None else out.zero_()
+    query, block_tables = _aligned(query), _idx(block_tables)
+    cu_seqlens_q, cu_seqlens_k = _idx(cu_seqlens_q), _idx(cu_seqlens_k)
+    keys = torch.empty((rows, hkv, d), dtype=query.dtype, device=device)
+    values = torch.empty_like(keys)
+    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows,
+            min(rows, width * bs))
+    return varlen_prefill(query, keys, values, cu_seqlens_q, cu_seqlens_k,
+                          max_seqlen_q=max_seqlen_q, scale=scale, out=out)
+
+
+def paged_attention_mxfp4_meta(query, key_pages, value_pages, metadata, *,
+                               scale: float | None = None) -> torch.Tensor:
+    """Backend dispatch on validated metadata, as ``paged_attention_meta`` over the 4-bit cache."""
+    if query.shape[0] == 0:
+        return torch.empty_like(query)
+    block_tables = metadata.block_tables
+    if block_tables is None:
+        raise ValueError("paged attention needs metadata.block_tables")
+    if metadata.is_decode and metadata.context_lens is not None:
+        return paged_decode_mxfp4(query, key_pages, value_pages, block_tables,
+                                  metadata.context_lens, scale=scale)
+    cu_q, cu_k = metadata.cu_seqlens_q, metadata.cu_seqlens_k
+    if cu_q is None:
+        cu_q = torch.tensor(metadata.cu_q_cpu, dtype=torch.int32, device=query.device)
+    if cu_k is None:
+        if metadata.context_lens is None:
+            raise ValueError("metadata needs cu_seqlens_k or context_lens")
+        cu_k = torch.zeros(metadata.context_lens.numel() + 1, dtype=torch.int32,
+                           device=query.device)
+        torch.cumsum(metadata.context_lens, 0, out=cu_k[1:])
+    max_q = metadata.max_seqlen_q or max(metadata.q_lens_cpu, default=0)
+    most = metadata.max_seqlen_k
+    return paged_prefill_mxfp4(query, key_pages, value_pages, cu_q, cu_k, block_tables,
+                               max_seqlen_q=max_q,
+                               total_k=most * block_tables.shape[0] if most else None, scale=scale)

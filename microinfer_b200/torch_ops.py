@@ -15,9 +15,11 @@ from __future__ import annotations
 
 import torch
 
+from microinfer_b200.layer import mxfp4_attention as _mx
 from microinfer_b200.layer import paged_attention as _pa
 from microinfer_b200.layer import prologue as _pro
 from microinfer_b200.worker import kv_store as _store
+from microinfer_b200.worker import mxfp4_cache as _mxc
 
 _NS = "microinfer_b200"
 
@@ -106,3 +108,43 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
 def _(qkv, q_weight, k_weight, positions, cos_table, sin_table, key_cache, value_cache,
       slot_mapping, num_q_heads, num_kv_heads, eps, interleaved=False):
     return qkv.new_empty((qkv.shape[0], num_q_heads, key_cache.shape[-1]))
+
+
+@torch.library.custom_op(f"{_NS}::store_kv_mxfp4", mutates_args=("key_pages", "value_pages"))
+def store_kv_mxfp4(key_pages: torch.Tensor, value_pages: torch.Tensor, slots: torch.Tensor,
+                   keys: torch.Tensor, values: torch.Tensor) -> None:
+    _mxc.store_kv_mxfp4(key_pages, value_pages, slots, keys, values)
+
+
+@store_kv_mxfp4.register_fake
+def _(key_pages, value_pages, slots, keys, values):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::paged_decode_mxfp4", mutates_args=())
+def paged_decode_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                       block_tables: torch.Tensor, context_lens: torch.Tensor,
+                       scale: float | None = None) -> torch.Tensor:
+    return _mx.paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens,
+                                  scale=scale)
+
+
+@paged_decode_mxfp4.register_fake
+def _(query, key_pages, value_pages, block_tables, context_lens, scale=None):
+    return torch.empty_like(query)
+
+
+@torch.library.custom_op(f"{_NS}::paged_prefill_mxfp4", mutates_args=())
+def paged_prefill_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                        cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                        block_tables: torch.Tensor, max_seqlen_q: int,
+                        total_k: int | None = None, scale: float | None = None) -> torch.Tensor:
+    return _mx.paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k,
+                                   block_tables, max_seqlen_q=max_seqlen_q, total_k=total_k,
+                                   scale=scale)
+
+
+@paged_prefill_mxfp4.register_fake
+def _(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, max_seqlen_q,
+      total_k=None, scale=None):
+    return torch.empty_like(query)
