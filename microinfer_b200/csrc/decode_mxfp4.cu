@@ -21,6 +21,12 @@
 
 namespace mi {
 
+bool mxfp4_mma_supported(int dtype, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
+                         int block_size, int64_t capacity);
+size_t mxfp4_mma_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
+                           int sms);
+cudaError_t launch_mxfp4_mma(const MxDecodeParams &p, int dtype, cudaStream_t stream);
+
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
@@ -242,16 +248,23 @@ int simt_splits(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t cap
 
 }  // namespace
 
+// The workspace of either form; it does not depend on the pool's size, which decides between
+// them for pools of 2^31 groups and more.
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                               int64_t capacity, int sms) {
-  (void)dtype;
   const int s = simt_splits(num_seqs, num_q_heads, num_kv_heads, capacity, sms);
-  return s == 1 ? 0 : static_cast<size_t>(num_seqs) * num_q_heads * s * (head_dim + 2) * sizeof(float);
+  const size_t simt =
+      s == 1 ? 0 : static_cast<size_t>(num_seqs) * num_q_heads * s * (head_dim + 2) * sizeof(float);
+  if (!mxfp4_mma_supported(dtype, num_q_heads, num_kv_heads, head_dim, 1, kMxGroup, capacity)) return simt;
+  const size_t mma = mxfp4_mma_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, capacity, sms);
+  return mma > simt ? mma : simt;
 }
 
 cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream) {
-  const int s = simt_splits(p.num_seqs, p.num_q_heads, p.num_kv_heads, p.bt_stride * p.block_size,
-                            sm_count_current());
+  const int64_t capacity = p.bt_stride * p.block_size;
+  if (mxfp4_mma_supported(dtype, p.num_q_heads, p.num_kv_heads, p.head_dim, p.num_blocks, p.block_size, capacity))
+    return launch_mxfp4_mma(p, dtype, stream);
+  const int s = simt_splits(p.num_seqs, p.num_q_heads, p.num_kv_heads, capacity, sm_count_current());
   if (dtype == MI_DTYPE_BFLOAT16) return launch_simt_t<__nv_bfloat16>(p, s, stream);
   if (dtype == MI_DTYPE_FLOAT16) return launch_simt_t<__half>(p, s, stream);
   return launch_simt_t<float>(p, s, stream);

@@ -82,12 +82,12 @@ def rows(pages, table, ctx):
 def attention(q, k, v, scale):
     """Causal attention of q [n, Hq, D], at the end of k / v [ctx, Hkv, D], in float64.
 
-    Returns the result, the sum of p |v| and the sum of scale |q| |k| of the largest
-    key (what rounding errors are measured against).
+    Returns the result and what rounding errors are measured against: the sum of p |v|, the
+    largest key's sum of scale |q| |k|, and ctx times the largest |v| of each block of 32.
     """
     n, hq, _ = q.shape
     ctx, hkv, d = k.shape
-    out, weight, size = (np.zeros((n, hq, d)) for _ in range(3))
+    out, weight, size, floor = (np.zeros((n, hq, d)) for _ in range(4))
     for h in range(hq if ctx else 0):
         kh, vh = k[:, h // (hq // hkv)], v[:, h // (hq // hkv)]
         x = q[:, h] @ kh.T * scale
@@ -98,4 +98,5 @@ def attention(q, k, v, scale):
         out[:, h] = p @ vh
         weight[:, h] = p @ np.abs(vh)
         size[:, h] = far.max(-1, keepdims=True)
-    return out, weight, size
+        floor[:, h] = ctx * np.abs(vh).reshape(ctx, -1, 32).max((0, 2)).repeat(32)
+    return out, weight, size, floor
