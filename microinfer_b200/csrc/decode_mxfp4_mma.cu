@@ -34,6 +34,7 @@
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
 // segment and the second launch has nothing to do.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -46,12 +47,13 @@ namespace mi {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kWarps = 16;
+constexpr int kWarps = 12;
 constexpr int kStages = 4;
 constexpr int kCols = 8;            // query heads of a segment: the MMA's N
 constexpr int kMaxSeqs = 2048;      // sequences of one launch (prefix sums in shared memory)
 constexpr float kLift = 12.f;       // p is held as 2^(x - m + kLift): f16 reaches 2^-37 of the largest p
 constexpr float kLag = 3.f;         // m may be this far behind: p <= 2^15
+constexpr uint32_t kLowestRef = 0x20202020u;  // R_b - 255 then has a bit of 0xf8 set, like every far scale
 constexpr int kAlignedSlack = 2;    // groups per warp that keeping a segment in one CTA may cost
 
 template <int NB>
@@ -63,19 +65,20 @@ struct MxCfg {
   static constexpr int kState = kCols * (D + 2);  // floats: acc [8][D], m [8], l [8]
   static constexpr int kSmemRing = kWarps * kRing;
   static constexpr int kSmemHeads = kWarps * kState * 4;  // parts that end before their warp's range does
+  static constexpr int kSmemUnits = kWarps * 64 * 16;  // two batches of 32 units per warp
   static constexpr int kSmemBars = kWarps * kStages * 8;
   static constexpr int kSmemPrefix = (kMaxSeqs + 1) * 4;
-  static constexpr int kSmemMisc = 4 * kWarps * 4 + 8 * kWarps + 64;
-  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemBars + kSmemPrefix + kSmemMisc;
+  static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kCols * 12 + 16;
+  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemBars + kSmemPrefix + kSmemMisc;
   static_assert(kState * 4 <= kRing, "a warp's last part goes into its own ring");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
-// What a CTA leaves in the workspace beside its states: the segment of its first
-// part if that began in an earlier CTA, whether it ends here, and the segment
-// of its last part if that began here and goes on (-1: none).
+// Beside its states (a part whose segment began in an earlier CTA, then one whose
+// segment goes on in the next) a CTA leaves in the workspace the segment that goes
+// on (-1: none) and how many CTAs hold parts of it.
 struct MxMeta {
-  int32_t head, head_ends, tail, pad;
+  int32_t segment, parts;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
@@ -92,13 +95,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t &r0, uint32_t &r1
 }
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -153,8 +155,103 @@ __device__ __forceinline__ void key_pairs(uint32_t v, uint32_t (&e)[4]) {
       "mov.b32 {b0, b1, b2, b3}, %5;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, b2;\n\t"
       "cvt.rn.f16x2.e2m1x2 %2, b3; }"
-      : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
+      : "=&r"(e[0]), "=&r"(e[1]), "=&r"(e[2]), "=&r"(e[3])  // written before y is read
       : "r"(x), "r"(y));
+}
+
+// P_b of this lane's keys times V's block b into `d0`, `d1` (rows j = 0, 1).
+__device__ __forceinline__ void value_block(uint32_t lo, uint32_t hi, uint32_t p0, uint32_t p1, float (&d0)[4],
+                                            float (&d1)[4]) {
+  uint32_t a[4], c[4];
+  key_pairs(lo, a);
+  key_pairs(hi, c);
+  mma_f16(d0, a[0], a[1], c[0], c[1], p0, p1);
+  mma_f16(d1, a[2], a[3], c[2], c[3], p0, p1);
+}
+
+// 2^(e - 127) (1 + 2^-23) of byte b: the low bit makes the byte 255 a NaN, and all scores share the factor.
+__device__ __forceinline__ float scale_of(uint32_t w, int b) {
+  const uint32_t v = b == 0 ? w << 23 : b == 1 ? w << 15 : b == 2 ? w << 7 : w >> 1;
+  return __uint_as_float((v & 0x7f800000u) | 1u);
+}
+
+// Scale byte of block b, key `which` (0, 1) of a key pair's words.
+template <int NB>
+__device__ __forceinline__ int byte_of(uint32_t w0, uint32_t w1, int b, int which) {
+  if constexpr (NB == 4)
+    return ((which ? w1 : w0) >> (8 * b)) & 255u;
+  else
+    return (w0 >> (16 * which + 8 * b)) & 255u;
+}
+
+// Scales that the window of 8 binades does not hold: raise R_b (a byte of `ref`, returned) where a
+// scale is above it, then take the keys window by window.  `o` is the caller's copy of its
+// accumulators; `pp0`, `pp1`: p of keys (2t, 2t+1) and (2t+8, 2t+9) of query g.  Out of line, so that
+// the loop around it keeps its registers.
+template <int NB>
+__device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vcodes, uint4 w, uint32_t pp0,
+                                            uint32_t pp1, int valid) {
+  const int lane = threadIdx.x & 31;
+  int deepest = 0;
+  const int key = (lane & 3) * 2;  // scales of keys that do not exist: none
+  if constexpr (NB == 4) {
+    if (key >= valid) w.x = 0;
+    if (key + 1 >= valid) w.y = 0;
+    if (key + 8 >= valid) w.z = 0;
+    if (key + 9 >= valid) w.w = 0;
+  } else {
+    w.x &= (key < valid ? 0xffffu : 0u) | (key + 1 < valid ? 0xffff0000u : 0u);
+    w.z &= (key + 8 < valid ? 0xffffu : 0u) | (key + 9 < valid ? 0xffff0000u : 0u);
+  }
+#pragma unroll 1
+  for (int b = 0; b < NB; ++b) {
+    int top = 0, low = 255;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = k < 2 ? byte_of<NB>(w.x, w.y, b, k & 1) : byte_of<NB>(w.z, w.w, b, k & 1);
+      if (s >= 1 && s <= 254) top = max(top, s), low = min(low, s);
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      top = max(top, __shfl_xor_sync(kAll, top, off));
+      low = min(low, __shfl_xor_sync(kAll, low, off));
+    }
+    int r = (ref >> (8 * b)) & 255;
+    if (top > r) {
+      const int next = min(top + 2, 254);
+      const float f = exp2i(r - next);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[b * 8 + i] *= f;
+      ref = (ref & ~(255u << (8 * b))) | (static_cast<uint32_t>(next) << (8 * b));
+      r = next;
+    }
+    if (low < 255) deepest = max(deepest, r - low);
+  }
+  uint32_t lo[NB], hi[NB];
+  load_codes<NB, true>(vcodes, lane, lo, hi);
+#pragma unroll 1
+  for (int window = 0; window <= deepest / 8; ++window) {
+    const float back = exp2i(-8 * window);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int r = (ref >> (8 * b)) & 255;
+      uint32_t f[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int s = k < 2 ? byte_of<NB>(w.x, w.y, b, k & 1) : byte_of<NB>(w.z, w.w, b, k & 1), d = r - s;
+        f[k] = s >= 1 && s <= 254 && (d >> 3) == window ? 0x3c00u - ((d & 7) << 10) : 0u;
+        if (s == 255 && window == 0) f[k] = 0x7e00u;
+      }
+      float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+      value_block(lo[b], hi[b], mul_f16x2(pp0, f[0] | f[1] << 16), mul_f16x2(pp1, f[2] | f[3] << 16), d0, d1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[b * 8 + i] = fmaf(d0[i], back, o[b * 8 + i]);
+        o[b * 8 + 4 + i] = fmaf(d1[i], back, o[b * 8 + 4 + i]);
+      }
+    }
+  }
+  return ref;
 }
 
 // One query head's state of a segment part, laid out [8][D] acc, [8] m, [8] l.
@@ -170,7 +267,7 @@ struct MxWarp {
   int lane, g, t;
 
   __device__ __forceinline__ void reset() {
-    ref = 0x20202020u;  // the lowest reference: a byte of 255 is then never mistaken for a near one
+    ref = kLowestRef;
 #pragma unroll
     for (int i = 0; i < NB * 2; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     m[0] = m[1] = -INFINITY;
@@ -211,83 +308,9 @@ struct MxWarp {
     xs[1] = __shfl_sync(kAll, back, 8 * t + 4);
   }
 
-  // P_b of this lane's keys times V's block b into `d0`, `d1` (rows j = 0, 1).
-  __device__ __forceinline__ static void value_block(uint32_t lo, uint32_t hi, uint32_t p0, uint32_t p1,
-                                                     float (&d0)[4], float (&d1)[4]) {
-    uint32_t a[4], c[4];
-    key_pairs(lo, a);
-    key_pairs(hi, c);
-    mma_f16(d0, a[0], a[1], c[0], c[1], p0, p1);
-    mma_f16(d1, a[2], a[3], c[2], c[3], p0, p1);
-  }
-
-  // Scale byte of key pair word(s), block b, key `which` (0, 1) of the pair.
-  __device__ __forceinline__ static uint32_t byte_of(const uint32_t (&w)[2], int b, int which) {
-    if constexpr (NB == 4)
-      return (w[which] >> (8 * b)) & 255u;
-    else
-      return (w[0] >> (16 * which + 8 * b)) & 255u;
-  }
-
-  // Scales that the window of 8 binades does not hold: raise R_b where a scale is above it,
-  // then take the keys window by window.  `pp`: p of keys (2t, 2t+1) and (2t+8, 2t+9) of query g.
-  __device__ __forceinline__ void value_slow(uint32_t vcodes, const uint32_t (&w0)[2], const uint32_t (&w1)[2],
-                                          uint32_t pp0, uint32_t pp1) {
-    int deepest = 0;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      int top = 0, low = 255;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = byte_of(k < 2 ? w0 : w1, b, k & 1);
-        if (s >= 1 && s <= 254) top = max(top, s), low = min(low, s);
-      }
-#pragma unroll
-      for (int off = 1; off < 4; off <<= 1) {
-        top = max(top, __shfl_xor_sync(kAll, top, off));
-        low = min(low, __shfl_xor_sync(kAll, low, off));
-      }
-      int r = (ref >> (8 * b)) & 255;
-      if (top > r) {
-        const int next = min(top + 2, 254);
-        const float f = exp2i(r - next);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[2 * b + j][i] *= f;
-        ref = (ref & ~(255u << (8 * b))) | (static_cast<uint32_t>(next) << (8 * b));
-        r = next;
-      }
-      if (low < 255) deepest = max(deepest, r - low);
-    }
-    uint32_t lo[NB], hi[NB];
-    load_codes<NB, true>(vcodes, lane, lo, hi);
-#pragma unroll 1
-    for (int window = 0; window <= deepest / 8; ++window) {
-      const float back = exp2i(-8 * window);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int r = (ref >> (8 * b)) & 255;
-        uint32_t f[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int s = byte_of(k < 2 ? w0 : w1, b, k & 1), d = r - s;
-          f[k] = s >= 1 && s <= 254 && (d >> 3) == window ? 0x3c00u - ((d & 7) << 10) : 0u;
-          if (s == 255 && window == 0) f[k] = 0x7e00u;
-        }
-        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-        value_block(lo[b], hi[b], mul_f16x2(pp0, f[0] | f[1] << 16), mul_f16x2(pp1, f[2] | f[3] << 16), d0, d1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[2 * b][i] = fmaf(d0[i], back, o[2 * b][i]);
-          o[2 * b + 1][i] = fmaf(d1[i], back, o[2 * b + 1][i]);
-        }
-      }
-    }
-  }
-
-  // One group: `kbase`, `vbase` its K and V bytes in shared memory, `valid` of its 16 keys exist.
-  __device__ __forceinline__ void process(uint32_t kbase, uint32_t vbase, int valid) {
+  // One group: `kbase`, `vbase` its K and V bytes in shared memory, `valid` of its 16 keys exist;
+  // `first`: the state holds none yet.
+  __device__ __forceinline__ void process(uint32_t kbase, uint32_t vbase, int valid, bool first) {
     float x[4] = {0.f, 0.f, 0.f, 0.f};  // (key g, queries 2t, 2t + 1), (key g + 8, ...)
     {
       uint32_t lo[NB], hi[NB], wl, wh;
@@ -307,15 +330,15 @@ struct MxWarp {
         float d[4] = {0.f, 0.f, 0.f, 0.f};
         mma_f16(d, a[0], c[0], a[1], c[1], q[2 * b][0], q[2 * b][1]);
         mma_f16(d, a[2], c[2], a[3], c[3], q[2 * b + 1][0], q[2 * b + 1][1]);
-        // 2^(e - 127) (1 + 2^-23): the low bit makes the byte 255 a NaN, and all scores share the factor
-        const float fl = __uint_as_float((((wl >> (8 * b)) & 255u) << 23) | 1u);
-        const float fh = __uint_as_float((((wh >> (8 * b)) & 255u) << 23) | 1u);
+        const float fl = scale_of(wl, b), fh = scale_of(wh, b);
         x[0] = fmaf(d[0], fl, x[0]);
         x[1] = fmaf(d[1], fl, x[1]);
         x[2] = fmaf(d[2], fh, x[2]);
         x[3] = fmaf(d[3], fh, x[3]);
       }
     }
+    uint32_t vlo[NB], vhi[NB];
+    load_codes<NB, true>(vbase, lane, vlo, vhi);
     // V's scales: words of keys 2t, 2t + 1 and 2t + 8, 2t + 9
     uint32_t w0[2], w1[2];
     if constexpr (NB == 4) {
@@ -327,6 +350,19 @@ struct MxWarp {
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
       asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
       w0[1] = w1[1] = 0;
+    }
+    if (first) {  // uniform: R_b starts at the largest scale here and two binades of room
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+        const uint32_t(&w)[2] = k < 2 ? w0 : w1;
+        uint32_t bytes = NB == 4 ? w[k & 1] : (w[0] >> (16 * (k & 1))) & 0xffffu;
+        if (key < valid) top = __vmaxu4(top, bytes);
+      }
+      top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 1));
+      top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 2));
+      ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] *= xs[i & 1];
@@ -367,34 +403,32 @@ struct MxWarp {
     l[1] += p[1] + p[3];
     const uint32_t pp0 = movm(pack_f16(p[0], p[1])), pp1 = movm(pack_f16(p[2], p[3]));
 
-    // how far below the reference each scale is, per byte
-    uint32_t d0[2], d1[2], bad;
+    // how far below the reference each scale is, per byte: 0 to 7, or a bit of 0xf8 is set
+    uint32_t u[2][NB / 2], bad = 0;  // [key pair][block pair]: bytes (key 0: b, b + 1; key 1: b, b + 1)
     if constexpr (NB == 4) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) d0[k] = ref - w0[k], d1[k] = ref - w1[k];
-      bad = (d0[0] | d0[1] | d1[0] | d1[1]) & 0xf8f8f8f8u;
+      const uint32_t a0 = ref - w0[0], a1 = ref - w0[1], c0 = ref - w1[0], c1 = ref - w1[1];
+      bad = (a0 | a1 | c0 | c1) & 0xf8f8f8f8u;
+      u[0][0] = __byte_perm(a0, a1, 0x5410), u[0][1] = __byte_perm(a0, a1, 0x7632);
+      u[1][0] = __byte_perm(c0, c1, 0x5410), u[1][1] = __byte_perm(c0, c1, 0x7632);
     } else {
       const uint32_t both = (ref & 0xffffu) * 0x10001u;
-      d0[0] = both - w0[0], d1[0] = both - w1[0];
-      bad = (d0[0] | d1[0]) & 0xf8f8f8f8u;
+      u[0][0] = both - w0[0], u[1][0] = both - w1[0];
+      bad = (u[0][0] | u[1][0]) & 0xf8f8f8f8u;
     }
     if (__any_sync(kAll, bad != 0)) {
-      value_slow(vbase, w0, w1, pp0, pp1);
+      float copy[NB * 8];
+#pragma unroll
+      for (int i = 0; i < NB * 8; ++i) copy[i] = o[i / 4][i % 4];
+      ref = value_slow<NB>(copy, ref, vbase, make_uint4(w0[0], w0[1], w1[0], w1[1]), pp0, pp1, valid);
+#pragma unroll
+      for (int i = 0; i < NB * 8; ++i) o[i / 4][i % 4] = copy[i];
     } else {
-      uint32_t lo[NB], hi[NB];
-      load_codes<NB, true>(vbase, lane, lo, hi);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint32_t z0, z1;  // d of the pair's keys in bits 8-11 and 24-27
-        if constexpr (NB == 4) {
-          z0 = __byte_perm(d0[0], d0[1], b << 4 | (b + 4) << 12);
-          z1 = __byte_perm(d1[0], d1[1], b << 4 | (b + 4) << 12);
-        } else {
-          z0 = __byte_perm(d0[0], 0, b << 4 | (b + 2) << 12);
-          z1 = __byte_perm(d1[0], 0, b << 4 | (b + 2) << 12);
-        }
-        const uint32_t f0 = 0x3c003c00u - ((z0 & 0x07000700u) << 2), f1 = 0x3c003c00u - ((z1 & 0x07000700u) << 2);
-        value_block(lo[b], hi[b], mul_f16x2(pp0, f0), mul_f16x2(pp1, f1), o[2 * b], o[2 * b + 1]);
+        // f16 2^-d: the exponent 15 - d is 15 ^ d
+        const uint32_t z0 = u[0][b / 2] << (b & 1 ? 2 : 10), z1 = u[1][b / 2] << (b & 1 ? 2 : 10);
+        const uint32_t f0 = (z0 & 0x1c001c00u) ^ 0x3c003c00u, f1 = (z1 & 0x1c001c00u) ^ 0x3c003c00u;
+        value_block(vlo[b], vhi[b], mul_f16x2(pp0, f0), mul_f16x2(pp1, f1), o[2 * b], o[2 * b + 1]);
       }
     }
   }
@@ -459,11 +493,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   constexpr int D = C::D;
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads);
+  int4 *unit_table = reinterpret_cast<int4 *>(smem + C::kSmemRing + C::kSmemHeads);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits);
   int *prefix = reinterpret_cast<int *>(bars + kWarps * kStages);  // groups before sequence s
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
   int *scan = part_flags + 2 * kWarps;      // [2 * kWarps]
+  float *factor = reinterpret_cast<float *>(scan + 2 * kWarps);               // [2 * kWarps][8]
+  float2 *run_ml = reinterpret_cast<float2 *>(                               // [2 * kWarps][8]
+      (reinterpret_cast<uintptr_t>(factor + 2 * kWarps * kCols) + 15) & ~static_cast<uintptr_t>(15));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t *wbar = bars + warp * kStages;
   uint8_t *ring = smem + warp * C::kRing;
@@ -483,7 +521,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   const int64_t cap = p.bt_stride * p.block_size;
   int c_max = 0;
   {
-    constexpr int kPer = kMaxSeqs / (kWarps * 32);
+    constexpr int kPer = (kMaxSeqs + kWarps * 32 - 1) / (kWarps * 32);
     int c[kPer], sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -576,34 +614,34 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     return r;
   };
   const int per_page = p.block_size / kMxGroup;
-  // A batch of 32 units, one per lane: the index of its group in the pools (-1: no
-  // such page) and what `process` has to know: keys in the group (bits 0-4),
-  // whether it is its segment's first (32) or last (64) group.
-  auto load_batch = [&](int first, int &where, int &what) {
-    where = -1, what = 0;
+  // Batches of 32 units, one per lane, in shared memory: x, the index of the unit's group in the
+  // pools (-1: no such page); y, the keys in it (bits 0-4) and whether it is its segment's first
+  // (32) or last (64) group; z, w, its sequence and head tile.
+  int4 *table = unit_table + warp * 64;
+  auto load_batch = [&](int first) {
     const int i = first + lane;
-    if (i >= units) return;
-    const Unit r = unit_of(i);
-    const int page = __ldg(p.block_tables + static_cast<int64_t>(r.seq) * p.bt_stride + r.group / per_page);
-    int valid = kMxGroup;
-    if (r.group == r.groups - 1) {
-      const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + r.seq)), cap));
-      valid = ctx - r.group * kMxGroup;
-      what |= 64;
+    if (i < units) {
+      const Unit r = unit_of(i);
+      const int page = __ldg(p.block_tables + static_cast<int64_t>(r.seq) * p.bt_stride + r.group / per_page);
+      int valid = kMxGroup, flags = r.group == 0 ? 32 : 0;
+      if (r.group == r.groups - 1) {
+        const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + r.seq)), cap));
+        valid = ctx - r.group * kMxGroup;
+        flags |= 64;
+      }
+      int where = -1;
+      if (page >= 0 && page < p.num_blocks)
+        where = (page * p.num_kv_heads + r.ht / tiles) * per_page + r.group % per_page;
+      else
+        flag_status(p.status, MI_DEV_BAD_BLOCK);
+      table[i & 63] = make_int4(where, valid | flags, r.seq, r.ht);
     }
-    what |= valid | (r.group == 0 ? 32 : 0);
-    if (page >= 0 && page < p.num_blocks)
-      where = (page * p.num_kv_heads + r.ht / tiles) * per_page + r.group % per_page;
-    else
-      flag_status(p.status, MI_DEV_BAD_BLOCK);
+    __syncwarp();
   };
-  int where_cur, what_cur, where_nxt, what_nxt;
-  load_batch(0, where_cur, what_cur);
-  load_batch(32, where_nxt, what_nxt);
-  auto issue = [&](int now, int i) {  // unit i, while unit `now` is being worked on
-    const int a = __shfl_sync(kAll, where_cur, i & 31), b = __shfl_sync(kAll, where_nxt, i & 31);
-    const int where = (i >> 5) == (now >> 5) ? a : b;
+  load_batch(0);
+  auto issue = [&](int i) {
     if (lane != 0) return;
+    const int where = table[i & 63].x;
     uint64_t *bar = &wbar[i % kStages];
     if (where < 0) {
       mbar_arrive(bar);
@@ -616,16 +654,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     bulk_g2s(dst + C::kGroup, p.value_pages + off, C::kGroup, bar);
   };
   int issued = 0;
-  for (; issued < kStages && issued < units; ++issued) issue(0, issued);
+  for (; issued < kStages && issued < units; ++issued) issue(issued);
 
   MxWarp<T, NB> st;
   st.lane = lane, st.g = lane >> 2, st.t = lane & 3;
   int seq = 0, ht = 0, heads = 0;
   bool has_first = false;
-  auto start_segment = [&](int i) {
-    const Unit r = unit_of(i);
-    seq = r.seq, ht = r.ht;
-    has_first = r.group == 0;
+  auto start_segment = [&](const int4 &unit) {
+    seq = unit.z, ht = unit.w;
+    has_first = (unit.y & 32) != 0;
     const int kvh = ht / tiles, h0 = (ht - kvh * tiles) * kCols;
     heads = min(kCols, G - h0);
     st.reset();
@@ -650,27 +687,22 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   bool timed_out = false;
 #pragma unroll 1
   for (int i = 0; i < units; ++i) {
-    const int what = __shfl_sync(kAll, what_cur, i & 31), where = __shfl_sync(kAll, where_cur, i & 31);
-    if (i == 0 || (what & 32)) start_segment(i);
+    if ((i & 31) == 0) load_batch(i + 32);  // the half that units i - 32 to i - 1 have left
+    const int4 unit = table[i & 63];
+    const bool fresh = i == 0 || (unit.y & 32);
+    if (fresh) start_segment(unit);
     if (!mbar_wait_bounded(&wbar[i % kStages], (i / kStages) & 1, p.status)) {
       timed_out = true;
       break;
     }
-    if (where >= 0) {
+    if (unit.x >= 0) {
       const uint32_t base = smem_addr(ring + i % kStages * C::kStage);
-      st.process(base, base + C::kGroup, what & 31);
+      st.process(base, base + C::kGroup, unit.y & 31, fresh);
     }
     __syncwarp();  // every lane has read the stage
     const bool final = i == units - 1;
-    if (issued < units) {
-      issue(i, issued);
-      ++issued;
-    }
-    if ((what & 64) || final) end_segment((what & 64) != 0, final);
-    if ((i & 31) == 31) {  // the next unit starts batch (i + 1) / 32
-      where_cur = where_nxt, what_cur = what_nxt;
-      load_batch(i + 33, where_nxt, what_nxt);
-    }
+    if (issued < units) issue(issued++);
+    if ((unit.y & 64) || final) end_segment((unit.y & 64) != 0, final);
   }
   if (timed_out) {  // the copies in flight land before the ring is given up
     if (lane == 0)
@@ -681,87 +713,138 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   __syncthreads();
 
   // ---- join the parts: runs of one segment over neighbouring warps ----
-  MxMeta meta = {-1, 0, -1, 0};
-  float *ws = p.workspace + static_cast<int64_t>(blockIdx.x) * 2 * C::kState;
+  // Every warp sees the list of parts, one per lane.
+  static_assert(2 * kWarps <= 32, "one lane per part");
+  const int my_seg = lane < 2 * kWarps ? part_seg[lane] : -1;
+  const unsigned present = __ballot_sync(kAll, my_seg >= 0);
+  const unsigned below = present & ((1u << lane) - 1u);
+  const int prev_seg = __shfl_sync(kAll, my_seg, below ? 31 - __clz(below) : lane);
+  const bool begins = my_seg >= 0 && (below == 0 || prev_seg != my_seg);
+  const unsigned starts = __ballot_sync(kAll, begins);
+  const int my_flags = my_seg >= 0 ? part_flags[lane] : 0;
   auto part = [&](int k) -> const float * {
     return k & 1 ? reinterpret_cast<const float *>(smem + (k >> 1) * C::kRing) : heads_smem + (k >> 1) * C::kState;
   };
-  for (int k = 0; k < 2 * kWarps;) {
-    const int seg = part_seg[k];
-    if (seg < 0) {
-      ++k;
-      continue;
+  // the parts' factors and sums: warp h takes query head h, lane k part k
+  for (int h = warp; h < kCols; h += kWarps) {
+    float m = -INFINITY, l = 0.f;
+    if (my_seg >= 0) m = part(lane)[kCols * D + h], l = part(lane)[kCols * D + kCols + h];
+    for (unsigned left = starts; left; left &= left - 1) {
+      const int k = __ffs(left) - 1;
+      const unsigned later = left & (left - 1);
+      const bool mine = my_seg >= 0 && lane >= k && (later == 0 || lane < __ffs(later) - 1);
+      float M = mine ? m : -INFINITY;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, off));
+      const float f = mine ? part_factor(m, l, M) : 0.f;
+      float L = f * l;
+      if (!mine) L = 0.f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(kAll, L, off);
+      if (mine) factor[lane * kCols + h] = f;
+      if (lane == k) run_ml[lane * kCols + h] = make_float2(M, L);
     }
-    int end = k, flags = 0;
-    for (; end < 2 * kWarps && (part_seg[end] == seg || part_seg[end] < 0); ++end)
-      if (part_seg[end] >= 0) flags |= part_flags[end];
+  }
+  __syncthreads();
+  float *ws = p.workspace + static_cast<int64_t>(blockIdx.x) * 2 * C::kState;
+  MxMeta meta = {-1, 0};
+  bool has_head = false;
+  for (unsigned left = starts; left; left &= left - 1) {
+    const int k = __ffs(left) - 1;
+    const unsigned later = left & (left - 1);
+    const unsigned in_run = present & ~((1u << k) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : kAll);
+    const int seg = __shfl_sync(kAll, my_seg, k);
+    const int flags = __reduce_or_sync(kAll, in_run >> lane & 1u ? my_flags : 0);
     const int s = seg / H, h_t = seg - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * kCols;
     const int hs = min(kCols, G - h0);
-    float *state = flags & 1 ? ws + C::kState : ws;  // began here / in an earlier CTA
+    if (flags != 3) {
+      if (flags & 1) {  // goes on in later CTAs, up to the one that holds its last unit
+        const uint64_t last = static_cast<uint64_t>(prefix[s]) * H + static_cast<uint64_t>(h_t + 1) * (prefix[s + 1] - prefix[s]) - 1;
+        meta.segment = seg;
+        meta.parts = static_cast<int>(((last + 1) * gridDim.x - 1) / total) - static_cast<int>(blockIdx.x) + 1;
+      } else {
+        has_head = true;
+      }
+    }
+    float *state = flags & 1 ? ws + C::kState : ws;
     T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
     for (int e = threadIdx.x; e < hs * D; e += blockDim.x) {
       const int h = e / D;
-      float M = -INFINITY, L = 0.f, A = 0.f;
-      for (int w = k; w < end; ++w)
-        if (part_seg[w] >= 0) M = fmaxf(M, part(w)[kCols * D + h]);
-      for (int w = k; w < end; ++w) {
-        if (part_seg[w] < 0) continue;
-        const float *x = part(w);
-        const float f = part_factor(x[kCols * D + h], x[kCols * D + kCols + h], M);
-        L += f * x[kCols * D + kCols + h];
-        A += f * x[e];
+      const float2 ml = run_ml[k * kCols + h];
+      float A = 0.f;
+      for (unsigned w = in_run; w; w &= w - 1) {
+        const int j = __ffs(w) - 1;
+        A = fmaf(factor[j * kCols + h], part(j)[e], A);
       }
       if (flags == 3) {
-        out[e] = Elem<T>::from_float(L == 0.f ? 0.f : A / L);
+        out[e] = Elem<T>::from_float(ml.y == 0.f ? 0.f : A / ml.y);
       } else {
         state[e] = A;
-        if (e - h * D == 0) state[kCols * D + h] = M, state[kCols * D + kCols + h] = L;
+        if (e - h * D == 0) state[kCols * D + h] = ml.x, state[kCols * D + kCols + h] = ml.y;
       }
     }
-    if (flags != 3) {
-      if (flags & 1)
-        meta.tail = seg;
-      else
-        meta.head = seg, meta.head_ends = flags >> 1;
-    }
-    k = end;
   }
-  if (threadIdx.x == 0 && p.workspace != nullptr)
-    reinterpret_cast<MxMeta *>(p.workspace + static_cast<int64_t>(gridDim.x) * 2 * C::kState)[blockIdx.x] = meta;
+  if (p.workspace != nullptr) {
+    if (threadIdx.x == 0)
+      reinterpret_cast<MxMeta *>(p.workspace + static_cast<int64_t>(gridDim.x) * 2 * C::kState)[blockIdx.x] = meta;
+    if (!has_head && threadIdx.x < kCols) {  // no part to give: one without keys
+      ws[kCols * D + threadIdx.x] = -INFINITY;
+      ws[kCols * D + kCols + threadIdx.x] = 0.f;
+    }
+  }
   pdl_launch_dependents();
 }
 
-// Segments that cross CTAs: the CTA in which one begins joins it.
+// Segments that cross CTAs: block (c, h) joins query head h of the one that goes
+// on from CTA c.  A thread takes one element; the quarters of the block take every fourth part.
+constexpr int kJoinWays = 4;
 template <typename T, int NB>
-__global__ void __launch_bounds__(512) mxfp4_decode_mma_join_kernel(const MxDecodeParams p, int tiles) {
+__global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
+    mxfp4_decode_mma_join_kernel(const MxDecodeParams p, int tiles) {
   using C = MxCfg<NB>;
   constexpr int D = C::D;
+  __shared__ float sums[kJoinWays][D];
+  __shared__ float ml[kJoinWays][2];
   pdl_wait();
-  const int ctas = gridDim.x;
-  const MxMeta *meta = reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState);
-  const int first = blockIdx.x, seg = meta[first].tail;
-  if (seg >= 0) {
-    int end = first + 1;  // one past the last CTA that has a part
-    while (end < ctas && meta[end].head == seg) {
-      ++end;
-      if (meta[end - 1].head_ends) break;
-    }
+  const int ctas = gridDim.x, first = blockIdx.x, h = blockIdx.y;
+  const MxMeta meta =
+      reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState)[first];
+  if (meta.segment >= 0) {
     const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * tiles;
-    const int s = seg / H, h_t = seg - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * kCols;
-    const int hs = min(kCols, G - h0);
-    T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
-    auto part = [&](int c) { return p.workspace + (static_cast<int64_t>(c) * 2 + (c == first ? 1 : 0)) * C::kState; };
-    for (int e = threadIdx.x; e < hs * D; e += blockDim.x) {
-      const int h = e / D;
-      float M = -INFINITY, L = 0.f, A = 0.f;
-      for (int c = first; c < end; ++c) M = fmaxf(M, part(c)[kCols * D + h]);
-      for (int c = first; c < end; ++c) {
-        const float *x = part(c);
-        const float f = part_factor(x[kCols * D + h], x[kCols * D + kCols + h], M);
-        L += f * x[kCols * D + kCols + h];
-        A += f * x[e];
+    const int s = meta.segment / H, h_t = meta.segment - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * kCols;
+    if (h0 + h < G) {  // uniform
+      const int d = threadIdx.x % D, way = threadIdx.x / D;
+      const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
+      const int parts = min(meta.parts, ctas - first);
+      auto part = [&](int k) { return base + (k == 0 ? 1 : 2 * k) * C::kState; };
+      float M = -INFINITY;
+#pragma unroll 4
+      for (int k = way; k < parts; k += kJoinWays) M = fmaxf(M, __ldcg(part(k) + kCols * D + h));
+      float L = 0.f, A = 0.f;
+#pragma unroll 4
+      for (int k = way; k < parts; k += kJoinWays) {
+        const float *x = part(k);
+        const float m = __ldcg(x + kCols * D + h), l = __ldcg(x + kCols * D + kCols + h), a = __ldcg(x + h * D + d);
+        const float f = part_factor(m, l, M);
+        L += f * l;
+        if (f != 0.f) A = fmaf(f, a, A);  // a part without keys has no sums
       }
-      out[e] = Elem<T>::from_float(L == 0.f ? 0.f : A / L);
+      sums[way][d] = A;
+      if (d == 0) ml[way][0] = M, ml[way][1] = L;
+      __syncthreads();
+      if (way == 0) {
+        M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWays; ++w) M = fmaxf(M, ml[w][0]);
+#pragma unroll
+        for (int w = 0; w < kJoinWays; ++w) {
+          const float f = part_factor(ml[w][0], ml[w][1], M);
+          L += f * ml[w][1];
+          A = fmaf(f, sums[w][d], A);
+        }
+        static_cast<T *>(p.out)[(static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0 + h) * D + d] =
+            Elem<T>::from_float(L == 0.f ? 0.f : A / L);
+      }
     }
   }
   pdl_launch_dependents();
@@ -781,7 +864,8 @@ cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, 
   }
   cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(kWarps * 32), C::kSmem, stream, p, tiles);
   if (e == cudaSuccess && join)
-    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB>, dim3(ctas), dim3(512), 0, stream, p, tiles);
+    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB>,
+                   dim3(ctas, std::min<int>(kCols, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, tiles);
   return e;
 }
 
