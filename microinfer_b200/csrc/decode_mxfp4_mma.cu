@@ -18,17 +18,20 @@
 //     8 binades, so no spread of scales loses more;
 //   - q is multiplied by a power of two that puts its largest element into
 //     [2^14, 2^15) and converted to f16 (exact for bf16 down to 2^-28 of that element).
-// Fragments need no transposition of codes: an ldmatrix of 8 keys x 16 bytes gives
-// each lane 8 consecutive codes of its key (K, dims in any order as long as q
-// follows it), and the transposed one gives 4 codes of two neighbouring keys, which two
-// bit-selects interleave to key pairs (V).  P goes from accumulator to operand
-// layout through two movmatrix.
+// No code is moved between lanes or interleaved.  An ldmatrix of 8 keys x 16 bytes gives each lane 8
+// consecutive codes of its key: K's A fragments, with dims in an order that q follows.  The
+// transposed one gives a lane two bytes of each of two keys, and each byte, two neighbouring dims of
+// one key, is an A register of V^T whose two k-slots are (key, even dim) and (key, odd dim);
+// the B operand then has a column for (query, even) and one for (query, odd), with P_b in one half of
+// a register and zero in the other, so a column gathers its own dims.  N = 8 holds 4 queries this
+// way (groups of up to 8 take two column tiles from the same decoded operands), and the scores' columns are
+// doubled to match, so that P goes from accumulator to operand layout through two movmatrix.
 //
-// Work: the groups of 16 keys of all (sequence, kv head, 8 query heads)
+// Work: the units of 32 keys of all (sequence, kv head, 4 or 8 query heads)
 // segments, in that order, are one list that is cut into equal ranges, one per
-// warp (16 warps to a CTA, one CTA to an SM), so ragged batches and single long
+// warp (one CTA to an SM), so ragged batches and single long
 // sequences load every SM alike.  A warp streams its range through a ring of bulk copies
-// (one of K and one of V per group; 4 stages, 139 KB in flight per SM at D = 128)
+// (one of K and one of V per group, 139 to 157 KB in flight per SM at D = 128)
 // that runs across segment borders.  Segments that lie within one
 // warp's range are written at once; the parts of others are joined in shared
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
@@ -47,31 +50,49 @@ namespace mi {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kWarps = 12;
-constexpr int kStages = 4;
-constexpr int kCols = 8;            // query heads of a segment: the MMA's N
+constexpr int kUnit = 2 * kMxGroup;  // keys of a unit of work
+constexpr int kQueries = 4;          // query heads of a column tile
 constexpr int kMaxSeqs = 2048;      // sequences of one launch (prefix sums in shared memory)
 constexpr float kLift = 12.f;       // p is held as 2^(x - m + kLift): f16 reaches 2^-37 of the largest p
 constexpr float kLag = 3.f;         // m may be this far behind: p <= 2^15
 constexpr uint32_t kLowestRef = 0x20202020u;  // R_b - 255 then has a bit of 0xf8 set, like every far scale
-constexpr int kAlignedSlack = 2;    // groups per warp that keeping a segment in one CTA may cost
+constexpr int kAlignedSlack = 1;    // units per warp that keeping a segment in one CTA may cost
 
-template <int NB>
+// NB blocks of 32 per head, CT column tiles of 4 query heads.  One tile leaves the registers for 16
+// warps, two for 12; the ring takes what shared memory the parts leave.
+template <int NB, int CT>
 struct MxCfg {
   static constexpr int D = NB * kMxBlock;
-  static constexpr int kGroup = NB * kMxBytes;  // bytes of one group of one operand
-  static constexpr int kStage = 2 * kGroup;
+  static constexpr int kWarps = CT == 1 ? 16 : 12;
+  static constexpr int kStages = CT == 1 ? 2 : 3;
+  static constexpr int kHeads = CT * kQueries;    // query heads of a segment
+  static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
+  static constexpr int kStage = 4 * kGroup;       // K of two groups, V of two groups
   static constexpr int kRing = kStages * kStage;  // per warp
-  static constexpr int kState = kCols * (D + 2);  // floats: acc [8][D], m [8], l [8]
+  static constexpr int kState = kHeads * (D + 2); // floats: acc [heads][D], m [heads], l [heads]
   static constexpr int kSmemRing = kWarps * kRing;
   static constexpr int kSmemHeads = kWarps * kState * 4;  // parts that end before their warp's range does
-  static constexpr int kSmemUnits = kWarps * 64 * 16;  // two batches of 32 units per warp
+  static constexpr int kSmemUnits = kWarps * 64 * 16;     // two batches of 32 units per warp
   static constexpr int kSmemBars = kWarps * kStages * 8;
   static constexpr int kSmemPrefix = (kMaxSeqs + 1) * 4;
-  static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kCols * 12 + 16;
+  static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kHeads * 12 + 16;
   static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemBars + kSmemPrefix + kSmemMisc;
   static_assert(kState * 4 <= kRing, "a warp's last part goes into its own ring");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+};
+
+// n / d by a multiplication, n below 2^31.
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+  explicit FastDiv(uint32_t d) {
+    shift = 31;
+    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return static_cast<uint32_t>(static_cast<uint64_t>(n) * mul >> shift);
+  }
 };
 
 // Beside its states (a part whose segment began in an earlier CTA, then one whose
@@ -104,6 +125,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
@@ -143,55 +171,31 @@ __device__ __forceinline__ void load_codes(uint32_t base, int lane, uint32_t (&l
   }
 }
 
-// Four codes of two keys (a: low 16 bits, b: high 16 bits) as f16 pairs (a_i, b_i).
-__device__ __forceinline__ void key_pairs(uint32_t v, uint32_t (&e)[4]) {
-  // bytes 2, 3 of x: (a1, b1), (a3, b3); of y: (a0, b0), (a2, b2)
-  const uint32_t x = (v & 0xf0f0f0f0u) | ((v << 12) & 0x0f0f0f0fu);
-  const uint32_t y = ((v << 4) & 0xf0f0f0f0u) | ((v << 16) & 0x0f0f0f0fu);
-  asm("{ .reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %5;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b3; }"
-      : "=&r"(e[0]), "=&r"(e[1]), "=&r"(e[2]), "=&r"(e[3])  // written before y is read
-      : "r"(x), "r"(y));
-}
-
-// P_b of this lane's keys times V's block b into `d0`, `d1` (rows j = 0, 1).
-__device__ __forceinline__ void value_block(uint32_t lo, uint32_t hi, uint32_t p0, uint32_t p1, float (&d0)[4],
-                                            float (&d1)[4]) {
-  uint32_t a[4], c[4];
-  key_pairs(lo, a);
-  key_pairs(hi, c);
-  mma_f16(d0, a[0], a[1], c[0], c[1], p0, p1);
-  mma_f16(d1, a[2], a[3], c[2], c[3], p0, p1);
-}
-
 // 2^(e - 127) (1 + 2^-23) of byte b: the low bit makes the byte 255 a NaN, and all scores share the factor.
 __device__ __forceinline__ float scale_of(uint32_t w, int b) {
   const uint32_t v = b == 0 ? w << 23 : b == 1 ? w << 15 : b == 2 ? w << 7 : w >> 1;
   return __uint_as_float((v & 0x7f800000u) | 1u);
 }
 
-// Scale byte of block b, key `which` (0, 1) of a key pair's words.
+// Scale byte of block b of a key: k = 0, 1: keys 2t, 2t + 1; k = 2, 3: keys 2t + 8, 2t + 9.  At D = 64
+// the two keys of a pair share a word.
 template <int NB>
-__device__ __forceinline__ int byte_of(uint32_t w0, uint32_t w1, int b, int which) {
+__device__ __forceinline__ int byte_of(const uint4 &w, int k, int b) {
   if constexpr (NB == 4)
-    return ((which ? w1 : w0) >> (8 * b)) & 255u;
+    return ((k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w) >> (8 * b)) & 255u;
   else
-    return (w0 >> (16 * which + 8 * b)) & 255u;
+    return ((k < 2 ? w.x : w.z) >> (16 * (k & 1) + 8 * b)) & 255u;
 }
 
 // Scales that the window of 8 binades does not hold: raise R_b (a byte of `ref`, returned) where a
-// scale is above it, then take the keys window by window.  `o` is the caller's copy of its
-// accumulators; `pp0`, `pp1`: p of keys (2t, 2t+1) and (2t+8, 2t+9) of query g.  Out of line, so that
-// the loop around it keeps its registers.
-template <int NB>
-__device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vcodes, uint4 w, uint32_t pp0,
-                                            uint32_t pp1, int valid) {
+// scale is above it, then take the keys window by window.  `o`: the caller's copy of its
+// accumulators [tile][block][4]; `p`: [tile][key], p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in both halves.
+// Out of line, so that the loop around it keeps its registers.
+template <int NB, int CT>
+__device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vcodes, uint4 w, const uint32_t *p,
+                                            int valid) {
   const int lane = threadIdx.x & 31;
+  const int shift = lane & 4 ? 16 : 0;  // g odd: the column of odd dims
   int deepest = 0;
   const int key = (lane & 3) * 2;  // scales of keys that do not exist: none
   if constexpr (NB == 4) {
@@ -208,7 +212,7 @@ __device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vco
     int top = 0, low = 255;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int s = k < 2 ? byte_of<NB>(w.x, w.y, b, k & 1) : byte_of<NB>(w.z, w.w, b, k & 1);
+      const int s = byte_of<NB>(w, k, b);
       if (s >= 1 && s <= 254) top = max(top, s), low = min(low, s);
     }
 #pragma unroll
@@ -221,7 +225,7 @@ __device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vco
       const int next = min(top + 2, 254);
       const float f = exp2i(r - next);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[b * 8 + i] *= f;
+      for (int i = 0; i < 4 * CT; ++i) o[(i / 4 * NB + b) * 4 + i % 4] *= f;
       ref = (ref & ~(255u << (8 * b))) | (static_cast<uint32_t>(next) << (8 * b));
       r = next;
     }
@@ -235,247 +239,334 @@ __device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vco
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int r = (ref >> (8 * b)) & 255;
-      uint32_t f[4];
+      uint32_t f[4], a[4], c[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int s = k < 2 ? byte_of<NB>(w.x, w.y, b, k & 1) : byte_of<NB>(w.z, w.w, b, k & 1), d = r - s;
+        const int s = byte_of<NB>(w, k, b), d = r - s;
         f[k] = s >= 1 && s <= 254 && (d >> 3) == window ? 0x3c00u - ((d & 7) << 10) : 0u;
         if (s == 255 && window == 0) f[k] = 0x7e00u;
+        f[k] <<= shift;
       }
-      float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-      value_block(lo[b], hi[b], mul_f16x2(pp0, f[0] | f[1] << 16), mul_f16x2(pp1, f[2] | f[3] << 16), d0, d1);
+      mx_codes_to_f16(lo[b], a);
+      mx_codes_to_f16(hi[b], c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[b * 8 + i] = fmaf(d0[i], back, o[b * 8 + i]);
-        o[b * 8 + 4 + i] = fmaf(d1[i], back, o[b * 8 + 4 + i]);
+      for (int i = 0; i < CT; ++i) {
+        float d[4];
+        mma_f16_zero(d, a[0], a[1], a[2], a[3], mul_f16x2(p[4 * i], f[0]), mul_f16x2(p[4 * i + 1], f[1]));
+        mma_f16(d, c[0], c[1], c[2], c[3], mul_f16x2(p[4 * i + 2], f[2]), mul_f16x2(p[4 * i + 3], f[3]));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[(i * NB + b) * 4 + j] = fmaf(d[j], back, o[(i * NB + b) * 4 + j]);
       }
     }
   }
   return ref;
 }
 
-// One query head's state of a segment part, laid out [8][D] acc, [8] m, [8] l.
-template <typename T, int NB>
+// A warp's state on a segment: 4 query heads to a column tile, lane (g, t) = (lane / 4, lane % 4).
+template <typename T, int NB, int CT>
 struct MxWarp {
-  using C = MxCfg<NB>;
+  using C = MxCfg<NB, CT>;
   static constexpr int D = C::D;
-  uint32_t q[NB * 2][2];  // B fragments of q
-  float xs[2];            // log2-domain scale of queries 2t, 2t + 1
-  float o[NB * 2][4];     // tile 2b + j: dims 32b + 4g + 2j (+ 1: [2], [3]), queries 2t, 2t + 1
-  float m[2], l[2];
-  uint32_t ref;           // R_b, one byte per block
+  uint32_t q[CT][NB * 2][2];  // B fragments of q: columns 2i and 2i + 1 both query i of the tile
+  float xs[CT];               // log2-domain scale of query t
+  float o[CT][NB][4];         // query t, dims 32b + 4g + 0 to 3, times 2^(R_b - 127)
+  float m[CT], l[CT];         // query t; l: this lane's keys only
+  uint32_t ref;               // R_b, one byte per block
+  uint32_t one, unit0, unit1; // f16 1.0 and the places of d's bits in the half of this lane's column
   int lane, g, t;
+
+  __device__ __forceinline__ void setup() {
+    lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int shift = g & 1 ? 16 : 0;
+    one = 0x3c00u << shift, unit0 = 1u << (10 + shift), unit1 = 1u << (2 + shift);
+  }
 
   __device__ __forceinline__ void reset() {
     ref = kLowestRef;
 #pragma unroll
-    for (int i = 0; i < NB * 2; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+    for (int c = 0; c < CT; ++c) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) o[c][b][0] = o[c][b][1] = o[c][b][2] = o[c][b][3] = 0.f;
+      m[c] = -INFINITY;
+      l[c] = 0.f;
+    }
   }
 
-  // Row `g` of the tile's query heads (heads of them exist).
+  // Query heads of the segment (heads of them exist).
   __device__ __forceinline__ void load_query(const T *query, int heads, float scale_log2) {
-    float x[NB][8];
-    uint32_t top = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (g < heads) v = *reinterpret_cast<const uint4 *>(query + g * D + b * 32 + t * 8);
-      float2 f[4];
-      Vec16<T>::unpack(v, f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[b][2 * i] = f[i].x, x[b][2 * i + 1] = f[i].y;
-        top = max(top, max(__float_as_uint(f[i].x) & 0x7fffffffu, __float_as_uint(f[i].y) & 0x7fffffffu));
-      }
-    }
-    top = max(top, __shfl_xor_sync(kAll, top, 1));
-    top = max(top, __shfl_xor_sync(kAll, top, 2));
-    int e = 14 - (static_cast<int>(top >> 23) - 127);  // largest element to [2^14, 2^15)
-    if (top >= 0x7f800000u) e = 0;                     // not finite: as it is
-    e = min(e, 126);
-    const float f = exp2i(e);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      q[2 * b][0] = pack_f16(x[b][0] * f, x[b][1] * f);
-      q[2 * b][1] = pack_f16(x[b][2] * f, x[b][3] * f);
-      q[2 * b + 1][0] = pack_f16(x[b][4] * f, x[b][5] * f);
-      q[2 * b + 1][1] = pack_f16(x[b][6] * f, x[b][7] * f);
-    }
-    const float back = exp2i(-e) * scale_log2;
-    xs[0] = __shfl_sync(kAll, back, 8 * t);  // lane of query 2t: g = 2t
-    xs[1] = __shfl_sync(kAll, back, 8 * t + 4);
-  }
-
-  // One group: `kbase`, `vbase` its K and V bytes in shared memory, `valid` of its 16 keys exist;
-  // `first`: the state holds none yet.
-  __device__ __forceinline__ void process(uint32_t kbase, uint32_t vbase, int valid, bool first) {
-    float x[4] = {0.f, 0.f, 0.f, 0.f};  // (key g, queries 2t, 2t + 1), (key g + 8, ...)
-    {
-      uint32_t lo[NB], hi[NB], wl, wh;
-      load_codes<NB, false>(kbase, lane, lo, hi);
-      if constexpr (NB == 4) {
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 4));
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 4 + 32));
-      } else {
-        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 2));
-        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 2 + 16));
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        uint32_t a[4], c[4];
-        mx_codes_to_f16(lo[b], a);
-        mx_codes_to_f16(hi[b], c);
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16(d, a[0], c[0], a[1], c[1], q[2 * b][0], q[2 * b][1]);
-        mma_f16(d, a[2], c[2], a[3], c[3], q[2 * b + 1][0], q[2 * b + 1][1]);
-        const float fl = scale_of(wl, b), fh = scale_of(wh, b);
-        x[0] = fmaf(d[0], fl, x[0]);
-        x[1] = fmaf(d[1], fl, x[1]);
-        x[2] = fmaf(d[2], fh, x[2]);
-        x[3] = fmaf(d[3], fh, x[3]);
-      }
-    }
-    uint32_t vlo[NB], vhi[NB];
-    load_codes<NB, true>(vbase, lane, vlo, vhi);
-    // V's scales: words of keys 2t, 2t + 1 and 2t + 8, 2t + 9
-    uint32_t w0[2], w1[2];
-    if constexpr (NB == 4) {
-      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w0[0]), "=r"(w0[1]) : "r"(vbase + NB * kMxBlockBytes + t * 8));
-      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                   : "=r"(w1[0]), "=r"(w1[1])
-                   : "r"(vbase + NB * kMxBlockBytes + t * 8 + 32));
-    } else {
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w0[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w1[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
-      w0[1] = w1[1] = 0;
-    }
-    if (first) {  // uniform: R_b starts at the largest scale here and two binades of room
+    for (int c = 0; c < CT; ++c) {
+      const int h = c * kQueries + (g >> 1);
+      float x[NB][8];
       uint32_t top = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-        const uint32_t(&w)[2] = k < 2 ? w0 : w1;
-        uint32_t bytes = NB == 4 ? w[k & 1] : (w[0] >> (16 * (k & 1))) & 0xffffu;
-        if (key < valid) top = __vmaxu4(top, bytes);
+      for (int b = 0; b < NB; ++b) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads) v = *reinterpret_cast<const uint4 *>(query + h * D + b * 32 + t * 8);
+        float2 f[4];
+        Vec16<T>::unpack(v, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[b][2 * i] = f[i].x, x[b][2 * i + 1] = f[i].y;
+          top = max(top, max(__float_as_uint(f[i].x) & 0x7fffffffu, __float_as_uint(f[i].y) & 0x7fffffffu));
+        }
       }
+      top = max(top, __shfl_xor_sync(kAll, top, 1));
+      top = max(top, __shfl_xor_sync(kAll, top, 2));
+      int e = 14 - (static_cast<int>(top >> 23) - 127);  // largest element to [2^14, 2^15)
+      if (top >= 0x7f800000u) e = 0;                     // not finite: as it is
+      e = min(e, 126);
+      const float f = exp2i(e);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        q[c][2 * b][0] = pack_f16(x[b][0] * f, x[b][1] * f);
+        q[c][2 * b][1] = pack_f16(x[b][2] * f, x[b][3] * f);
+        q[c][2 * b + 1][0] = pack_f16(x[b][4] * f, x[b][5] * f);
+        q[c][2 * b + 1][1] = pack_f16(x[b][6] * f, x[b][7] * f);
+      }
+      xs[c] = __shfl_sync(kAll, exp2i(-e) * scale_log2, 8 * t);  // a lane of query t: g = 2t
+    }
+  }
+
+  // Scores of a group's 16 keys for query t, still to be scaled by xs: x[c][0], key g; x[c][1], key g + 8.
+  __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[CT][2]) const {
+    uint32_t lo[NB], hi[NB], wl, wh;
+    load_codes<NB, false>(kbase, lane, lo, hi);
+    if constexpr (NB == 4) {
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 4));
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 4 + 32));
+    } else {
+      asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 2));
+      asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 2 + 16));
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t a[4], e[4];
+      mx_codes_to_f16(lo[b], a);
+      mx_codes_to_f16(hi[b], e);
+      const float fl = scale_of(wl, b), fh = scale_of(wh, b);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        float d[4];
+        mma_f16_zero(d, a[0], e[0], a[1], e[1], q[c][2 * b][0], q[c][2 * b][1]);
+        mma_f16(d, a[2], e[2], a[3], e[3], q[c][2 * b + 1][0], q[c][2 * b + 1][1]);
+        x[c][0] = b == 0 ? d[0] * fl : fmaf(d[0], fl, x[c][0]);
+        x[c][1] = b == 0 ? d[2] * fh : fmaf(d[2], fh, x[c][1]);
+      }
+    }
+  }
+
+  // V's scales of a group: words of keys 2t, 2t + 1 (w[0], w[1]) and 2t + 8, 2t + 9 (w[2], w[3]); at
+  // D = 64 a key pair has one word.
+  __device__ __forceinline__ void value_scales(uint32_t vbase, uint32_t (&w)[4]) const {
+    if constexpr (NB == 4) {
+      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                   : "=r"(w[0]), "=r"(w[1])
+                   : "r"(vbase + NB * kMxBlockBytes + t * 8));
+      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                   : "=r"(w[2]), "=r"(w[3])
+                   : "r"(vbase + NB * kMxBlockBytes + t * 8 + 32));
+    } else {
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[2]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
+      w[1] = w[3] = 0;
+    }
+  }
+
+  // The largest scale byte per block over the group's keys below `valid`, of this lane's keys.
+  __device__ __forceinline__ uint32_t largest_scales(const uint32_t (&w)[4], int valid) const {
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t bytes = NB == 4 ? w[k] : (w[k & 2] >> (16 * (k & 1))) & 0xffffu;
+      if (2 * t + (k & 1) + (k >> 1) * 8 < valid) top = __vmaxu4(top, bytes);
+    }
+    return top;
+  }
+
+  // Keys that do not exist: whatever their scale bytes are becomes the reference (their p is zero).
+  __device__ __forceinline__ void mask_scales(uint32_t (&w)[4], int valid) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (2 * t + (k & 1) + (k >> 1) * 8 < valid) continue;
+      if constexpr (NB == 4)
+        w[k] = ref;
+      else
+        w[k & 2] = k & 1 ? (w[k & 2] & 0xffffu) | ref << 16 : (w[k & 2] & 0xffff0000u) | (ref & 0xffffu);
+    }
+  }
+
+  // How far below the reference each scale is, per byte: 0 to 7, or a bit of 0xf8 is set in the result.
+  __device__ __forceinline__ uint32_t distances(const uint32_t (&w)[4], uint32_t (&d)[4]) const {
+    if constexpr (NB == 4) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = ref - w[k];
+      return (d[0] | d[1] | d[2] | d[3]) & 0xf8f8f8f8u;
+    } else {
+      const uint32_t both = (ref & 0xffffu) * 0x10001u;
+      d[0] = both - w[0], d[2] = both - w[2];
+      return (d[0] | d[2]) & 0xf8f8f8f8u;
+    }
+  }
+
+  // O += P_b V of a group, all scales within the window; p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9
+  // in both halves.
+  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[CT][4]) {
+    uint32_t lo[NB], hi[NB];
+    load_codes<NB, true>(vbase, lane, lo, hi);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t f[4];  // 2^-d in the half of this lane's column, zero in the other
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // bytes of blocks (b & ~1) and (b | 1) in the low half of the word
+        const uint32_t word = NB == 4 ? (b < 2 ? d[k] : d[k] >> 16) : (k & 1 ? d[k & 2] >> 16 : d[k & 2]);
+        f[k] = b & 1 ? one - (word & 0xff00u) * unit1 : one - (word & 0xffu) * unit0;
+      }
+      uint32_t a[4], e[4];
+      mx_codes_to_f16(lo[b], a);
+      mx_codes_to_f16(hi[b], e);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        mma_f16(o[c][b], a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
+        mma_f16(o[c][b], e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+      }
+    }
+  }
+
+  // One unit: K of its two groups at `base`, then V of both; `valid` of its 32 keys exist;
+  // `first`: the state holds none yet.
+  __device__ __forceinline__ void process(uint32_t base, int valid, bool first) {
+    const uint32_t vbase = base + 2 * C::kGroup;
+    float x[2][CT][2];
+    scores(base, x[0]);
+    scores(base + C::kGroup, x[1]);
+    uint32_t w[2][4];
+    value_scales(vbase, w[0]);
+    value_scales(vbase + C::kGroup, w[1]);
+    if (first) {  // uniform: R_b starts at the largest scale here and two binades of room
+      uint32_t top = __vmaxu4(largest_scales(w[0], valid), largest_scales(w[1], valid - kMxGroup));
       top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 1));
       top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 2));
       ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] *= xs[i & 1];
-    if (valid < kMxGroup) {  // uniform: the last group of a sequence
-      if (g >= valid) x[0] = x[1] = -INFINITY;
-      if (g + 8 >= valid) x[2] = x[3] = -INFINITY;
-      // stale scales of keys that do not exist become the reference (their p is zero)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (2 * t + (k & 1) + (k >> 1) * 8 < valid) continue;
-        uint32_t(&w)[2] = k < 2 ? w0 : w1;
-        if constexpr (NB == 4)
-          w[k & 1] = ref;
-        else
-          w[0] = k & 1 ? (w[0] & 0xffffu) | ref << 16 : (w[0] & 0xffff0000u) | (ref & 0xffffu);
+      for (int c = 0; c < CT; ++c) x[j][c][0] *= xs[c], x[j][c][1] *= xs[c];
+    if (valid < kUnit) {  // uniform: the last unit of a segment
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (j * kMxGroup + g >= valid) x[j][c][0] = -INFINITY;
+          if (j * kMxGroup + g + 8 >= valid) x[j][c][1] = -INFINITY;
+        }
+        mask_scales(w[j], valid - j * kMxGroup);
       }
     }
-    const bool behind = fmaxf(x[0], x[2]) > m[0] + kLag || fmaxf(x[1], x[3]) > m[1] + kLag;
+    // m follows the largest score, up to kLag binades behind it
+    float top[CT];
+    bool behind = false;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      top[c] = fmaxf(fmaxf(x[0][c][0], x[0][c][1]), fmaxf(x[1][c][0], x[1][c][1]));
+      behind |= top[c] > m[c] + kLag;
+    }
     if (__any_sync(kAll, behind)) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float mx = fmaxf(x[c], x[c + 2]);
+      for (int c = 0; c < CT; ++c) {
+        float mx = top[c];
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, off));
         if (mx > m[c]) {  // the lanes of a query agree
           const float f = m[c] == -INFINITY ? 0.f : fast_exp2(m[c] - mx);
 #pragma unroll
-          for (int i = 0; i < NB * 2; ++i) o[i][c] *= f, o[i][c + 2] *= f;
+          for (int i = 0; i < NB * 4; ++i) o[c][i / 4][i % 4] *= f;
           l[c] *= f;
           m[c] = mx;
         }
       }
     }
-    float p[4];
+    uint32_t p[2][CT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = fast_exp2(x[i] - m[i & 1] + kLift);
-    l[0] += p[0] + p[2];
-    l[1] += p[1] + p[3];
-    const uint32_t pp0 = movm(pack_f16(p[0], p[1])), pp1 = movm(pack_f16(p[2], p[3]));
-
-    // how far below the reference each scale is, per byte: 0 to 7, or a bit of 0xf8 is set
-    uint32_t u[2][NB / 2], bad = 0;  // [key pair][block pair]: bytes (key 0: b, b + 1; key 1: b, b + 1)
-    if constexpr (NB == 4) {
-      const uint32_t a0 = ref - w0[0], a1 = ref - w0[1], c0 = ref - w1[0], c1 = ref - w1[1];
-      bad = (a0 | a1 | c0 | c1) & 0xf8f8f8f8u;
-      u[0][0] = __byte_perm(a0, a1, 0x5410), u[0][1] = __byte_perm(a0, a1, 0x7632);
-      u[1][0] = __byte_perm(c0, c1, 0x5410), u[1][1] = __byte_perm(c0, c1, 0x7632);
-    } else {
-      const uint32_t both = (ref & 0xffffu) * 0x10001u;
-      u[0][0] = both - w0[0], u[1][0] = both - w1[0];
-      bad = (u[0][0] | u[1][0]) & 0xf8f8f8f8u;
-    }
-    if (__any_sync(kAll, bad != 0)) {
-      float copy[NB * 8];
+    for (int c = 0; c < CT; ++c) {
+      const float lift = kLift - m[c];
 #pragma unroll
-      for (int i = 0; i < NB * 8; ++i) copy[i] = o[i / 4][i % 4];
-      ref = value_slow<NB>(copy, ref, vbase, make_uint4(w0[0], w0[1], w1[0], w1[1]), pp0, pp1, valid);
-#pragma unroll
-      for (int i = 0; i < NB * 8; ++i) o[i / 4][i % 4] = copy[i];
-    } else {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        // f16 2^-d: the exponent 15 - d is 15 ^ d
-        const uint32_t z0 = u[0][b / 2] << (b & 1 ? 2 : 10), z1 = u[1][b / 2] << (b & 1 ? 2 : 10);
-        const uint32_t f0 = (z0 & 0x1c001c00u) ^ 0x3c003c00u, f1 = (z1 & 0x1c001c00u) ^ 0x3c003c00u;
-        value_block(vlo[b], vhi[b], mul_f16x2(pp0, f0), mul_f16x2(pp1, f1), o[2 * b], o[2 * b + 1]);
+      for (int j = 0; j < 2; ++j) {
+        const float p0 = fast_exp2(x[j][c][0] + lift), p1 = fast_exp2(x[j][c][1] + lift);
+        l[c] += p0 + p1;
+        // rows (keys) x columns (each query twice), transposed: keys 2t and 2t + 1 of query g / 2
+        const uint32_t k0 = movm(pack_f16(p0, p0)), k8 = movm(pack_f16(p1, p1));
+        p[j][c][0] = __byte_perm(k0, 0, 0x1010), p[j][c][1] = __byte_perm(k0, 0, 0x3232);
+        p[j][c][2] = __byte_perm(k8, 0, 0x1010), p[j][c][3] = __byte_perm(k8, 0, 0x3232);
       }
+    }
+    uint32_t d[2][4];
+    const uint32_t far = distances(w[0], d[0]) | distances(w[1], d[1]);
+    if (__any_sync(kAll, far != 0)) {
+      float copy[CT * NB * 4];
+      uint32_t pc[2][CT * 4];
+#pragma unroll
+      for (int i = 0; i < CT * NB * 4; ++i) copy[i] = o[i / (NB * 4)][i / 4 % NB][i % 4];
+#pragma unroll
+      for (int i = 0; i < CT * 8; ++i) pc[i / (CT * 4)][i % (CT * 4)] = p[i / (CT * 4)][i / 4 % CT][i % 4];
+#pragma unroll 1
+      for (int j = 0; j < 2; ++j)
+        ref = value_slow<NB, CT>(copy, ref, vbase + j * C::kGroup,
+                                 j ? make_uint4(w[1][0], w[1][1], w[1][2], w[1][3])
+                                   : make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]),
+                                 pc[j], valid - j * kMxGroup);
+#pragma unroll
+      for (int i = 0; i < CT * NB * 4; ++i) o[i / (NB * 4)][i / 4 % NB][i % 4] = copy[i];
+    } else {
+      values(vbase, d[0], p[0]);
+      values(vbase + C::kGroup, d[1], p[1]);
     }
   }
 
   // Sum l over the keys of the lanes, bring o to its true scale.
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < CT; ++c) {
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[c] += __shfl_xor_sync(kAll, l[c], off);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const float f = exp2i(static_cast<int>((ref >> (8 * b)) & 255u) - 127);
+      for (int b = 0; b < NB; ++b) {
+        const float f = exp2i(static_cast<int>((ref >> (8 * b)) & 255u) - 127);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[2 * b][i] *= f, o[2 * b + 1][i] *= f;
+        for (int i = 0; i < 4; ++i) o[c][b][i] *= f;
+      }
     }
   }
 
   __device__ __forceinline__ void write_out(T *out, int heads) const {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (2 * t + c >= heads) continue;
+    for (int c = 0; c < CT; ++c) {
+      if (c * kQueries + t >= heads) continue;
       const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         uint2 v;
         T *e = reinterpret_cast<T *>(&v);
-        e[0] = Elem<T>::from_float(o[2 * b][c] * inv);
-        e[1] = Elem<T>::from_float(o[2 * b][c + 2] * inv);
-        e[2] = Elem<T>::from_float(o[2 * b + 1][c] * inv);
-        e[3] = Elem<T>::from_float(o[2 * b + 1][c + 2] * inv);
-        *reinterpret_cast<uint2 *>(out + (2 * t + c) * D + b * 32 + g * 4) = v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_float(o[c][b][i] * inv);
+        *reinterpret_cast<uint2 *>(out + (c * kQueries + t) * D + b * 32 + g * 4) = v;
       }
     }
   }
 
   __device__ __forceinline__ void write_state(float *st, int heads) const {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (2 * t + c >= heads) continue;
+    for (int c = 0; c < CT; ++c) {
+      const int h = c * kQueries + t;
+      if (h >= heads) continue;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        *reinterpret_cast<float4 *>(st + (2 * t + c) * D + b * 32 + g * 4) =
-            make_float4(o[2 * b][c], o[2 * b][c + 2], o[2 * b + 1][c], o[2 * b + 1][c + 2]);
+        *reinterpret_cast<float4 *>(st + h * D + b * 32 + g * 4) = make_float4(o[c][b][0], o[c][b][1], o[c][b][2], o[c][b][3]);
       if (g == 0) {
-        st[kCols * D + 2 * t + c] = m[c];
-        st[kCols * D + kCols + 2 * t + c] = l[c];
+        st[C::kHeads * D + h] = m[c];
+        st[C::kHeads * D + C::kHeads + h] = l[c];
       }
     }
   }
@@ -487,21 +578,21 @@ __device__ __forceinline__ float part_factor(float m, float l, float M) {
   return fast_exp2(m - M);
 }
 
-template <typename T, int NB>
-__global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const MxDecodeParams p, int tiles) {
-  using C = MxCfg<NB>;
-  constexpr int D = C::D;
+template <typename T, int NB, int CT>
+__global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mma_kernel(const MxDecodeParams p, int tiles, FastDiv by_segments, FastDiv by_tiles, FastDiv by_page) {
+  using C = MxCfg<NB, CT>;
+  constexpr int D = C::D, kWarps = C::kWarps, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
   int4 *unit_table = reinterpret_cast<int4 *>(smem + C::kSmemRing + C::kSmemHeads);
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits);
-  int *prefix = reinterpret_cast<int *>(bars + kWarps * kStages);  // groups before sequence s
+  int *prefix = reinterpret_cast<int *>(bars + kWarps * kStages);  // units of a segment before sequence s
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
   int *scan = part_flags + 2 * kWarps;      // [2 * kWarps]
   float *factor = reinterpret_cast<float *>(scan + 2 * kWarps);               // [2 * kWarps][8]
   float2 *run_ml = reinterpret_cast<float2 *>(                               // [2 * kWarps][8]
-      (reinterpret_cast<uintptr_t>(factor + 2 * kWarps * kCols) + 15) & ~static_cast<uintptr_t>(15));
+      (reinterpret_cast<uintptr_t>(factor + 2 * kWarps * C::kHeads) + 15) & ~static_cast<uintptr_t>(15));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t *wbar = bars + warp * kStages;
   uint8_t *ring = smem + warp * C::kRing;
@@ -517,7 +608,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   }
   pdl_wait();
 
-  // ---- groups of each sequence, their prefix sums and largest ----
+  // ---- units of each sequence, their prefix sums and largest ----
   const int64_t cap = p.bt_stride * p.block_size;
   int c_max = 0;
   {
@@ -531,7 +622,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
         if (blockIdx.x == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
         ctx = static_cast<int>(cap);
       }
-      c[i] = ctx > 0 ? (ctx - 1) / kMxGroup + 1 : 0;
+      c[i] = ctx > 0 ? (ctx - 1) / kUnit + 1 : 0;
       sum += c[i];
       c_max = max(c_max, c[i]);
     }
@@ -570,7 +661,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
       *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
   }
 
-  // ---- this warp's range of units (unit: one group of one segment) ----
+  // ---- this warp's range of units (a unit: 32 keys of one segment) ----
   const uint32_t total = static_cast<uint32_t>(prefix[n]) * H;
   const uint32_t all_warps = gridDim.x * kWarps;
   uint32_t u0 = 0, u1 = 0;
@@ -590,81 +681,88 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   }
   const int units = static_cast<int>(u1 - u0);
 
-  // Unit u0 + i for lane-parallel use: its segment, group, and where its bytes are.
-  struct Unit {
-    int seq, ht, group, groups;
-  };
-  auto unit_of = [&](int i) -> Unit {
-    const uint32_t u = u0 + i;
-    const int per = static_cast<int>(u / H);
-    int a = 0, b = n - 1;  // the last sequence whose prefix is not above `per`
-    while (a < b) {
-      const int mid = (a + b + 1) >> 1;
-      if (prefix[mid] <= per)
-        a = mid;
-      else
-        b = mid - 1;
-    }
-    Unit r;
-    r.seq = a;
-    r.groups = prefix[a + 1] - prefix[a];
-    const int rest = static_cast<int>(u - static_cast<uint32_t>(prefix[a]) * H);
-    r.ht = rest / r.groups;
-    r.group = rest - r.ht * r.groups;
-    return r;
-  };
+  // Batches of 32 units, one per lane, in shared memory: x, y, the indices of the unit's two groups
+  // in the pools (-1: no such page, or no such keys); z, its keys (bits 0-5) and whether it is its
+  // segment's first (64) or last (128) unit; w, its segment.
   const int per_page = p.block_size / kMxGroup;
-  // Batches of 32 units, one per lane, in shared memory: x, the index of the unit's group in the
-  // pools (-1: no such page); y, the keys in it (bits 0-4) and whether it is its segment's first
-  // (32) or last (64) group; z, w, its sequence and head tile.
   int4 *table = unit_table + warp * 64;
   auto load_batch = [&](int first) {
     const int i = first + lane;
     if (i < units) {
-      const Unit r = unit_of(i);
-      const int page = __ldg(p.block_tables + static_cast<int64_t>(r.seq) * p.bt_stride + r.group / per_page);
-      int valid = kMxGroup, flags = r.group == 0 ? 32 : 0;
-      if (r.group == r.groups - 1) {
-        const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + r.seq)), cap));
-        valid = ctx - r.group * kMxGroup;
-        flags |= 64;
+      const uint32_t u = u0 + i;
+      const int per = static_cast<int>(by_segments.div(u));
+      int a = 0, b = n - 1;  // the last sequence whose prefix is not above `per`
+      while (a < b) {
+        const int mid = (a + b + 1) >> 1;
+        if (prefix[mid] <= per)
+          a = mid;
+        else
+          b = mid - 1;
       }
-      int where = -1;
-      if (page >= 0 && page < p.num_blocks)
-        where = (page * p.num_kv_heads + r.ht / tiles) * per_page + r.group % per_page;
-      else
-        flag_status(p.status, MI_DEV_BAD_BLOCK);
-      table[i & 63] = make_int4(where, valid | flags, r.seq, r.ht);
+      const int before = prefix[a], count = prefix[a + 1] - before;
+      const int rest = static_cast<int>(u - static_cast<uint32_t>(before) * H);
+      int ht = static_cast<int>(__fdividef(static_cast<float>(rest), static_cast<float>(count)));  // to one
+      if (ht * count > rest) --ht;
+      if (rest - ht * count >= count) ++ht;
+      const int unit = rest - ht * count;
+      int valid = kUnit, flags = unit == 0 ? 64 : 0;
+      if (unit == count - 1) {
+        const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + a)), cap));
+        valid = ctx - unit * kUnit;
+        flags |= 128;
+      }
+      const int32_t *row = p.block_tables + static_cast<int64_t>(a) * p.bt_stride;
+      const int kvh = static_cast<int>(by_tiles.div(ht));
+      int where[2] = {-1, -1};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j * kMxGroup >= valid) break;
+        const int group = 2 * unit + j, col = static_cast<int>(by_page.div(group));
+        const int page = __ldg(row + col);
+        if (page >= 0 && page < p.num_blocks)
+          where[j] = (page * p.num_kv_heads + kvh) * per_page + group - col * per_page;
+        else
+          flag_status(p.status, MI_DEV_BAD_BLOCK);
+      }
+      table[i & 63] = make_int4(where[0], where[1], valid | flags, a * H + ht);
     }
     __syncwarp();
   };
   load_batch(0);
-  auto issue = [&](int i) {
-    if (lane != 0) return;
-    const int where = table[i & 63].x;
+  // Lanes 4s to 4s + 3 of `lanes` bring unit first + s: K and V of its two groups.
+  auto issue = [&](int first, int count) {
+    const int i = first + (lane >> 2);
+    const bool on = (lane >> 2) < count;
+    int where = -1;
     uint64_t *bar = &wbar[i % kStages];
-    if (where < 0) {
-      mbar_arrive(bar);
-      return;
+    if (on) {
+      const int4 unit = table[i & 63];
+      where = lane & 1 ? unit.y : unit.x;
+      if ((lane & 3) == 0) {
+        const int groups = (unit.x >= 0) + (unit.y >= 0);
+        if (groups)
+          mbar_arrive_expect_tx(bar, groups * 2 * C::kGroup);
+        else
+          mbar_arrive(bar);
+      }
     }
-    uint8_t *dst = ring + i % kStages * C::kStage;
-    const int64_t off = static_cast<int64_t>(where) * C::kGroup;
-    mbar_arrive_expect_tx(bar, C::kStage);
-    bulk_g2s(dst, p.key_pages + off, C::kGroup, bar);
-    bulk_g2s(dst + C::kGroup, p.value_pages + off, C::kGroup, bar);
+    __syncwarp();
+    if (where >= 0)
+      bulk_g2s(ring + i % kStages * C::kStage + ((lane >> 1) & 1) * 2 * C::kGroup + (lane & 1) * C::kGroup,
+               (lane & 2 ? p.value_pages : p.key_pages) + static_cast<int64_t>(where) * C::kGroup, C::kGroup, bar);
   };
-  int issued = 0;
-  for (; issued < kStages && issued < units; ++issued) issue(issued);
+  int issued = min(kStages, units);
+  issue(0, issued);
 
-  MxWarp<T, NB> st;
-  st.lane = lane, st.g = lane >> 2, st.t = lane & 3;
+  MxWarp<T, NB, CT> st;
+  st.setup();
   int seq = 0, ht = 0, heads = 0;
   bool has_first = false;
   auto start_segment = [&](const int4 &unit) {
-    seq = unit.z, ht = unit.w;
-    has_first = (unit.y & 32) != 0;
-    const int kvh = ht / tiles, h0 = (ht - kvh * tiles) * kCols;
-    heads = min(kCols, G - h0);
+    seq = static_cast<int>(by_segments.div(unit.w)), ht = unit.w - seq * H;
+    has_first = (unit.z & 64) != 0;
+    const int kvh = static_cast<int>(by_tiles.div(ht)), h0 = (ht - kvh * tiles) * C::kHeads;
+    heads = min(C::kHeads, G - h0);
     st.reset();
     st.load_query(static_cast<const T *>(p.query) + (static_cast<int64_t>(seq) * p.num_q_heads + kvh * G + h0) * D,
                   heads, p.scale_log2);
@@ -672,7 +770,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
   auto end_segment = [&](bool has_last, bool final) {
     st.finish();
     if (has_first && has_last) {
-      const int kvh = ht / tiles, h0 = (ht - kvh * tiles) * kCols;
+      const int kvh = static_cast<int>(by_tiles.div(ht)), h0 = (ht - kvh * tiles) * C::kHeads;
       st.write_out(static_cast<T *>(p.out) + (static_cast<int64_t>(seq) * p.num_q_heads + kvh * G + h0) * D, heads);
       return;
     }
@@ -684,25 +782,31 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     }
   };
 
-  bool timed_out = false;
+  bool timed_out = false, fresh = true;
+  int stage = 0;
+  uint32_t phase = 0;
 #pragma unroll 1
   for (int i = 0; i < units; ++i) {
     if ((i & 31) == 0) load_batch(i + 32);  // the half that units i - 32 to i - 1 have left
     const int4 unit = table[i & 63];
-    const bool fresh = i == 0 || (unit.y & 32);
-    if (fresh) start_segment(unit);
-    if (!mbar_wait_bounded(&wbar[i % kStages], (i / kStages) & 1, p.status)) {
+    if (i == 0 || (unit.z & 64)) {
+      start_segment(unit);
+      fresh = true;
+    }
+    if (!mbar_wait_bounded(&wbar[stage], phase, p.status)) {
       timed_out = true;
       break;
     }
-    if (unit.x >= 0) {
-      const uint32_t base = smem_addr(ring + i % kStages * C::kStage);
-      st.process(base, base + C::kGroup, unit.y & 31, fresh);
+    const int valid = unit.z & 63;
+    if (unit.x >= 0 && (unit.y >= 0 || valid <= kMxGroup)) {  // else flagged: left out
+      st.process(smem_addr(ring + stage * C::kStage), valid, fresh);
+      fresh = false;
     }
     __syncwarp();  // every lane has read the stage
     const bool final = i == units - 1;
-    if (issued < units) issue(issued++);
-    if ((unit.y & 64) || final) end_segment((unit.y & 64) != 0, final);
+    if (issued < units) issue(issued++, 1);
+    if ((unit.z & 128) || final) end_segment((unit.z & 128) != 0, final);
+    if (++stage == kStages) stage = 0, phase ^= 1;
   }
   if (timed_out) {  // the copies in flight land before the ring is given up
     if (lane == 0)
@@ -726,9 +830,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     return k & 1 ? reinterpret_cast<const float *>(smem + (k >> 1) * C::kRing) : heads_smem + (k >> 1) * C::kState;
   };
   // the parts' factors and sums: warp h takes query head h, lane k part k
-  for (int h = warp; h < kCols; h += kWarps) {
+  for (int h = warp; h < C::kHeads; h += kWarps) {
     float m = -INFINITY, l = 0.f;
-    if (my_seg >= 0) m = part(lane)[kCols * D + h], l = part(lane)[kCols * D + kCols + h];
+    if (my_seg >= 0) m = part(lane)[C::kHeads * D + h], l = part(lane)[C::kHeads * D + C::kHeads + h];
     for (unsigned left = starts; left; left &= left - 1) {
       const int k = __ffs(left) - 1;
       const unsigned later = left & (left - 1);
@@ -741,8 +845,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
       if (!mine) L = 0.f;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(kAll, L, off);
-      if (mine) factor[lane * kCols + h] = f;
-      if (lane == k) run_ml[lane * kCols + h] = make_float2(M, L);
+      if (mine) factor[lane * C::kHeads + h] = f;
+      if (lane == k) run_ml[lane * C::kHeads + h] = make_float2(M, L);
     }
   }
   __syncthreads();
@@ -755,8 +859,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     const unsigned in_run = present & ~((1u << k) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : kAll);
     const int seg = __shfl_sync(kAll, my_seg, k);
     const int flags = __reduce_or_sync(kAll, in_run >> lane & 1u ? my_flags : 0);
-    const int s = seg / H, h_t = seg - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * kCols;
-    const int hs = min(kCols, G - h0);
+    const int s = seg / H, h_t = seg - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * C::kHeads;
+    const int hs = min(C::kHeads, G - h0);
     if (flags != 3) {
       if (flags & 1) {  // goes on in later CTAs, up to the one that holds its last unit
         const uint64_t last = static_cast<uint64_t>(prefix[s]) * H + static_cast<uint64_t>(h_t + 1) * (prefix[s + 1] - prefix[s]) - 1;
@@ -770,26 +874,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
     T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
     for (int e = threadIdx.x; e < hs * D; e += blockDim.x) {
       const int h = e / D;
-      const float2 ml = run_ml[k * kCols + h];
+      const float2 ml = run_ml[k * C::kHeads + h];
       float A = 0.f;
       for (unsigned w = in_run; w; w &= w - 1) {
         const int j = __ffs(w) - 1;
-        A = fmaf(factor[j * kCols + h], part(j)[e], A);
+        A = fmaf(factor[j * C::kHeads + h], part(j)[e], A);
       }
       if (flags == 3) {
         out[e] = Elem<T>::from_float(ml.y == 0.f ? 0.f : A / ml.y);
       } else {
         state[e] = A;
-        if (e - h * D == 0) state[kCols * D + h] = ml.x, state[kCols * D + kCols + h] = ml.y;
+        if (e - h * D == 0) state[C::kHeads * D + h] = ml.x, state[C::kHeads * D + C::kHeads + h] = ml.y;
       }
     }
   }
   if (p.workspace != nullptr) {
     if (threadIdx.x == 0)
       reinterpret_cast<MxMeta *>(p.workspace + static_cast<int64_t>(gridDim.x) * 2 * C::kState)[blockIdx.x] = meta;
-    if (!has_head && threadIdx.x < kCols) {  // no part to give: one without keys
-      ws[kCols * D + threadIdx.x] = -INFINITY;
-      ws[kCols * D + kCols + threadIdx.x] = 0.f;
+    if (!has_head && threadIdx.x < C::kHeads) {  // no part to give: one without keys
+      ws[C::kHeads * D + threadIdx.x] = -INFINITY;
+      ws[C::kHeads * D + C::kHeads + threadIdx.x] = 0.f;
     }
   }
   pdl_launch_dependents();
@@ -798,10 +902,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) mxfp4_decode_mma_kernel(const 
 // Segments that cross CTAs: block (c, h) joins query head h of the one that goes
 // on from CTA c.  A thread takes one element; the quarters of the block take every fourth part.
 constexpr int kJoinWays = 4;
-template <typename T, int NB>
+template <typename T, int NB, int CT>
 __global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
     mxfp4_decode_mma_join_kernel(const MxDecodeParams p, int tiles) {
-  using C = MxCfg<NB>;
+  using C = MxCfg<NB, CT>;
   constexpr int D = C::D;
   __shared__ float sums[kJoinWays][D];
   __shared__ float ml[kJoinWays][2];
@@ -811,7 +915,7 @@ __global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
       reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState)[first];
   if (meta.segment >= 0) {
     const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * tiles;
-    const int s = meta.segment / H, h_t = meta.segment - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * kCols;
+    const int s = meta.segment / H, h_t = meta.segment - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * C::kHeads;
     if (h0 + h < G) {  // uniform
       const int d = threadIdx.x % D, way = threadIdx.x / D;
       const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
@@ -819,12 +923,12 @@ __global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
       auto part = [&](int k) { return base + (k == 0 ? 1 : 2 * k) * C::kState; };
       float M = -INFINITY;
 #pragma unroll 4
-      for (int k = way; k < parts; k += kJoinWays) M = fmaxf(M, __ldcg(part(k) + kCols * D + h));
+      for (int k = way; k < parts; k += kJoinWays) M = fmaxf(M, __ldcg(part(k) + C::kHeads * D + h));
       float L = 0.f, A = 0.f;
 #pragma unroll 4
       for (int k = way; k < parts; k += kJoinWays) {
         const float *x = part(k);
-        const float m = __ldcg(x + kCols * D + h), l = __ldcg(x + kCols * D + kCols + h), a = __ldcg(x + h * D + d);
+        const float m = __ldcg(x + C::kHeads * D + h), l = __ldcg(x + C::kHeads * D + C::kHeads + h), a = __ldcg(x + h * D + d);
         const float f = part_factor(m, l, M);
         L += f * l;
         if (f != 0.f) A = fmaf(f, a, A);  // a part without keys has no sums
@@ -850,10 +954,10 @@ __global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
   pdl_launch_dependents();
 }
 
-template <typename T, int NB>
+template <typename T, int NB, int CT>
 cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, cudaStream_t stream) {
-  using C = MxCfg<NB>;
-  auto kern = mxfp4_decode_mma_kernel<T, NB>;
+  using C = MxCfg<NB, CT>;
+  auto kern = mxfp4_decode_mma_kernel<T, NB, CT>;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -862,20 +966,36 @@ cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, 
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_set[dev] = true;
   }
-  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(kWarps * 32), C::kSmem, stream, p, tiles);
+  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(C::kWarps * 32), C::kSmem, stream, p, tiles,
+                             FastDiv(p.num_kv_heads * tiles), FastDiv(tiles), FastDiv(p.block_size / kMxGroup));
   if (e == cudaSuccess && join)
-    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB>,
-                   dim3(ctas, std::min<int>(kCols, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, tiles);
+    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB, CT>,
+                   dim3(ctas, std::min<int>(C::kHeads, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, tiles);
   return e;
 }
 
-int mma_tiles(int num_q_heads, int num_kv_heads) { return (num_q_heads / num_kv_heads + kCols - 1) / kCols; }
+// Column tiles of a segment, and segments of a kv head.
+int mma_columns(int num_q_heads, int num_kv_heads) { return num_q_heads / num_kv_heads <= kQueries ? 1 : 2; }
+int mma_tiles(int num_q_heads, int num_kv_heads) {
+  const int heads = kQueries * mma_columns(num_q_heads, num_kv_heads);
+  return (num_q_heads / num_kv_heads + heads - 1) / heads;
+}
 
 // Whether some lengths that the table can hold need the second launch: not when
 // every segment has a CTA and a full table is no more than the slack per warp.
 bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t capacity, int sms) {
   const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads);
-  return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * kWarps * kMxGroup;
+  const int warps = mma_columns(num_q_heads, num_kv_heads) == 1 ? MxCfg<4, 1>::kWarps : MxCfg<4, 2>::kWarps;
+  return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * warps * kUnit;
+}
+
+template <typename T>
+cudaError_t launch_mma_t(const MxDecodeParams &p, int tiles, int columns, bool join, int ctas, cudaStream_t stream) {
+  if (p.head_dim == 64)
+    return columns == 1 ? launch_mma<T, 2, 1>(p, tiles, join, ctas, stream)
+                        : launch_mma<T, 2, 2>(p, tiles, join, ctas, stream);
+  return columns == 1 ? launch_mma<T, 4, 1>(p, tiles, join, ctas, stream)
+                      : launch_mma<T, 4, 2>(p, tiles, join, ctas, stream);
 }
 
 }  // namespace
@@ -887,21 +1007,24 @@ bool mxfp4_mma_supported(int dtype, int num_q_heads, int num_kv_heads, int head_
   if (head_dim != 64 && head_dim != 128) return false;
   const int64_t H = static_cast<int64_t>(num_kv_heads) * mma_tiles(num_q_heads, num_kv_heads);
   return num_blocks * num_kv_heads * (block_size / kMxGroup) < (int64_t{1} << 31) &&
-         (capacity / kMxGroup + 1) * H < (int64_t{1} << 31);
+         (capacity / kUnit + 1) * H < (int64_t{1} << 31);
 }
 
 size_t mxfp4_mma_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
                            int sms) {
   if (!mma_joins(num_seqs, num_q_heads, num_kv_heads, capacity, sms)) return 0;
-  return static_cast<size_t>(sms) * (2 * kCols * (head_dim + 2) * sizeof(float) + sizeof(MxMeta));
+  const size_t heads = kQueries * mma_columns(num_q_heads, num_kv_heads);
+  return static_cast<size_t>(sms) * (2 * heads * (head_dim + 2) * sizeof(float) + sizeof(MxMeta));
 }
 
 cudaError_t launch_mxfp4_mma(const MxDecodeParams &p, int dtype, cudaStream_t stream) {
-  const int tiles = mma_tiles(p.num_q_heads, p.num_kv_heads), sms = sm_count_current();
+  const int tiles = mma_tiles(p.num_q_heads, p.num_kv_heads), columns = mma_columns(p.num_q_heads, p.num_kv_heads);
+  const int sms = sm_count_current();
   const int64_t capacity = p.bt_stride * p.block_size;
   const int64_t H = static_cast<int64_t>(p.num_kv_heads) * tiles;
-  int64_t slice = ((int64_t{1} << 31) - 1) / ((capacity / kMxGroup + 1) * H);  // units stay in 32 bits
+  int64_t slice = ((int64_t{1} << 31) - 1) / ((capacity / kUnit + 1) * H);  // units stay in 32 bits
   if (slice > kMaxSeqs) slice = kMaxSeqs;
+  const bool join = mma_joins(p.num_seqs, p.num_q_heads, p.num_kv_heads, capacity, sms);
   for (int64_t s = 0; s < p.num_seqs; s += slice) {
     MxDecodeParams q = p;
     q.num_seqs = p.num_seqs - s < slice ? p.num_seqs - s : slice;
@@ -910,14 +1033,8 @@ cudaError_t launch_mxfp4_mma(const MxDecodeParams &p, int dtype, cudaStream_t st
     q.out = static_cast<char *>(p.out) + row;
     q.block_tables = p.block_tables + s * p.bt_stride;
     q.context_lens = p.context_lens + s;
-    const bool join = mma_joins(p.num_seqs, p.num_q_heads, p.num_kv_heads, capacity, sms);
-    cudaError_t e;
-    if (dtype == MI_DTYPE_BFLOAT16)
-      e = p.head_dim == 64 ? launch_mma<__nv_bfloat16, 2>(q, tiles, join, sms, stream)
-                           : launch_mma<__nv_bfloat16, 4>(q, tiles, join, sms, stream);
-    else
-      e = p.head_dim == 64 ? launch_mma<__half, 2>(q, tiles, join, sms, stream)
-                           : launch_mma<__half, 4>(q, tiles, join, sms, stream);
+    const cudaError_t e = dtype == MI_DTYPE_BFLOAT16 ? launch_mma_t<__nv_bfloat16>(q, tiles, columns, join, sms, stream)
+                                                     : launch_mma_t<__half>(q, tiles, columns, join, sms, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
