@@ -64,7 +64,7 @@ template <int NB, int CT>
 struct MxCfg {
   static constexpr int D = NB * kMxBlock;
   static constexpr int kWarps = CT == 1 ? 16 : 12;
-  static constexpr int kStages = CT == 1 ? 2 : 3;
+  static constexpr int kStages = 2;
   static constexpr int kHeads = CT * kQueries;    // query heads of a segment
   static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
   static constexpr int kStage = 4 * kGroup;       // K of two groups, V of two groups
@@ -73,10 +73,13 @@ struct MxCfg {
   static constexpr int kSmemRing = kWarps * kRing;
   static constexpr int kSmemHeads = kWarps * kState * 4;  // parts that end before their warp's range does
   static constexpr int kSmemUnits = kWarps * 64 * 16;     // two batches of 32 units per warp
+  static constexpr int kQuery = CT * NB * 512;            // q's B fragments, per warp
+  static constexpr int kSmemQuery = kWarps * kQuery;
   static constexpr int kSmemBars = kWarps * kStages * 8;
   static constexpr int kSmemPrefix = (kMaxSeqs + 1) * 4;
   static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kHeads * 12 + 16;
-  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemBars + kSmemPrefix + kSmemMisc;
+  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemQuery + kSmemBars + kSmemPrefix +
+                               kSmemMisc;
   static_assert(kState * 4 <= kRing, "a warp's last part goes into its own ring");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -177,89 +180,22 @@ __device__ __forceinline__ float scale_of(uint32_t w, int b) {
   return __uint_as_float((v & 0x7f800000u) | 1u);
 }
 
-// Scale byte of block b of a key: k = 0, 1: keys 2t, 2t + 1; k = 2, 3: keys 2t + 8, 2t + 9.  At D = 64
-// the two keys of a pair share a word.
+// V's scales of a group: words of keys 2t, 2t + 1 (w[0], w[1]) and 2t + 8, 2t + 9 (w[2], w[3]); at
+// D = 64 a key pair has one word.
 template <int NB>
-__device__ __forceinline__ int byte_of(const uint4 &w, int k, int b) {
-  if constexpr (NB == 4)
-    return ((k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w) >> (8 * b)) & 255u;
-  else
-    return ((k < 2 ? w.x : w.z) >> (16 * (k & 1) + 8 * b)) & 255u;
-}
-
-// Scales that the window of 8 binades does not hold: raise R_b (a byte of `ref`, returned) where a
-// scale is above it, then take the keys window by window.  `o`: the caller's copy of its
-// accumulators [tile][block][4]; `p`: [tile][key], p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in both halves.
-// Out of line, so that the loop around it keeps its registers.
-template <int NB, int CT>
-__device__ __noinline__ uint32_t value_slow(float *o, uint32_t ref, uint32_t vcodes, uint4 w, const uint32_t *p,
-                                            int valid) {
-  const int lane = threadIdx.x & 31;
-  const int shift = lane & 4 ? 16 : 0;  // g odd: the column of odd dims
-  int deepest = 0;
-  const int key = (lane & 3) * 2;  // scales of keys that do not exist: none
+__device__ __forceinline__ void load_scales(uint32_t vbase, int t, uint32_t (&w)[4]) {
   if constexpr (NB == 4) {
-    if (key >= valid) w.x = 0;
-    if (key + 1 >= valid) w.y = 0;
-    if (key + 8 >= valid) w.z = 0;
-    if (key + 9 >= valid) w.w = 0;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                 : "=r"(w[0]), "=r"(w[1])
+                 : "r"(vbase + NB * kMxBlockBytes + t * 8));
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                 : "=r"(w[2]), "=r"(w[3])
+                 : "r"(vbase + NB * kMxBlockBytes + t * 8 + 32));
   } else {
-    w.x &= (key < valid ? 0xffffu : 0u) | (key + 1 < valid ? 0xffff0000u : 0u);
-    w.z &= (key + 8 < valid ? 0xffffu : 0u) | (key + 9 < valid ? 0xffff0000u : 0u);
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[2]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
+    w[1] = w[3] = 0;
   }
-#pragma unroll 1
-  for (int b = 0; b < NB; ++b) {
-    int top = 0, low = 255;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int s = byte_of<NB>(w, k, b);
-      if (s >= 1 && s <= 254) top = max(top, s), low = min(low, s);
-    }
-#pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-      top = max(top, __shfl_xor_sync(kAll, top, off));
-      low = min(low, __shfl_xor_sync(kAll, low, off));
-    }
-    int r = (ref >> (8 * b)) & 255;
-    if (top > r) {
-      const int next = min(top + 2, 254);
-      const float f = exp2i(r - next);
-#pragma unroll
-      for (int i = 0; i < 4 * CT; ++i) o[(i / 4 * NB + b) * 4 + i % 4] *= f;
-      ref = (ref & ~(255u << (8 * b))) | (static_cast<uint32_t>(next) << (8 * b));
-      r = next;
-    }
-    if (low < 255) deepest = max(deepest, r - low);
-  }
-  uint32_t lo[NB], hi[NB];
-  load_codes<NB, true>(vcodes, lane, lo, hi);
-#pragma unroll 1
-  for (int window = 0; window <= deepest / 8; ++window) {
-    const float back = exp2i(-8 * window);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int r = (ref >> (8 * b)) & 255;
-      uint32_t f[4], a[4], c[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = byte_of<NB>(w, k, b), d = r - s;
-        f[k] = s >= 1 && s <= 254 && (d >> 3) == window ? 0x3c00u - ((d & 7) << 10) : 0u;
-        if (s == 255 && window == 0) f[k] = 0x7e00u;
-        f[k] <<= shift;
-      }
-      mx_codes_to_f16(lo[b], a);
-      mx_codes_to_f16(hi[b], c);
-#pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        float d[4];
-        mma_f16_zero(d, a[0], a[1], a[2], a[3], mul_f16x2(p[4 * i], f[0]), mul_f16x2(p[4 * i + 1], f[1]));
-        mma_f16(d, c[0], c[1], c[2], c[3], mul_f16x2(p[4 * i + 2], f[2]), mul_f16x2(p[4 * i + 3], f[3]));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[(i * NB + b) * 4 + j] = fmaf(d[j], back, o[(i * NB + b) * 4 + j]);
-      }
-    }
-  }
-  return ref;
 }
 
 // A warp's state on a segment: 4 query heads to a column tile, lane (g, t) = (lane / 4, lane % 4).
@@ -267,18 +203,20 @@ template <typename T, int NB, int CT>
 struct MxWarp {
   using C = MxCfg<NB, CT>;
   static constexpr int D = C::D;
-  uint32_t q[CT][NB * 2][2];  // B fragments of q: columns 2i and 2i + 1 both query i of the tile
+  uint32_t q;                 // shared address of this lane's B fragments of q (columns 2i and 2i + 1 both
+                              // query i of the tile): 4 words per block, 512 bytes between blocks
   float xs[CT];               // log2-domain scale of query t
   float o[CT][NB][4];         // query t, dims 32b + 4g + 0 to 3, times 2^(R_b - 127)
   float m[CT], l[CT];         // query t; l: this lane's keys only
   uint32_t ref;               // R_b, one byte per block
-  uint32_t one, unit0, unit1; // f16 1.0 and the places of d's bits in the half of this lane's column
+  uint32_t one, unit0, unit1; // f16 1.0 and minus the places of d's bits in the half of this lane's column
   int lane, g, t;
 
-  __device__ __forceinline__ void setup() {
+  __device__ __forceinline__ void setup(uint32_t query_smem) {
     lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    q = query_smem + lane * 16;
     const int shift = g & 1 ? 16 : 0;
-    one = 0x3c00u << shift, unit0 = 1u << (10 + shift), unit1 = 1u << (2 + shift);
+    one = 0x3c00u << shift, unit0 = 0u - (1u << (10 + shift)), unit1 = 0u - (1u << (2 + shift));
   }
 
   __device__ __forceinline__ void reset() {
@@ -318,81 +256,66 @@ struct MxWarp {
       e = min(e, 126);
       const float f = exp2i(e);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        q[c][2 * b][0] = pack_f16(x[b][0] * f, x[b][1] * f);
-        q[c][2 * b][1] = pack_f16(x[b][2] * f, x[b][3] * f);
-        q[c][2 * b + 1][0] = pack_f16(x[b][4] * f, x[b][5] * f);
-        q[c][2 * b + 1][1] = pack_f16(x[b][6] * f, x[b][7] * f);
-      }
+      for (int b = 0; b < NB; ++b)  // read by this lane alone
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q + (c * NB + b) * 512),
+                     "r"(pack_f16(x[b][0] * f, x[b][1] * f)), "r"(pack_f16(x[b][2] * f, x[b][3] * f)),
+                     "r"(pack_f16(x[b][4] * f, x[b][5] * f)), "r"(pack_f16(x[b][6] * f, x[b][7] * f))
+                     : "memory");
       xs[c] = __shfl_sync(kAll, exp2i(-e) * scale_log2, 8 * t);  // a lane of query t: g = 2t
     }
   }
 
-  // Scores of a group's 16 keys for query t, still to be scaled by xs: x[c][0], key g; x[c][1], key g + 8.
-  __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[CT][2]) const {
-    uint32_t lo[NB], hi[NB], wl, wh;
-    load_codes<NB, false>(kbase, lane, lo, hi);
-    if constexpr (NB == 4) {
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 4));
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 4 + 32));
-    } else {
-      asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl) : "r"(kbase + NB * kMxBlockBytes + g * 2));
-      asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh) : "r"(kbase + NB * kMxBlockBytes + g * 2 + 16));
+  // Scores of a unit's 32 keys for query t, still to be scaled by xs: x[j][c][0], key g of group j;
+  // x[j][c][1], its key g + 8.
+  __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[2][CT][2]) const {
+    uint32_t lo[2][NB], hi[2][NB], wl[2], wh[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t base = kbase + j * C::kGroup;
+      load_codes<NB, false>(base, lane, lo[j], hi[j]);
+      if constexpr (NB == 4) {
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl[j]) : "r"(base + NB * kMxBlockBytes + g * 4));
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh[j]) : "r"(base + NB * kMxBlockBytes + g * 4 + 32));
+      } else {
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl[j]) : "r"(base + NB * kMxBlockBytes + g * 2));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh[j]) : "r"(base + NB * kMxBlockBytes + g * 2 + 16));
+      }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t a[4], e[4];
-      mx_codes_to_f16(lo[b], a);
-      mx_codes_to_f16(hi[b], e);
-      const float fl = scale_of(wl, b), fh = scale_of(wh, b);
+      uint32_t f[CT][4];
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        float d[4];
-        mma_f16_zero(d, a[0], e[0], a[1], e[1], q[c][2 * b][0], q[c][2 * b][1]);
-        mma_f16(d, a[2], e[2], a[3], e[3], q[c][2 * b + 1][0], q[c][2 * b + 1][1]);
-        x[c][0] = b == 0 ? d[0] * fl : fmaf(d[0], fl, x[c][0]);
-        x[c][1] = b == 0 ? d[2] * fh : fmaf(d[2], fh, x[c][1]);
+      for (int c = 0; c < CT; ++c)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(f[c][0]), "=r"(f[c][1]), "=r"(f[c][2]), "=r"(f[c][3])
+                     : "r"(q + (c * NB + b) * 512));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t a[4], e[4];
+        mx_codes_to_f16(lo[j][b], a);
+        mx_codes_to_f16(hi[j][b], e);
+        const float fl = scale_of(wl[j], b), fh = scale_of(wh[j], b);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          float d[4];
+          mma_f16_zero(d, a[0], e[0], a[1], e[1], f[c][0], f[c][1]);
+          mma_f16(d, a[2], e[2], a[3], e[3], f[c][2], f[c][3]);
+          x[j][c][0] = b == 0 ? d[0] * fl : fmaf(d[0], fl, x[j][c][0]);
+          x[j][c][1] = b == 0 ? d[2] * fh : fmaf(d[2], fh, x[j][c][1]);
+        }
       }
     }
   }
 
-  // V's scales of a group: words of keys 2t, 2t + 1 (w[0], w[1]) and 2t + 8, 2t + 9 (w[2], w[3]); at
-  // D = 64 a key pair has one word.
-  __device__ __forceinline__ void value_scales(uint32_t vbase, uint32_t (&w)[4]) const {
-    if constexpr (NB == 4) {
-      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                   : "=r"(w[0]), "=r"(w[1])
-                   : "r"(vbase + NB * kMxBlockBytes + t * 8));
-      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                   : "=r"(w[2]), "=r"(w[3])
-                   : "r"(vbase + NB * kMxBlockBytes + t * 8 + 32));
-    } else {
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[2]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
-      w[1] = w[3] = 0;
-    }
-  }
-
-  // The largest scale byte per block over the group's keys below `valid`, of this lane's keys.
-  __device__ __forceinline__ uint32_t largest_scales(const uint32_t (&w)[4], int valid) const {
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t bytes = NB == 4 ? w[k] : (w[k & 2] >> (16 * (k & 1))) & 0xffffu;
-      if (2 * t + (k & 1) + (k >> 1) * 8 < valid) top = __vmaxu4(top, bytes);
-    }
-    return top;
-  }
-
-  // Keys that do not exist: whatever their scale bytes are becomes the reference (their p is zero).
-  __device__ __forceinline__ void mask_scales(uint32_t (&w)[4], int valid) const {
+  // Scale bytes of keys that do not exist become `with`'s.
+  __device__ __forceinline__ void mask_scales(uint32_t (&w)[4], int valid, uint32_t with) const {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (2 * t + (k & 1) + (k >> 1) * 8 < valid) continue;
       if constexpr (NB == 4)
-        w[k] = ref;
+        w[k] = with;
       else
-        w[k & 2] = k & 1 ? (w[k & 2] & 0xffffu) | ref << 16 : (w[k & 2] & 0xffff0000u) | (ref & 0xffffu);
+        w[k & 2] = k & 1 ? (w[k & 2] & 0xffffu) | with << 16 : (w[k & 2] & 0xffff0000u) | (with & 0xffffu);
     }
   }
 
@@ -409,9 +332,12 @@ struct MxWarp {
     }
   }
 
-  // O += P_b V of a group, all scales within the window; p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9
-  // in both halves.
-  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[CT][4]) {
+  // O += P_b V of a group.  d: distances per byte, 0 to 7, or 15 for no contribution (2^-15 has the f16
+  // exponent 0: zero); p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in both halves.  FAR: the
+  // products are `back` times what d says.
+  template <bool FAR>
+  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[CT][4],
+                                         float back = 1.f) {
     uint32_t lo[NB], hi[NB];
     load_codes<NB, true>(vbase, lane, lo, hi);
 #pragma unroll
@@ -421,16 +347,83 @@ struct MxWarp {
       for (int k = 0; k < 4; ++k) {
         // bytes of blocks (b & ~1) and (b | 1) in the low half of the word
         const uint32_t word = NB == 4 ? (b < 2 ? d[k] : d[k] >> 16) : (k & 1 ? d[k & 2] >> 16 : d[k & 2]);
-        f[k] = b & 1 ? one - (word & 0xff00u) * unit1 : one - (word & 0xffu) * unit0;
+        f[k] = b & 1 ? (word & 0xff00u) * unit1 + one : (word & 0xffu) * unit0 + one;
       }
       uint32_t a[4], e[4];
       mx_codes_to_f16(lo[b], a);
       mx_codes_to_f16(hi[b], e);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        mma_f16(o[c][b], a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
-        mma_f16(o[c][b], e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+        if constexpr (FAR) {
+          float r[4];
+          mma_f16_zero(r, a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
+          mma_f16(r, e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[c][b][i] = fmaf(r[i], back, o[c][b][i]);
+        } else {
+          mma_f16(o[c][b], a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
+          mma_f16(o[c][b], e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+        }
       }
+    }
+  }
+
+  // The largest byte of each block over the group's keys, from this lane's four.
+  __device__ __forceinline__ static uint32_t over_keys(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    uint32_t top = __vmaxu4(__vmaxu4(a, b), __vmaxu4(c, d));
+    if constexpr (NB == 2) top = __vmaxu4(top, top >> 16) & 0xffffu;
+    top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 1));
+    return __vmaxu4(top, __shfl_xor_sync(kAll, top, 2));
+  }
+
+  // As values() for scales that the window of 8 binades does not hold: raise R_b where a scale is above
+  // it, then take the keys window by window.
+  __device__ __forceinline__ void values_far(uint32_t vbase, const uint32_t (&p)[CT][4], int valid) {
+    uint32_t w[4], nan[4];
+    load_scales<NB>(vbase, t, w);
+    mask_scales(w, valid, 0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      nan[k] = __vcmpeq4(w[k], 0xffffffffu);
+      w[k] &= ~nan[k];
+    }
+    const uint32_t bad = over_keys(nan[0], nan[1], nan[2], nan[3]);
+    const uint32_t top = over_keys(w[0], w[1], w[2], w[3]);
+    const uint32_t above = __vcmpgtu4(top, ref);
+    const uint32_t next = (ref & ~above) | (__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu) & above);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float f = exp2i(static_cast<int>((ref >> (8 * b)) & 255u) - static_cast<int>((next >> (8 * b)) & 255u));
+#pragma unroll
+      for (int i = 0; i < CT * 4; ++i) o[i / 4][b][i % 4] *= f;
+    }
+    ref = next;
+    const uint32_t all = NB == 4 ? ref : (ref & 0xffffu) * 0x10001u;
+    uint32_t some[4];  // all ones where there is a scale
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      some[k] = __vcmpne4(w[k], 0u);
+      w[k] = (all - w[k]) & some[k];  // no byte is above the reference now
+    }
+    uint32_t deepest = over_keys(w[0], w[1], w[2], w[3]);
+    deepest = __vmaxu4(deepest, deepest >> 16);
+    deepest = max(deepest & 255u, (deepest >> 8) & 255u);
+#pragma unroll 1
+    for (uint32_t window = 0; window <= deepest / 8; ++window) {
+      uint32_t d[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t in = __vcmpeq4((w[k] >> 3) & 0x1f1f1f1fu, window * 0x01010101u) & some[k];
+        d[k] = (w[k] & 0x07070707u & in) | (0x0f0f0f0fu & ~in);
+      }
+      values<true>(vbase, d, p, exp2i(-8 * static_cast<int>(window)));
+    }
+    if (bad) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        if (bad >> (8 * b) & 255u)
+#pragma unroll
+          for (int i = 0; i < CT * 4; ++i) o[i / 4][b][i % 4] = __uint_as_float(0x7fffffffu);
     }
   }
 
@@ -439,15 +432,15 @@ struct MxWarp {
   __device__ __forceinline__ void process(uint32_t base, int valid, bool first) {
     const uint32_t vbase = base + 2 * C::kGroup;
     float x[2][CT][2];
-    scores(base, x[0]);
-    scores(base + C::kGroup, x[1]);
+    scores(base, x);
     uint32_t w[2][4];
-    value_scales(vbase, w[0]);
-    value_scales(vbase + C::kGroup, w[1]);
+    load_scales<NB>(vbase, t, w[0]);
+    load_scales<NB>(vbase + C::kGroup, t, w[1]);
     if (first) {  // uniform: R_b starts at the largest scale here and two binades of room
-      uint32_t top = __vmaxu4(largest_scales(w[0], valid), largest_scales(w[1], valid - kMxGroup));
-      top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 1));
-      top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 2));
+      mask_scales(w[0], valid, 0);
+      mask_scales(w[1], valid - kMxGroup, 0);
+      const uint32_t top = __vmaxu4(over_keys(w[0][0], w[0][1], w[0][2], w[0][3]),
+                                    over_keys(w[1][0], w[1][1], w[1][2], w[1][3]));
       ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
     }
 #pragma unroll
@@ -462,7 +455,7 @@ struct MxWarp {
           if (j * kMxGroup + g >= valid) x[j][c][0] = -INFINITY;
           if (j * kMxGroup + g + 8 >= valid) x[j][c][1] = -INFINITY;
         }
-        mask_scales(w[j], valid - j * kMxGroup);
+        mask_scales(w[j], valid - j * kMxGroup, ref);  // whatever they are: their p is zero
       }
     }
     // m follows the largest score, up to kLag binades behind it
@@ -505,23 +498,11 @@ struct MxWarp {
     uint32_t d[2][4];
     const uint32_t far = distances(w[0], d[0]) | distances(w[1], d[1]);
     if (__any_sync(kAll, far != 0)) {
-      float copy[CT * NB * 4];
-      uint32_t pc[2][CT * 4];
 #pragma unroll
-      for (int i = 0; i < CT * NB * 4; ++i) copy[i] = o[i / (NB * 4)][i / 4 % NB][i % 4];
-#pragma unroll
-      for (int i = 0; i < CT * 8; ++i) pc[i / (CT * 4)][i % (CT * 4)] = p[i / (CT * 4)][i / 4 % CT][i % 4];
-#pragma unroll 1
-      for (int j = 0; j < 2; ++j)
-        ref = value_slow<NB, CT>(copy, ref, vbase + j * C::kGroup,
-                                 j ? make_uint4(w[1][0], w[1][1], w[1][2], w[1][3])
-                                   : make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]),
-                                 pc[j], valid - j * kMxGroup);
-#pragma unroll
-      for (int i = 0; i < CT * NB * 4; ++i) o[i / (NB * 4)][i / 4 % NB][i % 4] = copy[i];
+      for (int j = 0; j < 2; ++j) values_far(vbase + j * C::kGroup, p[j], valid - j * kMxGroup);
     } else {
-      values(vbase, d[0], p[0]);
-      values(vbase + C::kGroup, d[1], p[1]);
+      values<false>(vbase, d[0], p[0]);
+      values<false>(vbase + C::kGroup, d[1], p[1]);
     }
   }
 
@@ -585,7 +566,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
   int4 *unit_table = reinterpret_cast<int4 *>(smem + C::kSmemRing + C::kSmemHeads);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery);
   int *prefix = reinterpret_cast<int *>(bars + kWarps * kStages);  // units of a segment before sequence s
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
@@ -755,7 +736,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
   issue(0, issued);
 
   MxWarp<T, NB, CT> st;
-  st.setup();
+  st.setup(smem_addr(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + warp * C::kQuery));
   int seq = 0, ht = 0, heads = 0;
   bool has_first = false;
   auto start_segment = [&](const int4 &unit) {
