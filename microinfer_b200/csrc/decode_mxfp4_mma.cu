@@ -98,6 +98,15 @@ struct FastDiv {
   }
 };
 
+// Launch constants: tiles of a kv head (segments), and divisions by what the host knows.
+struct MxPlan {
+  int tiles;
+  FastDiv by_segments;  // segments of a sequence: num_kv_heads * tiles
+  FastDiv by_tiles;
+  FastDiv by_page;      // groups of a page
+  FastDiv by_ctas;
+};
+
 // Beside its states (a part whose segment began in an earlier CTA, then one whose
 // segment goes on in the next) a CTA leaves in the workspace the segment that goes
 // on (-1: none) and how many CTAs hold parts of it.
@@ -230,19 +239,28 @@ struct MxWarp {
     }
   }
 
-  // Query heads of the segment (heads of them exist).
-  __device__ __forceinline__ void load_query(const T *query, int heads, float scale_log2) {
+  // q of the segment's query heads (heads of them exist): this lane's elements ...
+  __device__ __forceinline__ void fetch_query(const T *query, int heads, uint4 (&raw)[CT][NB]) const {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const int h = c * kQueries + (g >> 1);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        raw[c][b] = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads) raw[c][b] = *reinterpret_cast<const uint4 *>(query + h * D + b * 32 + t * 8);
+      }
+    }
+  }
+  // ... as f16 fragments.
+  __device__ __forceinline__ void set_query(const uint4 (&raw)[CT][NB], float scale_log2) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
       float x[NB][8];
       uint32_t top = 0;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (h < heads) v = *reinterpret_cast<const uint4 *>(query + h * D + b * 32 + t * 8);
         float2 f[4];
-        Vec16<T>::unpack(v, f);
+        Vec16<T>::unpack(raw[c][b], f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[b][2 * i] = f[i].x, x[b][2 * i + 1] = f[i].y;
@@ -560,7 +578,8 @@ __device__ __forceinline__ float part_factor(float m, float l, float M) {
 }
 
 template <typename T, int NB, int CT>
-__global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mma_kernel(const MxDecodeParams p, int tiles, FastDiv by_segments, FastDiv by_tiles, FastDiv by_page) {
+__global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
+    mxfp4_decode_mma_kernel(const MxDecodeParams p, const MxPlan plan) {
   using C = MxCfg<NB, CT>;
   constexpr int D = C::D, kWarps = C::kWarps, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -571,42 +590,63 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
   int *scan = part_flags + 2 * kWarps;      // [2 * kWarps]
-  float *factor = reinterpret_cast<float *>(scan + 2 * kWarps);               // [2 * kWarps][8]
-  float2 *run_ml = reinterpret_cast<float2 *>(                               // [2 * kWarps][8]
+  int *part_at = scan;                      // [2 * kWarps] after the scan: offsets of the parts, in floats
+  float *factor = reinterpret_cast<float *>(scan + 2 * kWarps);  // [2 * kWarps][heads]
+  float2 *run_ml = reinterpret_cast<float2 *>(                   // [2 * kWarps][heads]
       (reinterpret_cast<uintptr_t>(factor + 2 * kWarps * C::kHeads) + 15) & ~static_cast<uintptr_t>(15));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t *wbar = bars + warp * kStages;
   uint8_t *ring = smem + warp * C::kRing;
   const int n = static_cast<int>(p.num_seqs);
   const int G = p.num_q_heads / p.num_kv_heads;
-  const int H = p.num_kv_heads * tiles;  // segments of a sequence
+  const int tiles = plan.tiles, H = p.num_kv_heads * tiles;  // segments of a sequence
 
-  if (lane == 0) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) mbar_init(&wbar[s], 1);
-    fence_mbar_init();
-    part_seg[2 * warp] = part_seg[2 * warp + 1] = -1;
-  }
   pdl_wait();
+  pdl_launch_dependents();  // dependents wait for this grid's end; their blocks may come as its own leave
 
   // ---- units of each sequence, their prefix sums and largest ----
   const int64_t cap = p.bt_stride * p.block_size;
   int c_max = 0;
-  {
+  auto units_of = [&](int s) {
+    int ctx = s < n ? __ldg(p.context_lens + s) : 0;
+    if (ctx > cap) {
+      if (blockIdx.x == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+      ctx = static_cast<int>(cap);
+    }
+    return ctx > 0 ? (ctx - 1) / kUnit + 1 : 0;
+  };
+  auto setup_barriers = [&] {  // while the lengths are on their way
+    if (lane == 0) {
+#pragma unroll
+      for (int s = 0; s < kStages; ++s) mbar_init(&wbar[s], 1);
+      fence_mbar_init();
+      part_seg[2 * warp] = part_seg[2 * warp + 1] = -1;
+    }
+  };
+  if (n <= 32) {  // every warp for itself
+    const int c = units_of(lane);
+    setup_barriers();
+    int incl = c;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(kAll, incl, off);
+      if (lane >= off) incl += v;
+    }
+    c_max = __reduce_max_sync(kAll, c);
+    if (warp == 0) {
+      if (lane == 0) prefix[0] = 0;
+      if (lane < n) prefix[lane + 1] = incl;
+    }
+  } else {
     constexpr int kPer = (kMaxSeqs + kWarps * 32 - 1) / (kWarps * 32);
     int c[kPer], sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int s = threadIdx.x * kPer + i;
-      int ctx = s < n ? __ldg(p.context_lens + s) : 0;
-      if (ctx > cap) {
-        if (blockIdx.x == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
-        ctx = static_cast<int>(cap);
-      }
-      c[i] = ctx > 0 ? (ctx - 1) / kUnit + 1 : 0;
+      c[i] = units_of(threadIdx.x * kPer + i);
       sum += c[i];
       c_max = max(c_max, c[i]);
     }
+    setup_barriers();
     int incl = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -632,8 +672,8 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
         if (s == n - 1) prefix[n] = before;
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
   // sequences without a key: zeros
   for (int s = blockIdx.x; s < n; s += gridDim.x) {
     if (prefix[s + 1] != prefix[s]) continue;
@@ -642,83 +682,89 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
       *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
   }
 
-  // ---- this warp's range of units (a unit: 32 keys of one segment) ----
+  // ---- this CTA's range of units (a unit: 32 keys of one segment), split among its warps ----
   const uint32_t total = static_cast<uint32_t>(prefix[n]) * H;
-  const uint32_t all_warps = gridDim.x * kWarps;
-  uint32_t u0 = 0, u1 = 0;
-  const uint32_t share = (total + all_warps - 1) / all_warps;
+  const uint32_t share = plan.by_ctas.div(total), over = total - share * gridDim.x;  // `over` CTAs take one more
+  uint32_t u0, cta_units;
   if (static_cast<uint32_t>(n) * H <= gridDim.x &&
-      static_cast<uint32_t>((c_max + kWarps - 1) / kWarps) <= share + kAlignedSlack) {
-    if (blockIdx.x < static_cast<uint32_t>(n) * H) {  // one segment to a CTA
-      const int s = blockIdx.x / H, c = prefix[s + 1] - prefix[s];
-      const uint32_t base = static_cast<uint32_t>(prefix[s]) * H + (blockIdx.x - s * H) * c;
-      u0 = base + static_cast<uint32_t>(c) * warp / kWarps;
-      u1 = base + static_cast<uint32_t>(c) * (warp + 1) / kWarps;
-    }
+      static_cast<uint32_t>(c_max) <= share + (over != 0) + kAlignedSlack * kWarps) {
+    const int s = static_cast<int>(plan.by_segments.div(blockIdx.x));  // one segment to a CTA
+    cta_units = s < n ? prefix[s + 1] - prefix[s] : 0;
+    u0 = s < n ? static_cast<uint32_t>(prefix[s]) * H + (blockIdx.x - s * H) * cta_units : 0;
   } else {
-    const uint64_t j = blockIdx.x * kWarps + warp;
-    u0 = static_cast<uint32_t>(total * j / all_warps);
-    u1 = static_cast<uint32_t>(total * (j + 1) / all_warps);
+    cta_units = share + (blockIdx.x < over);
+    u0 = share * blockIdx.x + min(blockIdx.x, over);
   }
-  const int units = static_cast<int>(u1 - u0);
+  const int units = static_cast<int>(cta_units * (warp + 1) / kWarps - cta_units * warp / kWarps);
+  u0 += cta_units * warp / kWarps;
 
   // Batches of 32 units, one per lane, in shared memory: x, y, the indices of the unit's two groups
   // in the pools (-1: no such page, or no such keys); z, its keys (bits 0-5) and whether it is its
   // segment's first (64) or last (128) unit; w, its segment.
   const int per_page = p.block_size / kMxGroup;
   int4 *table = unit_table + warp * 64;
-  auto load_batch = [&](int first) {
-    const int i = first + lane;
+  struct Unit {
+    int seq, ht, unit, count;
+  };
+  auto unit_of = [&](int i) {
+    const uint32_t u = u0 + i;
+    const int per = static_cast<int>(plan.by_segments.div(u));
+    int a = 0, b = n - 1;  // the last sequence whose prefix is not above `per`
+    while (a < b) {
+      const int mid = (a + b + 1) >> 1;
+      if (prefix[mid] <= per)
+        a = mid;
+      else
+        b = mid - 1;
+    }
+    Unit r;
+    r.seq = a;
+    r.count = prefix[a + 1] - prefix[a];
+    const int rest = static_cast<int>(u - static_cast<uint32_t>(prefix[a]) * H);
+    r.ht = static_cast<int>(__fdividef(static_cast<float>(rest), static_cast<float>(r.count)));  // off by one at most
+    if (r.ht * r.count > rest) --r.ht;
+    if (rest - r.ht * r.count >= r.count) ++r.ht;
+    r.unit = rest - r.ht * r.count;
+    return r;
+  };
+  auto load_batch = [&](int i, const Unit &r) {
     if (i < units) {
-      const uint32_t u = u0 + i;
-      const int per = static_cast<int>(by_segments.div(u));
-      int a = 0, b = n - 1;  // the last sequence whose prefix is not above `per`
-      while (a < b) {
-        const int mid = (a + b + 1) >> 1;
-        if (prefix[mid] <= per)
-          a = mid;
-        else
-          b = mid - 1;
-      }
-      const int before = prefix[a], count = prefix[a + 1] - before;
-      const int rest = static_cast<int>(u - static_cast<uint32_t>(before) * H);
-      int ht = static_cast<int>(__fdividef(static_cast<float>(rest), static_cast<float>(count)));  // to one
-      if (ht * count > rest) --ht;
-      if (rest - ht * count >= count) ++ht;
-      const int unit = rest - ht * count;
-      int valid = kUnit, flags = unit == 0 ? 64 : 0;
-      if (unit == count - 1) {
-        const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + a)), cap));
-        valid = ctx - unit * kUnit;
+      int valid = kUnit, flags = r.unit == 0 ? 64 : 0;
+      if (r.unit == r.count - 1) {
+        const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + r.seq)), cap));
+        valid = ctx - r.unit * kUnit;
         flags |= 128;
       }
-      const int32_t *row = p.block_tables + static_cast<int64_t>(a) * p.bt_stride;
-      const int kvh = static_cast<int>(by_tiles.div(ht));
+      const int32_t *row = p.block_tables + static_cast<int64_t>(r.seq) * p.bt_stride;
+      const int kvh = static_cast<int>(plan.by_tiles.div(r.ht));
       int where[2] = {-1, -1};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j * kMxGroup >= valid) break;
-        const int group = 2 * unit + j, col = static_cast<int>(by_page.div(group));
+        const int group = 2 * r.unit + j, col = static_cast<int>(plan.by_page.div(group));
         const int page = __ldg(row + col);
         if (page >= 0 && page < p.num_blocks)
           where[j] = (page * p.num_kv_heads + kvh) * per_page + group - col * per_page;
         else
           flag_status(p.status, MI_DEV_BAD_BLOCK);
       }
-      table[i & 63] = make_int4(where[0], where[1], valid | flags, a * H + ht);
+      table[i & 63] = make_int4(where[0], where[1], valid | flags, r.seq * H + r.ht);
     }
     __syncwarp();
   };
-  load_batch(0);
-  // Lanes 4s to 4s + 3 of `lanes` bring unit first + s: K and V of its two groups.
+  // Lanes 4s to 4s + 3 bring unit first + s: K (0, 1) and V (2, 3) of its groups, both at once where
+  // they are neighbours.
   auto issue = [&](int first, int count) {
     const int i = first + (lane >> 2);
-    const bool on = (lane >> 2) < count;
-    int where = -1;
+    int where = -1, bytes = C::kGroup;
     uint64_t *bar = &wbar[i % kStages];
-    if (on) {
+    if ((lane >> 2) < count) {
       const int4 unit = table[i & 63];
       where = lane & 1 ? unit.y : unit.x;
+      if (unit.x >= 0 && unit.y == unit.x + 1) {
+        if (lane & 1) where = -1;
+        bytes = 2 * C::kGroup;
+      }
       if ((lane & 3) == 0) {
         const int groups = (unit.x >= 0) + (unit.y >= 0);
         if (groups)
@@ -730,48 +776,63 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
     __syncwarp();
     if (where >= 0)
       bulk_g2s(ring + i % kStages * C::kStage + ((lane >> 1) & 1) * 2 * C::kGroup + (lane & 1) * C::kGroup,
-               (lane & 2 ? p.value_pages : p.key_pages) + static_cast<int64_t>(where) * C::kGroup, C::kGroup, bar);
+               (lane & 2 ? p.value_pages : p.key_pages) + static_cast<int64_t>(where) * C::kGroup, bytes, bar);
   };
-  int issued = min(kStages, units);
-  issue(0, issued);
 
   MxWarp<T, NB, CT> st;
   st.setup(smem_addr(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + warp * C::kQuery));
-  int seq = 0, ht = 0, heads = 0;
+  int segment = 0, heads = 0;
+  int64_t row = 0;  // the segment's first query head, as a row of q and out
   bool has_first = false;
-  auto start_segment = [&](const int4 &unit) {
-    seq = static_cast<int>(by_segments.div(unit.w)), ht = unit.w - seq * H;
-    has_first = (unit.z & 64) != 0;
-    const int kvh = static_cast<int>(by_tiles.div(ht)), h0 = (ht - kvh * tiles) * C::kHeads;
+  auto place = [&](int seg) {
+    segment = seg;
+    const int seq = static_cast<int>(plan.by_segments.div(seg)), ht = seg - seq * H;
+    const int kvh = static_cast<int>(plan.by_tiles.div(ht)), h0 = (ht - kvh * tiles) * C::kHeads;
     heads = min(C::kHeads, G - h0);
-    st.reset();
-    st.load_query(static_cast<const T *>(p.query) + (static_cast<int64_t>(seq) * p.num_q_heads + kvh * G + h0) * D,
-                  heads, p.scale_log2);
+    row = static_cast<int64_t>(seq) * p.num_q_heads + kvh * G + h0;
   };
   auto end_segment = [&](bool has_last, bool final) {
     st.finish();
     if (has_first && has_last) {
-      const int kvh = static_cast<int>(by_tiles.div(ht)), h0 = (ht - kvh * tiles) * C::kHeads;
-      st.write_out(static_cast<T *>(p.out) + (static_cast<int64_t>(seq) * p.num_q_heads + kvh * G + h0) * D, heads);
+      st.write_out(static_cast<T *>(p.out) + row * D, heads);
       return;
     }
     const int slot = 2 * warp + (final ? 1 : 0);
     st.write_state(final ? reinterpret_cast<float *>(ring) : heads_smem + warp * C::kState, heads);
     if (lane == 0) {
-      part_seg[slot] = seq * H + ht;
+      part_seg[slot] = segment;
       part_flags[slot] = (has_first ? 1 : 0) | (has_last ? 2 : 0);
     }
   };
+
+  // The first segment's q is asked for before the ring's copies, which would keep it waiting.
+  uint4 raw[CT][NB];
+  int issued = min(kStages, units);
+  if (units > 0) {
+    const Unit r = unit_of(min(lane, units - 1));
+    place(__shfl_sync(kAll, r.seq * H + r.ht, 0));
+    st.fetch_query(static_cast<const T *>(p.query) + row * D, heads, raw);
+    load_batch(lane, r);
+    issue(0, issued);
+    st.set_query(raw, p.scale_log2);
+  }
 
   bool timed_out = false, fresh = true;
   int stage = 0;
   uint32_t phase = 0;
 #pragma unroll 1
   for (int i = 0; i < units; ++i) {
-    if ((i & 31) == 0) load_batch(i + 32);  // the half that units i - 32 to i - 1 have left
+    if ((i & 31) == 0 && i + 32 < units)  // into the half that units i - 32 to i - 1 have left
+      load_batch(i + 32 + lane, unit_of(min(i + 32 + lane, units - 1)));
     const int4 unit = table[i & 63];
     if (i == 0 || (unit.z & 64)) {
-      start_segment(unit);
+      if (i > 0) {
+        place(unit.w);
+        st.fetch_query(static_cast<const T *>(p.query) + row * D, heads, raw);
+        st.set_query(raw, p.scale_log2);
+      }
+      has_first = (unit.z & 64) != 0;
+      st.reset();
       fresh = true;
     }
     if (!mbar_wait_bounded(&wbar[stage], phase, p.status)) {
@@ -798,22 +859,22 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
   __syncthreads();
 
   // ---- join the parts: runs of one segment over neighbouring warps ----
-  // Every warp sees the list of parts, one per lane.
+  // Every warp sees the list of parts, one per lane; in shared memory they are without gaps.
   static_assert(2 * kWarps <= 32, "one lane per part");
   const int my_seg = lane < 2 * kWarps ? part_seg[lane] : -1;
   const unsigned present = __ballot_sync(kAll, my_seg >= 0);
   const unsigned below = present & ((1u << lane) - 1u);
+  const int rank = __popc(below);
   const int prev_seg = __shfl_sync(kAll, my_seg, below ? 31 - __clz(below) : lane);
-  const bool begins = my_seg >= 0 && (below == 0 || prev_seg != my_seg);
-  const unsigned starts = __ballot_sync(kAll, begins);
+  const unsigned starts = __ballot_sync(kAll, my_seg >= 0 && (below == 0 || prev_seg != my_seg));
   const int my_flags = my_seg >= 0 ? part_flags[lane] : 0;
-  auto part = [&](int k) -> const float * {
-    return k & 1 ? reinterpret_cast<const float *>(smem + (k >> 1) * C::kRing) : heads_smem + (k >> 1) * C::kState;
-  };
-  // the parts' factors and sums: warp h takes query head h, lane k part k
+  const float *my_part = lane & 1 ? reinterpret_cast<const float *>(smem + (lane >> 1) * C::kRing)
+                                  : heads_smem + (lane >> 1) * C::kState;
+  if (warp == 0 && my_seg >= 0) part_at[rank] = static_cast<int>(my_part - reinterpret_cast<const float *>(smem));
+  // their factors and sums: warp h takes query head h
   for (int h = warp; h < C::kHeads; h += kWarps) {
     float m = -INFINITY, l = 0.f;
-    if (my_seg >= 0) m = part(lane)[C::kHeads * D + h], l = part(lane)[C::kHeads * D + C::kHeads + h];
+    if (my_seg >= 0) m = my_part[C::kHeads * D + h], l = my_part[C::kHeads * D + C::kHeads + h];
     for (unsigned left = starts; left; left &= left - 1) {
       const int k = __ffs(left) - 1;
       const unsigned later = left & (left - 1);
@@ -822,12 +883,11 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, off));
       const float f = mine ? part_factor(m, l, M) : 0.f;
-      float L = f * l;
-      if (!mine) L = 0.f;
+      float L = mine ? f * l : 0.f;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(kAll, L, off);
-      if (mine) factor[lane * C::kHeads + h] = f;
-      if (lane == k) run_ml[lane * C::kHeads + h] = make_float2(M, L);
+      if (mine) factor[rank * C::kHeads + h] = f;
+      if (lane == k) run_ml[rank * C::kHeads + h] = make_float2(M, L);
     }
   }
   __syncthreads();
@@ -838,29 +898,28 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
     const int k = __ffs(left) - 1;
     const unsigned later = left & (left - 1);
     const unsigned in_run = present & ~((1u << k) - 1u) & (later ? (1u << (__ffs(later) - 1)) - 1u : kAll);
-    const int seg = __shfl_sync(kAll, my_seg, k);
+    const int j0 = __popc(present & ((1u << k) - 1u)), j1 = j0 + __popc(in_run);
     const int flags = __reduce_or_sync(kAll, in_run >> lane & 1u ? my_flags : 0);
-    const int s = seg / H, h_t = seg - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * C::kHeads;
-    const int hs = min(C::kHeads, G - h0);
-    if (flags != 3) {
-      if (flags & 1) {  // goes on in later CTAs, up to the one that holds its last unit
-        const uint64_t last = static_cast<uint64_t>(prefix[s]) * H + static_cast<uint64_t>(h_t + 1) * (prefix[s + 1] - prefix[s]) - 1;
-        meta.segment = seg;
-        meta.parts = static_cast<int>(((last + 1) * gridDim.x - 1) / total) - static_cast<int>(blockIdx.x) + 1;
-      } else {
-        has_head = true;
-      }
+    place(__shfl_sync(kAll, my_seg, k));
+    if (flags == 1) {  // goes on in later CTAs, up to the one that holds its last unit
+      const int s = static_cast<int>(plan.by_segments.div(segment));
+      const uint32_t last = static_cast<uint32_t>(prefix[s]) * H +
+                            static_cast<uint32_t>(segment - s * H + 1) * (prefix[s + 1] - prefix[s]) - 1;
+      const uint32_t edge = over * (share + 1);  // units of the CTAs that take one more
+      const uint32_t cta = last < edge ? last / (share + 1) : over + (last - edge) / share;
+      meta.segment = segment;
+      meta.parts = static_cast<int>(cta - blockIdx.x) + 1;
     }
+    has_head |= !(flags & 1);
     float *state = flags & 1 ? ws + C::kState : ws;
-    T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
-    for (int e = threadIdx.x; e < hs * D; e += blockDim.x) {
+    T *out = static_cast<T *>(p.out) + row * D;
+    for (int e = threadIdx.x; e < heads * D; e += blockDim.x) {
       const int h = e / D;
-      const float2 ml = run_ml[k * C::kHeads + h];
+      const float2 ml = run_ml[j0 * C::kHeads + h];
       float A = 0.f;
-      for (unsigned w = in_run; w; w &= w - 1) {
-        const int j = __ffs(w) - 1;
-        A = fmaf(factor[j * C::kHeads + h], part(j)[e], A);
-      }
+#pragma unroll 4
+      for (int j = j0; j < j1; ++j)
+        A = fmaf(factor[j * C::kHeads + h], reinterpret_cast<const float *>(smem)[part_at[j] + e], A);
       if (flags == 3) {
         out[e] = Elem<T>::from_float(ml.y == 0.f ? 0.f : A / ml.y);
       } else {
@@ -877,7 +936,6 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
       ws[C::kHeads * D + C::kHeads + threadIdx.x] = 0.f;
     }
   }
-  pdl_launch_dependents();
 }
 
 // Segments that cross CTAs: block (c, h) joins query head h of the one that goes
@@ -885,54 +943,52 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1) mxfp4_decode_mm
 constexpr int kJoinWays = 4;
 template <typename T, int NB, int CT>
 __global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
-    mxfp4_decode_mma_join_kernel(const MxDecodeParams p, int tiles) {
+    mxfp4_decode_mma_join_kernel(const MxDecodeParams p, const MxPlan plan) {
   using C = MxCfg<NB, CT>;
   constexpr int D = C::D;
   __shared__ float sums[kJoinWays][D];
   __shared__ float ml[kJoinWays][2];
   pdl_wait();
+  pdl_launch_dependents();
   const int ctas = gridDim.x, first = blockIdx.x, h = blockIdx.y;
   const MxMeta meta =
       reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState)[first];
-  if (meta.segment >= 0) {
-    const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * tiles;
-    const int s = meta.segment / H, h_t = meta.segment - s * H, kvh = h_t / tiles, h0 = (h_t - kvh * tiles) * C::kHeads;
-    if (h0 + h < G) {  // uniform
-      const int d = threadIdx.x % D, way = threadIdx.x / D;
-      const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
-      const int parts = min(meta.parts, ctas - first);
-      auto part = [&](int k) { return base + (k == 0 ? 1 : 2 * k) * C::kState; };
-      float M = -INFINITY;
+  if (meta.segment < 0) return;
+  const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * plan.tiles;
+  const int s = static_cast<int>(plan.by_segments.div(meta.segment)), ht = meta.segment - s * H;
+  const int kvh = static_cast<int>(plan.by_tiles.div(ht)), h0 = (ht - kvh * plan.tiles) * C::kHeads;
+  if (h0 + h >= G) return;  // uniform
+  const int d = threadIdx.x % D, way = threadIdx.x / D;
+  const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
+  const int parts = min(meta.parts, ctas - first);
+  float M = -INFINITY, L = 0.f, A = 0.f;
+  // the first CTA's second state, then the others' first
 #pragma unroll 4
-      for (int k = way; k < parts; k += kJoinWays) M = fmaxf(M, __ldcg(part(k) + C::kHeads * D + h));
-      float L = 0.f, A = 0.f;
-#pragma unroll 4
-      for (int k = way; k < parts; k += kJoinWays) {
-        const float *x = part(k);
-        const float m = __ldcg(x + C::kHeads * D + h), l = __ldcg(x + C::kHeads * D + C::kHeads + h), a = __ldcg(x + h * D + d);
-        const float f = part_factor(m, l, M);
-        L += f * l;
-        if (f != 0.f) A = fmaf(f, a, A);  // a part without keys has no sums
-      }
-      sums[way][d] = A;
-      if (d == 0) ml[way][0] = M, ml[way][1] = L;
-      __syncthreads();
-      if (way == 0) {
-        M = -INFINITY, L = 0.f, A = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWays; ++w) M = fmaxf(M, ml[w][0]);
-#pragma unroll
-        for (int w = 0; w < kJoinWays; ++w) {
-          const float f = part_factor(ml[w][0], ml[w][1], M);
-          L += f * ml[w][1];
-          A = fmaf(f, sums[w][d], A);
-        }
-        static_cast<T *>(p.out)[(static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0 + h) * D + d] =
-            Elem<T>::from_float(L == 0.f ? 0.f : A / L);
-      }
-    }
+  for (int k = way; k < parts; k += kJoinWays) {
+    const float *x = base + (k == 0 ? 1 : 2 * k) * C::kState;
+    const float m = __ldcg(x + C::kHeads * D + h), l = __ldcg(x + C::kHeads * D + C::kHeads + h);
+    const float a = __ldcg(x + h * D + d);
+    if (m == -INFINITY && l == 0.f) continue;  // a part without keys has no sums
+    const float next = fmaxf(M, m), f = part_factor(M, L, next), e = part_factor(m, l, next);
+    L = f * L + e * l;
+    A = f * A + e * a;
+    M = next;
   }
-  pdl_launch_dependents();
+  sums[way][d] = A;
+  if (d == 0) ml[way][0] = M, ml[way][1] = L;
+  __syncthreads();
+  if (way != 0) return;
+  M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWays; ++w) M = fmaxf(M, ml[w][0]);
+#pragma unroll
+  for (int w = 0; w < kJoinWays; ++w) {
+    const float f = part_factor(ml[w][0], ml[w][1], M);
+    L += f * ml[w][1];
+    A = fmaf(f, sums[w][d], A);
+  }
+  static_cast<T *>(p.out)[(static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0 + h) * D + d] =
+      Elem<T>::from_float(L == 0.f ? 0.f : A / L);
 }
 
 template <typename T, int NB, int CT>
@@ -947,11 +1003,12 @@ cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, 
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_set[dev] = true;
   }
-  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(C::kWarps * 32), C::kSmem, stream, p, tiles,
-                             FastDiv(p.num_kv_heads * tiles), FastDiv(tiles), FastDiv(p.block_size / kMxGroup));
+  const MxPlan plan = {tiles, FastDiv(p.num_kv_heads * tiles), FastDiv(tiles), FastDiv(p.block_size / kMxGroup),
+                       FastDiv(ctas)};
+  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(C::kWarps * 32), C::kSmem, stream, p, plan);
   if (e == cudaSuccess && join)
     e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB, CT>,
-                   dim3(ctas, std::min<int>(C::kHeads, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, tiles);
+                   dim3(ctas, std::min<int>(C::kHeads, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, plan);
   return e;
 }
 
