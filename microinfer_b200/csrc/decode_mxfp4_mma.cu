@@ -155,6 +155,20 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// Both halves of a times the low (HIGH: high) half of b.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t mul_f16x2_half(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (HIGH)
+    asm("{ .reg .b16 l, h; .reg .b32 x; mov.b32 {l, h}, %2; mov.b32 x, {h, h}; mul.rn.f16x2 %0, %1, x; }"
+        : "=r"(r)
+        : "r"(a), "r"(b));
+  else
+    asm("{ .reg .b16 l, h; .reg .b32 x; mov.b32 {l, h}, %2; mov.b32 x, {l, l}; mul.rn.f16x2 %0, %1, x; }"
+        : "=r"(r)
+        : "r"(a), "r"(b));
+  return r;
+}
 // 2^e for any e, through two factors where one has no normal exponent.
 __device__ __forceinline__ float exp2i(int e) {
   const int a = max(-126, min(127, e)), b = max(-126, min(127, e - a));
@@ -218,14 +232,13 @@ struct MxWarp {
   float o[CT][NB][4];         // query t, dims 32b + 4g + 0 to 3, times 2^(R_b - 127)
   float m[CT], l[CT];         // query t; l: this lane's keys only
   uint32_t ref;               // R_b, one byte per block
-  uint32_t one, unit0, unit1; // f16 1.0 and minus the places of d's bits in the half of this lane's column
+  uint32_t pick0, pick1;      // byte selectors: a pair's first (second) half to this lane's column, zeros
   int lane, g, t;
 
   __device__ __forceinline__ void setup(uint32_t query_smem) {
     lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     q = query_smem + lane * 16;
-    const int shift = g & 1 ? 16 : 0;
-    one = 0x3c00u << shift, unit0 = 0u - (1u << (10 + shift)), unit1 = 0u - (1u << (2 + shift));
+    pick0 = g & 1 ? 0x1044u : 0x4410u, pick1 = g & 1 ? 0x3244u : 0x4432u;
   }
 
   __device__ __forceinline__ void reset() {
@@ -351,36 +364,48 @@ struct MxWarp {
   }
 
   // O += P_b V of a group.  d: distances per byte, 0 to 7, or 15 for no contribution (2^-15 has the f16
-  // exponent 0: zero); p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in both halves.  FAR: the
-  // products are `back` times what d says.
+  // exponent 0: zero); p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in the half of this lane's
+  // column, zero in the other.  FAR: the products are `back` times what d says.
   template <bool FAR>
   __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[CT][4],
                                          float back = 1.f) {
     uint32_t lo[NB], hi[NB];
     load_codes<NB, true>(vbase, lane, lo, hi);
+    // f16 2^-d, two to a word: bytes 0 and 2 of d's word k, then bytes 1 and 3
+    uint32_t even[4], odd[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (NB == 2 && (k & 1)) continue;
+      even[k] = 0x3c003c00u - (d[k] & 0x00ff00ffu) * 1024u;
+      odd[k] = 0x3c003c00u - (d[k] & 0xff00ff00u) * 4u;
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      uint32_t f[4];  // 2^-d in the half of this lane's column, zero in the other
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // bytes of blocks (b & ~1) and (b | 1) in the low half of the word
-        const uint32_t word = NB == 4 ? (b < 2 ? d[k] : d[k] >> 16) : (k & 1 ? d[k & 2] >> 16 : d[k & 2]);
-        f[k] = b & 1 ? (word & 0xff00u) * unit1 + one : (word & 0xffu) * unit0 + one;
-      }
       uint32_t a[4], e[4];
       mx_codes_to_f16(lo[b], a);
       mx_codes_to_f16(hi[b], e);
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
+        uint32_t s[4];  // p times the scale of V's block b
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (NB == 4) {
+            const uint32_t f = b & 1 ? odd[k] : even[k];
+            s[k] = b < 2 ? mul_f16x2_half<false>(p[c][k], f) : mul_f16x2_half<true>(p[c][k], f);
+          } else {
+            const uint32_t f = b & 1 ? odd[k & 2] : even[k & 2];
+            s[k] = k & 1 ? mul_f16x2_half<true>(p[c][k], f) : mul_f16x2_half<false>(p[c][k], f);
+          }
+        }
         if constexpr (FAR) {
           float r[4];
-          mma_f16_zero(r, a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
-          mma_f16(r, e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+          mma_f16_zero(r, a[0], a[1], a[2], a[3], s[0], s[1]);
+          mma_f16(r, e[0], e[1], e[2], e[3], s[2], s[3]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[c][b][i] = fmaf(r[i], back, o[c][b][i]);
         } else {
-          mma_f16(o[c][b], a[0], a[1], a[2], a[3], mul_f16x2(p[c][0], f[0]), mul_f16x2(p[c][1], f[1]));
-          mma_f16(o[c][b], e[0], e[1], e[2], e[3], mul_f16x2(p[c][2], f[2]), mul_f16x2(p[c][3], f[3]));
+          mma_f16(o[c][b], a[0], a[1], a[2], a[3], s[0], s[1]);
+          mma_f16(o[c][b], e[0], e[1], e[2], e[3], s[2], s[3]);
         }
       }
     }
@@ -445,27 +470,27 @@ struct MxWarp {
     }
   }
 
-  // One unit: K of its two groups at `base`, then V of both; `valid` of its 32 keys exist;
-  // `first`: the state holds none yet.
-  __device__ __forceinline__ void process(uint32_t base, int valid, bool first) {
+  // One unit: K of its two groups at `base`, then V of both; `valid` of its 32 keys exist; `special`:
+  // that may be fewer than 32, or it is the `first` that the state meets.
+  __device__ __forceinline__ void process(uint32_t base, bool special, int valid, bool first) {
     const uint32_t vbase = base + 2 * C::kGroup;
     float x[2][CT][2];
     scores(base, x);
     uint32_t w[2][4];
     load_scales<NB>(vbase, t, w[0]);
     load_scales<NB>(vbase + C::kGroup, t, w[1]);
-    if (first) {  // uniform: R_b starts at the largest scale here and two binades of room
-      mask_scales(w[0], valid, 0);
-      mask_scales(w[1], valid - kMxGroup, 0);
-      const uint32_t top = __vmaxu4(over_keys(w[0][0], w[0][1], w[0][2], w[0][3]),
-                                    over_keys(w[1][0], w[1][1], w[1][2], w[1][3]));
-      ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
-    }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int c = 0; c < CT; ++c) x[j][c][0] *= xs[c], x[j][c][1] *= xs[c];
-    if (valid < kUnit) {  // uniform: the last unit of a segment
+    if (special) {  // uniform
+      if (first) {  // R_b starts at the largest scale here and two binades of room
+        mask_scales(w[0], valid, 0);
+        mask_scales(w[1], valid - kMxGroup, 0);
+        const uint32_t top = __vmaxu4(over_keys(w[0][0], w[0][1], w[0][2], w[0][3]),
+                                      over_keys(w[1][0], w[1][1], w[1][2], w[1][3]));
+        ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -509,8 +534,8 @@ struct MxWarp {
         l[c] += p0 + p1;
         // rows (keys) x columns (each query twice), transposed: keys 2t and 2t + 1 of query g / 2
         const uint32_t k0 = movm(pack_f16(p0, p0)), k8 = movm(pack_f16(p1, p1));
-        p[j][c][0] = __byte_perm(k0, 0, 0x1010), p[j][c][1] = __byte_perm(k0, 0, 0x3232);
-        p[j][c][2] = __byte_perm(k8, 0, 0x1010), p[j][c][3] = __byte_perm(k8, 0, 0x3232);
+        p[j][c][0] = __byte_perm(k0, 0, pick0), p[j][c][1] = __byte_perm(k0, 0, pick1);
+        p[j][c][2] = __byte_perm(k8, 0, pick0), p[j][c][3] = __byte_perm(k8, 0, pick1);
       }
     }
     uint32_t d[2][4];
@@ -698,9 +723,13 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   const int units = static_cast<int>(cta_units * (warp + 1) / kWarps - cta_units * warp / kWarps);
   u0 += cta_units * warp / kWarps;
 
-  // Batches of 32 units, one per lane, in shared memory: x, y, the indices of the unit's two groups
-  // in the pools (-1: no such page, or no such keys); z, its keys (bits 0-5) and whether it is its
-  // segment's first (64) or last (128) unit; w, its segment.
+  // Batches of 32 units, one per lane, in shared memory: x, y, the indices of the unit's two groups in
+  // the pools (0 where there is none: every unit brings two); z, its keys (bits 0-5) and flags; w, its segment.
+  constexpr int kStarts = 64;   // the warp's first unit of its segment
+  constexpr int kEnds = 128;    // its last
+  constexpr int kFirst = 256;   // the segment's first unit
+  constexpr int kLast = 512;    // the segment's last
+  constexpr int kNoPage = 1024; // a page that is none: flagged, left out
   const int per_page = p.block_size / kMxGroup;
   int4 *table = unit_table + warp * 64;
   struct Unit {
@@ -729,54 +758,48 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   };
   auto load_batch = [&](int i, const Unit &r) {
     if (i < units) {
-      int valid = kUnit, flags = r.unit == 0 ? 64 : 0;
+      int valid = kUnit, flags = 0;
+      if (r.unit == 0) flags |= kStarts | kFirst;
+      if (i == 0) flags |= kStarts;
+      if (i == units - 1) flags |= kEnds;
       if (r.unit == r.count - 1) {
         const int ctx = static_cast<int>(min(static_cast<int64_t>(__ldg(p.context_lens + r.seq)), cap));
         valid = ctx - r.unit * kUnit;
-        flags |= 128;
+        flags |= kEnds | kLast;
       }
       const int32_t *row = p.block_tables + static_cast<int64_t>(r.seq) * p.bt_stride;
       const int kvh = static_cast<int>(plan.by_tiles.div(r.ht));
-      int where[2] = {-1, -1};
+      int where[2] = {0, 0};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j * kMxGroup >= valid) break;
         const int group = 2 * r.unit + j, col = static_cast<int>(plan.by_page.div(group));
         const int page = __ldg(row + col);
-        if (page >= 0 && page < p.num_blocks)
+        if (page >= 0 && page < p.num_blocks) {
           where[j] = (page * p.num_kv_heads + kvh) * per_page + group - col * per_page;
-        else
+        } else {
           flag_status(p.status, MI_DEV_BAD_BLOCK);
+          flags |= kNoPage;
+        }
       }
       table[i & 63] = make_int4(where[0], where[1], valid | flags, r.seq * H + r.ht);
     }
     __syncwarp();
   };
-  // Lanes 4s to 4s + 3 bring unit first + s: K (0, 1) and V (2, 3) of its groups, both at once where
-  // they are neighbours.
-  auto issue = [&](int first, int count) {
-    const int i = first + (lane >> 2);
-    int where = -1, bytes = C::kGroup;
-    uint64_t *bar = &wbar[i % kStages];
-    if ((lane >> 2) < count) {
-      const int4 unit = table[i & 63];
-      where = lane & 1 ? unit.y : unit.x;
-      if (unit.x >= 0 && unit.y == unit.x + 1) {
-        if (lane & 1) where = -1;
-        bytes = 2 * C::kGroup;
-      }
-      if ((lane & 3) == 0) {
-        const int groups = (unit.x >= 0) + (unit.y >= 0);
-        if (groups)
-          mbar_arrive_expect_tx(bar, groups * 2 * C::kGroup);
-        else
-          mbar_arrive(bar);
-      }
-    }
-    __syncwarp();
-    if (where >= 0)
-      bulk_g2s(ring + i % kStages * C::kStage + ((lane >> 1) & 1) * 2 * C::kGroup + (lane & 1) * C::kGroup,
-               (lane & 2 ? p.value_pages : p.key_pages) + static_cast<int64_t>(where) * C::kGroup, bytes, bar);
+  // Lanes 4s to 4s + 3 bring unit first + s: K (lanes 0, 1) and V (2, 3) of its groups.
+  const uint8_t *my_pages = lane & 2 ? p.value_pages : p.key_pages;
+  const uint32_t my_place = smem_addr(ring) + (lane & 3) * C::kGroup;
+  const uint32_t my_bar = smem_addr(wbar);
+  auto issue = [&](int i, int at) {  // unit i to stage `at`, by four lanes
+    if ((lane & 3) == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(my_bar + at * 8), "r"(C::kStage)
+                   : "memory");
+    const int where = reinterpret_cast<const int *>(table + (i & 63))[lane & 1];
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            my_place + at * C::kStage),
+        "l"(my_pages + static_cast<int64_t>(where) * C::kGroup), "r"(C::kGroup), "r"(my_bar + at * 8)
+        : "memory");
   };
 
   MxWarp<T, NB, CT> st;
@@ -807,52 +830,55 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
 
   // The first segment's q is asked for before the ring's copies, which would keep it waiting.
   uint4 raw[CT][NB];
-  int issued = min(kStages, units);
+  const int ahead = min(kStages, units);
   if (units > 0) {
     const Unit r = unit_of(min(lane, units - 1));
     place(__shfl_sync(kAll, r.seq * H + r.ht, 0));
     st.fetch_query(static_cast<const T *>(p.query) + row * D, heads, raw);
     load_batch(lane, r);
-    issue(0, issued);
+    if ((lane >> 2) < ahead) issue(lane >> 2, lane >> 2);
+    __syncwarp();
     st.set_query(raw, p.scale_log2);
   }
 
   bool timed_out = false, fresh = true;
-  int stage = 0;
+  int stage = 0, stop = 0;
   uint32_t phase = 0;
 #pragma unroll 1
   for (int i = 0; i < units; ++i) {
     if ((i & 31) == 0 && i + 32 < units)  // into the half that units i - 32 to i - 1 have left
       load_batch(i + 32 + lane, unit_of(min(i + 32 + lane, units - 1)));
     const int4 unit = table[i & 63];
-    if (i == 0 || (unit.z & 64)) {
+    const int what = unit.z;
+    if (what & kStarts) {
       if (i > 0) {
         place(unit.w);
         st.fetch_query(static_cast<const T *>(p.query) + row * D, heads, raw);
         st.set_query(raw, p.scale_log2);
       }
-      has_first = (unit.z & 64) != 0;
+      has_first = (what & kFirst) != 0;
       st.reset();
       fresh = true;
     }
     if (!mbar_wait_bounded(&wbar[stage], phase, p.status)) {
       timed_out = true;
+      stop = i;
       break;
     }
-    const int valid = unit.z & 63;
-    if (unit.x >= 0 && (unit.y >= 0 || valid <= kMxGroup)) {  // else flagged: left out
-      st.process(smem_addr(ring + stage * C::kStage), valid, fresh);
+    const bool special = what != kUnit || fresh;
+    if (!(what & kNoPage)) {
+      st.process(smem_addr(ring) + stage * C::kStage, special, what & 63, fresh);
       fresh = false;
     }
     __syncwarp();  // every lane has read the stage
-    const bool final = i == units - 1;
-    if (issued < units) issue(issued++, 1);
-    if ((unit.z & 128) || final) end_segment((unit.z & 128) != 0, final);
+    if (i + kStages < units && lane < 4) issue(i + kStages, stage);
+    __syncwarp();
+    if (what & kEnds) end_segment((what & kLast) != 0, i == units - 1);
     if (++stage == kStages) stage = 0, phase ^= 1;
   }
   if (timed_out) {  // the copies in flight land before the ring is given up
     if (lane == 0)
-      for (int k = max(0, issued - kStages); k < issued; ++k)
+      for (int k = stop; k < min(stop + kStages, units); ++k)
         if (!mbar_wait_bounded(&wbar[k % kStages], (k / kStages) & 1, p.status)) break;
     __syncwarp();
   }
