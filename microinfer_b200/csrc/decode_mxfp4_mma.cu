@@ -37,7 +37,6 @@
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
 // segment and the second launch has nothing to do.
-#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -148,11 +147,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // Both halves of a times the low (HIGH: high) half of b.
@@ -964,57 +958,92 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   }
 }
 
-// Segments that cross CTAs: block (c, h) joins query head h of the one that goes
-// on from CTA c.  A thread takes one element; the quarters of the block take every fourth part.
+// Segments that cross CTAs: block c joins the one that goes on from CTA c.  A thread takes 4 elements;
+// the quarters of the block take every fourth part.  The first four parts are read while
+// the block is still finding out whether they are any.  (Joining in the first launch, by the
+// CTA that arrives last, took longer: its fences and the atomic cost 5 us at 1 x 131072, this launch 4.)
 constexpr int kJoinWays = 4;
+constexpr int kJoinLanes = 128;
 template <typename T, int NB, int CT>
-__global__ void __launch_bounds__(NB * kMxBlock * kJoinWays)
+__global__ void __launch_bounds__(kJoinLanes * kJoinWays)
     mxfp4_decode_mma_join_kernel(const MxDecodeParams p, const MxPlan plan) {
   using C = MxCfg<NB, CT>;
-  constexpr int D = C::D;
-  __shared__ float sums[kJoinWays][D];
-  __shared__ float ml[kJoinWays][2];
+  constexpr int D = C::D, kVecs = C::kHeads * D / 4;
+  constexpr int kPer = (kVecs + kJoinLanes - 1) / kJoinLanes;
+  __shared__ float4 sums[kJoinWays][kVecs];
+  __shared__ float2 ml[kJoinWays][C::kHeads];
+  const int ctas = gridDim.x, first = blockIdx.x;
+  const int lane = threadIdx.x % kJoinLanes, way = threadIdx.x / kJoinLanes;
+  const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
+  struct Part {
+    float m[kPer], l[kPer];
+    float4 a[kPer];
+  };
+  auto read = [&](int k, Part &x) {  // k = 0: the first CTA's second state, then the others' first
+    const float *st = base + (k == 0 ? 1 : 2 * k) * C::kState;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int v = lane + i * kJoinLanes;
+      if (v >= kVecs) break;
+      x.m[i] = __ldcg(st + C::kHeads * D + v * 4 / D);
+      x.l[i] = __ldcg(st + C::kHeads * D + C::kHeads + v * 4 / D);
+      x.a[i] = __ldcg(reinterpret_cast<const float4 *>(st) + v);
+    }
+  };
   pdl_wait();
   pdl_launch_dependents();
-  const int ctas = gridDim.x, first = blockIdx.x, h = blockIdx.y;
   const MxMeta meta =
       reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState)[first];
+  Part x;
+  if (first + way < ctas) read(way, x);
   if (meta.segment < 0) return;
+  const int parts = min(meta.parts, ctas - first);
+  float M[kPer], L[kPer];
+  float4 A[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) M[i] = -INFINITY, L[i] = 0.f, A[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = way; k < parts; k += kJoinWays) {
+    Part y;
+    if (k + kJoinWays < parts) read(k + kJoinWays, y);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (lane + i * kJoinLanes >= kVecs) break;
+      if (x.m[i] == -INFINITY && x.l[i] == 0.f) continue;  // a part without keys has no sums
+      const float next = fmaxf(M[i], x.m[i]);
+      const float f = part_factor(M[i], L[i], next), e = part_factor(x.m[i], x.l[i], next);
+      L[i] = f * L[i] + e * x.l[i];
+      A[i].x = f * A[i].x + e * x.a[i].x, A[i].y = f * A[i].y + e * x.a[i].y;
+      A[i].z = f * A[i].z + e * x.a[i].z, A[i].w = f * A[i].w + e * x.a[i].w;
+      M[i] = next;
+    }
+    x = y;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int v = lane + i * kJoinLanes;
+    if (v >= kVecs) break;
+    sums[way][v] = A[i];
+    if (v * 4 % D == 0) ml[way][v * 4 / D] = make_float2(M[i], L[i]);
+  }
+  __syncthreads();
   const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * plan.tiles;
   const int s = static_cast<int>(plan.by_segments.div(meta.segment)), ht = meta.segment - s * H;
   const int kvh = static_cast<int>(plan.by_tiles.div(ht)), h0 = (ht - kvh * plan.tiles) * C::kHeads;
-  if (h0 + h >= G) return;  // uniform
-  const int d = threadIdx.x % D, way = threadIdx.x / D;
-  const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
-  const int parts = min(meta.parts, ctas - first);
-  float M = -INFINITY, L = 0.f, A = 0.f;
-  // the first CTA's second state, then the others' first
-#pragma unroll 4
-  for (int k = way; k < parts; k += kJoinWays) {
-    const float *x = base + (k == 0 ? 1 : 2 * k) * C::kState;
-    const float m = __ldcg(x + C::kHeads * D + h), l = __ldcg(x + C::kHeads * D + C::kHeads + h);
-    const float a = __ldcg(x + h * D + d);
-    if (m == -INFINITY && l == 0.f) continue;  // a part without keys has no sums
-    const float next = fmaxf(M, m), f = part_factor(M, L, next), e = part_factor(m, l, next);
-    L = f * L + e * l;
-    A = f * A + e * a;
-    M = next;
-  }
-  sums[way][d] = A;
-  if (d == 0) ml[way][0] = M, ml[way][1] = L;
-  __syncthreads();
-  if (way != 0) return;
-  M = -INFINITY, L = 0.f, A = 0.f;
+  const int heads = min(C::kHeads, G - h0);
+  T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
+  for (int e = threadIdx.x; e < heads * D; e += kJoinLanes * kJoinWays) {
+    const int h = e / D;
+    float m = -INFINITY, l = 0.f, a = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWays; ++w) M = fmaxf(M, ml[w][0]);
+    for (int w = 0; w < kJoinWays; ++w) m = fmaxf(m, ml[w][h].x);
 #pragma unroll
-  for (int w = 0; w < kJoinWays; ++w) {
-    const float f = part_factor(ml[w][0], ml[w][1], M);
-    L += f * ml[w][1];
-    A = fmaf(f, sums[w][d], A);
+    for (int w = 0; w < kJoinWays; ++w) {
+      const float f = part_factor(ml[w][h].x, ml[w][h].y, m);
+      l += f * ml[w][h].y;
+      a = fmaf(f, reinterpret_cast<const float *>(sums[w])[e], a);
+    }
+    out[e] = Elem<T>::from_float(l == 0.f ? 0.f : a / l);
   }
-  static_cast<T *>(p.out)[(static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0 + h) * D + d] =
-      Elem<T>::from_float(L == 0.f ? 0.f : A / L);
 }
 
 template <typename T, int NB, int CT>
@@ -1033,8 +1062,8 @@ cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, 
                        FastDiv(ctas)};
   cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(C::kWarps * 32), C::kSmem, stream, p, plan);
   if (e == cudaSuccess && join)
-    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB, CT>,
-                   dim3(ctas, std::min<int>(C::kHeads, p.num_q_heads / p.num_kv_heads)), dim3(C::D * kJoinWays), 0, stream, p, plan);
+    e = launch_pdl(mxfp4_decode_mma_join_kernel<T, NB, CT>, dim3(ctas), dim3(kJoinLanes * kJoinWays), 0, stream, p,
+                   plan);
   return e;
 }
 
