@@ -62,7 +62,7 @@ constexpr int kAlignedSlack = 1;    // units per warp that keeping a segment in 
 template <int NB, int CT>
 struct MxCfg {
   static constexpr int D = NB * kMxBlock;
-  static constexpr int kWarps = CT == 1 ? 16 : 12;
+  static constexpr int kWarps = CT == 1 || NB == 2 ? 16 : 12;
   static constexpr int kStages = 2;
   static constexpr int kHeads = CT * kQueries;    // query heads of a segment
   static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
@@ -621,7 +621,6 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   const int tiles = plan.tiles, H = p.num_kv_heads * tiles;  // segments of a sequence
 
   pdl_wait();
-  pdl_launch_dependents();  // dependents wait for this grid's end; their blocks may come as its own leave
 
   // ---- units of each sequence, their prefix sums and largest ----
   const int64_t cap = p.bt_stride * p.block_size;
@@ -956,6 +955,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
       ws[C::kHeads * D + C::kHeads + threadIdx.x] = 0.f;
     }
   }
+  pdl_launch_dependents();
 }
 
 // Segments that cross CTAs: block c joins the one that goes on from CTA c.  A thread takes 4 elements;
@@ -1078,7 +1078,7 @@ int mma_tiles(int num_q_heads, int num_kv_heads) {
 // every segment has a CTA and a full table is no more than the slack per warp.
 bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t capacity, int sms) {
   const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads);
-  const int warps = mma_columns(num_q_heads, num_kv_heads) == 1 ? MxCfg<4, 1>::kWarps : MxCfg<4, 2>::kWarps;
+  constexpr int warps = MxCfg<4, 2>::kWarps;  // the fewest
   return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * warps * kUnit;
 }
 
