@@ -83,20 +83,6 @@ struct MxCfg {
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
-// n / d by a multiplication, n below 2^31.
-struct FastDiv {
-  uint32_t mul;
-  int shift;
-  explicit FastDiv(uint32_t d) {
-    shift = 31;
-    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
-    mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    return static_cast<uint32_t>(static_cast<uint64_t>(n) * mul >> shift);
-  }
-};
-
 // Launch constants: tiles of a kv head (segments), and divisions by what the host knows.
 struct MxPlan {
   int tiles;

@@ -25,6 +25,20 @@ __host__ __device__ constexpr int mx_group_bytes(int head_dim) {
   return head_dim / kMxBlock * kMxBytes;
 }
 
+// n / d by a multiplication, n below 2^31.
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+  explicit FastDiv(uint32_t d) {
+    shift = 31;
+    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
+    mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    return static_cast<uint32_t>(static_cast<uint64_t>(n) * mul >> shift);
+  }
+};
+
 // Byte offset of the group that holds `slot` (block * block_size + offset) of kv head h.
 __device__ __forceinline__ int64_t mx_group_offset(int64_t slot, int h, int block_size, int num_kv_heads,
                                                    int head_dim) {
@@ -61,7 +75,7 @@ __device__ __forceinline__ void mx_codes_to_f32(uint32_t w, float scale, float (
   }
 }
 
-// Two floats -> one byte of two codes (lo in the low nibble): round to
+// Four floats -> 16 bits of codes (a in the lowest nibble), twice: round to
 // nearest, ties to even, saturating at 6.
 __device__ __forceinline__ uint32_t mx_encode4(float a, float b, float c, float d) {
   uint32_t r;

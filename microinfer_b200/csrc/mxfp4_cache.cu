@@ -6,15 +6,17 @@
 // nearest e2m1 value (ties to even, saturating at 6).  The division by a power
 // of two is exact, so codes and scales do not depend on the order of any sum.
 // A zero block has the byte 0, a block with an infinity or a NaN the byte 255.
-// Four lanes hold a block (8 elements each, one 16-byte load of a 16-bit
-// type), two shuffles give a.  Reads 2 or 4 bytes per element and writes 4.25 bits:
-// HBM-bound on the read.
+// A warp takes 8 consecutive tokens of one kv head, four lanes to a token: a lane loads
+// 8 elements of every block of K and V before it uses any, two shuffles give a
+// block's a, and the tokens' codes of one block are 128 consecutive bytes, their scales 32 (at
+// D = 128) where the slots are consecutive.  Reads 2 or 4 bytes per element and writes 4.25
+// bits: HBM-bound on the read.
 //
 // Gather: rows of each request in logical order, request-major, as
 // code * scale in the requested type (exact in fp32 and bf16 short of
-// overflow; fp16 rounds).  One warp per group of 16 tokens and kv head; a lane
-// reads 4 bytes of codes (8 elements, 128 consecutive bytes per warp load) and writes
-// them as one or two 16-byte vectors.  HBM-bound on the rows that it writes.
+// overflow; fp16 rounds).  A warp takes a group of 16 positions of one kv head, four lanes to a token as
+// above; the heads of a group go to neighbouring warps, which write whole rows
+// together.  HBM-bound on the rows that it writes.
 #include <type_traits>
 
 #include "common.cuh"
@@ -42,55 +44,96 @@ __device__ __forceinline__ void load8(const T *src, float (&x)[8]) {
   }
 }
 
-// Quantise 8 of a block's 32 elements (the quad's lanes hold the rest) and
-// write their codes; lane 0 of the quad writes the scale.
-__device__ __forceinline__ void store8(const float (&x)[8], uint32_t quad, int j, uint8_t *codes,
-                                       uint8_t *scale) {
+// Quantise 8 of a block's 32 elements (the quad's other lanes hold the rest); returns the codes, `byte`
+// the block's scale.
+__device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t &byte) {
   uint32_t top = 0;  // largest magnitude as bits: orders like the floats, NaN above infinity
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(quad, top, 1));
-  top = max(top, __shfl_xor_sync(quad, top, 2));
-  uint32_t byte = top >> 23;
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  byte = top >> 23;
   byte = byte > 3 ? byte - 2 : 1;  // the lowest scale is 2^-126
   const float inv = __uint_as_float((254u - byte) << 23);
   uint32_t w = mx_encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv) & 0xffffu;
   w |= mx_encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv) << 16;
   if (top == 0) byte = 0;
   if (top >= 0x7f800000u) byte = 255, w = 0;
-  *reinterpret_cast<uint32_t *>(codes + j * 4) = w;
-  if (j == 0) *scale = static_cast<uint8_t>(byte);
+  return w;
 }
 
-// block (bx, by): x walks the row's 8-element vectors, y the tokens.
-template <typename T, typename I, bool VEC>
-__global__ void __launch_bounds__(256) mxfp4_store_kernel(const MxStoreParams p) {
+// Blocks of a head: the template's, or at run time where that is 0.
+template <int NB>
+__device__ __forceinline__ int blocks_of(int head_dim) {
+  return NB > 0 ? NB : head_dim / kMxBlock;
+}
+
+// One warp per (8 tokens, kv head).  WIDE: slots past 32 bits.
+template <typename T, typename I, bool VEC, int NB, bool WIDE>
+__global__ void __launch_bounds__(128) mxfp4_store_kernel(const MxStoreParams p, const FastDiv by_heads,
+                                                          const FastDiv by_block) {
   pdl_wait();
-  const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31;
-  const uint32_t quad = 0xfu << (lane & ~3);
-  const int per_head = p.head_dim / 8;
-  const int vecs = p.num_kv_heads * per_head;
-  const int nb = p.head_dim / kMxBlock;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.num_tokens;
-       t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    const int64_t slot = static_cast<int64_t>(static_cast<const I *>(p.slots)[t]);
-    if (slot < 0 || slot >= p.num_slots) {
-      if (slot != -1 && threadIdx.x == 0) flag_status(p.status, MI_DEV_BAD_SLOT);
-      continue;  // every lane of a quad holds the same token
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const uint32_t task = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const uint32_t chunk = by_heads.div(task);
+  const int h = static_cast<int>(task - chunk * p.num_kv_heads);
+  const int64_t t = static_cast<int64_t>(chunk) * 8 + (lane >> 2);
+  const int nb = blocks_of<NB>(p.head_dim);
+  int64_t slot = -1;
+  if (t < p.num_tokens) slot = static_cast<int64_t>(static_cast<const I *>(p.slots)[t]);
+  if (slot < -1 || slot >= p.num_slots) {
+    if (j == 0 && h == 0) flag_status(p.status, MI_DEV_BAD_SLOT);
+    slot = -1;
+  }
+  const T *krow = static_cast<const T *>(p.keys) + t * p.key_stride + h * p.head_dim + j * 8;
+  const T *vrow = static_cast<const T *>(p.values) + t * p.value_stride + h * p.head_dim + j * 8;
+  int64_t page, offset;
+  if constexpr (WIDE) {
+    page = (slot < 0 ? 0 : slot) / p.block_size;
+    offset = (slot < 0 ? 0 : slot) - page * p.block_size;
+  } else {
+    const uint32_t s = slot < 0 ? 0 : static_cast<uint32_t>(slot);
+    page = by_block.div(s);
+    offset = s - static_cast<uint32_t>(page) * p.block_size;
+  }
+  const int tok = static_cast<int>(offset % kMxGroup);
+  const int64_t group = ((page * p.num_kv_heads + h) * (p.block_size / kMxGroup) + offset / kMxGroup) *
+                        (nb * kMxBytes);
+  uint8_t *kg = p.key_pages + group, *vg = p.value_pages + group;
+  constexpr int kAhead = NB > 0 ? NB : 1;  // blocks loaded before any is used
+  for (int b0 = 0; b0 < nb; b0 += kAhead) {
+    float k8[kAhead][8], v8[kAhead][8];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) k8[i][u] = v8[i][u] = 0.f;
+      if (slot >= 0) {
+        load8<T, VEC>(krow + (b0 + i) * kMxBlock, k8[i]);
+        load8<T, VEC>(vrow + (b0 + i) * kMxBlock, v8[i]);
+      }
     }
-    const T *krow = static_cast<const T *>(p.keys) + t * p.key_stride;
-    const T *vrow = static_cast<const T *>(p.values) + t * p.value_stride;
-    const int tok = static_cast<int>(slot % kMxGroup);  // block_size is a multiple of the group
-    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-      float k8[8], v8[8];
-      load8<T, VEC>(krow + v * 8, k8);
-      load8<T, VEC>(vrow + v * 8, v8);
-      const int h = v / per_head, in_head = v - h * per_head;
-      const int b = in_head >> 2, j = in_head & 3;
-      const int64_t group = mx_group_offset(slot, h, p.block_size, p.num_kv_heads, p.head_dim);
-      const int code = b * kMxBlockBytes + tok * 16, scale = nb * kMxBlockBytes + tok * nb + b;
-      store8(k8, quad, j, p.key_pages + group + code, p.key_pages + group + scale);
-      store8(v8, quad, j, p.value_pages + group + code, p.value_pages + group + scale);
+    uint64_t ks = 0, vs = 0;  // scale bytes of the blocks
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      uint32_t byte;
+      const uint32_t kw = encode8(k8[i], byte);
+      ks |= static_cast<uint64_t>(byte) << (8 * i);
+      const uint32_t vw = encode8(v8[i], byte);
+      vs |= static_cast<uint64_t>(byte) << (8 * i);
+      if (slot < 0) continue;
+      const int at = (b0 + i) * kMxBlockBytes + tok * 16 + j * 4;
+      *reinterpret_cast<uint32_t *>(kg + at) = kw;
+      *reinterpret_cast<uint32_t *>(vg + at) = vw;
+    }
+    if (slot < 0 || j > 1) continue;
+    uint8_t *to = (j ? vg : kg) + nb * kMxBlockBytes + tok * nb + b0;  // lane 0 writes K's, lane 1 V's
+    const uint64_t bytes = j ? vs : ks;
+    if constexpr (NB == 4) {
+      *reinterpret_cast<uint32_t *>(to) = static_cast<uint32_t>(bytes);
+    } else if constexpr (NB == 2) {
+      *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(bytes);
+    } else {
+      *to = static_cast<uint8_t>(bytes);
     }
   }
   pdl_launch_dependents();
@@ -111,64 +154,97 @@ __device__ __forceinline__ void write8(T *dst, const float (&x)[8]) {
 }
 
 // grid (groups of 16 positions x kv heads, 8 warps to a CTA; sequences).
-template <typename T>
-__global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams p) {
+template <typename T, int NB>
+__global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams p, const FastDiv by_heads,
+                                                           const FastDiv by_page) {
   pdl_wait();
-  const int64_t seq = blockIdx.y;
+  const int seq = blockIdx.y;
   const int64_t base = p.cu_seqlens_k[seq];
   const int64_t ctx = p.cu_seqlens_k[seq + 1] - base;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + warp;
-  const int64_t g = unit / p.num_kv_heads;
-  const int h = static_cast<int>(unit - g * p.num_kv_heads);
-  const int64_t pos0 = g * kMxGroup;
-  if (pos0 < ctx) {
-    const int64_t col = pos0 / p.block_size;
-    const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
-    if (blk < 0 || blk >= p.num_blocks) {
-      if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
-    } else {
-      const int nb = p.head_dim / kMxBlock;
-      const int64_t off =
-          mx_group_offset(blk * p.block_size + pos0 % p.block_size, h, p.block_size, p.num_kv_heads, p.head_dim);
-      const int j = lane & 3;
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const uint32_t task = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t g = by_heads.div(task);
+  const int h = static_cast<int>(task - g * p.num_kv_heads);
+  const int64_t pos0 = static_cast<int64_t>(g) * kMxGroup;
+  if (pos0 >= ctx) return;
+  const int64_t col = by_page.div(g);  // groups of a page
+  const int per_page = p.block_size / kMxGroup;
+  const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
+  if (blk < 0 || blk >= p.num_blocks) {
+    if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+    return;
+  }
+  const int nb = blocks_of<NB>(p.head_dim);
+  const int64_t off = ((blk * p.num_kv_heads + h) * per_page + (g - col * per_page)) * (nb * kMxBytes);
+  const uint8_t *kg = p.key_pages + off, *vg = p.value_pages + off;
+  constexpr int kAhead = NB > 0 ? NB : 1;
+  for (int b0 = 0; b0 < nb; b0 += kAhead) {
+    uint32_t kw[2][kAhead], vw[2][kAhead];
+    uint32_t ks[2][kAhead], vs[2][kAhead];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int tok = half * 8 + (lane >> 2);
-        const int64_t row = base + pos0 + tok;
-        if (pos0 + tok >= ctx) continue;
-        if (row < 0 || row >= p.out_rows) {
-          flag_status(p.status, MI_DEV_BAD_SLOT);
-          continue;
-        }
-        for (int b = 0; b < nb; ++b) {
-          const int code = b * kMxBlockBytes + tok * 16 + j * 4, scale = nb * kMxBlockBytes + tok * nb + b;
-          const uint32_t kw = *reinterpret_cast<const uint32_t *>(p.key_pages + off + code);
-          const uint32_t vw = *reinterpret_cast<const uint32_t *>(p.value_pages + off + code);
-          const float ks = mx_scale(p.key_pages[off + scale]), vs = mx_scale(p.value_pages[off + scale]);
-          const int64_t dst = (row * p.num_kv_heads + h) * p.head_dim + b * kMxBlock + j * 8;
-          float x[8];
-          mx_codes_to_f32(kw, ks, x);
-          write8(static_cast<T *>(p.out_keys) + dst, x);
-          mx_codes_to_f32(vw, vs, x);
-          write8(static_cast<T *>(p.out_values) + dst, x);
-        }
+    for (int half = 0; half < 2; ++half) {  // every code and scale is in the page: read whether wanted or not
+      const int tok = half * 8 + (lane >> 2);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int code = (b0 + i) * kMxBlockBytes + tok * 16 + j * 4, scale = nb * kMxBlockBytes + tok * nb + b0 + i;
+        kw[half][i] = __ldg(reinterpret_cast<const uint32_t *>(kg + code));
+        vw[half][i] = __ldg(reinterpret_cast<const uint32_t *>(vg + code));
+        ks[half][i] = __ldg(kg + scale);
+        vs[half][i] = __ldg(vg + scale);
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int tok = half * 8 + (lane >> 2);
+      const int64_t row = base + pos0 + tok;
+      if (pos0 + tok >= ctx) continue;
+      if (row < 0 || row >= p.out_rows) {
+        flag_status(p.status, MI_DEV_BAD_SLOT);
+        continue;
+      }
+      const int64_t dst = (row * p.num_kv_heads + h) * p.head_dim + b0 * kMxBlock + j * 8;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        float x[8];
+        mx_codes_to_f32(kw[half][i], mx_scale(ks[half][i]), x);
+        write8(static_cast<T *>(p.out_keys) + dst + i * kMxBlock, x);
+        mx_codes_to_f32(vw[half][i], mx_scale(vs[half][i]), x);
+        write8(static_cast<T *>(p.out_values) + dst + i * kMxBlock, x);
       }
     }
   }
   pdl_launch_dependents();
 }
 
+template <typename T, typename I, int NB>
+cudaError_t launch_store_tin(const MxStoreParams &p, bool vec, cudaStream_t stream) {
+  const int64_t tasks = (p.num_tokens + 7) / 8 * p.num_kv_heads;
+  if (tasks >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>((tasks + 3) / 4)), block(128);
+  const FastDiv by_heads(p.num_kv_heads), by_block(p.block_size);
+  if (p.num_slots >= (int64_t{1} << 31))
+    return vec ? launch_pdl(mxfp4_store_kernel<T, I, true, NB, true>, grid, block, 0, stream, p, by_heads, by_block)
+               : launch_pdl(mxfp4_store_kernel<T, I, false, NB, true>, grid, block, 0, stream, p, by_heads, by_block);
+  return vec ? launch_pdl(mxfp4_store_kernel<T, I, true, NB, false>, grid, block, 0, stream, p, by_heads, by_block)
+             : launch_pdl(mxfp4_store_kernel<T, I, false, NB, false>, grid, block, 0, stream, p, by_heads, by_block);
+}
+
 template <typename T, typename I>
 cudaError_t launch_store_ti(const MxStoreParams &p, bool vec, cudaStream_t stream) {
-  const int vecs = p.num_kv_heads * (p.head_dim / 8);
-  const int bx = vecs < 256 ? vecs : 256, by = 256 / bx;
-  int64_t blocks = (p.num_tokens + by - 1) / by;
-  const int64_t cap = static_cast<int64_t>(sm_count_current()) * 16;
-  if (blocks > cap) blocks = cap;
-  const dim3 grid(static_cast<unsigned>(blocks)), block(bx, by);
-  return vec ? launch_pdl(mxfp4_store_kernel<T, I, true>, grid, block, 0, stream, p)
-             : launch_pdl(mxfp4_store_kernel<T, I, false>, grid, block, 0, stream, p);
+  if (p.head_dim == 128) return launch_store_tin<T, I, 4>(p, vec, stream);
+  if (p.head_dim == 64) return launch_store_tin<T, I, 2>(p, vec, stream);
+  return launch_store_tin<T, I, 0>(p, vec, stream);
+}
+
+template <typename T>
+cudaError_t launch_gather_t(const MxGatherParams &p, int64_t num_seqs, int64_t max_context, cudaStream_t stream) {
+  const int64_t tasks = (max_context + kMxGroup - 1) / kMxGroup * p.num_kv_heads;
+  if (tasks >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>((tasks + 7) / 8), static_cast<unsigned>(num_seqs)), block(256);
+  const FastDiv by_heads(p.num_kv_heads), by_page(p.block_size / kMxGroup);
+  if (p.head_dim == 128) return launch_pdl(mxfp4_gather_kernel<T, 4>, grid, block, 0, stream, p, by_heads, by_page);
+  if (p.head_dim == 64) return launch_pdl(mxfp4_gather_kernel<T, 2>, grid, block, 0, stream, p, by_heads, by_page);
+  return launch_pdl(mxfp4_gather_kernel<T, 0>, grid, block, 0, stream, p, by_heads, by_page);
 }
 
 template <typename T>
@@ -188,13 +264,9 @@ cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtyp
 
 cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
                                 cudaStream_t stream) {
-  const int64_t units = (max_context + kMxGroup - 1) / kMxGroup * p.num_kv_heads;
-  const dim3 grid(static_cast<unsigned>((units + 7) / 8), static_cast<unsigned>(num_seqs));
-  if (dtype == MI_DTYPE_BFLOAT16)
-    return launch_pdl(mxfp4_gather_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
-  if (dtype == MI_DTYPE_FLOAT16)
-    return launch_pdl(mxfp4_gather_kernel<__half>, grid, dim3(256), 0, stream, p);
-  return launch_pdl(mxfp4_gather_kernel<float>, grid, dim3(256), 0, stream, p);
+  if (dtype == MI_DTYPE_BFLOAT16) return launch_gather_t<__nv_bfloat16>(p, num_seqs, max_context, stream);
+  if (dtype == MI_DTYPE_FLOAT16) return launch_gather_t<__half>(p, num_seqs, max_context, stream);
+  return launch_gather_t<float>(p, num_seqs, max_context, stream);
 }
 
 }  // namespace mi

@@ -66,6 +66,8 @@ int mi_store_kv_mxfp4(void *key_pages, void *value_pages, int64_t num_blocks, in
   if (num_tokens < 0) return capi_fail(MI_ERR_INVALID, "num_tokens must be >= 0");
   if (key_token_stride < 0 || value_token_stride < 0)
     return capi_fail(MI_ERR_INVALID, "token strides must be >= 0");
+  if (num_tokens / 8 + 1 >= (int64_t{1} << 31) / num_kv_heads)
+    return capi_fail(MI_ERR_UNSUPPORTED, "too many tokens for one call");
   if (num_tokens == 0) return MI_OK;
   if (!key_pages || !value_pages || !keys || !values || !slots) return capi_fail(MI_ERR_INVALID, "null pointer");
   if (!aligned16(key_pages) || !aligned16(value_pages))
@@ -102,7 +104,7 @@ int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void *key_p
     return capi_fail(MI_ERR_INVALID, "negative sizes");
   if (num_seqs > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences in one call");
   if (num_seqs == 0 || max_context == 0 || out_rows == 0) return MI_OK;
-  if (max_context / kMxGroup > (int64_t{1} << 33) / num_kv_heads)
+  if (max_context / kMxGroup + 1 >= (int64_t{1} << 31) / num_kv_heads)
     return capi_fail(MI_ERR_UNSUPPORTED, "max_context too large for one call");
   if (!out_keys || !out_values || !key_pages || !value_pages || !block_tables || !cu_seqlens_k)
     return capi_fail(MI_ERR_INVALID, "null pointer");

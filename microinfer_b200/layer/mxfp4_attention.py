@@ -26,17 +26,21 @@ from microinfer_b200.worker.mxfp4_cache import page_dims
 
 
 def _check_query(query, hkv, d, out):
-    if query.ndim != 3:
+    """(tokens, Hq) of a query over a cache of these heads."""
+    shape = query.shape
+    if len(shape) != 3:
         raise ValueError("query must have shape [tokens, Hq, D]")
-    if query.shape[2] != d:
+    tokens, hq, query_dim = shape
+    if query_dim != d:
         raise ValueError("query and cache head dimensions differ")
-    if query.shape[1] == 0 or query.shape[1] % hkv:
+    if hq == 0 or hq % hkv:
         raise ValueError("Hq must be divisible by Hkv")
     if out is not None:
-        if out.shape != query.shape or out.dtype != query.dtype or not out.is_contiguous():
+        if out.shape != shape or out.dtype != query.dtype or not out.is_contiguous():
             raise ValueError("out must be contiguous, of the query's shape and dtype")
         if out.device != query.device:
             raise ValueError("out must be on the query's device")
+    return tokens, hq
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -60,17 +64,17 @@ def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens
                                                            block_tables, context_lens, scale)
         return res if out is None else out.copy_(res)
     nb, bs, hkv, d = page_dims(key_pages, value_pages)
-    _check_query(query, hkv, d, out)
-    n, hq, _ = query.shape
+    n, hq = _check_query(query, hkv, d, out)
     dtype = _lib.dtype_code(query.dtype)
-    if block_tables.ndim != 2 or block_tables.shape[0] != n:
+    table_shape = block_tables.shape
+    if len(table_shape) != 2 or table_shape[0] != n:
         raise ValueError("block_tables must have one row per request")
     if context_lens.shape != (n,):
         raise ValueError("context_lens must have one entry per request")
     if n == 0:
         return torch.empty_like(query) if out is None else out
     device = _lib.require_cuda(query, key_pages, value_pages, block_tables, context_lens)
-    width = block_tables.shape[1]
+    width = table_shape[1]
     if width == 0:  # no request can have a key
         return torch.zeros_like(query) if out is None else out.zero_()
     query, block_tables, context_lens = _aligned(query), _idx(block_tables), _idx(context_lens)

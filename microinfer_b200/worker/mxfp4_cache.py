@@ -30,13 +30,14 @@ MX_BYTES = 272  # bytes of one block of 32 elements of a group's 16 tokens
 
 def page_dims(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple[int, int, int, int]:
     """(num_blocks, block_size, Hkv, D) of a layer's pages; raises if they are none."""
-    if key_pages.ndim != 4 or value_pages.shape != key_pages.shape:
+    shape = key_pages.shape
+    if len(shape) != 4 or value_pages.shape != shape:
         raise ValueError("pages must be matching [blocks, Hkv, block_size / 16, bytes] tensors")
     if key_pages.dtype != torch.uint8 or value_pages.dtype != torch.uint8:
         raise ValueError("pages must be uint8")
     if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
         raise ValueError("pages must be contiguous")
-    blocks, hkv, groups, size = key_pages.shape
+    blocks, hkv, groups, size = shape
     if size == 0 or size % MX_BYTES:
         raise ValueError(f"the last dimension of pages must be head_dim / {MX} * {MX_BYTES} bytes")
     return blocks, groups * GROUP, hkv, size // MX_BYTES * MX
