@@ -441,12 +441,13 @@ MI_API int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void
  * keys gives zeros.  query / out are contiguous [num_seqs, num_q_heads, head_dim]
  * in `dtype`, 16-byte aligned.  The workspace holds partial states for the
  * duration of the call and needs no initial value; calls that can run at the
- * same time need one each.  `max_context` of the size query is
- * block_table_stride * block_size.
+ * same time need one each.
  */
-MI_API size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int32_t num_q_heads,
+MI_API size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int64_t num_blocks,
+                                             int32_t block_size, int32_t num_q_heads,
                                              int32_t num_kv_heads, int32_t head_dim,
-                                             int32_t dtype, int64_t max_context, int device);
+                                             int32_t dtype, int64_t block_table_stride,
+                                             int device);
 MI_API int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages,
                           const void *value_pages, int64_t num_blocks, int32_t block_size,
                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,

@@ -92,7 +92,7 @@ SIGNATURES = {
         [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P, _I64, _I64, _I64, _P, _P],
     ),
     "mi_paged_decode_mxfp4_workspace_bytes": (
-        _SZ, [_I64, _I32, _I32, _I32, _I32, _I64, ctypes.c_int],
+        _SZ, [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, ctypes.c_int],
     ),
     "mi_paged_decode_mxfp4": (
         ctypes.c_int,

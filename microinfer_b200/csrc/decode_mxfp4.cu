@@ -248,16 +248,12 @@ int simt_splits(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t cap
 
 }  // namespace
 
-// The workspace of either form; it does not depend on the pool's size, which decides between
-// them for pools of 2^31 groups and more.
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
-                              int64_t capacity, int sms) {
+                              int64_t num_blocks, int block_size, int64_t capacity, int sms) {
+  if (mxfp4_mma_supported(dtype, num_q_heads, num_kv_heads, head_dim, num_blocks, block_size, capacity))
+    return mxfp4_mma_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, capacity, sms);
   const int s = simt_splits(num_seqs, num_q_heads, num_kv_heads, capacity, sms);
-  const size_t simt =
-      s == 1 ? 0 : static_cast<size_t>(num_seqs) * num_q_heads * s * (head_dim + 2) * sizeof(float);
-  if (!mxfp4_mma_supported(dtype, num_q_heads, num_kv_heads, head_dim, 1, kMxGroup, capacity)) return simt;
-  const size_t mma = mxfp4_mma_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, capacity, sms);
-  return mma > simt ? mma : simt;
+  return s == 1 ? 0 : static_cast<size_t>(num_seqs) * num_q_heads * s * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream) {

@@ -19,7 +19,7 @@ cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_
                                 cudaStream_t stream);
 cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream);
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
-                              int64_t capacity, int sms);
+                              int64_t num_blocks, int block_size, int64_t capacity, int sms);
 
 }  // namespace mi
 
@@ -129,13 +129,14 @@ int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void *key_p
       launch_mxfp4_gather(p, dtype, num_seqs, max_context, static_cast<cudaStream_t>(stream)));
 }
 
-size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
-                                             int32_t head_dim, int32_t dtype, int64_t max_context, int device) {
-  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context <= 0 ||
-      num_q_heads % num_kv_heads != 0)
+size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int64_t num_blocks, int32_t block_size,
+                                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t dtype, int64_t block_table_stride, int device) {
+  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_table_stride <= 0 ||
+      num_q_heads % num_kv_heads != 0 || check_cache(num_blocks, block_size, num_kv_heads, head_dim) != MI_OK)
     return 0;
-  return mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, max_context,
-                                sm_count_of(device < 0 ? 0 : device));
+  return mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, num_blocks, block_size,
+                                block_table_stride * block_size, sm_count_of(device < 0 ? 0 : device));
 }
 
 int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, const void *value_pages,
@@ -159,8 +160,8 @@ int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, c
   if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
     return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
-  const size_t need = mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype,
-                                             block_table_stride * block_size, sm_count_current());
+  const size_t need = mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, num_blocks,
+                                             block_size, block_table_stride * block_size, sm_count_current());
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_decode_mxfp4_workspace_bytes)");
   if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");

@@ -49,8 +49,8 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 @lru_cache(maxsize=4096)
-def _decode_workspace_bytes(n, hq, hkv, d, dtype, capacity, device):
-    return _lib.load().mi_paged_decode_mxfp4_workspace_bytes(n, hq, hkv, d, dtype, capacity, device)
+def _decode_workspace_bytes(*shape):
+    return _lib.load().mi_paged_decode_mxfp4_workspace_bytes(*shape)
 
 
 def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens, *,
@@ -80,7 +80,7 @@ def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens
     query, block_tables, context_lens = _aligned(query), _idx(block_tables), _idx(context_lens)
     if out is None:
         out = torch.empty_like(query)
-    need = _decode_workspace_bytes(n, hq, hkv, d, dtype, width * bs, device.index or 0)
+    need = _decode_workspace_bytes(n, nb, bs, hq, hkv, d, dtype, width, device.index or 0)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _lib.call(
         "mi_paged_decode_mxfp4", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),

@@ -178,7 +178,7 @@ def test_c_entries_refuse_bad_arguments():
 
     assert gather(n=0) == 0 and gather(most=0) == 0 and gather(rows=0) == 0
     assert gather(n=-1) < 0 and gather(dtype=5) < 0 and gather(n=70000) < 0
-    assert lib.mi_paged_decode_mxfp4_workspace_bytes(0, 4, 2, 64, 2, 100, 0) == 0
+    assert lib.mi_paged_decode_mxfp4_workspace_bytes(0, 8, 16, 4, 2, 64, 2, 100, 0) == 0
 
 
 # ---------------------------------------------------------------------------
