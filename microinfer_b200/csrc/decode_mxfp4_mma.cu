@@ -1,5 +1,5 @@
-// Paged decode over the 4-bit cache on the warp-level tensor cores (bf16 and
-// fp16, head_dim 64 or 128, any GQA group; other shapes: decode_mxfp4.cu).
+// Paged decode over the 4-bit cache on the warp-level tensor cores (head_dim 64 or 128, any type
+// and GQA group; other shapes: decode_mxfp4.cu).
 //
 // Decode moves 4.25 bits per cached element and does 2 flops per element and
 // query head on it, so the bound is HBM as long as turning codes into MMA
@@ -26,6 +26,8 @@
 // a register and zero in the other, so a column gathers its own dims.  N = 8 holds 4 queries this
 // way (groups of up to 8 take two column tiles from the same decoded operands), and the scores' columns are
 // doubled to match, so that P goes from accumulator to operand layout through two movmatrix.
+// For fp32 the two columns of a query hold the upper and lower f16 of q, 22 bits together at no cost, and
+// P_b goes in twice, its rounding error in f16 after it.
 //
 // Work: the units of 32 keys of all (sequence, kv head, 4 or 8 query heads)
 // segments, in that order, are one list that is cut into equal ranges, one per
@@ -57,12 +59,12 @@ constexpr float kLag = 3.f;         // m may be this far behind: p <= 2^15
 constexpr uint32_t kLowestRef = 0x20202020u;  // R_b - 255 then has a bit of 0xf8 set, like every far scale
 constexpr int kAlignedSlack = 1;    // units per warp that keeping a segment in one CTA may cost
 
-// NB blocks of 32 per head, CT column tiles of 4 query heads.  One tile leaves the registers for 16
-// warps, two for 12; the ring takes what shared memory the parts leave.
-template <int NB, int CT>
+// NB blocks of 32 per head, CT column tiles of 4 query heads, SPLIT: fp32.  One tile leaves the registers for
+// 16 warps, two at D = 128 and fp32 for 12.
+template <int NB, int CT, bool SPLIT>
 struct MxCfg {
   static constexpr int D = NB * kMxBlock;
-  static constexpr int kWarps = CT == 1 || NB == 2 ? 16 : 12;
+  static constexpr int kWarps = (CT == 1 || NB == 2) && !SPLIT ? 16 : 12;
   static constexpr int kStages = 2;
   static constexpr int kHeads = CT * kQueries;    // query heads of a segment
   static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
@@ -204,8 +206,10 @@ __device__ __forceinline__ void load_scales(uint32_t vbase, int t, uint32_t (&w)
 // A warp's state on a segment: 4 query heads to a column tile, lane (g, t) = (lane / 4, lane % 4).
 template <typename T, int NB, int CT>
 struct MxWarp {
-  using C = MxCfg<NB, CT>;
+  static constexpr bool kSplit = std::is_same<T, float>::value;
+  using C = MxCfg<NB, CT, kSplit>;
   static constexpr int D = C::D;
+  static constexpr int kParts = kSplit ? 2 : 1;  // f16 parts of p
   uint32_t q;                 // shared address of this lane's B fragments of q (columns 2i and 2i + 1 both
                               // query i of the tile): 4 words per block, 512 bytes between blocks
   float xs[CT];               // log2-domain scale of query t
@@ -233,32 +237,43 @@ struct MxWarp {
   }
 
   // q of the segment's query heads (heads of them exist): this lane's elements ...
-  __device__ __forceinline__ void fetch_query(const T *query, int heads, uint4 (&raw)[CT][NB]) const {
+  static constexpr int kRaw = 8 * static_cast<int>(sizeof(T)) / 16;
+  using Raw = uint4[CT][NB][kRaw];
+  __device__ __forceinline__ void fetch_query(const T *query, int heads, Raw &raw) const {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const int h = c * kQueries + (g >> 1);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        raw[c][b] = make_uint4(0u, 0u, 0u, 0u);
-        if (h < heads) raw[c][b] = *reinterpret_cast<const uint4 *>(query + h * D + b * 32 + t * 8);
+      for (int i = 0; i < NB * kRaw; ++i) {
+        uint4 &v = raw[c][i / kRaw][i % kRaw];
+        v = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads) v = reinterpret_cast<const uint4 *>(query + h * D + i / kRaw * 32 + t * 8)[i % kRaw];
       }
     }
   }
   // ... as f16 fragments.
-  __device__ __forceinline__ void set_query(const uint4 (&raw)[CT][NB], float scale_log2) {
+  __device__ __forceinline__ void set_query(const Raw &raw, float scale_log2) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float x[NB][8];
       uint32_t top = 0;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float2 f[4];
-        Vec16<T>::unpack(raw[c][b], f);
+        if constexpr (kSplit) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[b][2 * i] = f[i].x, x[b][2 * i + 1] = f[i].y;
-          top = max(top, max(__float_as_uint(f[i].x) & 0x7fffffffu, __float_as_uint(f[i].y) & 0x7fffffffu));
+          for (int i = 0; i < 2; ++i) {
+            const uint4 &v = raw[c][b][i];
+            x[b][4 * i] = __uint_as_float(v.x), x[b][4 * i + 1] = __uint_as_float(v.y);
+            x[b][4 * i + 2] = __uint_as_float(v.z), x[b][4 * i + 3] = __uint_as_float(v.w);
+          }
+        } else {
+          float2 f[4];
+          Vec16<T>::unpack(raw[c][b][0], f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[b][2 * i] = f[i].x, x[b][2 * i + 1] = f[i].y;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[b][i]) & 0x7fffffffu);
       }
       top = max(top, __shfl_xor_sync(kAll, top, 1));
       top = max(top, __shfl_xor_sync(kAll, top, 2));
@@ -267,11 +282,18 @@ struct MxWarp {
       e = min(e, 126);
       const float f = exp2i(e);
 #pragma unroll
-      for (int b = 0; b < NB; ++b)  // read by this lane alone
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[b][i] *= f;
+          if (kSplit && (g & 1)) x[b][i] -= __half2float(__float2half_rn(x[b][i]));  // what the other column leaves
+        }
+        // read by this lane alone
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q + (c * NB + b) * 512),
-                     "r"(pack_f16(x[b][0] * f, x[b][1] * f)), "r"(pack_f16(x[b][2] * f, x[b][3] * f)),
-                     "r"(pack_f16(x[b][4] * f, x[b][5] * f)), "r"(pack_f16(x[b][6] * f, x[b][7] * f))
+                     "r"(pack_f16(x[b][0], x[b][1])), "r"(pack_f16(x[b][2], x[b][3])),
+                     "r"(pack_f16(x[b][4], x[b][5])), "r"(pack_f16(x[b][6], x[b][7]))
                      : "memory");
+      }
       xs[c] = __shfl_sync(kAll, exp2i(-e) * scale_log2, 8 * t);  // a lane of query t: g = 2t
     }
   }
@@ -311,6 +333,7 @@ struct MxWarp {
           float d[4];
           mma_f16_zero(d, a[0], e[0], a[1], e[1], f[c][0], f[c][1]);
           mma_f16(d, a[2], e[2], a[3], e[3], f[c][2], f[c][3]);
+          if constexpr (kSplit) d[0] += d[1], d[2] += d[3];
           x[j][c][0] = b == 0 ? d[0] * fl : fmaf(d[0], fl, x[j][c][0]);
           x[j][c][1] = b == 0 ? d[2] * fh : fmaf(d[2], fh, x[j][c][1]);
         }
@@ -344,10 +367,10 @@ struct MxWarp {
   }
 
   // O += P_b V of a group.  d: distances per byte, 0 to 7, or 15 for no contribution (2^-15 has the f16
-  // exponent 0: zero); p[c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in the half of this lane's
-  // column, zero in the other.  FAR: the products are `back` times what d says.
+  // exponent 0: zero); p[part][c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in the half of this lane's
+  // column, zero in the other (fp32: its upper f16, then its lower).  FAR: the products are `back` times what d says.
   template <bool FAR>
-  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[CT][4],
+  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[kParts][CT][4],
                                          float back = 1.f) {
     uint32_t lo[NB], hi[NB];
     load_codes<NB, true>(vbase, lane, lo, hi);
@@ -365,16 +388,18 @@ struct MxWarp {
       mx_codes_to_f16(lo[b], a);
       mx_codes_to_f16(hi[b], e);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
+      for (int part = 0; part < kParts * CT; ++part) {
+        const int c = part / kParts, half = part % kParts;
         uint32_t s[4];  // p times the scale of V's block b
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+          const uint32_t pk = p[half][c][k];
           if constexpr (NB == 4) {
             const uint32_t f = b & 1 ? odd[k] : even[k];
-            s[k] = b < 2 ? mul_f16x2_half<false>(p[c][k], f) : mul_f16x2_half<true>(p[c][k], f);
+            s[k] = b < 2 ? mul_f16x2_half<false>(pk, f) : mul_f16x2_half<true>(pk, f);
           } else {
             const uint32_t f = b & 1 ? odd[k & 2] : even[k & 2];
-            s[k] = k & 1 ? mul_f16x2_half<true>(p[c][k], f) : mul_f16x2_half<false>(p[c][k], f);
+            s[k] = k & 1 ? mul_f16x2_half<true>(pk, f) : mul_f16x2_half<false>(pk, f);
           }
         }
         if constexpr (FAR) {
@@ -401,7 +426,7 @@ struct MxWarp {
 
   // As values() for scales that the window of 8 binades does not hold: raise R_b where a scale is above
   // it, then take the keys window by window.
-  __device__ __forceinline__ void values_far(uint32_t vbase, const uint32_t (&p)[CT][4], int valid) {
+  __device__ __forceinline__ void values_far(uint32_t vbase, const uint32_t (&p)[kParts][CT][4], int valid) {
     uint32_t w[4], nan[4];
     load_scales<NB>(vbase, t, w);
     mask_scales(w, valid, 0);
@@ -504,18 +529,22 @@ struct MxWarp {
         }
       }
     }
-    uint32_t p[2][CT][4];
+    uint32_t p[2][kParts][CT][4];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const float lift = kLift - m[c];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float p0 = fast_exp2(x[j][c][0] + lift), p1 = fast_exp2(x[j][c][1] + lift);
+        float p0 = fast_exp2(x[j][c][0] + lift), p1 = fast_exp2(x[j][c][1] + lift);
         l[c] += p0 + p1;
-        // rows (keys) x columns (each query twice), transposed: keys 2t and 2t + 1 of query g / 2
-        const uint32_t k0 = movm(pack_f16(p0, p0)), k8 = movm(pack_f16(p1, p1));
-        p[j][c][0] = __byte_perm(k0, 0, pick0), p[j][c][1] = __byte_perm(k0, 0, pick1);
-        p[j][c][2] = __byte_perm(k8, 0, pick0), p[j][c][3] = __byte_perm(k8, 0, pick1);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          // rows (keys) x columns (each query twice), transposed: keys 2t and 2t + 1 of query g / 2
+          const uint32_t k0 = movm(pack_f16(p0, p0)), k8 = movm(pack_f16(p1, p1));
+          p[j][part][c][0] = __byte_perm(k0, 0, pick0), p[j][part][c][1] = __byte_perm(k0, 0, pick1);
+          p[j][part][c][2] = __byte_perm(k8, 0, pick0), p[j][part][c][3] = __byte_perm(k8, 0, pick1);
+          if (part + 1 < kParts) p0 -= __half2float(__float2half_rn(p0)), p1 -= __half2float(__float2half_rn(p1));
+        }
       }
     }
     uint32_t d[2][4];
@@ -551,11 +580,12 @@ struct MxWarp {
       const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        uint2 v;
+        using V = typename std::conditional<kSplit, uint4, uint2>::type;
+        V v;
         T *e = reinterpret_cast<T *>(&v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_float(o[c][b][i] * inv);
-        *reinterpret_cast<uint2 *>(out + (c * kQueries + t) * D + b * 32 + g * 4) = v;
+        *reinterpret_cast<V *>(out + (c * kQueries + t) * D + b * 32 + g * 4) = v;
       }
     }
   }
@@ -583,9 +613,9 @@ __device__ __forceinline__ float part_factor(float m, float l, float M) {
 }
 
 template <typename T, int NB, int CT>
-__global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
+__global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::kWarps * 32, 1)
     mxfp4_decode_mma_kernel(const MxDecodeParams p, const MxPlan plan) {
-  using C = MxCfg<NB, CT>;
+  using C = MxCfg<NB, CT, std::is_same<T, float>::value>;
   constexpr int D = C::D, kWarps = C::kWarps, kStages = C::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
@@ -682,7 +712,8 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   for (int s = blockIdx.x; s < n; s += gridDim.x) {
     if (prefix[s + 1] != prefix[s]) continue;
     T *out = static_cast<T *>(p.out) + static_cast<int64_t>(s) * p.num_q_heads * D;
-    for (int i = threadIdx.x * 8; i < p.num_q_heads * D; i += blockDim.x * 8)
+    constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+    for (int i = threadIdx.x * kVec; i < p.num_q_heads * D; i += blockDim.x * kVec)
       *reinterpret_cast<uint4 *>(out + i) = make_uint4(0u, 0u, 0u, 0u);
   }
 
@@ -808,7 +839,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT>::kWarps * 32, 1)
   };
 
   // The first segment's q is asked for before the ring's copies, which would keep it waiting.
-  uint4 raw[CT][NB];
+  typename MxWarp<T, NB, CT>::Raw raw;
   const int ahead = min(kStages, units);
   if (units > 0) {
     const Unit r = unit_of(min(lane, units - 1));
@@ -953,7 +984,7 @@ constexpr int kJoinLanes = 128;
 template <typename T, int NB, int CT>
 __global__ void __launch_bounds__(kJoinLanes * kJoinWays)
     mxfp4_decode_mma_join_kernel(const MxDecodeParams p, const MxPlan plan) {
-  using C = MxCfg<NB, CT>;
+  using C = MxCfg<NB, CT, std::is_same<T, float>::value>;
   constexpr int D = C::D, kVecs = C::kHeads * D / 4;
   constexpr int kPer = (kVecs + kJoinLanes - 1) / kJoinLanes;
   __shared__ float4 sums[kJoinWays][kVecs];
@@ -1034,7 +1065,7 @@ __global__ void __launch_bounds__(kJoinLanes * kJoinWays)
 
 template <typename T, int NB, int CT>
 cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, cudaStream_t stream) {
-  using C = MxCfg<NB, CT>;
+  using C = MxCfg<NB, CT, std::is_same<T, float>::value>;
   auto kern = mxfp4_decode_mma_kernel<T, NB, CT>;
   static bool attr_set[64] = {};
   int dev = 0;
@@ -1064,7 +1095,7 @@ int mma_tiles(int num_q_heads, int num_kv_heads) {
 // every segment has a CTA and a full table is no more than the slack per warp.
 bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t capacity, int sms) {
   const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads);
-  constexpr int warps = MxCfg<4, 2>::kWarps;  // the fewest
+  constexpr int warps = MxCfg<4, 2, true>::kWarps;  // the fewest
   return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * warps * kUnit;
 }
 
@@ -1082,7 +1113,7 @@ cudaError_t launch_mma_t(const MxDecodeParams &p, int tiles, int columns, bool j
 // Shapes of this kernel: 32-bit unit and group counts, sequences in one launch's reach.
 bool mxfp4_mma_supported(int dtype, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
                          int block_size, int64_t capacity) {
-  if (dtype != MI_DTYPE_BFLOAT16 && dtype != MI_DTYPE_FLOAT16) return false;
+  (void)dtype;
   if (head_dim != 64 && head_dim != 128) return false;
   const int64_t H = static_cast<int64_t>(num_kv_heads) * mma_tiles(num_q_heads, num_kv_heads);
   return num_blocks * num_kv_heads * (block_size / kMxGroup) < (int64_t{1} << 31) &&
@@ -1107,13 +1138,14 @@ cudaError_t launch_mxfp4_mma(const MxDecodeParams &p, int dtype, cudaStream_t st
   for (int64_t s = 0; s < p.num_seqs; s += slice) {
     MxDecodeParams q = p;
     q.num_seqs = p.num_seqs - s < slice ? p.num_seqs - s : slice;
-    const int64_t row = s * p.num_q_heads * p.head_dim * 2;
+    const int64_t row = s * p.num_q_heads * p.head_dim * (dtype == MI_DTYPE_FLOAT32 ? 4 : 2);
     q.query = static_cast<const char *>(p.query) + row;
     q.out = static_cast<char *>(p.out) + row;
     q.block_tables = p.block_tables + s * p.bt_stride;
     q.context_lens = p.context_lens + s;
     const cudaError_t e = dtype == MI_DTYPE_BFLOAT16 ? launch_mma_t<__nv_bfloat16>(q, tiles, columns, join, sms, stream)
-                                                     : launch_mma_t<__half>(q, tiles, columns, join, sms, stream);
+                          : dtype == MI_DTYPE_FLOAT16  ? launch_mma_t<__half>(q, tiles, columns, join, sms, stream)
+                                                       : launch_mma_t<float>(q, tiles, columns, join, sms, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

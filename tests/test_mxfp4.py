@@ -5,7 +5,8 @@ Store and gather are exact (the scale is a power of two).  Attention is held to
 with u half a step of the output type and c from the kernels' roundings:
   scores: fp32 sums of D products, off by at most D 2^-23 S with S = scale * sum |q||k|;
           that and the exponential's 2^-21 move p by as much, in the numerator and the sum;
-  p:      rounded once to f16 before the tensor-core product (2^-11, in fp32 not at all).
+  p:      rounded once to f16 before the tensor-core product (2^-11); fp32 carries the error in a second
+          f16 (2^-22, within the exponential's term).
           f16 ends: p times a power of two that puts the sum above 2^12 and V's scale
           into [2^-7, 1] (at most 4 above the block's largest) loses at most half of 2^-24 a key,
           which is 2^-37 * 4 * 2^s_max * 6 of the result, and 2^s_max <= max|v| / 4 over the block:
@@ -32,8 +33,7 @@ def _bound(want, weight, size, floor, dtype, d, p_step):
     u = torch.finfo(dtype).eps / 2
     c = 2 * (d * 2.0 ** -23 * size + 2.0 ** -21) + p_step
     # below the smallest normal number the steps stay as they are there: half of one is u * smallest_normal
-    return u * np.maximum(np.abs(want), torch.finfo(dtype).smallest_normal) + (c + u) * weight + (
-        floor * 2.0 ** -34 if p_step else 0.0) + 1e-30
+    return u * np.maximum(np.abs(want), torch.finfo(dtype).smallest_normal) + (c + u) * weight + floor * 2.0 ** -34
 
 
 def _close(got, want, weight, size, floor, dtype, p_step):
