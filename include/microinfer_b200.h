@@ -457,6 +457,27 @@ MI_API int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_p
                           size_t workspace_bytes, int32_t *dev_status, void *stream);
 
 /*
+ * Causal chunked prefill from the 4-bit cache (also mixed batches): rows as
+ * mi_paged_prefill, any GQA group, f32/f16/bf16, head_dim 64 or 128
+ * (MI_ERR_UNSUPPORTED otherwise: gather and mi_varlen_prefill).  `max_seqlen_q`
+ * bounds the launch shape, `max_context` (a bound on the contexts, or less) the split over the keys
+ * of few rows, whose states take the workspace for the duration of the call.
+ */
+MI_API size_t mi_paged_prefill_mxfp4_workspace_bytes(int64_t num_seqs, int64_t num_tokens,
+                                              int64_t max_seqlen_q, int32_t num_q_heads,
+                                              int32_t num_kv_heads, int32_t head_dim,
+                                              int64_t max_context, int device);
+MI_API int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages,
+                           const void *value_pages, int64_t num_blocks, int32_t block_size,
+                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t dtype, const int32_t *cu_seqlens_q,
+                           const int32_t *cu_seqlens_k, const int32_t *block_tables,
+                           int64_t block_table_stride, int64_t num_seqs, int64_t num_tokens,
+                           int64_t max_seqlen_q, int64_t max_context, float scale,
+                           void *workspace, size_t workspace_bytes, int32_t *dev_status,
+                           void *stream);
+
+/*
  * Bounded-wait self test: one thread spins on `flag` (device int32) until it
  * becomes non-zero or `timeout_ns` passes, then ORs MI_DEV_TIMEOUT into
  * dev_status if it ran out.  Exercises the same bounded-wait helper every

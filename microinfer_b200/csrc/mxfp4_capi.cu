@@ -21,6 +21,12 @@ cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                               int64_t num_blocks, int block_size, int64_t capacity, int sms);
 
+bool mxfp4_prefill_supported(int head_dim);
+int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
+                         int64_t capacity, int sms);
+cudaError_t launch_mxfp4_prefill(const MxPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
+                                 int64_t max_seqlen_q, cudaStream_t stream);
+
 }  // namespace mi
 
 using namespace mi;
@@ -183,6 +189,81 @@ int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, c
   p.scale_log2 = scale * kLog2eHost;
   p.status = dev_status;
   return capi_cuda_status(launch_mxfp4_decode(p, dtype, static_cast<cudaStream_t>(stream)));
+}
+
+static int prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
+                          int64_t max_context, int sms) {
+  return mxfp4_prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context, sms);
+}
+
+static size_t prefill_workspace(int splits, int64_t num_tokens, int32_t num_q_heads, int32_t head_dim) {
+  return splits <= 1 ? 0
+                     : static_cast<size_t>(splits) * num_tokens * num_q_heads * (head_dim + 2) * sizeof(float);
+}
+
+size_t mi_paged_prefill_mxfp4_workspace_bytes(int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen_q,
+                                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int64_t max_context, int device) {
+  if (num_seqs <= 0 || num_tokens <= 0 || max_seqlen_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0 || head_dim <= 0 || max_context < 0)
+    return 0;
+  const int splits = prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context,
+                                    sm_count_of(device < 0 ? 0 : device));
+  return prefill_workspace(splits, num_tokens, num_q_heads, head_dim);
+}
+
+int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, const void *value_pages,
+                           int64_t num_blocks, int32_t block_size, int32_t num_q_heads, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t dtype, const int32_t *cu_seqlens_q,
+                           const int32_t *cu_seqlens_k, const int32_t *block_tables, int64_t block_table_stride,
+                           int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen_q, int64_t max_context,
+                           float scale, void *workspace, size_t workspace_bytes, int32_t *dev_status,
+                           void *stream) {
+  if (!known_dtype(dtype)) return capi_fail(MI_ERR_INVALID, "unknown dtype");
+  if (const int s = check_cache(num_blocks, block_size, num_kv_heads, head_dim)) return s;
+  if (num_seqs < 0 || num_tokens < 0 || max_context < 0 || block_table_stride < 0)
+    return capi_fail(MI_ERR_INVALID, "negative sizes");
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0)
+    return capi_fail(MI_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads");
+  if (!mxfp4_prefill_supported(head_dim))
+    return capi_fail(MI_ERR_UNSUPPORTED, "prefill from the 4-bit cache takes head_dim 64 or 128; gather other ones");
+  if (num_seqs > 65535 || num_kv_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
+  if (num_seqs == 0 || num_tokens == 0) return MI_OK;
+  if (max_seqlen_q <= 0) return capi_fail(MI_ERR_INVALID, "max_seqlen_q must be positive");
+  if (max_seqlen_q > (int64_t{1} << 24) || max_seqlen_q * (num_q_heads / num_kv_heads) >= (int64_t{1} << 31) ||
+      block_table_stride * block_size > INT32_MAX)
+    return capi_fail(MI_ERR_UNSUPPORTED, "sequence too long for one call");
+  if (!out || !query || !key_pages || !value_pages || !cu_seqlens_q || !cu_seqlens_k || !block_tables)
+    return capi_fail(MI_ERR_INVALID, "null pointer");
+  if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
+    return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
+  if (const int s = capi_select_device(key_pages)) return s;
+  const int splits = prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context,
+                                    sm_count_current());
+  const size_t need = prefill_workspace(splits, num_tokens, num_q_heads, head_dim);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_prefill_mxfp4_workspace_bytes)");
+  if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  MxPrefillParams p = {};
+  p.out = out;
+  p.query = query;
+  p.key_pages = static_cast<const uint8_t *>(key_pages);
+  p.value_pages = static_cast<const uint8_t *>(value_pages);
+  p.block_tables = block_tables;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.cu_seqlens_k = cu_seqlens_k;
+  p.workspace = static_cast<float *>(workspace);
+  p.bt_stride = block_table_stride;
+  p.num_blocks = num_blocks;
+  p.num_tokens = num_tokens;
+  p.num_splits = splits;
+  p.block_size = block_size;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.scale_log2 = scale * kLog2eHost;
+  p.status = dev_status;
+  return capi_cuda_status(
+      launch_mxfp4_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -187,6 +187,26 @@ struct MxDecodeParams {
   int32_t *status;
 };
 
+struct MxPrefillParams {
+  void *out;
+  const void *query;
+  const uint8_t *key_pages;
+  const uint8_t *value_pages;
+  const int32_t *block_tables;
+  const int32_t *cu_seqlens_q;
+  const int32_t *cu_seqlens_k;
+  float *workspace;  // num_splits > 1: [split][token][q head][2 + D]
+  int64_t bt_stride;
+  int64_t num_blocks;
+  int64_t num_tokens;
+  int32_t num_splits;
+  int32_t block_size;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  float scale_log2;
+  int32_t *status;
+};
+
 // Per-step runner metadata from the device page table (runner_meta.cu).
 struct RunnerMetaParams {
   int32_t *page_table;  // [max_rows, max_pages]

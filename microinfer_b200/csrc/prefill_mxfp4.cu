@@ -1,0 +1,510 @@
+// Causal chunked prefill straight from the 4-bit cache (layout: mxfp4.cuh) on
+// the warp-level tensor cores, for what the dense tcgen05 kernel behind the gather does
+// not take (head_dim 64, fp32, other groups) and for chunks too small to fill it.
+//
+// A CTA takes 128 rows of one kv head, a row being (token, query head of the group), so any group
+// fills the tiles; 8 warps of 16 rows.  It walks the keys 64 at a time: codes and scales of
+// the next tile are on their way in registers while this one is worked on, then become
+// 16-bit K and V rows in the other half of shared memory, decoded once for the 8 warps.  S = Q K^T and
+// O += P V are m16n8k16 with fp32 accumulators, P passes from the one to the
+// other in registers; online softmax in fp32, the maximum followed 3 binades behind at most.
+// Types: bf16 holds every value of the cache (short of overflow), fp16 rounds
+// those outside its range, as the gather does; p in fp16 is lifted by 2^12, which keeps a key down to 2^-26 of
+// the largest at full precision.  fp32: K and V are exact in bf16, q and p go in as three bf16 parts
+// (24 bits), three MMAs for one.
+// A NaN block of V is held as zero and its dims are set to NaN in the rows that
+// see the key, so it never reaches rows before it.
+// Few rows over a long context are split over the keys; a second launch joins
+// the splits.  mma.sync bounds this at about 1/3 of the tcgen05 rate.
+#include <type_traits>
+
+#include "common.cuh"
+#include "launch.cuh"
+#include "mxfp4.cuh"
+#include "params.cuh"
+
+namespace mi {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kRows = 128;
+constexpr int kThreads = 256;
+constexpr int kKeys = 64;  // keys of a tile
+constexpr int kGroups = kKeys / kMxGroup;
+
+template <typename T, int NB>
+struct PfCfg {
+  static constexpr bool kSplit = std::is_same<T, float>::value;
+  using E = typename std::conditional<kSplit, __nv_bfloat16, T>::type;  // MMA operands
+  static constexpr int kParts = kSplit ? 3 : 1;
+  static constexpr int D = NB * kMxBlock;
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kTile = kKeys * kRowBytes;      // K or V of a tile
+  static constexpr int kQuery = kRows * kRowBytes;     // one part of q
+  static constexpr int kWords = kKeys * NB * 4 / kThreads;  // code words of K (and of V) per thread and tile
+  static constexpr int kSmem = kParts * kQuery + 4 * kTile + 2 * (kKeys + 4 * kGroups);
+};
+
+// Byte offset of 16-byte chunk c of a row, chunks swizzled so that 8 rows' reads of one chunk touch every bank.
+template <int NB>
+__device__ __forceinline__ uint32_t at(int row, int c) {
+  return static_cast<uint32_t>(row * (NB * 64) + ((c ^ (row & 7)) << 4));
+}
+
+__device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename E>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<E, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename E>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<E, __nv_bfloat16>::value)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// What a value leaves after its rounding to E.
+template <typename E>
+__device__ __forceinline__ float rest(float x) {
+  return x - Elem<E>::to_float(Elem<E>::from_float(x));
+}
+
+}  // namespace
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
+    mxfp4_prefill_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
+  using C = PfCfg<T, NB>;
+  using E = typename C::E;
+  constexpr int D = C::D, kParts = C::kParts;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *tiles = smem + kParts * C::kQuery;  // [2][K, V]
+  uint8_t *nan_v = tiles + 4 * C::kTile;       // [2][keys]: NaN blocks of V, a bit each
+  int *group_ok = reinterpret_cast<int *>(nan_v + 2 * kKeys);  // [2][groups]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_wait();
+
+  const int seq = blockIdx.z, kvh = blockIdx.y;
+  const int tile = (gridDim.x - 1 - blockIdx.x) / p.num_splits;  // the last rows, with the most keys, first
+  const int split = (gridDim.x - 1 - blockIdx.x) % p.num_splits;
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int64_t q0 = p.cu_seqlens_q[seq];
+  const int64_t q_len = p.cu_seqlens_q[seq + 1] - q0;
+  const int64_t row0 = static_cast<int64_t>(tile) * kRows;
+  if (row0 >= q_len * G) return;
+  int64_t ctx = static_cast<int64_t>(p.cu_seqlens_k[seq + 1]) - p.cu_seqlens_k[seq];
+  const int64_t prefix = ctx - q_len;
+  if (ctx > p.bt_stride * p.block_size) {
+    if (threadIdx.x == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+    ctx = p.bt_stride * p.block_size;
+  }
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), q_len * G - row0));
+  const int64_t last_pos = prefix + by_group.div(static_cast<uint32_t>(row0 + rows - 1));
+  const int keys = static_cast<int>(max(int64_t{0}, min(ctx, last_pos + 1)));
+  const int all_tiles = (keys + kKeys - 1) / kKeys;
+  const int per_split = (all_tiles + p.num_splits - 1) / p.num_splits;
+  const int k_begin = split * per_split, k_end = min(all_tiles, k_begin + per_split);
+
+  // q into shared memory, as `kParts` operands
+  for (int i = threadIdx.x; i < kRows * (D / 8); i += kThreads) {
+    const int r = i / (D / 8), c = i % (D / 8);
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = 0.f;
+    const uint32_t row = static_cast<uint32_t>(row0) + r;
+    const int64_t token = q0 + by_group.div(row);
+    if (r < rows && token >= 0 && token < p.num_tokens) {
+      const T *src = static_cast<const T *>(p.query) +
+                     (token * p.num_q_heads + kvh * G + (row - by_group.div(row) * G)) * D + c * 8;
+      if constexpr (C::kSplit) {
+        const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      } else {
+        float2 f[4];
+        Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(src), f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[2 * u] = f[u].x, x[2 * u + 1] = f[u].y;
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      *reinterpret_cast<uint4 *>(smem + part * C::kQuery + at<NB>(r, c)) =
+          make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
+      if (part + 1 < kParts)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = rest<E>(x[u]);
+    }
+  }
+
+  // A thread's code words of a tile: word i is (group, block, token, quarter) in the order of memory.
+  struct Words {
+    uint32_t k[C::kWords], v[C::kWords];
+    uint32_t scales[C::kWords];  // K's byte, V's byte, whether the page is one
+  };
+  const int per_page = p.block_size / kMxGroup;
+  const int32_t *table = p.block_tables + seq * p.bt_stride;
+  const int j = threadIdx.x & 3, tok = (threadIdx.x >> 2) & 15, combo = threadIdx.x >> 6;  // 4 (group, block) at a time
+  auto fetch = [&](int kt, Words &w) {
+#pragma unroll
+    for (int i = 0; i < C::kWords; ++i) {
+      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB;
+      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + group;
+      w.k[i] = w.v[i] = 0;
+      w.scales[i] = 1u << 16;  // keys that do not exist: zeros
+      if (static_cast<int>(index) * kMxGroup + tok >= keys) continue;
+      const uint32_t col = by_page.div(index);
+      const int page = __ldg(table + col);
+      if (page < 0 || page >= p.num_blocks) {
+        w.scales[i] = 0;
+        continue;
+      }
+      const int64_t off = ((static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page + (index - col * per_page)) *
+                          (NB * kMxBytes);
+      const int code = b * kMxBlockBytes + tok * 16 + j * 4, scale = NB * kMxBlockBytes + tok * NB + b;
+      w.k[i] = *reinterpret_cast<const uint32_t *>(p.key_pages + off + code);
+      w.v[i] = *reinterpret_cast<const uint32_t *>(p.value_pages + off + code);
+      w.scales[i] |= p.key_pages[off + scale] | static_cast<uint32_t>(p.value_pages[off + scale]) << 8;
+    }
+  };
+  auto place = [&](const Words &w, int buf) {
+    uint8_t *kt = tiles + buf * 2 * C::kTile, *vt = kt + C::kTile;
+#pragma unroll
+    for (int i = 0; i < C::kWords; ++i) {
+      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB, key = group * kMxGroup + tok;
+      const uint32_t ks = w.scales[i] & 255u, vs = (w.scales[i] >> 8) & 255u;
+      float x[8];
+      mx_codes_to_f32(w.k[i], mx_scale(ks), x);
+      *reinterpret_cast<uint4 *>(kt + at<NB>(key, b * 4 + j)) =
+          make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
+      mx_codes_to_f32(vs == 255u ? 0u : w.v[i], vs == 255u ? 0.f : mx_scale(vs), x);
+      *reinterpret_cast<uint4 *>(vt + at<NB>(key, b * 4 + j)) =
+          make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
+      if (tok == 0 && j == 0 && b == 0) {
+        const bool ok = (w.scales[i] >> 16) != 0;
+        group_ok[buf * kGroups + group] = ok;
+        if (!ok) flag_status(p.status, MI_DEV_BAD_BLOCK);
+      }
+    }
+  };
+  // NaN blocks of V: found by one lane per key (its codes' neighbours hold the same bytes)
+  auto note_nan = [&](const Words &w, int buf) -> bool {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < C::kWords; ++i) any |= ((w.scales[i] >> 8) & 255u) == 255u;
+    if (threadIdx.x < kKeys) nan_v[buf * kKeys + threadIdx.x] = 0;
+    return any;
+  };
+  auto mark_nan = [&](const Words &w, int buf) {
+#pragma unroll
+    for (int i = 0; i < C::kWords; ++i) {
+      const int gb = combo + 4 * i, key = gb / NB * kMxGroup + tok;
+      if (((w.scales[i] >> 8) & 255u) == 255u && j == 0)
+        atomicOr(reinterpret_cast<unsigned *>(nan_v + buf * kKeys) + key / 4, 1u << (key % 4 * 8 + gb % NB));
+    }
+  };
+
+  // this thread's rows: g and g + 8 of its warp's 16
+  int pos[2];  // positions are below 2^31 as contexts are
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = warp * 16 + g + 8 * i;
+    pos[i] = r < rows ? static_cast<int>(prefix + by_group.div(static_cast<uint32_t>(row0) + r)) : -1;
+  }
+  const int first_pos = static_cast<int>(prefix + by_group.div(static_cast<uint32_t>(row0) + min(warp * 16, rows - 1)));
+  // m follows the largest score, up to kLag binades behind it: p <= 2^(kLift + kLag) is within f16
+  constexpr float kLift = std::is_same<E, __half>::value ? 12.f : 0.f, kLag = 3.f;
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+  bool has_nan = false;
+  if (k_begin < k_end) {
+    Words w;
+    fetch(k_begin, w);
+    place(w, 0);
+    const bool mine = note_nan(w, 0);
+    has_nan = __syncthreads_or(mine);
+    if (has_nan) {
+      mark_nan(w, 0);
+      __syncthreads();
+    }
+  }
+  const uint32_t q_base = smem_addr(smem), t_base = smem_addr(tiles);
+  const int mi = lane >> 3, rr = lane & 7;
+#pragma unroll 1
+  for (int kt = k_begin; kt < k_end; ++kt) {
+    const int buf = (kt - k_begin) & 1;
+    Words w;
+    const bool more = kt + 1 < k_end;
+    if (more) fetch(kt + 1, w);
+    const uint32_t k_base = t_base + buf * 2 * C::kTile, v_base = k_base + C::kTile;
+    float s[kKeys / 8][4];
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t a[kParts][4];
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+        ldsm(q_base + part * C::kQuery + at<NB>(warp * 16 + (mi & 1) * 8 + rr, ks * 2 + (mi >> 1)), a[part]);
+#pragma unroll
+      for (int n = 0; n < kKeys / 16; ++n) {  // 16 keys: dims lo, hi of keys 0-7, then of keys 8-15
+        uint32_t b[4];
+        ldsm(k_base + at<NB>(n * 16 + (mi >> 1) * 8 + rr, ks * 2 + (mi & 1)), b);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          mma<E>(s[2 * n], a[part], b[0], b[1]);
+          mma<E>(s[2 * n + 1], a[part], b[2], b[3]);
+        }
+      }
+    }
+    const int key0 = kt * kKeys;
+    bool pages = true;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) pages &= group_ok[buf * kGroups + i] != 0;
+    const bool masked = key0 + kKeys - 1 > first_pos || key0 + kKeys > keys || !pages;  // uniform in the warp
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s[i][u] *= p.scale_log2;
+        if (masked) {
+          const int key = key0 + i * 8 + 2 * t + (u & 1);
+          if (key > pos[u >> 1] || key >= keys || !group_ok[buf * kGroups + i / 2]) s[i][u] = -INFINITY;
+        }
+        top[u >> 1] = fmaxf(top[u >> 1], s[i][u]);
+      }
+    }
+    if (__any_sync(kAll, top[0] > m[0] + kLag || top[1] > m[1] + kLag)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(kAll, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(kAll, top[i], 2));
+        const float next = fmaxf(m[i], top[i]);
+        const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - next);
+        l[i] *= f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][2 * i] *= f, o[n][2 * i + 1] *= f;
+        m[i] = next;
+      }
+    }
+    float base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) base[i] = m[i] == -INFINITY ? 0.f : kLift - m[i];  // no key yet: exp2(-inf) = 0
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        s[i][u] = fast_exp2(s[i][u] + base[u >> 1]);
+        l[u >> 1] += s[i][u];
+      }
+#pragma unroll
+    for (int ks = 0; ks < kKeys / 16; ++ks) {
+      uint32_t a[kParts][4];
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          a[part][2 * u] = pack<E>(s[2 * ks + u][0], s[2 * ks + u][1]);
+          a[part][2 * u + 1] = pack<E>(s[2 * ks + u][2], s[2 * ks + u][3]);
+          if (part + 1 < kParts)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[2 * ks + u][c] = rest<E>(s[2 * ks + u][c]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {  // 16 dims: keys lo, hi of dims 0-7, then of dims 8-15
+        uint32_t b[4];
+        ldsm_t(v_base + at<NB>(ks * 16 + (mi & 1) * 8 + rr, n * 2 + (mi >> 1)), b);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          mma<E>(o[2 * n], a[part], b[0], b[1]);
+          mma<E>(o[2 * n + 1], a[part], b[2], b[3]);
+        }
+      }
+    }
+    if (has_nan) {  // uniform in the CTA
+#pragma unroll 1
+      for (int key = 0; key < kKeys; ++key) {
+        const unsigned blocks = nan_v[buf * kKeys + key];
+        if (!blocks) continue;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          if (!(blocks >> (n / 4) & 1u)) continue;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (key0 + key <= pos[u >> 1]) o[n][u] = __uint_as_float(0x7fffffffu);
+        }
+      }
+    }
+    if (more) {
+      place(w, buf ^ 1);
+      const bool mine = note_nan(w, buf ^ 1);
+      has_nan = __syncthreads_or(mine);
+      if (has_nan) {
+        mark_nan(w, buf ^ 1);
+        __syncthreads();
+      }
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(kAll, l[i], 1);
+    l[i] += __shfl_xor_sync(kAll, l[i], 2);
+    const int r = warp * 16 + g + 8 * i;
+    if (r >= rows) continue;
+    const uint32_t row = static_cast<uint32_t>(row0) + r;
+    const int64_t token = q0 + by_group.div(row);
+    if (token < 0 || token >= p.num_tokens) {
+      flag_status(p.status, MI_DEV_BAD_SLOT);
+      continue;
+    }
+    const int64_t at_row = token * p.num_q_heads + kvh * G + (row - by_group.div(row) * G);
+    if (p.num_splits == 1) {
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      T *out = static_cast<T *>(p.out) + at_row * D + 2 * t;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) {
+        if constexpr (C::kSplit)
+          *reinterpret_cast<float2 *>(out + n * 8) = make_float2(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+        else
+          *reinterpret_cast<uint32_t *>(out + n * 8) = pack<E>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+      }
+    } else {
+      float *st = p.workspace + (split * p.num_tokens * p.num_q_heads + at_row) * (D + 2);
+      if (t == 0) st[0] = m[i], st[1] = l[i];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2 *>(st + 2 + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+  }
+  pdl_launch_dependents();
+}
+
+// Join the splits: a warp to a row, the rows of the sequences only.
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads) mxfp4_prefill_join_kernel(const MxPrefillParams p, const FastDiv by_group) {
+  constexpr int D = NB * kMxBlock;
+  pdl_wait();
+  const int seq = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31;
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int64_t q0 = p.cu_seqlens_q[seq];
+  const int64_t rows = (p.cu_seqlens_q[seq + 1] - q0) * G;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (row < rows) {
+    const int64_t token = q0 + by_group.div(static_cast<uint32_t>(row));
+    if (token >= 0 && token < p.num_tokens) {
+      const int64_t at_row =
+          token * p.num_q_heads + kvh * G + (row - by_group.div(static_cast<uint32_t>(row)) * static_cast<int64_t>(G));
+      const int64_t stride = p.num_tokens * p.num_q_heads * (D + 2);
+      const float *st = p.workspace + at_row * (D + 2);
+      float M = -INFINITY, L = 0.f, A[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) A[b] = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < p.num_splits; ++s, st += stride) {
+        const float m = __ldcg(st), l = __ldcg(st + 1);
+        float a[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) a[b] = __ldcg(st + 2 + b * 32 + lane);
+        if (m == -INFINITY && l == 0.f) continue;  // no keys
+        const float next = fmaxf(M, m);
+        const float f = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : fast_exp2(M - next);
+        const float e = m == -INFINITY ? 1.f : fast_exp2(m - next);
+        L = f * L + e * l;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) A[b] = f * A[b] + e * a[b];
+        M = next;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        static_cast<T *>(p.out)[at_row * D + b * 32 + lane] = Elem<T>::from_float(L == 0.f ? 0.f : A[b] / L);
+    }
+  }
+  pdl_launch_dependents();
+}
+
+namespace {
+
+template <typename T, int NB>
+cudaError_t launch_pf(const MxPrefillParams &p, int64_t num_seqs, int64_t max_seqlen_q, cudaStream_t stream) {
+  using C = PfCfg<T, NB>;
+  auto kern = mxfp4_prefill_kernel<T, NB>;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int64_t tiles = (max_seqlen_q * G + kRows - 1) / kRows;
+  const FastDiv by_group(G), by_page(p.block_size / kMxGroup);
+  cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.num_splits), p.num_kv_heads,
+                                        static_cast<unsigned>(num_seqs)),
+                             dim3(kThreads), C::kSmem, stream, p, by_group, by_page);
+  if (e == cudaSuccess && p.num_splits > 1)
+    e = launch_pdl(mxfp4_prefill_join_kernel<T, NB>,
+                   dim3(static_cast<unsigned>((max_seqlen_q * G + kThreads / 32 - 1) / (kThreads / 32)),
+                        p.num_kv_heads, static_cast<unsigned>(num_seqs)),
+                   dim3(kThreads), 0, stream, p, by_group);
+  return e;
+}
+
+template <typename T>
+cudaError_t launch_pf_t(const MxPrefillParams &p, int head_dim, int64_t num_seqs, int64_t max_seqlen_q,
+                        cudaStream_t stream) {
+  return head_dim == 64 ? launch_pf<T, 2>(p, num_seqs, max_seqlen_q, stream)
+                        : launch_pf<T, 4>(p, num_seqs, max_seqlen_q, stream);
+}
+
+}  // namespace
+
+bool mxfp4_prefill_supported(int head_dim) { return head_dim == 64 || head_dim == 128; }
+
+// Splits over the keys: enough CTAs for two per SM, each split at least 4 tiles of a full table.
+int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
+                         int64_t capacity, int sms) {
+  const int64_t rows = max_seqlen_q * (num_q_heads / num_kv_heads);
+  const int64_t ctas = (rows + kRows - 1) / kRows * num_kv_heads * num_seqs;
+  int64_t s = 2 * sms / ctas;
+  const int64_t most = capacity / (4 * kKeys);
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+cudaError_t launch_mxfp4_prefill(const MxPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
+                                 int64_t max_seqlen_q, cudaStream_t stream) {
+  if (dtype == MI_DTYPE_BFLOAT16) return launch_pf_t<__nv_bfloat16>(p, head_dim, num_seqs, max_seqlen_q, stream);
+  if (dtype == MI_DTYPE_FLOAT16) return launch_pf_t<__half>(p, head_dim, num_seqs, max_seqlen_q, stream);
+  return launch_pf_t<float>(p, head_dim, num_seqs, max_seqlen_q, stream);
+}
+
+}  // namespace mi

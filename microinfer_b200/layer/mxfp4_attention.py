@@ -5,10 +5,11 @@
 * ``gather_paged_kv_mxfp4``     rows in logical order, as ``gather_paged_kv``
 * ``paged_attention_mxfp4_meta``  dispatch on the step's metadata, as ``paged_attention_meta``
 
-Decode reads the codes and decodes them in registers.  Prefill decodes each
+Decode reads the codes and decodes them in registers.  Prefill of a large chunk decodes each
 context once into a workspace of the query's type and attends to that with the
 dense tensor-core kernel: a chunk of n tokens does 4 * n * Hq flops for each of the
-Hkv elements decoded, so the extra pass is a few percent of a chunk of ordinary size.
+Hkv elements decoded, so the extra pass is a few percent.  Small chunks, and shapes that kernel does not
+take, are computed from the pages.
 Workspaces come from torch's allocator for the length of the call, so that calls on several
 streams, and captured graphs, each have their own.
 """
@@ -150,6 +151,28 @@ def gather_paged_kv_mxfp4(key_pages, value_pages, block_tables, contexts, *,
     return keys, values
 
 
+@lru_cache(maxsize=4096)
+def _prefill_workspace_bytes(*shape):
+    return _lib.load().mi_paged_prefill_mxfp4_workspace_bytes(*shape)
+
+
+@lru_cache(maxsize=4096)
+def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
+    """Whether prefill reads the pages itself instead of gathering for the dense kernel.
+
+    It does where the tcgen05 kernel does not take the shape, and where that would leave three
+    quarters of the SMs without a tile of 128 rows: reading the pages splits the keys
+    (64 tokens on 16000, 32/8 heads of 128: 113 us, gathered 295; 256 tokens: 438 and 297).
+    """
+    if d not in (64, 128):
+        return False
+    lib = _lib.load()
+    if lib.mi_prefill_kernel_for(dtype, d, hq, hkv, 0) != 2:
+        return True
+    tiles = requests * hkv * -(-max_seqlen_q * (hq // hkv) // 128)
+    return 4 * tiles <= lib.mi_device_sm_count(device)
+
+
 def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, *,
                         max_seqlen_q: int, total_k: int | None = None, scale: float | None = None,
                         out: torch.Tensor | None = None) -> torch.Tensor:
@@ -188,10 +211,27 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
         return torch.zeros_like(query) if out is None else out.zero_()
     query, block_tables = _aligned(query), _idx(block_tables)
     cu_seqlens_q, cu_seqlens_k = _idx(cu_seqlens_q), _idx(cu_seqlens_k)
+    tokens, hq, _ = query.shape
+    most = min(rows, width * bs)  # keys of one request
+    dtype = _lib.dtype_code(query.dtype)
+    if _reads_pages(dtype, hq, hkv, d, requests, int(max_seqlen_q), device.index or 0):
+        if out is None:
+            out = torch.empty_like(query)
+        shape = (requests, tokens, int(max_seqlen_q), hq, hkv, d, most, device.index or 0)
+        need = _prefill_workspace_bytes(*shape)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _lib.call(
+            "mi_paged_prefill_mxfp4", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),
+            value_pages.data_ptr(), dims[0], bs, hq, hkv, d, dtype,
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), block_tables.data_ptr(), width,
+            requests, tokens, int(max_seqlen_q), most,
+            1.0 / math.sqrt(d) if scale is None else float(scale), _lib.ptr(workspace), need,
+            _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
+        )
+        return out
     keys = torch.empty((rows, hkv, d), dtype=query.dtype, device=device)
     values = torch.empty_like(keys)
-    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows,
-            min(rows, width * bs))
+    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most)
     return varlen_prefill(query, keys, values, cu_seqlens_q, cu_seqlens_k,
                           max_seqlen_q=max_seqlen_q, scale=scale, out=out)
 
