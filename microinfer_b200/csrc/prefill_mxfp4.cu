@@ -149,6 +149,9 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
         for (int u = 0; u < 4; ++u) x[2 * u] = f[u].x, x[2 * u + 1] = f[u].y;
       }
     }
+    if (p.scale_log2 < 0.f)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = -x[u];
 #pragma unroll
     for (int part = 0; part < kParts; ++part) {
       *reinterpret_cast<uint4 *>(smem + part * C::kQuery + at<NB>(r, c)) =
@@ -235,6 +238,9 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   }
   const int first_pos = static_cast<int>(prefix + by_group.div(static_cast<uint32_t>(row0) + min(warp * 16, rows - 1)));
   // m follows the largest score, up to kLag binades behind it: p <= 2^(kLift + kLag) is within f16
+  // q goes in with the sign of the scale, so that the largest product is the largest score; a scale of 0
+  // becomes one that leaves every score at 0
+  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
   constexpr float kLift = std::is_same<E, __half>::value ? 12.f : 0.f, kLag = 3.f;
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -252,15 +258,22 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       __syncthreads();
     }
   }
-  const uint32_t q_base = smem_addr(smem), t_base = smem_addr(tiles);
+  // ldmatrix addresses: the swizzle only touches bits 4 to 6, so a lane's row and chunk parity go into a
+  // base and even chunk 2n is one exclusive or (and an immediate offset past 8 chunks)
   const int mi = lane >> 3, rr = lane & 7;
+  const uint32_t q_lane = (smem_addr(smem) + (warp * 16 + (mi & 1) * 8 + rr) * C::kRowBytes) | ((rr ^ (mi >> 1)) << 4);
+  const uint32_t k_lane = (((mi >> 1) * 8 + rr) * C::kRowBytes) | ((rr ^ (mi & 1)) << 4);
+  const uint32_t v_lane = (((mi & 1) * 8 + rr) * C::kRowBytes) | ((rr ^ (mi >> 1)) << 4);
+  const uint32_t t_base = smem_addr(tiles);
+  auto even_chunk = [](uint32_t lane_base, int n) { return (lane_base ^ ((2 * n & 7) << 4)) + (n >> 2) * 128; };
 #pragma unroll 1
   for (int kt = k_begin; kt < k_end; ++kt) {
     const int buf = (kt - k_begin) & 1;
     Words w;
     const bool more = kt + 1 < k_end;
     if (more) fetch(kt + 1, w);
-    const uint32_t k_base = t_base + buf * 2 * C::kTile, v_base = k_base + C::kTile;
+    const uint32_t k_base = t_base + buf * 2 * C::kTile + k_lane;
+    const uint32_t v_base = t_base + buf * 2 * C::kTile + C::kTile + v_lane;
     float s[kKeys / 8][4];
 #pragma unroll
     for (int i = 0; i < kKeys / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -269,11 +282,11 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       uint32_t a[kParts][4];
 #pragma unroll
       for (int part = 0; part < kParts; ++part)
-        ldsm(q_base + part * C::kQuery + at<NB>(warp * 16 + (mi & 1) * 8 + rr, ks * 2 + (mi >> 1)), a[part]);
+        ldsm(even_chunk(q_lane, ks) + part * C::kQuery, a[part]);
 #pragma unroll
       for (int n = 0; n < kKeys / 16; ++n) {  // 16 keys: dims lo, hi of keys 0-7, then of keys 8-15
         uint32_t b[4];
-        ldsm(k_base + at<NB>(n * 16 + (mi >> 1) * 8 + rr, ks * 2 + (mi & 1)), b);
+        ldsm(even_chunk(k_base, ks) + n * 16 * C::kRowBytes, b);
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           mma<E>(s[2 * n], a[part], b[0], b[1]);
@@ -291,7 +304,6 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     for (int i = 0; i < kKeys / 8; ++i) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        s[i][u] *= p.scale_log2;
         if (masked) {
           const int key = key0 + i * 8 + 2 * t + (u & 1);
           if (key > pos[u >> 1] || key >= keys || !group_ok[buf * kGroups + i / 2]) s[i][u] = -INFINITY;
@@ -299,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
         top[u >> 1] = fmaxf(top[u >> 1], s[i][u]);
       }
     }
+    top[0] *= scale, top[1] *= scale;
     if (__any_sync(kAll, top[0] > m[0] + kLag || top[1] > m[1] + kLag)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        s[i][u] = fast_exp2(s[i][u] + base[u >> 1]);
+        s[i][u] = fast_exp2(fmaf(s[i][u], scale, base[u >> 1]));
         l[u >> 1] += s[i][u];
       }
 #pragma unroll
@@ -339,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {  // 16 dims: keys lo, hi of dims 0-7, then of dims 8-15
         uint32_t b[4];
-        ldsm_t(v_base + at<NB>(ks * 16 + (mi & 1) * 8 + rr, n * 2 + (mi >> 1)), b);
+        ldsm_t(even_chunk(v_base, n) + ks * 16 * C::kRowBytes, b);
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           mma<E>(o[2 * n], a[part], b[0], b[1]);
