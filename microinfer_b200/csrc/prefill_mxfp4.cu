@@ -170,26 +170,32 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   const int per_page = p.block_size / kMxGroup;
   const int32_t *table = p.block_tables + seq * p.bt_stride;
   const int j = threadIdx.x & 3, tok = (threadIdx.x >> 2) & 15, combo = threadIdx.x >> 6;  // 4 (group, block) at a time
+  // Pages of a tile's words are looked up a tile before their codes: kNone past the keys.
+  constexpr int kNone = INT32_MIN;
+  int pages_at[C::kWords];
+  auto look_up = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < C::kWords; ++i) {
+      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + (combo + 4 * i) / NB;
+      pages_at[i] = kNone;
+      if (static_cast<int>(index) * kMxGroup + tok < keys) pages_at[i] = max(-1, __ldg(table + by_page.div(index)));
+    }
+  };
   auto fetch = [&](int kt, Words &w) {
 #pragma unroll
     for (int i = 0; i < C::kWords; ++i) {
-      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB;
-      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + group;
+      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB, page = pages_at[i];
       w.k[i] = w.v[i] = 0;
-      w.scales[i] = 1u << 16;  // keys that do not exist: zeros
-      if (static_cast<int>(index) * kMxGroup + tok >= keys) continue;
-      const uint32_t col = by_page.div(index);
-      const int page = __ldg(table + col);
-      if (page < 0 || page >= p.num_blocks) {
-        w.scales[i] = 0;
-        continue;
-      }
-      const int64_t off = ((static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page + (index - col * per_page)) *
+      w.scales[i] = page == kNone ? 1u << 16 : 0u;  // keys that do not exist: zeros
+      if (page < 0 || page >= p.num_blocks) continue;
+      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + group;
+      const int64_t off = ((static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page +
+                           (index - by_page.div(index) * per_page)) *
                           (NB * kMxBytes);
       const int code = b * kMxBlockBytes + tok * 16 + j * 4, scale = NB * kMxBlockBytes + tok * NB + b;
       w.k[i] = *reinterpret_cast<const uint32_t *>(p.key_pages + off + code);
       w.v[i] = *reinterpret_cast<const uint32_t *>(p.value_pages + off + code);
-      w.scales[i] |= p.key_pages[off + scale] | static_cast<uint32_t>(p.value_pages[off + scale]) << 8;
+      w.scales[i] = p.key_pages[off + scale] | static_cast<uint32_t>(p.value_pages[off + scale]) << 8 | 1u << 16;
     }
   };
   auto place = [&](const Words &w, int buf) {
@@ -249,7 +255,9 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   bool has_nan = false;
   if (k_begin < k_end) {
     Words w;
+    look_up(k_begin);
     fetch(k_begin, w);
+    look_up(k_begin + 1);
     place(w, 0);
     const bool mine = note_nan(w, 0);
     has_nan = __syncthreads_or(mine);
@@ -271,7 +279,10 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     const int buf = (kt - k_begin) & 1;
     Words w;
     const bool more = kt + 1 < k_end;
-    if (more) fetch(kt + 1, w);
+    if (more) {
+      fetch(kt + 1, w);
+      look_up(kt + 2);
+    }
     const uint32_t k_base = t_base + buf * 2 * C::kTile + k_lane;
     const uint32_t v_base = t_base + buf * 2 * C::kTile + C::kTile + v_lane;
     float s[kKeys / 8][4];
