@@ -415,6 +415,39 @@ def test_decode_large_values_with_no_weight(cuda_device, name):
 
 
 @gpu
+def test_decode_more_sequences_than_one_launch_takes(cuda_device):
+    rng = np.random.default_rng(21)
+    ctxs = rng.integers(0, 20, 2500).tolist()
+    got, want, dtype = _decode_case(cuda_device, "bf16", 1, 4, 64, 16, ctxs)
+    mi.check_device_status(cuda_device)
+    _close(got, *want, dtype, DECODE_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+def test_decode_many_keys_of_little_weight(cuda_device, name):
+    """One key takes nearly everything and its value is zero: the rest of a long context, each key about 2^-20
+    of it, decides the result."""
+    ctx, d = 9000, 64
+    rng = np.random.default_rng(22)
+    nb = ctx // 16 + 2
+    kc, kb = mo.encode(rng.standard_normal((nb, 16, 1, d)) * 0.01)
+    vc, vb = mo.encode(rng.standard_normal((nb, 16, 1, d)) + 1.0)
+    table = _table(rng, [ctx], nb, 16)
+    sink = table[0, 3], 5
+    kc[sink], kb[sink] = 2, 127  # all 1.0
+    vc[sink], vb[sink] = 0, 0
+    kp, vp = mo.pack(kc, kb), mo.pack(vc, vb)
+    query = _cuda(np.full((1, 4, d), 1.0), cuda_device, DTYPES[name])
+    scale = 14.0 / d  # the sink is exp(14) = 2^20 above the others
+    got = mi.paged_decode_mxfp4(query, _cuda(kp, cuda_device), _cuda(vp, cuda_device), _cuda(table, cuda_device),
+                                torch.tensor([ctx], dtype=torch.int32, device=cuda_device), scale=scale)
+    want = mo.attention(np.full((1, 4, d), 1.0), mo.rows(kp, table[0], ctx), mo.rows(vp, table[0], ctx), scale)
+    assert 0.001 < np.abs(want[0]).max() < 0.1
+    _close(got, *want, DTYPES[name], DECODE_STEP[DTYPES[name]])
+
+
+@gpu
 @pytest.mark.parametrize("name", ["bf16", "f32"])
 def test_decode_ignores_what_lies_past_the_context(cuda_device, name):
     """Stale rows of the last page and pages past the context hold NaN scales; columns past it bad ids."""
@@ -567,28 +600,99 @@ def test_cache_past_32_bit_offsets(cuda_device):
 PREFILL_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -10, torch.float32: 0.0}
 
 
-@gpu
-@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("hkv,group,d,bs", [(8, 2, 128, 16), (2, 4, 64, 64), (1, 3, 96, 32)])
-def test_prefill_matches_the_formula(cuda_device, name, hkv, group, d, bs):
-    rng = np.random.default_rng(d + group)
+def _prefill_case(device, name, hkv, group, d, bs, q_lens, ctxs, seed=0, scale=None, edit=None, **kw):
+    rng = np.random.default_rng(seed + d + group)
     dtype = DTYPES[name]
-    q_lens, ctxs = [1, 40, 7, 130, 1], [90, 40, 135, 201, 1]
     nb = sum(-(-c // bs) for c in ctxs) + 2
     kp, vp = _pages(rng, nb, bs, hkv, d)
     table = _table(rng, ctxs, nb, bs)
-    query = _cuda(rng.standard_normal((sum(q_lens), hkv * group, d)), cuda_device, dtype)
-    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=cuda_device) for x in (q_lens, ctxs))
-    args = (query, _cuda(kp, cuda_device), _cuda(vp, cuda_device), cu_q, cu_k, _cuda(table, cuda_device))
-    got = mi.paged_prefill_mxfp4(*args, max_seqlen_q=max(q_lens), total_k=sum(ctxs))
-    free = mi.paged_prefill_mxfp4(*args, max_seqlen_q=max(q_lens))
-    mi.check_device_status(cuda_device)
-    assert torch.equal(got, free)
+    if edit is not None:
+        edit(kp, vp, table)
+    query = _cuda(rng.standard_normal((sum(q_lens), hkv * group, d)), device, dtype)
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=device) for x in (q_lens, ctxs))
+    args = (query, _cuda(kp, device), _cuda(vp, device), cu_q, cu_k, _cuda(table, device))
+    got = mi.paged_prefill_mxfp4(*args, max_seqlen_q=max(q_lens), total_k=sum(ctxs), scale=scale, **kw)
+    free = mi.paged_prefill_mxfp4(*args, max_seqlen_q=max(q_lens), scale=scale)
+    mi.check_device_status(device)
     q = query.double().cpu().numpy()
     at = np.cumsum([0, *q_lens])
-    parts = [mo.attention(q[at[r]:at[r + 1]], mo.rows(kp, table[r], c), mo.rows(vp, table[r], c), d ** -0.5)
-             for r, c in enumerate(ctxs)]
-    _close(got, *(np.concatenate(x) for x in zip(*parts)), dtype, PREFILL_STEP[dtype])
+    parts = [mo.attention(q[at[r]:at[r + 1]], mo.rows(kp, table[r], c), mo.rows(vp, table[r], c),
+                          d ** -0.5 if scale is None else scale) for r, c in enumerate(ctxs)]
+    return got, free, [np.concatenate(x) for x in zip(*parts)], dtype
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("hkv,group,d,bs", [
+    (8, 2, 128, 16), (2, 4, 64, 64), (1, 3, 96, 32), (2, 7, 128, 32), (1, 5, 64, 16), (1, 16, 64, 256), (4, 1, 128, 48)])
+def test_prefill_matches_the_formula(cuda_device, name, hkv, group, d, bs):
+    q_lens, ctxs = [1, 40, 7, 130, 1], [90, 40, 135, 201, 1]
+    got, free, want, dtype = _prefill_case(cuda_device, name, hkv, group, d, bs, q_lens, ctxs)
+    for x in (got, free):  # the bound on the contexts only decides the split over the keys
+        _close(x, *want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_lens,ctxs", [([3], [5000]), ([64], [2000]), ([1, 17], [4097, 63]), ([33], [33])])
+def test_prefill_small_chunks_over_long_contexts(cuda_device, name, d, q_lens, ctxs):
+    got, free, want, dtype = _prefill_case(cuda_device, name, 2, 4, d, 16, q_lens, ctxs)
+    for x in (got, free):
+        _close(x, *want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("scale", [2.0, 0.0, -0.3])
+def test_prefill_scales(cuda_device, name, scale):
+    got, _, want, dtype = _prefill_case(cuda_device, name, 1, 3, 64, 16, [50, 20], [70, 150], scale=scale)
+    _close(got, *want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_nan_blocks_reach_only_rows_that_see_them(cuda_device, name, d):
+    """A NaN value block of a key in the chunk: NaN in its 32 dims for the rows from it on; a NaN key block: those
+    rows alone."""
+    place = {}
+
+    def edit(kp, vp, table):
+        kc, kb = mo.unpack(kp)
+        vc, vb = mo.unpack(vp)
+        vb[table[0, 60 // 16], 60 % 16, 0, 1] = 255  # position 60 of 90, row 10 of 40
+        kb[table[0, 80 // 16], 80 % 16, 0, 0] = 255  # position 80, row 30
+        kp[:], vp[:] = mo.pack(kc, kb), mo.pack(vc, vb)
+
+    got, _, _, _ = _prefill_case(cuda_device, name, 1, 3, d, 16, [40], [90], edit=edit)
+    nan = torch.isnan(got).cpu()
+    assert not bool(nan[:10].any()) and bool(nan[30:].all())
+    assert bool(nan[10:30, :, 32:64].all()) and int(nan[10:30].sum()) == 20 * 3 * 32
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_leaves_rows_of_no_sequence_and_flags_bad_pages(cuda_device, d):
+    rng = np.random.default_rng(31)
+    kp, vp = _pages(rng, 6, 16, 1, d)
+    query = torch.randn(12, 2, d, device=cuda_device, dtype=torch.float16)
+    cu_q = torch.tensor([0, 3, 8], dtype=torch.int32, device=cuda_device)
+    cu_k = torch.tensor([0, 20, 60], dtype=torch.int32, device=cuda_device)
+    table = torch.tensor([[0, 1, -1], [2, 3, 4]], dtype=torch.int32, device=cuda_device)
+    out = torch.full_like(query, 7.0)
+    args = (query, _cuda(kp, cuda_device), _cuda(vp, cuda_device), cu_q, cu_k)
+    mi.paged_prefill_mxfp4(*args, table, max_seqlen_q=5, out=out)
+    mi.check_device_status(cuda_device)
+    assert bool((out[8:] == 7.0).all()) and not bool((out[:8] == 7.0).all(-1).any())
+    table[1, 1] = 9
+    mi.paged_prefill_mxfp4(*args, table, max_seqlen_q=5)
+    assert mi.read_device_status(cuda_device) == _lib.DEV_BAD_BLOCK
+    # a context past the table's columns
+    cu_k[2] = 20 + 70
+    table[1, 1] = 3
+    mi.paged_prefill_mxfp4(*args, table, max_seqlen_q=5)
+    assert mi.read_device_status(cuda_device) & _lib.DEV_BAD_BLOCK
 
 
 @gpu
