@@ -160,7 +160,9 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    status = getattr(_lib or load(), name)(*args)
+    if status != 0:
+        check(status)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -45,7 +45,8 @@ def _check_query(query, hkv, d, out):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
+    if not t.is_contiguous():
+        return t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -92,14 +93,12 @@ def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens
     return out
 
 
-def _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most):
-    nb, bs, hkv, d = dims
-    device = key_pages.device
+def _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most, device):
+    requests, width = block_tables.shape
     _lib.call(
         "mi_gather_paged_kv_mxfp4", keys.data_ptr(), values.data_ptr(), key_pages.data_ptr(),
-        value_pages.data_ptr(), nb, bs, hkv, d, _lib.dtype_code(keys.dtype),
-        block_tables.data_ptr(), block_tables.shape[1], cu_seqlens_k.data_ptr(),
-        block_tables.shape[0], rows, most, _lib.status_buffer(device).data_ptr(),
+        value_pages.data_ptr(), *dims, _lib.dtype_code(keys.dtype), block_tables.data_ptr(), width,
+        cu_seqlens_k.data_ptr(), requests, rows, most, _lib.status_buffer(device).data_ptr(),
         _lib.stream_of(device),
     )
 
@@ -115,12 +114,13 @@ def gather_paged_kv_mxfp4(key_pages, value_pages, block_tables, contexts, *,
     """
     dims = page_dims(key_pages, value_pages)
     _, bs, hkv, d = dims
-    device = _lib.require_cuda(key_pages, value_pages, block_tables)
+    device = _lib.require_cuda(key_pages, value_pages, block_tables, cu_seqlens_k)
     contexts = [int(c) for c in contexts]
-    if any(c < 0 for c in contexts):
-        raise ValueError("contexts must be non-negative")
-    if block_tables.ndim != 2 or len(contexts) != block_tables.shape[0]:
+    table_shape = block_tables.shape
+    if len(table_shape) != 2 or len(contexts) != table_shape[0]:
         raise ValueError("one context per block-table row")
+    if contexts and min(contexts) < 0:
+        raise ValueError("contexts must be non-negative")
     total = sum(contexts)
     if out is None:
         _lib.dtype_code(dtype)
@@ -129,14 +129,15 @@ def gather_paged_kv_mxfp4(key_pages, value_pages, block_tables, contexts, *,
     else:
         keys, values = out
         want = (total, hkv, d)
-        if (tuple(keys.shape) != want or tuple(values.shape) != want or keys.dtype != values.dtype
+        if (keys.shape != want or values.shape != want or keys.dtype != values.dtype
                 or not (keys.is_contiguous() and values.is_contiguous())):
             raise ValueError("out must be two contiguous [sum(contexts), Hkv, D] tensors of one dtype")
         _lib.dtype_code(keys.dtype)
         _lib.require_cuda(key_pages, keys, values)
     if total == 0:
         return keys, values
-    if max(contexts) > block_tables.shape[1] * bs:
+    most = max(contexts)
+    if most > table_shape[1] * bs:
         raise ValueError("a context is longer than its block-table row")
     if cu_seqlens_k is None:
         cu = [0]
@@ -145,9 +146,8 @@ def gather_paged_kv_mxfp4(key_pages, value_pages, block_tables, contexts, *,
         cu_seqlens_k = torch.tensor(cu, dtype=torch.int32).to(device, non_blocking=True)
     elif cu_seqlens_k.shape != (len(contexts) + 1,):
         raise ValueError("cu_seqlens_k must have num_requests + 1 entries")
-    _lib.require_cuda(key_pages, cu_seqlens_k)
     _gather(keys, values, key_pages, value_pages, dims, _idx(block_tables), _idx(cu_seqlens_k),
-            total, max(contexts))
+            total, most, device)
     return keys, values
 
 
@@ -231,7 +231,8 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
         return out
     keys = torch.empty((rows, hkv, d), dtype=query.dtype, device=device)
     values = torch.empty_like(keys)
-    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most)
+    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most,
+            device)
     return varlen_prefill(query, keys, values, cu_seqlens_q, cu_seqlens_k,
                           max_seqlen_q=max_seqlen_q, scale=scale, out=out)
 

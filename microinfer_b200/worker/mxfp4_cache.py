@@ -21,7 +21,6 @@ import torch
 
 from microinfer_b200 import _lib
 from microinfer_b200.worker.kv_cache import copy_blocks
-from microinfer_b200.worker.kv_store import _check_kv_rows
 
 GROUP = 16  # tokens of a group
 MX = 32  # elements that share a scale
@@ -52,10 +51,15 @@ def store_kv_mxfp4(key_pages, value_pages, slots, keys, values):
         torch.ops.microinfer_b200.store_kv_mxfp4(key_pages, value_pages, slots, keys, values)
         return
     nb, bs, hkv, d = page_dims(key_pages, value_pages)
-    _check_kv_rows(keys, values)
-    tokens = keys.shape[0]
-    if keys.shape[1] != hkv or keys.shape[2] != d:
+    shape = keys.shape
+    if len(shape) != 3 or values.shape != shape:
+        raise ValueError("K/V shapes differ")
+    tokens, heads, dim = shape
+    if heads != hkv or dim != d:
         raise ValueError("K/V heads do not match the cache")
+    key_stride, value_stride = keys.stride(), values.stride()
+    if key_stride[1:] != (d, 1) or value_stride[1:] != (d, 1):
+        raise ValueError("K/V inner dimensions must be contiguous")
     if keys.dtype != values.dtype:
         raise ValueError("K/V must share a dtype")
     dtype = _lib.dtype_code(keys.dtype)
@@ -65,12 +69,11 @@ def store_kv_mxfp4(key_pages, value_pages, slots, keys, values):
     if tokens == 0:
         return
     device = _lib.require_cuda(key_pages, value_pages, slots, keys, values)
-    if not slots.is_contiguous():
-        slots = slots.contiguous()
+    slots = slots.contiguous()
     _lib.call(
         "mi_store_kv_mxfp4", key_pages.data_ptr(), value_pages.data_ptr(), nb, bs, hkv, d,
-        slots.data_ptr(), index, keys.data_ptr(), values.data_ptr(), dtype, keys.stride(0),
-        values.stride(0), tokens, _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
+        slots.data_ptr(), index, keys.data_ptr(), values.data_ptr(), dtype, key_stride[0],
+        value_stride[0], tokens, _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
     )
 
 
