@@ -32,9 +32,10 @@
 // Work: the units of 32 keys of all (sequence, kv head, 4 or 8 query heads)
 // segments, in that order, are one list that is cut into equal ranges, one per
 // warp (one CTA to an SM), so ragged batches and single long
-// sequences load every SM alike.  A warp streams its range through a ring of bulk copies
-// (one of K and one of V per group, 139 to 157 KB in flight per SM at D = 128)
-// that runs across segment borders.  Segments that lie within one
+// sequences load every SM alike.  A warp streams its range through a ring of its own, two units
+// deep, that runs across segment borders (139 KB in flight per SM with 16 warps at D = 128, 104 KB with 12).
+// Its lanes fill it with 16-byte cp.async; four bulk copies a unit, waited for on an
+// mbarrier, took 5 to 9% longer (96 x 8192, 32/8 heads of 128: 168 us, now 155).  Segments that lie within one
 // warp's range are written at once; the parts of others are joined in shared
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
@@ -76,10 +77,9 @@ struct MxCfg {
   static constexpr int kSmemUnits = kWarps * 64 * 16;     // two batches of 32 units per warp
   static constexpr int kQuery = CT * NB * 512;            // q's B fragments, per warp
   static constexpr int kSmemQuery = kWarps * kQuery;
-  static constexpr int kSmemBars = kWarps * kStages * 8;
   static constexpr int kSmemPrefix = (kMaxSeqs + 1) * 4;
   static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kHeads * 12 + 16;
-  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemQuery + kSmemBars + kSmemPrefix +
+  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemQuery + kSmemPrefix +
                                kSmemMisc;
   static_assert(kState * 4 <= kRing, "a warp's last part goes into its own ring");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -620,8 +620,8 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
   int4 *unit_table = reinterpret_cast<int4 *>(smem + C::kSmemRing + C::kSmemHeads);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery);
-  int *prefix = reinterpret_cast<int *>(bars + kWarps * kStages);  // units of a segment before sequence s
+  int *prefix =
+      reinterpret_cast<int *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery);  // units of a segment before sequence s
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
   int *scan = part_flags + 2 * kWarps;      // [2 * kWarps]
@@ -630,7 +630,6 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
   float2 *run_ml = reinterpret_cast<float2 *>(                   // [2 * kWarps][heads]
       (reinterpret_cast<uintptr_t>(factor + 2 * kWarps * C::kHeads) + 15) & ~static_cast<uintptr_t>(15));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t *wbar = bars + warp * kStages;
   uint8_t *ring = smem + warp * C::kRing;
   const int n = static_cast<int>(p.num_seqs);
   const int G = p.num_q_heads / p.num_kv_heads;
@@ -649,17 +648,9 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
     }
     return ctx > 0 ? (ctx - 1) / kUnit + 1 : 0;
   };
-  auto setup_barriers = [&] {  // while the lengths are on their way
-    if (lane == 0) {
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) mbar_init(&wbar[s], 1);
-      fence_mbar_init();
-      part_seg[2 * warp] = part_seg[2 * warp + 1] = -1;
-    }
-  };
+  if (lane == 0) part_seg[2 * warp] = part_seg[2 * warp + 1] = -1;
   if (n <= 32) {  // every warp for itself
     const int c = units_of(lane);
-    setup_barriers();
     int incl = c;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -680,7 +671,6 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
       sum += c[i];
       c_max = max(c_max, c[i]);
     }
-    setup_barriers();
     int incl = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -796,21 +786,31 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
     }
     __syncwarp();
   };
-  // Lanes 4s to 4s + 3 bring unit first + s: K (lanes 0, 1) and V (2, 3) of its groups.
-  const uint8_t *my_pages = lane & 2 ? p.value_pages : p.key_pages;
-  const uint32_t my_place = smem_addr(ring) + (lane & 3) * C::kGroup;
-  const uint32_t my_bar = smem_addr(wbar);
-  auto issue = [&](int i, int at) {  // unit i to stage `at`, by four lanes
-    if ((lane & 3) == 0)
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(my_bar + at * 8), "r"(C::kStage)
-                   : "memory");
-    const int where = reinterpret_cast<const int *>(table + (i & 63))[lane & 1];
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-            my_place + at * C::kStage),
-        "l"(my_pages + static_cast<int64_t>(where) * C::kGroup), "r"(C::kGroup), "r"(my_bar + at * 8)
-        : "memory");
+  // Copies of unit i to stage `at`, K and V of its two groups: 16 bytes a lane, whole rows of 32 lanes,
+  // then what is left of the four runs in one.
+  constexpr int kVecs = C::kGroup / 16, kFull = kVecs / 32, kLeft = kVecs % 32;
+  const uint32_t my_place = smem_addr(ring) + lane * 16;
+  const uint8_t *my_keys = p.key_pages + lane * 16, *my_values = p.value_pages + lane * 16;
+  const int left_run = lane / kLeft, left_at = (kFull * 32 + lane % kLeft) * 16;
+  const uint8_t *my_left = (left_run & 2 ? p.value_pages : p.key_pages) + left_at;
+  const uint32_t my_left_place = smem_addr(ring) + left_run * C::kGroup + left_at;
+  auto copy16 = [](uint32_t to, const uint8_t *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
   };
+  auto issue = [&](int i, int at) {
+    const int2 where = *reinterpret_cast<const int2 *>(table + (i & 63));
+    const uint32_t to = my_place + at * C::kStage;
+#pragma unroll
+    for (int run = 0; run < 4; ++run) {
+      const uint8_t *from = (run & 2 ? my_values : my_keys) + static_cast<int64_t>(run & 1 ? where.y : where.x) * C::kGroup;
+#pragma unroll
+      for (int v = 0; v < kFull; ++v) copy16(to + run * C::kGroup + v * 512, from + v * 512);
+    }
+    if (lane < 4 * kLeft)
+      copy16(my_left_place + at * C::kStage,
+             my_left + static_cast<int64_t>(left_run & 1 ? where.y : where.x) * C::kGroup);
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
   MxWarp<T, NB, CT> st;
   st.setup(smem_addr(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + warp * C::kQuery));
@@ -840,20 +840,21 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
 
   // The first segment's q is asked for before the ring's copies, which would keep it waiting.
   typename MxWarp<T, NB, CT>::Raw raw;
-  const int ahead = min(kStages, units);
   if (units > 0) {
     const Unit r = unit_of(min(lane, units - 1));
     place(__shfl_sync(kAll, r.seq * H + r.ht, 0));
     st.fetch_query(static_cast<const T *>(p.query) + row * D, heads, raw);
     load_batch(lane, r);
-    if ((lane >> 2) < ahead) issue(lane >> 2, lane >> 2);
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      if (i < units) issue(i, i);
+      commit();
+    }
     st.set_query(raw, p.scale_log2);
   }
 
-  bool timed_out = false, fresh = true;
-  int stage = 0, stop = 0;
-  uint32_t phase = 0;
+  bool fresh = true;
+  int stage = 0;
 #pragma unroll 1
   for (int i = 0; i < units; ++i) {
     if ((i & 31) == 0 && i + 32 < units)  // into the half that units i - 32 to i - 1 have left
@@ -870,27 +871,18 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
       st.reset();
       fresh = true;
     }
-    if (!mbar_wait_bounded(&wbar[stage], phase, p.status)) {
-      timed_out = true;
-      stop = i;
-      break;
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");  // this lane's copies of unit i
+    __syncwarp();                                                         // every lane's
     const bool special = what != kUnit || fresh;
     if (!(what & kNoPage)) {
       st.process(smem_addr(ring) + stage * C::kStage, special, what & 63, fresh);
       fresh = false;
     }
     __syncwarp();  // every lane has read the stage
-    if (i + kStages < units && lane < 4) issue(i + kStages, stage);
-    __syncwarp();
+    if (i + kStages < units) issue(i + kStages, stage);
+    commit();
     if (what & kEnds) end_segment((what & kLast) != 0, i == units - 1);
-    if (++stage == kStages) stage = 0, phase ^= 1;
-  }
-  if (timed_out) {  // the copies in flight land before the ring is given up
-    if (lane == 0)
-      for (int k = stop; k < min(stop + kStages, units); ++k)
-        if (!mbar_wait_bounded(&wbar[k % kStages], (k / kStages) & 1, p.status)) break;
-    __syncwarp();
+    if (++stage == kStages) stage = 0;
   }
   __syncthreads();
 
