@@ -37,6 +37,8 @@ def page_dims(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple[int, 
     if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
         raise ValueError("pages must be contiguous")
     blocks, hkv, groups, size = shape
+    if hkv == 0 or groups == 0:
+        raise ValueError("pages must have kv heads and tokens")
     if size == 0 or size % MX_BYTES:
         raise ValueError(f"the last dimension of pages must be head_dim / {MX} * {MX_BYTES} bytes")
     return blocks, groups * GROUP, hkv, size // MX_BYTES * MX

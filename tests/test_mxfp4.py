@@ -154,6 +154,16 @@ def test_refusals_before_any_launch():
         mi.gather_paged_kv_mxfp4(pages, pages, table, [1, 1, 1])
 
 
+@pytest.mark.parametrize("shape", [(4, 0, 1, 544), (4, 2, 0, 544), (4, 2, 1, 0)])
+def test_pages_without_heads_or_tokens_are_refused(shape):
+    pages = torch.zeros(shape, dtype=torch.uint8)
+    table, lens = torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="pages"):
+        mi.paged_decode_mxfp4(torch.zeros(3, 4, 64), pages, pages, table, lens)
+    with pytest.raises(ValueError, match="pages"):
+        mi.gather_paged_kv_mxfp4(pages, pages, table, [1, 1, 1])
+
+
 def test_c_entries_refuse_bad_arguments():
     lib = _lib.load()
     buf = ctypes.create_string_buffer(64)
