@@ -74,11 +74,11 @@ def paged_decode_mxfp4(query, key_pages, value_pages, block_tables, context_lens
     if context_lens.shape != (n,):
         raise ValueError("context_lens must have one entry per request")
     if n == 0:
-        return torch.empty_like(query) if out is None else out
+        return query.new_empty(query.shape) if out is None else out
     device = _lib.require_cuda(query, key_pages, value_pages, block_tables, context_lens)
     width = table_shape[1]
     if width == 0:  # no request can have a key
-        return torch.zeros_like(query) if out is None else out.zero_()
+        return query.new_zeros(query.shape) if out is None else out.zero_()
     query, block_tables, context_lens = _aligned(query), _idx(block_tables), _idx(context_lens)
     if out is None:
         out = torch.empty_like(query)
@@ -198,7 +198,7 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
     if cu_seqlens_q.shape != (requests + 1,) or cu_seqlens_k.shape != (requests + 1,):
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have num_requests + 1 entries")
     if query.shape[0] == 0 or requests == 0:
-        return torch.empty_like(query) if out is None else out
+        return query.new_empty(query.shape) if out is None else out
     if max_seqlen_q <= 0:
         raise ValueError("max_seqlen_q must be positive")
     if total_k is not None and total_k < 0:
@@ -208,7 +208,7 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
     if total_k is not None:
         rows = min(rows, int(total_k))
     if rows == 0:  # no request can have a key
-        return torch.zeros_like(query) if out is None else out.zero_()
+        return query.new_zeros(query.shape) if out is None else out.zero_()
     query, block_tables = _aligned(query), _idx(block_tables)
     cu_seqlens_q, cu_seqlens_k = _idx(cu_seqlens_q), _idx(cu_seqlens_k)
     tokens, hq, _ = query.shape

@@ -131,7 +131,7 @@ def paged_decode_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_pages
 
 @paged_decode_mxfp4.register_fake
 def _(query, key_pages, value_pages, block_tables, context_lens, scale=None):
-    return torch.empty_like(query)
+    return query.new_empty(query.shape)  # contiguous, whatever the query's strides
 
 
 @torch.library.custom_op(f"{_NS}::paged_prefill_mxfp4", mutates_args=())
@@ -147,4 +147,4 @@ def paged_prefill_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_page
 @paged_prefill_mxfp4.register_fake
 def _(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, max_seqlen_q,
       total_k=None, scale=None):
-    return torch.empty_like(query)
+    return query.new_empty(query.shape)  # contiguous, whatever the query's strides

@@ -164,6 +164,19 @@ def test_pages_without_heads_or_tokens_are_refused(shape):
         mi.gather_paged_kv_mxfp4(pages, pages, table, [1, 1, 1])
 
 
+def test_fake_results_are_contiguous_like_the_real_ones():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        query = torch.empty(4, 3, 64).transpose(0, 1)
+        pages = torch.empty(4, 2, 1, 544, dtype=torch.uint8)
+        table, lens, cu = (torch.empty(n, dtype=torch.int32) for n in ((3, 1), 3, 4))
+        ops = torch.ops.microinfer_b200
+        for got in (ops.paged_decode_mxfp4(query, pages, pages, table, lens),
+                    ops.paged_prefill_mxfp4(query, pages, pages, cu, cu, table, 1)):
+            assert got.shape == query.shape and got.is_contiguous()
+
+
 def test_c_entries_refuse_bad_arguments():
     lib = _lib.load()
     buf = ctypes.create_string_buffer(64)
@@ -814,3 +827,55 @@ def test_under_torch_compile(cuda_device):
     want = fn(q, k, v, kt.clone(), vt.clone())
     got = torch.compile(fn, fullgraph=True, backend="aot_eager")(q, k, v, kt, vt)
     assert torch.equal(got, want)
+
+
+@gpu
+def test_transposed_query_under_torch_compile(cuda_device):
+    rng = np.random.default_rng(14)
+    kp, vp = _pages(rng, 6, 16, 2, 64)
+    kt, vt = _cuda(kp, cuda_device), _cuda(vp, cuda_device)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([20, 32], dtype=torch.int32, device=cuda_device)
+    cu_q = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda_device)
+    cu_k = torch.tensor([0, 20, 52], dtype=torch.int32, device=cuda_device)
+    heads_first = torch.randn(4, 2, 64, device=cuda_device, dtype=torch.bfloat16)
+
+    def fn(x):
+        q = x.transpose(0, 1)
+        a = mi.paged_decode_mxfp4(q, kt, vt, table, lens)
+        b = mi.paged_prefill_mxfp4(q, kt, vt, cu_q, cu_k, table, max_seqlen_q=1)
+        return a.view(2, 256), b.view(2, 256)
+
+    for got, want in zip(torch.compile(fn, fullgraph=True, backend="aot_eager")(heads_first), fn(heads_first)):
+        assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_results_over_the_query_and_shared_pages(cuda_device, name, d):
+    """`out` may be the query itself; rows of the table may name the same pages, and one page twice."""
+    rng = np.random.default_rng(15)
+    dtype = DTYPES[name]
+    kp, vp = _pages(rng, 40, 16, 2, d)
+    pages = _cuda(kp, cuda_device), _cuda(vp, cuda_device)
+    one = rng.integers(0, 40, 200).astype(np.int32)
+    one[7] = one[3]
+    table = _cuda(np.stack([one, one, one[::-1]]), cuda_device)
+    lens = torch.tensor([3200, 3185, 1700], dtype=torch.int32, device=cuda_device)
+    query = _cuda(rng.standard_normal((3, 8, d)), cuda_device, dtype)
+    q = query.double().cpu().numpy()
+    names = [one, one, one[::-1]]
+    parts = [mo.attention(q[r:r + 1], mo.rows(kp, names[r], int(c)), mo.rows(vp, names[r], int(c)), d ** -0.5)
+             for r, c in enumerate(lens.tolist())]
+    want = [np.concatenate(x) for x in zip(*parts)]
+    over = query.clone()
+    assert mi.paged_decode_mxfp4(over, *pages, table, lens, out=over) is over
+    _close(over, *want, dtype, DECODE_STEP[dtype])
+    over = query.clone()
+    cu_q = torch.arange(4, dtype=torch.int32, device=cuda_device)
+    cu_k = torch.cat([cu_q[:1], lens.cumsum(0).int()])
+    if d != 96:  # computed from the pages: the rows are read before they are written
+        mi.paged_prefill_mxfp4(over, *pages, cu_q, cu_k, table, max_seqlen_q=1, out=over)
+        _close(over, *want, dtype, PREFILL_STEP[dtype])
+    mi.check_device_status(cuda_device)
