@@ -1,5 +1,5 @@
-// Paged decode over the 4-bit cache on the warp-level tensor cores (head_dim 64 or 128, any type
-// and GQA group; other shapes: decode_mxfp4.cu).
+// Paged decode over the 4-bit cache (layout: mxfp4.cuh) on the warp-level tensor cores: one query
+// token per sequence, out = softmax(scale * K q) V, any type, head_dim and GQA group.
 //
 // Decode moves 4.25 bits per cached element and does 2 flops per element and
 // query head on it, so the bound is HBM as long as turning codes into MMA
@@ -61,12 +61,15 @@ constexpr uint32_t kLowestRef = 0x20202020u;  // R_b - 255 then has a bit of 0xf
 constexpr int kAlignedSlack = 1;    // units per warp that keeping a segment in one CTA may cost
 
 // NB blocks of 32 per head, CT column tiles of 4 query heads, SPLIT: fp32.  One tile leaves the registers for
-// 16 warps, two at D = 128 and fp32 for 12.
+// 16 warps, two at D = 128 and fp32 for 12; past D = 128 shared memory holds the rings of 8 (and one tile).
 template <int NB, int CT, bool SPLIT>
 struct MxCfg {
   static constexpr int D = NB * kMxBlock;
-  static constexpr int kWarps = (CT == 1 || NB == 2) && !SPLIT ? 16 : 12;
+  static constexpr int kWarps = NB > 4 ? 8 : (CT == 1 || NB <= 2) && !SPLIT ? 16 : 12;
   static constexpr int kStages = 2;
+  // Scale bytes are held four to a word, a word per 4 blocks of a key; at D = 64 a word has two keys'.
+  static constexpr int kQuads = (NB + 3) / 4;
+  static constexpr bool kBytes = NB != 2 && NB % 4 != 0;  // a key's bytes do not make words in memory
   static constexpr int kHeads = CT * kQueries;    // query heads of a segment
   static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
   static constexpr int kStage = 4 * kGroup;       // K of two groups, V of two groups
@@ -157,7 +160,8 @@ __device__ __forceinline__ float exp2i(int e) {
   return __uint_as_float(static_cast<uint32_t>(a + 127) << 23) * __uint_as_float(static_cast<uint32_t>(b + 127) << 23);
 }
 
-// The codes of a group as MMA A fragments.  NB registers for keys 0-7 and 8-15 each.
+// The codes of a group as MMA A fragments: its 2 NB matrices of 8 keys x 16 bytes lie one after the other.
+// NB registers for keys 0-7 and 8-15 each.
 template <int NB, bool TRANS>
 __device__ __forceinline__ void load_codes(uint32_t base, int lane, uint32_t (&lo)[NB], uint32_t (&hi)[NB]) {
   const int mi = lane >> 3, rr = lane & 7;
@@ -171,11 +175,16 @@ __device__ __forceinline__ void load_codes(uint32_t base, int lane, uint32_t (&l
       ldsm4(addr + 128, hi[0], hi[1], hi[2], hi[3]);
     }
   } else {
-    const uint32_t addr = base + (mi >> 1) * kMxBlockBytes + (mi & 1) * 128 + rr * 16;
-    if constexpr (TRANS)
-      ldsm4t(addr, lo[0], hi[0], lo[1], hi[1]);
-    else
-      ldsm4(addr, lo[0], hi[0], lo[1], hi[1]);
+#pragma unroll
+    for (int b = 0; b < NB; b += 2) {
+      uint32_t lo1, hi1;  // an odd NB's last block is read twice
+      const uint32_t addr = base + b * kMxBlockBytes + (b + 1 < NB ? lane : lane & 15) * 16;
+      if constexpr (TRANS)
+        ldsm4t(addr, lo[b], hi[b], lo1, hi1);
+      else
+        ldsm4(addr, lo[b], hi[b], lo1, hi1);
+      if (b + 1 < NB) lo[b + 1 < NB ? b + 1 : 0] = lo1, hi[b + 1 < NB ? b + 1 : 0] = hi1;
+    }
   }
 }
 
@@ -185,21 +194,41 @@ __device__ __forceinline__ float scale_of(uint32_t w, int b) {
   return __uint_as_float((v & 0x7f800000u) | 1u);
 }
 
-// V's scales of a group: words of keys 2t, 2t + 1 (w[0], w[1]) and 2t + 8, 2t + 9 (w[2], w[3]); at
-// D = 64 a key pair has one word.
-template <int NB>
-__device__ __forceinline__ void load_scales(uint32_t vbase, int t, uint32_t (&w)[4]) {
+__device__ __forceinline__ uint32_t lds8(uint32_t addr) {
+  uint32_t r;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(addr));
+  return r;
+}
+
+// V's scales of a group, words of blocks 4i to 4i + 3: of keys 2t, 2t + 1 (w[i][0], w[i][1]) and 2t + 8, 2t + 9
+// (w[i][2], w[i][3]); at D = 64 a key pair has one word.  Bytes of blocks that do not exist are kPadScale.
+constexpr uint32_t kPadScale = kLowestRef & 255u;
+template <int NB, int Q>
+__device__ __forceinline__ void load_scales(uint32_t vbase, int t, uint32_t (&w)[Q][4]) {
+  const uint32_t at = vbase + NB * kMxBlockBytes;
   if constexpr (NB == 4) {
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                 : "=r"(w[0]), "=r"(w[1])
-                 : "r"(vbase + NB * kMxBlockBytes + t * 8));
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                 : "=r"(w[2]), "=r"(w[3])
-                 : "r"(vbase + NB * kMxBlockBytes + t * 8 + 32));
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0][0]), "=r"(w[0][1]) : "r"(at + t * 8));
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0][2]), "=r"(w[0][3]) : "r"(at + t * 8 + 32));
+  } else if constexpr (NB == 2) {
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0][0]) : "r"(at + t * 4));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0][2]) : "r"(at + t * 4 + 16));
+    w[0][1] = w[0][3] = 0;
+  } else if constexpr (NB == 8) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[0][k]), "=r"(w[1][k]), "=r"(w[0][k + 1]), "=r"(w[1][k + 1])
+                   : "r"(at + t * 16 + k * 32));
   } else {
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(vbase + NB * kMxBlockBytes + t * 4));
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[2]) : "r"(vbase + NB * kMxBlockBytes + t * 4 + 16));
-    w[1] = w[3] = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        w[i][k] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          w[i][k] |= (4 * i + b < NB ? lds8(at + (2 * t + (k & 1) + (k >> 1) * 8) * NB + 4 * i + b) : kPadScale) << (8 * b);
+      }
   }
 }
 
@@ -210,12 +239,13 @@ struct MxWarp {
   using C = MxCfg<NB, CT, kSplit>;
   static constexpr int D = C::D;
   static constexpr int kParts = kSplit ? 2 : 1;  // f16 parts of p
+  static constexpr int Q = C::kQuads;
   uint32_t q;                 // shared address of this lane's B fragments of q (columns 2i and 2i + 1 both
                               // query i of the tile): 4 words per block, 512 bytes between blocks
   float xs[CT];               // log2-domain scale of query t
   float o[CT][NB][4];         // query t, dims 32b + 4g + 0 to 3, times 2^(R_b - 127)
   float m[CT], l[CT];         // query t; l: this lane's keys only
-  uint32_t ref;               // R_b, one byte per block
+  uint32_t ref[Q];            // R_b, one byte per block
   uint32_t pick0, pick1;      // byte selectors: a pair's first (second) half to this lane's column, zeros
   int lane, g, t;
 
@@ -226,7 +256,8 @@ struct MxWarp {
   }
 
   __device__ __forceinline__ void reset() {
-    ref = kLowestRef;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) ref[i] = kLowestRef;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
 #pragma unroll
@@ -301,17 +332,24 @@ struct MxWarp {
   // Scores of a unit's 32 keys for query t, still to be scaled by xs: x[j][c][0], key g of group j;
   // x[j][c][1], its key g + 8.
   __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[2][CT][2]) const {
-    uint32_t lo[2][NB], hi[2][NB], wl[2], wh[2];
+    constexpr int kWords = C::kBytes ? NB : Q;  // scales of a key: bytes of their own, or words of four
+    uint32_t lo[2][NB], hi[2][NB], wl[2][kWords], wh[2][kWords];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint32_t base = kbase + j * C::kGroup;
+      const uint32_t base = kbase + j * C::kGroup, at = base + NB * kMxBlockBytes + g * NB;
       load_codes<NB, false>(base, lane, lo[j], hi[j]);
       if constexpr (NB == 4) {
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl[j]) : "r"(base + NB * kMxBlockBytes + g * 4));
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh[j]) : "r"(base + NB * kMxBlockBytes + g * 4 + 32));
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wl[j][0]) : "r"(at));
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wh[j][0]) : "r"(at + 8 * NB));
+      } else if constexpr (NB == 2) {
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl[j][0]) : "r"(at));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh[j][0]) : "r"(at + 8 * NB));
+      } else if constexpr (NB == 8) {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wl[j][0]), "=r"(wl[j][1]) : "r"(at));
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wh[j][0]), "=r"(wh[j][1]) : "r"(at + 8 * NB));
       } else {
-        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wl[j]) : "r"(base + NB * kMxBlockBytes + g * 2));
-        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(wh[j]) : "r"(base + NB * kMxBlockBytes + g * 2 + 16));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) wl[j][b] = lds8(at + b), wh[j][b] = lds8(at + 8 * NB + b);
       }
     }
 #pragma unroll
@@ -327,7 +365,8 @@ struct MxWarp {
         uint32_t a[4], e[4];
         mx_codes_to_f16(lo[j][b], a);
         mx_codes_to_f16(hi[j][b], e);
-        const float fl = scale_of(wl[j], b), fh = scale_of(wh[j], b);
+        const float fl = C::kBytes ? scale_of(wl[j][b % kWords], 0) : scale_of(wl[j][b / 4 % kWords], b % 4);
+        const float fh = C::kBytes ? scale_of(wh[j][b % kWords], 0) : scale_of(wh[j][b / 4 % kWords], b % 4);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           float d[4];
@@ -342,27 +381,35 @@ struct MxWarp {
   }
 
   // Scale bytes of keys that do not exist become `with`'s.
-  __device__ __forceinline__ void mask_scales(uint32_t (&w)[4], int valid, uint32_t with) const {
+  __device__ __forceinline__ void mask_scales(uint32_t (&w)[Q][4], int valid, const uint32_t (&with)[Q]) const {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (2 * t + (k & 1) + (k >> 1) * 8 < valid) continue;
-      if constexpr (NB == 4)
-        w[k] = with;
-      else
-        w[k & 2] = k & 1 ? (w[k & 2] & 0xffffu) | with << 16 : (w[k & 2] & 0xffff0000u) | (with & 0xffffu);
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        if constexpr (NB == 2)
+          w[i][k & 2] = k & 1 ? (w[i][k & 2] & 0xffffu) | with[i] << 16 : (w[i][k & 2] & 0xffff0000u) | (with[i] & 0xffffu);
+        else
+          w[i][k] = with[i];
+      }
     }
   }
 
   // How far below the reference each scale is, per byte: 0 to 7, or a bit of 0xf8 is set in the result.
-  __device__ __forceinline__ uint32_t distances(const uint32_t (&w)[4], uint32_t (&d)[4]) const {
-    if constexpr (NB == 4) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) d[k] = ref - w[k];
-      return (d[0] | d[1] | d[2] | d[3]) & 0xf8f8f8f8u;
+  __device__ __forceinline__ uint32_t distances(const uint32_t (&w)[Q][4], uint32_t (&d)[Q][4]) const {
+    if constexpr (NB == 2) {
+      const uint32_t both = (ref[0] & 0xffffu) * 0x10001u;
+      d[0][0] = both - w[0][0], d[0][2] = both - w[0][2];
+      return (d[0][0] | d[0][2]) & 0xf8f8f8f8u;
     } else {
-      const uint32_t both = (ref & 0xffffu) * 0x10001u;
-      d[0] = both - w[0], d[2] = both - w[2];
-      return (d[0] | d[2]) & 0xf8f8f8f8u;
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[i][k] = ref[i] - w[i][k];
+        any |= d[i][0] | d[i][1] | d[i][2] | d[i][3];
+      }
+      return any & 0xf8f8f8f8u;
     }
   }
 
@@ -370,18 +417,20 @@ struct MxWarp {
   // exponent 0: zero); p[part][c][k]: p of keys 2t, 2t + 1, 2t + 8, 2t + 9 in the half of this lane's
   // column, zero in the other (fp32: its upper f16, then its lower).  FAR: the products are `back` times what d says.
   template <bool FAR>
-  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[4], const uint32_t (&p)[kParts][CT][4],
+  __device__ __forceinline__ void values(uint32_t vbase, const uint32_t (&d)[Q][4], const uint32_t (&p)[kParts][CT][4],
                                          float back = 1.f) {
     uint32_t lo[NB], hi[NB];
     load_codes<NB, true>(vbase, lane, lo, hi);
     // f16 2^-d, two to a word: bytes 0 and 2 of d's word k, then bytes 1 and 3
-    uint32_t even[4], odd[4];
+    uint32_t even[Q][4], odd[Q][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (NB == 2 && (k & 1)) continue;
-      even[k] = 0x3c003c00u - (d[k] & 0x00ff00ffu) * 1024u;
-      odd[k] = 0x3c003c00u - (d[k] & 0xff00ff00u) * 4u;
-    }
+    for (int i = 0; i < Q; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (NB == 2 && (k & 1)) continue;
+        even[i][k] = 0x3c003c00u - (d[i][k] & 0x00ff00ffu) * 1024u;
+        odd[i][k] = 0x3c003c00u - (d[i][k] & 0xff00ff00u) * 4u;
+      }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       uint32_t a[4], e[4];
@@ -394,12 +443,12 @@ struct MxWarp {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t pk = p[half][c][k];
-          if constexpr (NB == 4) {
-            const uint32_t f = b & 1 ? odd[k] : even[k];
-            s[k] = b < 2 ? mul_f16x2_half<false>(pk, f) : mul_f16x2_half<true>(pk, f);
-          } else {
-            const uint32_t f = b & 1 ? odd[k & 2] : even[k & 2];
+          if constexpr (NB == 2) {
+            const uint32_t f = b & 1 ? odd[0][k & 2] : even[0][k & 2];
             s[k] = k & 1 ? mul_f16x2_half<true>(pk, f) : mul_f16x2_half<false>(pk, f);
+          } else {
+            const uint32_t f = b & 1 ? odd[b / 4][k] : even[b / 4][k];
+            s[k] = b % 4 < 2 ? mul_f16x2_half<false>(pk, f) : mul_f16x2_half<true>(pk, f);
           }
         }
         if constexpr (FAR) {
@@ -417,8 +466,8 @@ struct MxWarp {
   }
 
   // The largest byte of each block over the group's keys, from this lane's four.
-  __device__ __forceinline__ static uint32_t over_keys(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    uint32_t top = __vmaxu4(__vmaxu4(a, b), __vmaxu4(c, d));
+  __device__ __forceinline__ static uint32_t over_keys(const uint32_t (&w)[4]) {
+    uint32_t top = __vmaxu4(__vmaxu4(w[0], w[1]), __vmaxu4(w[2], w[3]));
     if constexpr (NB == 2) top = __vmaxu4(top, top >> 16) & 0xffffu;
     top = __vmaxu4(top, __shfl_xor_sync(kAll, top, 1));
     return __vmaxu4(top, __shfl_xor_sync(kAll, top, 2));
@@ -427,49 +476,57 @@ struct MxWarp {
   // As values() for scales that the window of 8 binades does not hold: raise R_b where a scale is above
   // it, then take the keys window by window.
   __device__ __forceinline__ void values_far(uint32_t vbase, const uint32_t (&p)[kParts][CT][4], int valid) {
-    uint32_t w[4], nan[4];
+    uint32_t w[Q][4], some[Q][4], bad[Q], any_bad = 0, deepest = 0;  // some: all ones where there is a scale
+    const uint32_t none[Q] = {};
     load_scales<NB>(vbase, t, w);
-    mask_scales(w, valid, 0);
+    mask_scales(w, valid, none);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      nan[k] = __vcmpeq4(w[k], 0xffffffffu);
-      w[k] &= ~nan[k];
+    for (int i = 0; i < Q; ++i) {
+      uint32_t nan[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        nan[k] = __vcmpeq4(w[i][k], 0xffffffffu);
+        w[i][k] &= ~nan[k];
+      }
+      bad[i] = over_keys(nan);
+      any_bad |= bad[i];
+      const uint32_t top = over_keys(w[i]);
+      const uint32_t above = __vcmpgtu4(top, ref[i]);
+      const uint32_t next = (ref[i] & ~above) | (__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu) & above);
+#pragma unroll
+      for (int b = 4 * i; b < NB && b < 4 * i + 4; ++b) {
+        const float f = exp2i(static_cast<int>((ref[i] >> (8 * (b % 4))) & 255u) -
+                              static_cast<int>((next >> (8 * (b % 4))) & 255u));
+#pragma unroll
+        for (int u = 0; u < CT * 4; ++u) o[u / 4][b][u % 4] *= f;
+      }
+      ref[i] = next;
+      const uint32_t all = NB == 2 ? (ref[i] & 0xffffu) * 0x10001u : ref[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        some[i][k] = __vcmpne4(w[i][k], 0u);
+        w[i][k] = (all - w[i][k]) & some[i][k];  // no byte is above the reference now
+      }
+      deepest = __vmaxu4(deepest, over_keys(w[i]));
     }
-    const uint32_t bad = over_keys(nan[0], nan[1], nan[2], nan[3]);
-    const uint32_t top = over_keys(w[0], w[1], w[2], w[3]);
-    const uint32_t above = __vcmpgtu4(top, ref);
-    const uint32_t next = (ref & ~above) | (__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu) & above);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const float f = exp2i(static_cast<int>((ref >> (8 * b)) & 255u) - static_cast<int>((next >> (8 * b)) & 255u));
-#pragma unroll
-      for (int i = 0; i < CT * 4; ++i) o[i / 4][b][i % 4] *= f;
-    }
-    ref = next;
-    const uint32_t all = NB == 4 ? ref : (ref & 0xffffu) * 0x10001u;
-    uint32_t some[4];  // all ones where there is a scale
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      some[k] = __vcmpne4(w[k], 0u);
-      w[k] = (all - w[k]) & some[k];  // no byte is above the reference now
-    }
-    uint32_t deepest = over_keys(w[0], w[1], w[2], w[3]);
     deepest = __vmaxu4(deepest, deepest >> 16);
     deepest = max(deepest & 255u, (deepest >> 8) & 255u);
 #pragma unroll 1
     for (uint32_t window = 0; window <= deepest / 8; ++window) {
-      uint32_t d[4];
+      uint32_t d[Q][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t in = __vcmpeq4((w[k] >> 3) & 0x1f1f1f1fu, window * 0x01010101u) & some[k];
-        d[k] = (w[k] & 0x07070707u & in) | (0x0f0f0f0fu & ~in);
-      }
+      for (int i = 0; i < Q; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t in = __vcmpeq4((w[i][k] >> 3) & 0x1f1f1f1fu, window * 0x01010101u) & some[i][k];
+          d[i][k] = (w[i][k] & 0x07070707u & in) | (0x0f0f0f0fu & ~in);
+        }
       values<true>(vbase, d, p, exp2i(-8 * static_cast<int>(window)));
     }
-    if (bad) {
+    if (any_bad) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        if (bad >> (8 * b) & 255u)
+        if (bad[b / 4] >> (8 * (b % 4)) & 255u)
 #pragma unroll
           for (int i = 0; i < CT * 4; ++i) o[i / 4][b][i % 4] = __uint_as_float(0x7fffffffu);
     }
@@ -481,7 +538,7 @@ struct MxWarp {
     const uint32_t vbase = base + 2 * C::kGroup;
     float x[2][CT][2];
     scores(base, x);
-    uint32_t w[2][4];
+    uint32_t w[2][Q][4];
     load_scales<NB>(vbase, t, w[0]);
     load_scales<NB>(vbase + C::kGroup, t, w[1]);
 #pragma unroll
@@ -490,11 +547,14 @@ struct MxWarp {
       for (int c = 0; c < CT; ++c) x[j][c][0] *= xs[c], x[j][c][1] *= xs[c];
     if (special) {  // uniform
       if (first) {  // R_b starts at the largest scale here and two binades of room
-        mask_scales(w[0], valid, 0);
-        mask_scales(w[1], valid - kMxGroup, 0);
-        const uint32_t top = __vmaxu4(over_keys(w[0][0], w[0][1], w[0][2], w[0][3]),
-                                      over_keys(w[1][0], w[1][1], w[1][2], w[1][3]));
-        ref = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
+        const uint32_t none[Q] = {};
+        mask_scales(w[0], valid, none);
+        mask_scales(w[1], valid - kMxGroup, none);
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          const uint32_t top = __vmaxu4(over_keys(w[0][i]), over_keys(w[1][i]));
+          ref[i] = __vmaxu4(__vminu4(__vaddus4(top, 0x02020202u), 0xfefefefeu), kLowestRef);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -547,7 +607,7 @@ struct MxWarp {
         }
       }
     }
-    uint32_t d[2][4];
+    uint32_t d[2][Q][4];
     const uint32_t far = distances(w[0], d[0]) | distances(w[1], d[1]);
     if (__any_sync(kAll, far != 0)) {
 #pragma unroll
@@ -566,7 +626,7 @@ struct MxWarp {
       for (int off = 4; off < 32; off <<= 1) l[c] += __shfl_xor_sync(kAll, l[c], off);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const float f = exp2i(static_cast<int>((ref >> (8 * b)) & 255u) - 127);
+        const float f = exp2i(static_cast<int>((ref[b / 4] >> (8 * (b % 4))) & 255u) - 127);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[c][b][i] *= f;
       }
@@ -787,7 +847,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
     __syncwarp();
   };
   // Copies of unit i to stage `at`, K and V of its two groups: 16 bytes a lane, whole rows of 32 lanes,
-  // then what is left of the four runs in one.
+  // then what is left of the four runs, in one where a row holds it.
   constexpr int kVecs = C::kGroup / 16, kFull = kVecs / 32, kLeft = kVecs % 32;
   const uint32_t my_place = smem_addr(ring) + lane * 16;
   const uint8_t *my_keys = p.key_pages + lane * 16, *my_values = p.value_pages + lane * 16;
@@ -805,8 +865,9 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
       const uint8_t *from = (run & 2 ? my_values : my_keys) + static_cast<int64_t>(run & 1 ? where.y : where.x) * C::kGroup;
 #pragma unroll
       for (int v = 0; v < kFull; ++v) copy16(to + run * C::kGroup + v * 512, from + v * 512);
+      if (kLeft > 8 && lane < kLeft) copy16(to + run * C::kGroup + kFull * 512, from + kFull * 512);
     }
-    if (lane < 4 * kLeft)
+    if (kLeft <= 8 && lane < 4 * kLeft)
       copy16(my_left_place + at * C::kStage,
              my_left + static_cast<int64_t>(left_run & 1 ? where.y : where.x) * C::kGroup);
   };
@@ -1076,57 +1137,68 @@ cudaError_t launch_mma(const MxDecodeParams &p, int tiles, bool join, int ctas, 
   return e;
 }
 
-// Column tiles of a segment, and segments of a kv head.
-int mma_columns(int num_q_heads, int num_kv_heads) { return num_q_heads / num_kv_heads <= kQueries ? 1 : 2; }
-int mma_tiles(int num_q_heads, int num_kv_heads) {
-  const int heads = kQueries * mma_columns(num_q_heads, num_kv_heads);
+// Column tiles of a segment (two rings' worth of sums do not fit past D = 128), and segments of a kv head.
+int mma_columns(int num_q_heads, int num_kv_heads, int head_dim) {
+  return num_q_heads / num_kv_heads <= kQueries || head_dim > 128 ? 1 : 2;
+}
+int mma_tiles(int num_q_heads, int num_kv_heads, int head_dim) {
+  const int heads = kQueries * mma_columns(num_q_heads, num_kv_heads, head_dim);
   return (num_q_heads / num_kv_heads + heads - 1) / heads;
 }
 
 // Whether some lengths that the table can hold need the second launch: not when
 // every segment has a CTA and a full table is no more than the slack per warp.
-bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t capacity, int sms) {
-  const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads);
-  constexpr int warps = MxCfg<4, 2, true>::kWarps;  // the fewest
+bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity, int sms) {
+  const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads, head_dim);
+  const int warps = head_dim > 128 ? MxCfg<8, 1, true>::kWarps : MxCfg<4, 2, true>::kWarps;  // the fewest
   return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * warps * kUnit;
 }
 
 template <typename T>
 cudaError_t launch_mma_t(const MxDecodeParams &p, int tiles, int columns, bool join, int ctas, cudaStream_t stream) {
-  if (p.head_dim == 64)
-    return columns == 1 ? launch_mma<T, 2, 1>(p, tiles, join, ctas, stream)
-                        : launch_mma<T, 2, 2>(p, tiles, join, ctas, stream);
-  return columns == 1 ? launch_mma<T, 4, 1>(p, tiles, join, ctas, stream)
-                      : launch_mma<T, 4, 2>(p, tiles, join, ctas, stream);
+  switch (p.head_dim / kMxBlock * 2 + columns) {
+    case 3: return launch_mma<T, 1, 1>(p, tiles, join, ctas, stream);
+    case 4: return launch_mma<T, 1, 2>(p, tiles, join, ctas, stream);
+    case 5: return launch_mma<T, 2, 1>(p, tiles, join, ctas, stream);
+    case 6: return launch_mma<T, 2, 2>(p, tiles, join, ctas, stream);
+    case 7: return launch_mma<T, 3, 1>(p, tiles, join, ctas, stream);
+    case 8: return launch_mma<T, 3, 2>(p, tiles, join, ctas, stream);
+    case 9: return launch_mma<T, 4, 1>(p, tiles, join, ctas, stream);
+    case 10: return launch_mma<T, 4, 2>(p, tiles, join, ctas, stream);
+    case 11: return launch_mma<T, 5, 1>(p, tiles, join, ctas, stream);
+    case 13: return launch_mma<T, 6, 1>(p, tiles, join, ctas, stream);
+    case 15: return launch_mma<T, 7, 1>(p, tiles, join, ctas, stream);
+    case 17: return launch_mma<T, 8, 1>(p, tiles, join, ctas, stream);
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-// Shapes of this kernel: 32-bit unit and group counts, sequences in one launch's reach.
-bool mxfp4_mma_supported(int dtype, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
-                         int block_size, int64_t capacity) {
-  (void)dtype;
-  if (head_dim != 64 && head_dim != 128) return false;
-  const int64_t H = static_cast<int64_t>(num_kv_heads) * mma_tiles(num_q_heads, num_kv_heads);
-  return num_blocks * num_kv_heads * (block_size / kMxGroup) < (int64_t{1} << 31) &&
-         (capacity / kUnit + 1) * H < (int64_t{1} << 31);
+// 32-bit unit and group counts: more than any memory holds, or a table of more than 2^31 units a sequence.
+bool mxfp4_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
+                            int64_t capacity) {
+  const int64_t H = static_cast<int64_t>(num_kv_heads) * mma_tiles(num_q_heads, num_kv_heads, head_dim);
+  return num_blocks < (int64_t{1} << 31) / num_kv_heads / (block_size / kMxGroup) &&
+         capacity / kUnit + 1 < (int64_t{1} << 31) / H;
 }
 
-size_t mxfp4_mma_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
-                           int sms) {
-  if (!mma_joins(num_seqs, num_q_heads, num_kv_heads, capacity, sms)) return 0;
-  const size_t heads = kQueries * mma_columns(num_q_heads, num_kv_heads);
+size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
+                              int sms) {
+  if (!mma_joins(num_seqs, num_q_heads, num_kv_heads, head_dim, capacity, sms)) return 0;
+  const size_t heads = kQueries * mma_columns(num_q_heads, num_kv_heads, head_dim);
   return static_cast<size_t>(sms) * (2 * heads * (head_dim + 2) * sizeof(float) + sizeof(MxMeta));
 }
 
-cudaError_t launch_mxfp4_mma(const MxDecodeParams &p, int dtype, cudaStream_t stream) {
-  const int tiles = mma_tiles(p.num_q_heads, p.num_kv_heads), columns = mma_columns(p.num_q_heads, p.num_kv_heads);
+cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream) {
+  const int tiles = mma_tiles(p.num_q_heads, p.num_kv_heads, p.head_dim);
+  const int columns = mma_columns(p.num_q_heads, p.num_kv_heads, p.head_dim);
   const int sms = sm_count_current();
   const int64_t capacity = p.bt_stride * p.block_size;
   const int64_t H = static_cast<int64_t>(p.num_kv_heads) * tiles;
   int64_t slice = ((int64_t{1} << 31) - 1) / ((capacity / kUnit + 1) * H);  // units stay in 32 bits
   if (slice > kMaxSeqs) slice = kMaxSeqs;
-  const bool join = mma_joins(p.num_seqs, p.num_q_heads, p.num_kv_heads, capacity, sms);
+  const bool join = mma_joins(p.num_seqs, p.num_q_heads, p.num_kv_heads, p.head_dim, capacity, sms);
   for (int64_t s = 0; s < p.num_seqs; s += slice) {
     MxDecodeParams q = p;
     q.num_seqs = p.num_seqs - s < slice ? p.num_seqs - s : slice;

@@ -18,8 +18,10 @@ cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtyp
 cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
                                 cudaStream_t stream);
 cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream);
-size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
-                              int64_t num_blocks, int block_size, int64_t capacity, int sms);
+bool mxfp4_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
+                            int64_t capacity);
+size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
+                              int sms);
 
 bool mxfp4_prefill_supported(int head_dim);
 int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
@@ -141,8 +143,8 @@ size_t mi_paged_decode_mxfp4_workspace_bytes(int64_t num_seqs, int64_t num_block
   if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || block_table_stride <= 0 ||
       num_q_heads % num_kv_heads != 0 || check_cache(num_blocks, block_size, num_kv_heads, head_dim) != MI_OK)
     return 0;
-  return mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, num_blocks, block_size,
-                                block_table_stride * block_size, sm_count_of(device < 0 ? 0 : device));
+  return mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, block_table_stride * block_size,
+                                sm_count_of(device < 0 ? 0 : device));
 }
 
 int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, const void *value_pages,
@@ -160,14 +162,17 @@ int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, c
     return capi_fail(MI_ERR_INVALID, "block_table_stride out of range");
   if (num_seqs > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences in one call");
   if (num_q_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 query heads");
+  if (!mxfp4_decode_supported(num_q_heads, num_kv_heads, head_dim, num_blocks, block_size,
+                              block_table_stride * block_size))
+    return capi_fail(MI_ERR_UNSUPPORTED, "pages or block table too large for one call");
   if (num_seqs == 0) return MI_OK;
   if (!out || !query || !key_pages || !value_pages || !block_tables || !context_lens)
     return capi_fail(MI_ERR_INVALID, "null pointer");
   if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
     return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
-  const size_t need = mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, num_blocks,
-                                             block_size, block_table_stride * block_size, sm_count_current());
+  const size_t need = mxfp4_decode_workspace(num_seqs, num_q_heads, num_kv_heads, head_dim,
+                                             block_table_stride * block_size, sm_count_current());
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_decode_mxfp4_workspace_bytes)");
   if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");

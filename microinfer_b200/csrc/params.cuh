@@ -175,7 +175,7 @@ struct MxDecodeParams {
   const uint8_t *value_pages;
   const int32_t *block_tables;
   const int32_t *context_lens;
-  float *workspace;  // partial states, see decode_mxfp4.cu
+  float *workspace;  // partial states, see decode_mxfp4_mma.cu
   int64_t bt_stride;
   int64_t num_blocks;
   int64_t num_seqs;

@@ -879,3 +879,48 @@ def test_results_over_the_query_and_shared_pages(cuda_device, name, d):
         mi.paged_prefill_mxfp4(over, *pages, cu_q, cu_k, table, max_seqlen_q=1, out=over)
         _close(over, *want, dtype, PREFILL_STEP[dtype])
     mi.check_device_status(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("group", [1, 6, 9])
+def test_decode_every_head_dim(cuda_device, name, d, group):
+    """Long and short contexts of every head_dim, scales far apart, sequences that cross CTAs."""
+    ctxs = [7000, 0, 1, 31, 33, 1500]
+    got, want, dtype = _decode_case(cuda_device, name, 2, group, d, 32, ctxs, spread=6.0)
+    mi.check_device_status(cuda_device)
+    assert bool((got[1] == 0).all())
+    if dtype == torch.float16:
+        # V reaches 6 * 2^17 here, and a result from 65520 on (half a step past 65504) is an infinity in
+        # fp16: those have to be one, of the right sign, and leave the comparison with what may round either way.
+        exact = want[0]
+        slack = _bound(exact, *want[1:], dtype, d, DECODE_STEP[dtype])
+        out = got.double().cpu().numpy()
+        past, near = np.abs(exact) - slack >= 65520, np.abs(exact) + slack >= 65504
+        assert np.array_equal(out[past], np.sign(exact[past]) * np.inf)
+        got = torch.from_numpy(np.where(near, exact, out))
+    _close(got, *want, dtype, DECODE_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_decode_nan_and_zero_blocks_of_every_head_dim(cuda_device, d):
+    """A NaN block of V is NaN in its 32 dims of its sequence alone; a NaN of K in all; zero blocks are zeros."""
+    nb = d // 32
+    rng = np.random.default_rng(d)
+    kp, vp = _pages(rng, 12, 16, 1, d)
+    scales = vp.reshape(12, 1, 1, -1)[..., nb * 256:].reshape(12, 16, nb)  # a view
+    kscales = kp.reshape(12, 1, 1, -1)[..., nb * 256:].reshape(12, 16, nb)
+    scales[2, 5, nb - 1] = 255
+    scales[6, 3, :] = 0
+    kscales[9, 0, 0] = 255
+    table = np.arange(12, dtype=np.int32).reshape(3, 4)
+    kt, vt, tt = _cuda(kp, cuda_device), _cuda(vp, cuda_device), _cuda(table, cuda_device)
+    query = torch.randn(3, 4, d, device=cuda_device)
+    got = mi.paged_decode_mxfp4(query, kt, vt, tt, torch.full((3,), 60, dtype=torch.int32, device=cuda_device))
+    nan = torch.isnan(got)
+    assert bool(nan[0, :, d - 32:].all()) and not bool(nan[0, :, :d - 32].any())
+    assert not bool(nan[1].any()) and bool(nan[2].all())
+    want = mo.attention(query[1:2].double().cpu().numpy(), mo.rows(kp, table[1], 60), mo.rows(vp, table[1], 60), d ** -0.5)
+    _close(got[1:2], *want, torch.float32, DECODE_STEP[torch.float32])
