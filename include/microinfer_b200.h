@@ -458,8 +458,8 @@ MI_API int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_p
 
 /*
  * Causal chunked prefill from the 4-bit cache (also mixed batches): rows as
- * mi_paged_prefill, any GQA group, f32/f16/bf16, head_dim 64 or 128
- * (MI_ERR_UNSUPPORTED otherwise: gather and mi_varlen_prefill).  `max_seqlen_q`
+ * mi_paged_prefill, any GQA group and head_dim in f16/bf16, up to head_dim 128 in f32
+ * (MI_ERR_UNSUPPORTED above: gather and mi_varlen_prefill).  `max_seqlen_q`
  * bounds the launch shape, `max_context` (a bound on the contexts, or less) the split over the keys
  * of few rows, whose states take the workspace for the duration of the call.
  */

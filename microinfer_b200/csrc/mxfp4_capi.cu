@@ -23,7 +23,7 @@ bool mxfp4_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
                               int sms);
 
-bool mxfp4_prefill_supported(int head_dim);
+bool mxfp4_prefill_supported(int dtype, int head_dim);
 int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
                          int64_t capacity, int sms);
 cudaError_t launch_mxfp4_prefill(const MxPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
@@ -230,8 +230,8 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
     return capi_fail(MI_ERR_INVALID, "negative sizes");
   if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0)
     return capi_fail(MI_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads");
-  if (!mxfp4_prefill_supported(head_dim))
-    return capi_fail(MI_ERR_UNSUPPORTED, "prefill from the 4-bit cache takes head_dim 64 or 128; gather other ones");
+  if (!mxfp4_prefill_supported(dtype, head_dim))
+    return capi_fail(MI_ERR_UNSUPPORTED, "prefill from the 4-bit cache takes fp32 up to head_dim 128; gather above");
   if (num_seqs > 65535 || num_kv_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
   if (num_seqs == 0 || num_tokens == 0) return MI_OK;
   if (max_seqlen_q <= 0) return capi_fail(MI_ERR_INVALID, "max_seqlen_q must be positive");

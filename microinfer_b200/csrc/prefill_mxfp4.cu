@@ -1,6 +1,6 @@
 // Causal chunked prefill straight from the 4-bit cache (layout: mxfp4.cuh) on
 // the warp-level tensor cores, for what the dense tcgen05 kernel behind the gather does
-// not take (head_dim 64, fp32, other groups) and for chunks too small to fill it.
+// not take (head_dim other than 128, fp32, other groups) and for chunks too small to fill it.
 //
 // A CTA takes 128 rows of one kv head, a row being (token, query head of the group), so any group
 // fills the tiles; 8 warps of 16 rows.  It walks the keys 64 at a time: codes and scales of
@@ -39,17 +39,18 @@ struct PfCfg {
   using E = typename std::conditional<kSplit, __nv_bfloat16, T>::type;  // MMA operands
   static constexpr int kParts = kSplit ? 3 : 1;
   static constexpr int D = NB * kMxBlock;
-  static constexpr int kRowBytes = D * 2;
+  static constexpr int kRowBytes = (NB + 1) / 2 * 128;  // rows of whole 128 bytes, for the swizzle
   static constexpr int kTile = kKeys * kRowBytes;      // K or V of a tile
   static constexpr int kQuery = kRows * kRowBytes;     // one part of q
   static constexpr int kWords = kKeys * NB * 4 / kThreads;  // code words of K (and of V) per thread and tile
   static constexpr int kSmem = kParts * kQuery + 4 * kTile + 2 * (kKeys + 4 * kGroups);
+  static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // Byte offset of 16-byte chunk c of a row, chunks swizzled so that 8 rows' reads of one chunk touch every bank.
 template <int NB>
 __device__ __forceinline__ uint32_t at(int row, int c) {
-  return static_cast<uint32_t>(row * (NB * 64) + ((c ^ (row & 7)) << 4));
+  return static_cast<uint32_t>(row * ((NB + 1) / 2 * 128) + ((c ^ (row & 7)) << 4));
 }
 
 __device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
@@ -504,13 +505,29 @@ cudaError_t launch_pf(const MxPrefillParams &p, int64_t num_seqs, int64_t max_se
 template <typename T>
 cudaError_t launch_pf_t(const MxPrefillParams &p, int head_dim, int64_t num_seqs, int64_t max_seqlen_q,
                         cudaStream_t stream) {
-  return head_dim == 64 ? launch_pf<T, 2>(p, num_seqs, max_seqlen_q, stream)
-                        : launch_pf<T, 4>(p, num_seqs, max_seqlen_q, stream);
+  switch (head_dim / kMxBlock) {
+    case 1: return launch_pf<T, 1>(p, num_seqs, max_seqlen_q, stream);
+    case 2: return launch_pf<T, 2>(p, num_seqs, max_seqlen_q, stream);
+    case 3: return launch_pf<T, 3>(p, num_seqs, max_seqlen_q, stream);
+    case 4: return launch_pf<T, 4>(p, num_seqs, max_seqlen_q, stream);
+  }
+  if constexpr (!std::is_same<T, float>::value) {
+    switch (head_dim / kMxBlock) {
+      case 5: return launch_pf<T, 5>(p, num_seqs, max_seqlen_q, stream);
+      case 6: return launch_pf<T, 6>(p, num_seqs, max_seqlen_q, stream);
+      case 7: return launch_pf<T, 7>(p, num_seqs, max_seqlen_q, stream);
+      case 8: return launch_pf<T, 8>(p, num_seqs, max_seqlen_q, stream);
+    }
+  }
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-bool mxfp4_prefill_supported(int head_dim) { return head_dim == 64 || head_dim == 128; }
+// Shared memory holds q's three parts in fp32 up to head_dim 128.
+bool mxfp4_prefill_supported(int dtype, int head_dim) {
+  return head_dim % kMxBlock == 0 && head_dim <= (dtype == MI_DTYPE_FLOAT32 ? 128 : 256);
+}
 
 // Splits over the keys: enough CTAs for two per SM, each split at least 4 tiles of a full table.
 int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,

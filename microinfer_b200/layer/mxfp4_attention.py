@@ -164,7 +164,7 @@ def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
     quarters of the SMs without a tile of 128 rows: reading the pages splits the keys
     (64 tokens on 16000, 32/8 heads of 128: 113 us, gathered 295; 256 tokens: 438 and 297).
     """
-    if d not in (64, 128):
+    if dtype == _lib.dtype_code(torch.float32) and d > 128:  # q's three parts outgrow shared memory
         return False
     lib = _lib.load()
     if lib.mi_prefill_kernel_for(dtype, d, hq, hkv, 0) != 2:

@@ -93,8 +93,10 @@ def attention(q, k, v, scale):
         x = q[:, h] @ kh.T * scale
         far = np.abs(q[:, h]) @ np.abs(kh).T * scale
         x = np.where(np.arange(ctx)[None] > np.arange(ctx - n, ctx)[:, None], -np.inf, x)
-        p = np.exp(x - x.max(-1, keepdims=True))
-        p /= p.sum(-1, keepdims=True)
+        top = x.max(-1, keepdims=True)
+        p = np.exp(x - np.where(np.isneginf(top), 0, top))
+        total = p.sum(-1, keepdims=True)
+        p /= np.where(total == 0, 1, total)  # a row before the first key: zeros
         out[:, h] = p @ vh
         weight[:, h] = p @ np.abs(vh)
         size[:, h] = far.max(-1, keepdims=True)

@@ -924,3 +924,35 @@ def test_decode_nan_and_zero_blocks_of_every_head_dim(cuda_device, d):
     assert not bool(nan[1].any()) and bool(nan[2].all())
     want = mo.attention(query[1:2].double().cpu().numpy(), mo.rows(kp, table[1], 60), mo.rows(vp, table[1], 60), d ** -0.5)
     _close(got[1:2], *want, torch.float32, DECODE_STEP[torch.float32])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("group", [1, 5])
+def test_prefill_every_head_dim(cuda_device, name, d, group):
+    """Chunks of one token and of several tiles, a context split over its keys; in shapes that are computed
+    from the pages also a context shorter than its chunk, whose first rows see no key."""
+    short = d != 128 and not (name == "f32" and d > 128)
+    q_lens, ctxs = [140, 1, 3, 20, 9], [140, 3000, 3, 77, 5 if short else 9]
+    got, free, want, dtype = _prefill_case(cuda_device, name, 2, group, d, 32, q_lens, ctxs)
+    if short:
+        assert bool((got[164:168] == 0).all())
+    _close(got, *want, dtype, PREFILL_STEP[dtype])
+    _close(free, *want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("d", [32, 96, 160, 192, 224, 256])
+def test_prefill_nan_blocks_of_every_head_dim(cuda_device, d):
+    nb = d // 32
+    rng = np.random.default_rng(d)
+    kp, vp = _pages(rng, 6, 16, 1, d)
+    vp.reshape(6, 1, 1, -1)[..., nb * 256:].reshape(6, 16, nb)[4, 6, nb - 1] = 255  # key 70
+    table = np.arange(6, dtype=np.int32).reshape(1, 6)
+    cu = torch.tensor([0, 96], dtype=torch.int32, device=cuda_device)
+    query = torch.randn(96, 3, d, device=cuda_device, dtype=torch.bfloat16)
+    got = mi.paged_prefill_mxfp4(query, _cuda(kp, cuda_device), _cuda(vp, cuda_device), cu, cu,
+                                 _cuda(table, cuda_device), max_seqlen_q=96)
+    nan = torch.isnan(got)
+    assert bool(nan[70:, :, d - 32:].all()) and int(nan.sum()) == 26 * 3 * 32
