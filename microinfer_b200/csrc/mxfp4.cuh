@@ -52,6 +52,7 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) {
 }
 
 // Eight codes of a word, in element order, as four f16 pairs (exact).
+// (Pass a word of memory: from a byte load, zero-extended, nvcc 12.9's conversions gave 0.)
 __device__ __forceinline__ void mx_codes_to_f16(uint32_t w, uint32_t (&r)[4]) {
   asm("{ .reg .b8 b0, b1, b2, b3;\n\t"
       "mov.b32 {b0, b1, b2, b3}, %4;\n\t"

@@ -9,13 +9,18 @@
 // O += P V are m16n8k16 with fp32 accumulators, P passes from the one to the
 // other in registers; online softmax in fp32, the maximum followed 3 binades behind at most.
 // Types: bf16 holds every value of the cache (short of overflow), fp16 rounds
-// those outside its range, as the gather does; p in fp16 is lifted by 2^12, which keeps a key down to 2^-26 of
+// K outside its range, as the gather does; p in fp16 is lifted by 2^12, which keeps a key down to 2^-26 of
 // the largest at full precision.  fp32: K and V are exact in bf16, q and p go in as three bf16 parts
 // (24 bits), three MMAs for one.
 // A NaN block of V is held as zero and its dims are set to NaN in the rows that
-// see the key, so it never reaches rows before it.
+// see the key, so it never reaches rows before it.  So is one that fp16 does not hold, and its products are
+// added in fp32 to those rows.
 // Few rows over a long context are split over the keys; a second launch joins
-// the splits.  mma.sync bounds this at about 1/3 of the tcgen05 rate.
+// the splits.
+// Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2960 us, 174 TFLOP/s; 8 x 250 on 2000, 16/8
+// heads of 64: 110 us, 139 TFLOP/s, of 256: 405 us, 152; fp32, of 128: 388 us, 79.  Latency bounds it: two
+// CTAs to an SM (128 registers a thread) wait at a barrier per tile (ALU 37%, shared memory 44%); mma.sync itself would
+// bound this at about 560 TFLOP/s.  With the pages looked up a tile ahead 110 us, else 116.
 #include <type_traits>
 
 #include "common.cuh"
@@ -38,6 +43,9 @@ struct PfCfg {
   static constexpr bool kSplit = std::is_same<T, float>::value;
   using E = typename std::conditional<kSplit, __nv_bfloat16, T>::type;  // MMA operands
   static constexpr int kParts = kSplit ? 3 : 1;
+  // Scale bytes of V from here on are not for the MMA: fp16 ends at 65504 = 3.998 * 2^14.
+  static constexpr bool kHalf = std::is_same<T, __half>::value;
+  static constexpr uint32_t kApart = kHalf ? 127 + 14 : 255;
   static constexpr int D = NB * kMxBlock;
   static constexpr int kRowBytes = (NB + 1) / 2 * 128;  // rows of whole 128 bytes, for the swizzle
   static constexpr int kTile = kKeys * kRowBytes;      // K or V of a tile
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       mx_codes_to_f32(w.k[i], mx_scale(ks), x);
       *reinterpret_cast<uint4 *>(kt + at<NB>(key, b * 4 + j)) =
           make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
-      mx_codes_to_f32(vs == 255u ? 0u : w.v[i], vs == 255u ? 0.f : mx_scale(vs), x);
+      mx_codes_to_f32(vs >= C::kApart ? 0u : w.v[i], vs >= C::kApart ? 0.f : mx_scale(vs), x);
       *reinterpret_cast<uint4 *>(vt + at<NB>(key, b * 4 + j)) =
           make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
       if (tok == 0 && j == 0 && b == 0) {
@@ -219,11 +227,12 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       }
     }
   };
-  // NaN blocks of V: found by one lane per key (its codes' neighbours hold the same bytes)
+  // NaN blocks of V, and those fp16 does not hold: found by one lane per key (its codes' neighbours hold
+  // the same bytes)
   auto note_nan = [&](const Words &w, int buf) -> bool {
     bool any = false;
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) any |= ((w.scales[i] >> 8) & 255u) == 255u;
+    for (int i = 0; i < C::kWords; ++i) any |= ((w.scales[i] >> 8) & 255u) >= C::kApart;
     if (threadIdx.x < kKeys) nan_v[buf * kKeys + threadIdx.x] = 0;
     return any;
   };
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 #pragma unroll
     for (int i = 0; i < C::kWords; ++i) {
       const int gb = combo + 4 * i, key = gb / NB * kMxGroup + tok;
-      if (((w.scales[i] >> 8) & 255u) == 255u && j == 0)
+      if (((w.scales[i] >> 8) & 255u) >= C::kApart && j == 0)
         atomicOr(reinterpret_cast<unsigned *>(nan_v + buf * kKeys) + key / 4, 1u << (key % 4 * 8 + gb % NB));
     }
   };
@@ -377,12 +386,34 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       for (int key = 0; key < kKeys; ++key) {
         const unsigned blocks = nan_v[buf * kKeys + key];
         if (!blocks) continue;
+        float pk[2] = {0.f, 0.f};  // p of this key in this thread's rows
+        const uint8_t *codes = nullptr;
+        if constexpr (C::kHalf) {
+#pragma unroll
+          for (int i = 0; i < kKeys / 8; ++i)
+            if (i == key / 8) pk[0] = key & 1 ? s[i][1] : s[i][0], pk[1] = key & 1 ? s[i][3] : s[i][2];
+          pk[0] = __shfl_sync(kAll, pk[0], (lane & ~3) | (key % 8 / 2));
+          pk[1] = __shfl_sync(kAll, pk[1], (lane & ~3) | (key % 8 / 2));
+          const uint32_t index = static_cast<uint32_t>(kt) * kGroups + key / kMxGroup, col = by_page.div(index);
+          codes = p.value_pages +  // a marked key has a page
+                  ((static_cast<int64_t>(__ldg(table + col)) * p.num_kv_heads + kvh) * per_page + (index - col * per_page)) *
+                      (NB * kMxBytes);
+        }
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
           if (!(blocks >> (n / 4) & 1u)) continue;
+          float v[8];
+          v[0] = v[1] = __uint_as_float(0x7fffffffu);
+          if constexpr (C::kHalf) {
+            const int tok = key % kMxGroup;
+            const uint32_t byte = codes[NB * kMxBlockBytes + tok * NB + n / 4];
+            if (byte != 255u)
+              mx_codes_to_f32(*reinterpret_cast<const uint32_t *>(codes + n / 4 * kMxBlockBytes + tok * 16 + n % 4 * 4) >> (8 * t),
+                              mx_scale(byte), v);
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (key0 + key <= pos[u >> 1]) o[n][u] = __uint_as_float(0x7fffffffu);
+            if (key0 + key <= pos[u >> 1]) o[n][u] = C::kHalf ? fmaf(pk[u >> 1], v[u & 1], o[n][u]) : v[0];
         }
       }
     }

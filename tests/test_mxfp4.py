@@ -45,6 +45,18 @@ def _close(got, want, weight, size, floor, dtype, p_step):
     assert worst <= 1, f"{worst:.3g} of the bound"
 
 
+def _close_or_past(got, want, weight, size, floor, dtype, p_step):
+    """As _close, for fp16 with results past its range: from 65520 on (half a step past 65504) a result has
+    to be an infinity of the right sign; what may round either way leaves the comparison."""
+    if dtype == torch.float16:
+        slack = _bound(want, weight, size, floor, dtype, got.shape[-1], p_step)
+        out = got.double().cpu().numpy()
+        past, near = np.abs(want) - slack >= 65520, np.abs(want) + slack >= 65504
+        assert np.array_equal(out[past], np.sign(want[past]) * np.inf)
+        got = torch.from_numpy(np.where(near, want, out))
+    _close(got, want, weight, size, floor, dtype, p_step)
+
+
 DECODE_STEP = {torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -11, torch.float32: 0.0}
 
 
@@ -891,16 +903,7 @@ def test_decode_every_head_dim(cuda_device, name, d, group):
     got, want, dtype = _decode_case(cuda_device, name, 2, group, d, 32, ctxs, spread=6.0)
     mi.check_device_status(cuda_device)
     assert bool((got[1] == 0).all())
-    if dtype == torch.float16:
-        # V reaches 6 * 2^17 here, and a result from 65520 on (half a step past 65504) is an infinity in
-        # fp16: those have to be one, of the right sign, and leave the comparison with what may round either way.
-        exact = want[0]
-        slack = _bound(exact, *want[1:], dtype, d, DECODE_STEP[dtype])
-        out = got.double().cpu().numpy()
-        past, near = np.abs(exact) - slack >= 65520, np.abs(exact) + slack >= 65504
-        assert np.array_equal(out[past], np.sign(exact[past]) * np.inf)
-        got = torch.from_numpy(np.where(near, exact, out))
-    _close(got, *want, dtype, DECODE_STEP[dtype])
+    _close_or_past(got, *want, dtype, DECODE_STEP[dtype])
 
 
 @gpu
@@ -956,3 +959,21 @@ def test_prefill_nan_blocks_of_every_head_dim(cuda_device, d):
                                  _cuda(table, cuda_device), max_seqlen_q=96)
     nan = torch.isnan(got)
     assert bool(nan[70:, :, d - 32:].all()) and int(nan.sum()) == 26 * 3 * 32
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 96, 256])
+def test_prefill_values_past_fp16(cuda_device, name, d):
+    """V blocks of 2^14 to 2^40 reach the rows that see them, with their weight, and no row before."""
+    def edit(kp, vp, table):
+        code, byte = mo.unpack(vp)
+        for i, pos in enumerate([5, 6, 17, 40, 63, 64, 70, 89]):
+            byte[table[0, pos // 16], pos % 16, 0, i % (d // 32)] = 127 + [14, 15, 20, 40][i % 4]
+        vp[:] = mo.pack(code, byte)
+
+    got, free, want, dtype = _prefill_case(cuda_device, name, 1, 3, d, 16, [86], [90], edit=edit)
+    for x in (got, free):
+        _close_or_past(x, *want, dtype, PREFILL_STEP[dtype])
+    assert bool(torch.isfinite(got[0]).all())  # position 4: before the first of them
+
