@@ -40,6 +40,12 @@
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
 // segment and the second launch has nothing to do.
+//
+// Measured (bf16, 32/8 heads): 96 x 8192, head_dim 128: 155 us, 5.5 TB/s (86% of the copy rate), 64% of the
+// ALU pipe's cycles, which the conversions, masks and shifts of the scales take; 32 x 8192, head_dim 256:
+// 104 us, 5.5 TB/s; 96: 58 us, 3.7 TB/s (its scales are read byte by byte); 1 x 131072, head_dim 128: 34.8 us,
+// of which 24 are the loop, the rest the start's dependent reads (lengths, table, pages) and the second launch.
+// 12 warps of three stages at head_dim 128: 168 us where 16 of two take 155; a third stage at 64 gains nothing.
 #include <type_traits>
 
 #include "common.cuh"
