@@ -320,18 +320,21 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) pages &= group_ok[buf * kGroups + i] != 0;
     const bool masked = key0 + kKeys - 1 > first_pos || key0 + kKeys > keys || !pages;  // uniform in the warp
-    float top[2] = {-INFINITY, -INFINITY};
+    if (masked) {
 #pragma unroll
-    for (int i = 0; i < kKeys / 8; ++i) {
+      for (int i = 0; i < kKeys / 8; ++i) {
+        const int key = key0 + i * 8 + 2 * t;
+        const bool none = !group_ok[buf * kGroups + i / 2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (masked) {
-          const int key = key0 + i * 8 + 2 * t + (u & 1);
-          if (key > pos[u >> 1] || key >= keys || !group_ok[buf * kGroups + i / 2]) s[i][u] = -INFINITY;
-        }
-        top[u >> 1] = fmaxf(top[u >> 1], s[i][u]);
+        for (int u = 0; u < 4; ++u)
+          if (key + (u & 1) > min(pos[u >> 1], keys - 1) || none) s[i][u] = -INFINITY;
       }
     }
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) top[u >> 1] = fmaxf(top[u >> 1], s[i][u]);
     top[0] *= scale, top[1] *= scale;
     if (__any_sync(kAll, top[0] > m[0] + kLag || top[1] > m[1] + kLag)) {
 #pragma unroll
