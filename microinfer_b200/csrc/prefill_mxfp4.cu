@@ -50,7 +50,8 @@ struct PfCfg {
   static constexpr int kRowBytes = (NB + 1) / 2 * 128;  // rows of whole 128 bytes, for the swizzle
   static constexpr int kTile = kKeys * kRowBytes;      // K or V of a tile
   static constexpr int kQuery = kRows * kRowBytes;     // one part of q
-  static constexpr int kWords = kKeys * NB * 4 / kThreads;  // code words of K (and of V) per thread and tile
+  static constexpr int kChunks = 2 * kKeys * NB;  // a tile's (operand, key, block): 16 bytes of codes and a scale
+  static constexpr int kPer = (kChunks + kThreads - 1) / kThreads;  // of those per thread
   static constexpr int kSmem = kParts * kQuery + 4 * kTile + 2 * (kKeys + 4 * kGroups);
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
@@ -171,77 +172,97 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     }
   }
 
-  // A thread's code words of a tile: word i is (group, block, token, quarter) in the order of memory.
+  // A thread's chunks of a tile, in the order of memory: K's, then V's, (group, block, token).
   struct Words {
-    uint32_t k[C::kWords], v[C::kWords];
-    uint32_t scales[C::kWords];  // K's byte, V's byte, whether the page is one
+    uint4 codes[C::kPer];
+    uint32_t scales[C::kPer];  // the scale byte, then whether the page is one
+  };
+  struct Chunk {
+    bool exists, value;
+    int group, b;
+  };
+  auto chunk = [&](int i) {
+    const int id = i * kThreads + static_cast<int>(threadIdx.x);
+    Chunk c;
+    c.exists = C::kChunks % kThreads == 0 || id < C::kChunks;
+    c.value = id >= C::kChunks / 2;
+    const int gb = (c.value ? id - C::kChunks / 2 : id) / kMxGroup;
+    c.group = gb / NB, c.b = gb % NB;
+    return c;
   };
   const int per_page = p.block_size / kMxGroup;
   const int32_t *table = p.block_tables + seq * p.bt_stride;
-  const int j = threadIdx.x & 3, tok = (threadIdx.x >> 2) & 15, combo = threadIdx.x >> 6;  // 4 (group, block) at a time
-  // Pages of a tile's words are looked up a tile before their codes: kNone past the keys.
+  const int tok = threadIdx.x % kMxGroup;
+  // Pages of a tile's chunks are looked up a tile before their codes: kNone past the keys.
   constexpr int kNone = INT32_MIN;
-  int pages_at[C::kWords];
+  int pages_at[C::kPer];
   auto look_up = [&](int kt) {
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) {
-      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + (combo + 4 * i) / NB;
+    for (int i = 0; i < C::kPer; ++i) {
+      const Chunk c = chunk(i);
+      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + c.group;
       pages_at[i] = kNone;
-      if (static_cast<int>(index) * kMxGroup + tok < keys) pages_at[i] = max(-1, __ldg(table + by_page.div(index)));
+      if (c.exists && static_cast<int>(index) * kMxGroup + tok < keys)
+        pages_at[i] = max(-1, __ldg(table + by_page.div(index)));
     }
   };
   auto fetch = [&](int kt, Words &w) {
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) {
-      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB, page = pages_at[i];
-      w.k[i] = w.v[i] = 0;
+    for (int i = 0; i < C::kPer; ++i) {
+      const Chunk c = chunk(i);
+      const int page = pages_at[i];
+      w.codes[i] = make_uint4(0u, 0u, 0u, 0u);
       w.scales[i] = page == kNone ? 1u << 16 : 0u;  // keys that do not exist: zeros
       if (page < 0 || page >= p.num_blocks) continue;
-      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + group;
-      const int64_t off = ((static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page +
-                           (index - by_page.div(index) * per_page)) *
-                          (NB * kMxBytes);
-      const int code = b * kMxBlockBytes + tok * 16 + j * 4, scale = NB * kMxBlockBytes + tok * NB + b;
-      w.k[i] = *reinterpret_cast<const uint32_t *>(p.key_pages + off + code);
-      w.v[i] = *reinterpret_cast<const uint32_t *>(p.value_pages + off + code);
-      w.scales[i] = p.key_pages[off + scale] | static_cast<uint32_t>(p.value_pages[off + scale]) << 8 | 1u << 16;
+      const uint32_t index = static_cast<uint32_t>(kt) * kGroups + c.group;
+      const uint8_t *from = (c.value ? p.value_pages : p.key_pages) +
+                            ((static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page +
+                             (index - by_page.div(index) * per_page)) *
+                                (NB * kMxBytes);
+      w.codes[i] = *reinterpret_cast<const uint4 *>(from + c.b * kMxBlockBytes + tok * 16);
+      w.scales[i] = from[NB * kMxBlockBytes + tok * NB + c.b] | 1u << 16;
     }
   };
   auto place = [&](const Words &w, int buf) {
-    uint8_t *kt = tiles + buf * 2 * C::kTile, *vt = kt + C::kTile;
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) {
-      const int gb = combo + 4 * i, group = gb / NB, b = gb % NB, key = group * kMxGroup + tok;
-      const uint32_t ks = w.scales[i] & 255u, vs = (w.scales[i] >> 8) & 255u;
-      float x[8];
-      mx_codes_to_f32(w.k[i], mx_scale(ks), x);
-      *reinterpret_cast<uint4 *>(kt + at<NB>(key, b * 4 + j)) =
-          make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
-      mx_codes_to_f32(vs >= C::kApart ? 0u : w.v[i], vs >= C::kApart ? 0.f : mx_scale(vs), x);
-      *reinterpret_cast<uint4 *>(vt + at<NB>(key, b * 4 + j)) =
-          make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
-      if (tok == 0 && j == 0 && b == 0) {
+    for (int i = 0; i < C::kPer; ++i) {
+      const Chunk c = chunk(i);
+      if (!c.exists) continue;
+      uint8_t *to = tiles + (buf * 2 + c.value) * C::kTile;
+      const int key = c.group * kMxGroup + tok;
+      const uint32_t byte = w.scales[i] & 255u;
+      const bool apart = c.value && byte >= C::kApart;
+      const float f = apart ? 0.f : mx_scale(byte);
+      const uint32_t word[4] = {w.codes[i].x, w.codes[i].y, w.codes[i].z, w.codes[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[8];
+        mx_codes_to_f32(word[j], f, x);
+        *reinterpret_cast<uint4 *>(to + at<NB>(key, c.b * 4 + j)) =
+            make_uint4(pack<E>(x[0], x[1]), pack<E>(x[2], x[3]), pack<E>(x[4], x[5]), pack<E>(x[6], x[7]));
+      }
+      if (tok == 0 && c.b == 0 && !c.value) {
         const bool ok = (w.scales[i] >> 16) != 0;
-        group_ok[buf * kGroups + group] = ok;
+        group_ok[buf * kGroups + c.group] = ok;
         if (!ok) flag_status(p.status, MI_DEV_BAD_BLOCK);
       }
     }
   };
-  // NaN blocks of V, and those fp16 does not hold: found by one lane per key (its codes' neighbours hold
-  // the same bytes)
+  // NaN blocks of V, and those fp16 does not hold
   auto note_nan = [&](const Words &w, int buf) -> bool {
     bool any = false;
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) any |= ((w.scales[i] >> 8) & 255u) >= C::kApart;
+    for (int i = 0; i < C::kPer; ++i) any |= chunk(i).value && (w.scales[i] & 255u) >= C::kApart;
     if (threadIdx.x < kKeys) nan_v[buf * kKeys + threadIdx.x] = 0;
     return any;
   };
   auto mark_nan = [&](const Words &w, int buf) {
 #pragma unroll
-    for (int i = 0; i < C::kWords; ++i) {
-      const int gb = combo + 4 * i, key = gb / NB * kMxGroup + tok;
-      if (((w.scales[i] >> 8) & 255u) >= C::kApart && j == 0)
-        atomicOr(reinterpret_cast<unsigned *>(nan_v + buf * kKeys) + key / 4, 1u << (key % 4 * 8 + gb % NB));
+    for (int i = 0; i < C::kPer; ++i) {
+      const Chunk c = chunk(i);
+      const int key = c.group * kMxGroup + tok;
+      if (c.exists && c.value && (w.scales[i] & 255u) >= C::kApart)
+        atomicOr(reinterpret_cast<unsigned *>(nan_v + buf * kKeys) + key / 4, 1u << (key % 4 * 8 + c.b));
     }
   };
 
