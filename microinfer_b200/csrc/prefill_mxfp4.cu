@@ -17,10 +17,12 @@
 // added in fp32 to those rows.
 // Few rows over a long context are split over the keys; a second launch joins
 // the splits.
-// Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2960 us, 174 TFLOP/s; 8 x 250 on 2000, 16/8
-// heads of 64: 110 us, 139 TFLOP/s, of 256: 405 us, 152; fp32, of 128: 388 us, 79.  Latency bounds it: two
-// CTAs to an SM (128 registers a thread) wait at a barrier per tile (ALU 37%, shared memory 44%); mma.sync itself would
-// bound this at about 560 TFLOP/s.  With the pages looked up a tile ahead 110 us, else 116.
+// Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2313 us, 223 TFLOP/s; 8 x 250 on 2000, 16/8
+// heads of 64: 88 us, 174 TFLOP/s, of 256: 342 us, 180; fp32, of 128: 320 us, 96.  mma.sync itself would
+// bound this at about 560 TFLOP/s; what does is latency, 16 warps an SM (128 registers a thread) meeting at a
+// barrier per tile.  What it took, 2048 on 6144, 32/8 heads of 64: pages looked up a tile ahead (116 to 110 us at 8 x 250);
+// a branch of its own for masked tiles (762 to 651); chunks of 16 bytes a thread, not words (595).
+// 32 rows a warp, which halves the reads of K and V fragments, leaves 8 warps and was slower (786 against 762).
 #include <type_traits>
 
 #include "common.cuh"

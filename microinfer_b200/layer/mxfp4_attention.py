@@ -161,9 +161,9 @@ def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
     """Whether prefill reads the pages itself instead of gathering for the dense kernel.
 
     It does where the tcgen05 kernel does not take the shape (8 x 250 tokens on 2000, 16/8 heads of
-    256: 405 us, gathered 19114; 8 x 8 on nothing: 14 and 39), and where that would leave three
+    256: 342 us, gathered 19103; 8 x 8 on nothing: 14 and 29), and where that would leave three
     quarters of the SMs without a tile of 128 rows: reading the pages splits the keys
-    (64 tokens on 16000, 32/8 heads of 128: 106 us, gathered 295; 256 tokens: 438 and 297).
+    (128 tokens on 16000, 32/8 heads of 128: 151 us, gathered 294; 256 tokens: 317 and 297).
     """
     if dtype == _lib.dtype_code(torch.float32) and d > 128:  # q's three parts outgrow shared memory
         return False
