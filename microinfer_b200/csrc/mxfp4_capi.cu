@@ -183,7 +183,7 @@ int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, c
   p.value_pages = static_cast<const uint8_t *>(value_pages);
   p.block_tables = block_tables;
   p.context_lens = context_lens;
-  p.workspace = static_cast<float *>(workspace);
+  p.workspace = need > 0 ? static_cast<float *>(workspace) : nullptr;  // unasked for: of any size, not written
   p.bt_stride = block_table_stride;
   p.num_blocks = num_blocks;
   p.num_seqs = num_seqs;
@@ -257,7 +257,7 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
   p.block_tables = block_tables;
   p.cu_seqlens_q = cu_seqlens_q;
   p.cu_seqlens_k = cu_seqlens_k;
-  p.workspace = static_cast<float *>(workspace);
+  p.workspace = need > 0 ? static_cast<float *>(workspace) : nullptr;
   p.bt_stride = block_table_stride;
   p.num_blocks = num_blocks;
   p.num_tokens = num_tokens;

@@ -1,0 +1,41 @@
+"""The C entries of the 4-bit cache, called as a C program would call them."""
+
+import numpy as np
+import pytest
+import torch
+
+import microinfer_b200 as mi
+from microinfer_b200 import _lib
+from tests.test_mxfp4 import _cuda, _pages
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("d,hq", [(64, 8), (128, 4), (128, 16), (256, 4)])
+def test_a_workspace_that_is_not_needed_is_left_alone(cuda_device, d, hq):
+    """Short tables need no workspace, so one that the caller has all the same may be of any size."""
+    lib = _lib.load()
+    rng = np.random.default_rng(d)
+    kp, vp = _pages(rng, 4, 16, 2, d)
+    kt, vt = _cuda(kp, cuda_device), _cuda(vp, cuda_device)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([20, 0], dtype=torch.int32, device=cuda_device)
+    query = torch.randn(2, hq, d, device=cuda_device, dtype=torch.bfloat16)
+    assert lib.mi_paged_decode_mxfp4_workspace_bytes(2, 4, 16, hq, 2, d, 2, 2, 0) == 0
+    around = torch.full((8 << 20,), 0x5A, dtype=torch.uint8, device=cuda_device)
+    small = around[64:80]
+    out = torch.empty_like(query)
+    code = _lib.dtype_code(query.dtype)
+    _lib.call("mi_paged_decode_mxfp4", out.data_ptr(), query.data_ptr(), kt.data_ptr(), vt.data_ptr(), 4, 16, hq, 2, d,
+              code, table.data_ptr(), 2, lens.data_ptr(), 2, d ** -0.5, small.data_ptr(), small.numel(),
+              _lib.status_buffer(cuda_device).data_ptr(), _lib.stream_of(cuda_device))
+    assert torch.equal(out, mi.paged_decode_mxfp4(query, kt, vt, table, lens))
+    cu_q = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda_device)
+    cu_k = torch.tensor([0, 20, 21], dtype=torch.int32, device=cuda_device)
+    assert lib.mi_paged_prefill_mxfp4_workspace_bytes(2, 2, 1, hq, 2, d, 32, 0) == 0
+    _lib.call("mi_paged_prefill_mxfp4", out.data_ptr(), query.data_ptr(), kt.data_ptr(), vt.data_ptr(), 4, 16, hq, 2, d,
+              code, cu_q.data_ptr(), cu_k.data_ptr(), table.data_ptr(), 2, 2, 2, 1, 32, d ** -0.5, small.data_ptr(),
+              small.numel(), _lib.status_buffer(cuda_device).data_ptr(), _lib.stream_of(cuda_device))
+    mi.check_device_status(cuda_device)
+    assert bool((around == 0x5A).all())
