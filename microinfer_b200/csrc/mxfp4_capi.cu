@@ -235,8 +235,9 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
   if (num_seqs > 65535 || num_kv_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
   if (num_seqs == 0 || num_tokens == 0) return MI_OK;
   if (max_seqlen_q <= 0) return capi_fail(MI_ERR_INVALID, "max_seqlen_q must be positive");
+  // positions are 32 bits, and pages are looked up as many as three tiles of keys past the last
   if (max_seqlen_q > (int64_t{1} << 24) || max_seqlen_q * (num_q_heads / num_kv_heads) >= (int64_t{1} << 31) ||
-      block_table_stride * block_size > INT32_MAX)
+      block_table_stride > (INT32_MAX - 256) / block_size)
     return capi_fail(MI_ERR_UNSUPPORTED, "sequence too long for one call");
   if (!out || !query || !key_pages || !value_pages || !cu_seqlens_q || !cu_seqlens_k || !block_tables)
     return capi_fail(MI_ERR_INVALID, "null pointer");

@@ -39,3 +39,20 @@ def test_a_workspace_that_is_not_needed_is_left_alone(cuda_device, d, hq):
               small.numel(), _lib.status_buffer(cuda_device).data_ptr(), _lib.stream_of(cuda_device))
     mi.check_device_status(cuda_device)
     assert bool((around == 0x5A).all())
+
+
+def test_prefill_refuses_tables_whose_positions_pass_32_bits():
+    """Up to three tiles of 64 keys past the last one are looked up, so a table may hold 256 positions less than 2^31."""
+    lib = _lib.load()
+    p = np.zeros(64, dtype=np.uint8).ctypes.data
+
+    def prefill(block_size, width):
+        # the misaligned query is refused after the sizes and before any launch
+        return lib.mi_paged_prefill_mxfp4(p, p | 1, p, p, 4, block_size, 4, 2, 64, 2, p, p, p, width, 1, 1, 1, 16, 0.1, None,
+                                          0, None, None)
+
+    unsupported, alignment = -2, prefill(16, 2)
+    assert alignment < 0 and alignment != unsupported
+    assert prefill(16, (2 ** 31 - 16) // 16) == unsupported  # 2^31 - 16 positions
+    assert prefill(1 << 20, 2047) == alignment
+    assert prefill(16, 2 ** 60) == unsupported
