@@ -335,8 +335,8 @@ struct MxWarp {
     }
   }
 
-  // Scores of a unit's 32 keys for query t, still to be scaled by xs: x[j][c][0], key g of group j;
-  // x[j][c][1], its key g + 8.
+  // Scores of a unit's 32 keys for query t: x[j][c][0], key g of group j; x[j][c][1], its key g + 8.
+  // K's scale comes before xs, which takes q's lift back: one multiplication a score for that.
   __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[2][CT][2]) const {
     constexpr int kWords = C::kBytes ? NB : Q;  // scales of a key: bytes of their own, or words of four
     uint32_t lo[2][NB], hi[2][NB], wl[2][kWords], wh[2][kWords];
@@ -381,6 +381,50 @@ struct MxWarp {
           if constexpr (kSplit) d[0] += d[1], d[2] += d[3];
           x[j][c][0] = b == 0 ? d[0] * fl : fmaf(d[0], fl, x[j][c][0]);
           x[j][c][1] = b == 0 ? d[2] * fh : fmaf(d[2], fh, x[j][c][1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) x[j][c][0] *= xs[c], x[j][c][1] *= xs[c];
+  }
+
+  // d * scale * x, the scales first: their product is in the range of the term itself where d is not far from q's
+  // lift (a d of zero, or of q's smallest elements, leaves them apart).
+  __device__ __forceinline__ static float far_term(float d, float scale, float x) {
+    const float both = scale * x;
+    return fabsf(both) <= 0x1p127f ? d * both : d * x * scale;
+  }
+
+  // As scores() where its order of the factors leaves fp32's range though the score may not: q is up to 2^15 here,
+  // so keys of 2^105 do.
+  // Rolled up: unrolled like the other it costs 16 bytes of spills at D = 128.
+  __device__ __forceinline__ void scores_far(uint32_t kbase, float (&x)[2][CT][2]) const {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t base = kbase + j * C::kGroup, at = base + NB * kMxBlockBytes + g * NB;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) x[j][c][0] = x[j][c][1] = 0.f;
+#pragma unroll 1
+      for (int b = 0; b < NB; ++b) {
+        uint32_t lo, hi, again[2], a[4], e[4];
+        ldsm4(base + b * kMxBlockBytes + (lane & 15) * 16, lo, hi, again[0], again[1]);
+        mx_codes_to_f16(lo, a);
+        mx_codes_to_f16(hi, e);
+        const float fl = scale_of(lds8(at + b), 0), fh = scale_of(lds8(at + 8 * NB + b), 0);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          uint32_t f[4];
+          float d[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3])
+                       : "r"(q + (c * NB + b) * 512));
+          mma_f16_zero(d, a[0], e[0], a[1], e[1], f[0], f[1]);
+          mma_f16(d, a[2], e[2], a[3], e[3], f[2], f[3]);
+          if constexpr (kSplit) d[0] += d[1], d[2] += d[3];
+          x[j][c][0] += far_term(d[0], fl, xs[c]);
+          x[j][c][1] += far_term(d[2], fh, xs[c]);
         }
       }
     }
@@ -547,10 +591,11 @@ struct MxWarp {
     uint32_t w[2][Q][4];
     load_scales<NB>(vbase, t, w[0]);
     load_scales<NB>(vbase + C::kGroup, t, w[1]);
+    bool far_scores = false;  // a score may not be finite because of how it was multiplied
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int c = 0; c < CT; ++c) x[j][c][0] *= xs[c], x[j][c][1] *= xs[c];
+    for (int c = 0; c < CT; ++c)
+      far_scores |= !(fabsf((x[0][c][0] + x[0][c][1]) + (x[1][c][0] + x[1][c][1])) <= 0x1p126f);
+    if (__any_sync(kAll, far_scores)) scores_far(base, x);
     if (special) {  // uniform
       if (first) {  // R_b starts at the largest scale here and two binades of room
         const uint32_t none[Q] = {};
