@@ -80,7 +80,7 @@ struct MxCfg {
   static constexpr int kGroup = NB * kMxBytes;    // bytes of one group of one operand
   static constexpr int kStage = 4 * kGroup;       // K of two groups, V of two groups
   static constexpr int kRing = kStages * kStage;  // per warp
-  static constexpr int kState = kHeads * (D + 2); // floats: acc [heads][D], m [heads], l [heads]
+  static constexpr int kState = kHeads * (D + 2); // floats: mean of V [heads][D], m [heads], l [heads]
   static constexpr int kSmemRing = kWarps * kRing;
   static constexpr int kSmemHeads = kWarps * kState * 4;  // parts that end before their warp's range does
   static constexpr int kSmemUnits = kWarps * 64 * 16;     // two batches of 32 units per warp
@@ -669,33 +669,34 @@ struct MxWarp {
     }
   }
 
-  // Sum l over the keys of the lanes, bring o to its true scale.
+  // Sum l over the keys of the lanes.
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[c] += __shfl_xor_sync(kAll, l[c], off);
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const float f = exp2i(static_cast<int>((ref[b / 4] >> (8 * (b % 4))) & 255u) - 127);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[c][b][i] *= f;
-      }
-    }
+  }
+
+  // The mean of V over the keys seen: o is divided by l, which holds the lift of p as o does, before the scale comes
+  // back, so that the result is in range where V is.
+  __device__ __forceinline__ float inverse(int c) const { return l[c] == 0.f ? 0.f : __fdividef(1.f, l[c]); }
+  __device__ __forceinline__ float scale_back(int b) const {
+    return exp2i(static_cast<int>((ref[b / 4] >> (8 * (b % 4))) & 255u) - 127);
   }
 
   __device__ __forceinline__ void write_out(T *out, int heads) const {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       if (c * kQueries + t >= heads) continue;
-      const float inv = l[c] == 0.f ? 0.f : 1.f / l[c];
+      const float inv = inverse(c);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         using V = typename std::conditional<kSplit, uint4, uint2>::type;
+        const float f = scale_back(b);
         V v;
         T *e = reinterpret_cast<T *>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_float(o[c][b][i] * inv);
+        for (int i = 0; i < 4; ++i) e[i] = Elem<T>::from_float(o[c][b][i] * inv * f);
         *reinterpret_cast<V *>(out + (c * kQueries + t) * D + b * 32 + g * 4) = v;
       }
     }
@@ -706,9 +707,13 @@ struct MxWarp {
     for (int c = 0; c < CT; ++c) {
       const int h = c * kQueries + t;
       if (h >= heads) continue;
+      const float inv = inverse(c);
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-        *reinterpret_cast<float4 *>(st + h * D + b * 32 + g * 4) = make_float4(o[c][b][0], o[c][b][1], o[c][b][2], o[c][b][3]);
+      for (int b = 0; b < NB; ++b) {
+        const float f = scale_back(b);
+        *reinterpret_cast<float4 *>(st + h * D + b * 32 + g * 4) = make_float4(
+            o[c][b][0] * inv * f, o[c][b][1] * inv * f, o[c][b][2] * inv * f, o[c][b][3] * inv * f);
+      }
       if (g == 0) {
         st[C::kHeads * D + h] = m[c];
         st[C::kHeads * D + C::kHeads + h] = l[c];
@@ -1026,7 +1031,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
       float L = mine ? f * l : 0.f;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(kAll, L, off);
-      if (mine) factor[rank * C::kHeads + h] = f;
+      if (mine) factor[rank * C::kHeads + h] = L == 0.f ? 0.f : __fdividef(f * l, L);  // its share of the mean
       if (lane == k) run_ml[rank * C::kHeads + h] = make_float2(M, L);
     }
   }
@@ -1055,16 +1060,18 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
     T *out = static_cast<T *>(p.out) + row * D;
     for (int e = threadIdx.x; e < heads * D; e += blockDim.x) {
       const int h = e / D;
-      const float2 ml = run_ml[j0 * C::kHeads + h];
       float A = 0.f;
 #pragma unroll 4
       for (int j = j0; j < j1; ++j)
         A = fmaf(factor[j * C::kHeads + h], reinterpret_cast<const float *>(smem)[part_at[j] + e], A);
       if (flags == 3) {
-        out[e] = Elem<T>::from_float(ml.y == 0.f ? 0.f : A / ml.y);
+        out[e] = Elem<T>::from_float(A);
       } else {
         state[e] = A;
-        if (e - h * D == 0) state[C::kHeads * D + h] = ml.x, state[C::kHeads * D + C::kHeads + h] = ml.y;
+        if (e - h * D == 0) {
+          const float2 ml = run_ml[j0 * C::kHeads + h];
+          state[C::kHeads * D + h] = ml.x, state[C::kHeads * D + C::kHeads + h] = ml.y;
+        }
       }
     }
   }
@@ -1079,72 +1086,93 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
   pdl_launch_dependents();
 }
 
-// Segments that cross CTAs: block c joins the one that goes on from CTA c.  A thread takes 4 elements;
-// the quarters of the block take every fourth part.  The first four parts are read while
-// the block is still finding out whether they are any.  (Joining in the first launch, by the
-// CTA that arrives last, took longer: its fences and the atomic cost 5 us at 1 x 131072, this launch 4.)
+// Segments that cross CTAs: block c joins the one that goes on from CTA c.  A warp takes a query head's m and l,
+// a lane to a part, and turns them into the parts' shares of the mean; then a thread takes 4 elements, the quarters of the
+// block every fourth part.  The first parts are read while the block is still finding out whether they are
+// any.  (Joining in the first launch, by the CTA that arrives last, took longer: its fences and the atomic
+// cost 5 us at 1 x 131072, this launch 4.)
 constexpr int kJoinWays = 4;
 constexpr int kJoinLanes = 128;
+constexpr int kMaxCtas = 192;  // of the first launch
 template <typename T, int NB, int CT>
 __global__ void __launch_bounds__(kJoinLanes * kJoinWays)
     mxfp4_decode_mma_join_kernel(const MxDecodeParams p, const MxPlan plan) {
   using C = MxCfg<NB, CT, std::is_same<T, float>::value>;
   constexpr int D = C::D, kVecs = C::kHeads * D / 4;
   constexpr int kPer = (kVecs + kJoinLanes - 1) / kJoinLanes;
+  constexpr int kBatches = kMaxCtas / 32;
+  constexpr float kNone = -1.f;  // the share of a part without keys, whose sums are not read
+  static_assert(C::kHeads <= kJoinLanes * kJoinWays / 32, "a warp to a query head");
   __shared__ float4 sums[kJoinWays][kVecs];
-  __shared__ float2 ml[kJoinWays][C::kHeads];
+  __shared__ float share[kMaxCtas][C::kHeads];
   const int ctas = gridDim.x, first = blockIdx.x;
   const int lane = threadIdx.x % kJoinLanes, way = threadIdx.x / kJoinLanes;
+  const int head = threadIdx.x / 32, part = threadIdx.x % 32;
   const float *base = p.workspace + static_cast<int64_t>(first) * 2 * C::kState;
-  struct Part {
-    float m[kPer], l[kPer];
-    float4 a[kPer];
+  auto state_of = [&](int k) {  // the first CTA's second state, then the others' first
+    return base + (k == 0 ? 1 : 2 * k) * C::kState;
   };
-  auto read = [&](int k, Part &x) {  // k = 0: the first CTA's second state, then the others' first
-    const float *st = base + (k == 0 ? 1 : 2 * k) * C::kState;
+  auto read = [&](int k, float4 (&a)[kPer]) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int v = lane + i * kJoinLanes;
-      if (v >= kVecs) break;
-      x.m[i] = __ldcg(st + C::kHeads * D + v * 4 / D);
-      x.l[i] = __ldcg(st + C::kHeads * D + C::kHeads + v * 4 / D);
-      x.a[i] = __ldcg(reinterpret_cast<const float4 *>(st) + v);
+      if (v < kVecs) a[i] = __ldcg(reinterpret_cast<const float4 *>(state_of(k)) + v);
     }
   };
   pdl_wait();
   pdl_launch_dependents();
   const MxMeta meta =
       reinterpret_cast<const MxMeta *>(p.workspace + static_cast<int64_t>(ctas) * 2 * C::kState)[first];
-  Part x;
+  float4 x[kPer];
   if (first + way < ctas) read(way, x);
   if (meta.segment < 0) return;
   const int parts = min(meta.parts, ctas - first);
-  float M[kPer], L[kPer];
+  if (head < C::kHeads) {
+    float m[kBatches], l[kBatches], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+      if (i * 32 + part >= parts) continue;
+      const float *st = state_of(i * 32 + part) + C::kHeads * D + head;
+      m[i] = __ldcg(st), l[i] = __ldcg(st + C::kHeads);
+      M = fmaxf(M, m[i]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(kAll, M, off));
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) L += part_factor(m[i], l[i], M) * l[i];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(kAll, L, off);
+#pragma unroll
+    for (int i = 0; i < kBatches; ++i) {
+      if (i * 32 + part >= parts) break;
+      const bool none = m[i] == -INFINITY && l[i] == 0.f;
+      share[i * 32 + part][head] = none ? kNone : L == 0.f ? 0.f : __fdividef(part_factor(m[i], l[i], M) * l[i], L);
+    }
+  }
+  __syncthreads();
   float4 A[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) M[i] = -INFINITY, L[i] = 0.f, A[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < kPer; ++i) A[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = way; k < parts; k += kJoinWays) {
-    Part y;
+    float4 y[kPer];
     if (k + kJoinWays < parts) read(k + kJoinWays, y);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (lane + i * kJoinLanes >= kVecs) break;
-      if (x.m[i] == -INFINITY && x.l[i] == 0.f) continue;  // a part without keys has no sums
-      const float next = fmaxf(M[i], x.m[i]);
-      const float f = part_factor(M[i], L[i], next), e = part_factor(x.m[i], x.l[i], next);
-      L[i] = f * L[i] + e * x.l[i];
-      A[i].x = f * A[i].x + e * x.a[i].x, A[i].y = f * A[i].y + e * x.a[i].y;
-      A[i].z = f * A[i].z + e * x.a[i].z, A[i].w = f * A[i].w + e * x.a[i].w;
-      M[i] = next;
+      const int v = lane + i * kJoinLanes;
+      if (v >= kVecs) break;
+      const float s = share[k][v * 4 / D];
+      if (s == kNone) continue;
+      A[i].x = fmaf(s, x[i].x, A[i].x), A[i].y = fmaf(s, x[i].y, A[i].y);
+      A[i].z = fmaf(s, x[i].z, A[i].z), A[i].w = fmaf(s, x[i].w, A[i].w);
     }
-    x = y;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = y[i];
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int v = lane + i * kJoinLanes;
-    if (v >= kVecs) break;
-    sums[way][v] = A[i];
-    if (v * 4 % D == 0) ml[way][v * 4 / D] = make_float2(M[i], L[i]);
+    if (v < kVecs) sums[way][v] = A[i];
   }
   __syncthreads();
   const int G = p.num_q_heads / p.num_kv_heads, H = p.num_kv_heads * plan.tiles;
@@ -1153,17 +1181,10 @@ __global__ void __launch_bounds__(kJoinLanes * kJoinWays)
   const int heads = min(C::kHeads, G - h0);
   T *out = static_cast<T *>(p.out) + (static_cast<int64_t>(s) * p.num_q_heads + kvh * G + h0) * D;
   for (int e = threadIdx.x; e < heads * D; e += kJoinLanes * kJoinWays) {
-    const int h = e / D;
-    float m = -INFINITY, l = 0.f, a = 0.f;
+    float a = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWays; ++w) m = fmaxf(m, ml[w][h].x);
-#pragma unroll
-    for (int w = 0; w < kJoinWays; ++w) {
-      const float f = part_factor(ml[w][h].x, ml[w][h].y, m);
-      l += f * ml[w][h].y;
-      a = fmaf(f, reinterpret_cast<const float *>(sums[w])[e], a);
-    }
-    out[e] = Elem<T>::from_float(l == 0.f ? 0.f : a / l);
+    for (int w = 0; w < kJoinWays; ++w) a += reinterpret_cast<const float *>(sums[w])[e];
+    out[e] = Elem<T>::from_float(a);
   }
 }
 
@@ -1196,6 +1217,8 @@ int mma_tiles(int num_q_heads, int num_kv_heads, int head_dim) {
   const int heads = kQueries * mma_columns(num_q_heads, num_kv_heads, head_dim);
   return (num_q_heads / num_kv_heads + heads - 1) / heads;
 }
+
+int mma_ctas(int sms) { return sms < kMaxCtas ? sms : kMaxCtas; }
 
 // Whether some lengths that the table can hold need the second launch: not when
 // every segment has a CTA and a full table is no more than the slack per warp.
@@ -1236,6 +1259,7 @@ bool mxfp4_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int
 
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
                               int sms) {
+  sms = mma_ctas(sms);
   if (!mma_joins(num_seqs, num_q_heads, num_kv_heads, head_dim, capacity, sms)) return 0;
   const size_t heads = kQueries * mma_columns(num_q_heads, num_kv_heads, head_dim);
   return static_cast<size_t>(sms) * (2 * heads * (head_dim + 2) * sizeof(float) + sizeof(MxMeta));
@@ -1244,7 +1268,7 @@ size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_head
 cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream) {
   const int tiles = mma_tiles(p.num_q_heads, p.num_kv_heads, p.head_dim);
   const int columns = mma_columns(p.num_q_heads, p.num_kv_heads, p.head_dim);
-  const int sms = sm_count_current();
+  const int sms = mma_ctas(sm_count_current());
   const int64_t capacity = p.bt_stride * p.block_size;
   const int64_t H = static_cast<int64_t>(p.num_kv_heads) * tiles;
   int64_t slice = ((int64_t{1} << 31) - 1) / ((capacity / kUnit + 1) * H);  // units stay in 32 bits

@@ -24,7 +24,7 @@ def _at(rng, nb, bs, hkv, d, power):
 @pytest.mark.parametrize("name", ["bf16", "f32"])
 @pytest.mark.parametrize("d,group", [(32, 4), (64, 7), (96, 2), (128, 4), (128, 8), (256, 4)])
 @pytest.mark.parametrize("k_power,q_power,v_power", [
-    (118, -118, 0), (104, -104, 0), (-110, 112, -100)])
+    (118, -118, 0), (104, -104, 0), (-110, 112, -100), (0, 0, 110), (0, 0, 124), (118, -118, 124), (0, 0, -122)])
 def test_decode_over_the_whole_range_of_scales(cuda_device, name, d, group, k_power, q_power, v_power):
     """Scores of ordinary size from keys and queries of 2^+-118, values up to fp32's end; sequences within a warp,
     over warps and over CTAs."""
