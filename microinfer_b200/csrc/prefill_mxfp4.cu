@@ -9,12 +9,12 @@
 // O += P V are m16n8k16 with fp32 accumulators, P passes from the one to the
 // other in registers; online softmax in fp32, the maximum followed 3 binades behind at most.
 // Types: bf16 holds every value of the cache (short of overflow), fp16 rounds
-// K outside its range, as the gather does; p in fp16 is lifted by 2^12, which keeps a key down to 2^-26 of
+// what lies below its smallest step; p in fp16 is lifted by 2^12, which keeps a key down to 2^-26 of
 // the largest at full precision.  fp32: K and V are exact in bf16, q and p go in as three bf16 parts
 // (24 bits), three MMAs for one.
 // A NaN block of V is held as zero and its dims are set to NaN in the rows that
-// see the key, so it never reaches rows before it.  So is one that fp16 does not hold, and its products are
-// added in fp32 to those rows.
+// see the key, so it never reaches rows before it.  So are blocks of K and V that fp16 does not hold, and their products
+// are added in fp32, K's to the scores and V's to those rows.
 // Few rows over a long context are split over the keys; a second launch joins
 // the splits.
 // Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2313 us, 223 TFLOP/s; 8 x 250 on 2000, 16/8
@@ -45,16 +45,17 @@ struct PfCfg {
   static constexpr bool kSplit = std::is_same<T, float>::value;
   using E = typename std::conditional<kSplit, __nv_bfloat16, T>::type;  // MMA operands
   static constexpr int kParts = kSplit ? 3 : 1;
-  // Scale bytes of V from here on are not for the MMA: fp16 ends at 65504 = 3.998 * 2^14.
+  // Scale bytes from here on are not for the MMA (of K in fp16 alone): fp16 ends at 65504 = 3.998 * 2^14.
   static constexpr bool kHalf = std::is_same<T, __half>::value;
   static constexpr uint32_t kApart = kHalf ? 127 + 14 : 255;
+  static constexpr int kMarks = kHalf ? 2 : 1;  // operands with such blocks: V, K
   static constexpr int D = NB * kMxBlock;
   static constexpr int kRowBytes = (NB + 1) / 2 * 128;  // rows of whole 128 bytes, for the swizzle
   static constexpr int kTile = kKeys * kRowBytes;      // K or V of a tile
   static constexpr int kQuery = kRows * kRowBytes;     // one part of q
   static constexpr int kChunks = 2 * kKeys * NB;  // a tile's (operand, key, block): 16 bytes of codes and a scale
   static constexpr int kPer = (kChunks + kThreads - 1) / kThreads;  // of those per thread
-  static constexpr int kSmem = kParts * kQuery + 4 * kTile + 2 * (kKeys + 4 * kGroups);
+  static constexpr int kSmem = kParts * kQuery + 4 * kTile + 2 * (kMarks * kKeys + 4 * kGroups);
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -104,6 +105,32 @@ __device__ __forceinline__ float rest(float x) {
   return x - Elem<E>::to_float(Elem<E>::from_float(x));
 }
 
+// fp16: rows `row` and row + 8 of q times the blocks of one key that fp16 does not hold, over the four lanes of a row,
+// each of which takes 8 dims of a block.  Called among what masked tiles do (a branch of its own after the products took 192 us at
+// 8 x 250 on 2000, 16/8 heads of 96, where this takes 172).
+template <int NB>
+__device__ __noinline__ float2 apart_scores(const uint8_t *codes, unsigned blocks, int tok, const uint8_t *q, int row, int t) {
+  float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+  for (int b = 0; b < NB; ++b) {
+    if (!(blocks >> b & 1u)) continue;
+    float k8[8];
+    mx_codes_to_f32(*reinterpret_cast<const uint32_t *>(codes + b * kMxBlockBytes + tok * 16 + t * 4),
+                    mx_scale(codes[NB * kMxBlockBytes + tok * NB + b]), k8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 f[4];
+      Vec16<__half>::unpack(*reinterpret_cast<const uint4 *>(q + at<NB>(row + 8 * i, b * 4 + t)), f);
+      float &to = i ? sum.y : sum.x;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) to = fmaf(f[u].x, k8[2 * u], fmaf(f[u].y, k8[2 * u + 1], to));
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) sum.x += __shfl_xor_sync(kAll, sum.x, off), sum.y += __shfl_xor_sync(kAll, sum.y, off);
+  return sum;
+}
+
 }  // namespace
 
 template <typename T, int NB>
@@ -114,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   constexpr int D = C::D, kParts = C::kParts;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *tiles = smem + kParts * C::kQuery;  // [2][K, V]
-  uint8_t *nan_v = tiles + 4 * C::kTile;       // [2][keys]: NaN blocks of V, a bit each
-  int *group_ok = reinterpret_cast<int *>(nan_v + 2 * kKeys);  // [2][groups]
+  uint8_t *marks = tiles + 4 * C::kTile;  // [2][V, K][keys]: blocks that are not for the MMA, a bit each
+  int *group_ok = reinterpret_cast<int *>(marks + 2 * C::kMarks * kKeys);  // [2][groups]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   pdl_wait();
 
@@ -225,6 +252,9 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       w.scales[i] = from[NB * kMxBlockBytes + tok * NB + c.b] | 1u << 16;
     }
   };
+  auto is_apart = [](bool value, uint32_t byte) {  // a NaN of K only meets its own scores
+    return byte >= C::kApart && (value || (C::kHalf && byte != 255u));
+  };
   auto place = [&](const Words &w, int buf) {
 #pragma unroll
     for (int i = 0; i < C::kPer; ++i) {
@@ -233,8 +263,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       uint8_t *to = tiles + (buf * 2 + c.value) * C::kTile;
       const int key = c.group * kMxGroup + tok;
       const uint32_t byte = w.scales[i] & 255u;
-      const bool apart = c.value && byte >= C::kApart;
-      const float f = apart ? 0.f : mx_scale(byte);
+      const float f = is_apart(c.value, byte) ? 0.f : mx_scale(byte);
       const uint32_t word[4] = {w.codes[i].x, w.codes[i].y, w.codes[i].z, w.codes[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -250,22 +279,29 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       }
     }
   };
-  // NaN blocks of V, and those fp16 does not hold
-  auto note_nan = [&](const Words &w, int buf) -> bool {
+  // NaN blocks of V, and those of K and V that fp16 does not hold
+  auto note_apart = [&](const Words &w, int buf) -> bool {
     bool any = false;
 #pragma unroll
-    for (int i = 0; i < C::kPer; ++i) any |= chunk(i).value && (w.scales[i] & 255u) >= C::kApart;
-    if (threadIdx.x < kKeys) nan_v[buf * kKeys + threadIdx.x] = 0;
+    for (int i = 0; i < C::kPer; ++i) any |= (C::kHalf || chunk(i).value) && (w.scales[i] & 255u) >= C::kApart;
+    if (threadIdx.x < C::kMarks * kKeys) marks[buf * C::kMarks * kKeys + threadIdx.x] = 0;
     return any;
   };
-  auto mark_nan = [&](const Words &w, int buf) {
+  auto mark_apart = [&](const Words &w, int buf) {
 #pragma unroll
     for (int i = 0; i < C::kPer; ++i) {
       const Chunk c = chunk(i);
       const int key = c.group * kMxGroup + tok;
-      if (c.exists && c.value && (w.scales[i] & 255u) >= C::kApart)
-        atomicOr(reinterpret_cast<unsigned *>(nan_v + buf * kKeys) + key / 4, 1u << (key % 4 * 8 + c.b));
+      if (c.exists && is_apart(c.value, w.scales[i] & 255u))
+        atomicOr(reinterpret_cast<unsigned *>(marks + (buf * C::kMarks + !c.value) * kKeys) + key / 4,
+                 1u << (key % 4 * 8 + c.b));
     }
+  };
+  // the group of a marked key of tile kt, which has a page
+  auto group_of = [&](const uint8_t *pool, int kt, int key) {
+    const uint32_t index = static_cast<uint32_t>(kt) * kGroups + key / kMxGroup, col = by_page.div(index);
+    return pool + ((static_cast<int64_t>(__ldg(table + col)) * p.num_kv_heads + kvh) * per_page + (index - col * per_page)) *
+                      (NB * kMxBytes);
   };
 
   // this thread's rows: g and g + 8 of its warp's 16
@@ -285,17 +321,17 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  bool has_nan = false;
+  bool has_apart = false;
   if (k_begin < k_end) {
     Words w;
     look_up(k_begin);
     fetch(k_begin, w);
     look_up(k_begin + 1);
     place(w, 0);
-    const bool mine = note_nan(w, 0);
-    has_nan = __syncthreads_or(mine);
-    if (has_nan) {
-      mark_nan(w, 0);
+    const bool mine = note_apart(w, 0);
+    has_apart = __syncthreads_or(mine);
+    if (has_apart) {
+      mark_apart(w, 0);
       __syncthreads();
     }
   }
@@ -342,8 +378,28 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     bool pages = true;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) pages &= group_ok[buf * kGroups + i] != 0;
-    const bool masked = key0 + kKeys - 1 > first_pos || key0 + kKeys > keys || !pages;  // uniform in the warp
+    const bool masked = key0 + kKeys - 1 > first_pos || key0 + kKeys > keys || !pages || (C::kHalf && has_apart);  // uniform in the warp
     if (masked) {
+      if constexpr (C::kHalf) {
+        if (has_apart) {  // K's blocks past fp16
+#pragma unroll 1
+          for (int key = 0; key < kKeys; ++key) {
+            const unsigned blocks = marks[(buf * C::kMarks + 1) * kKeys + key];
+            if (!blocks) continue;
+            const float2 sum = apart_scores<NB>(group_of(p.key_pages, kt, key), blocks, key % kMxGroup, smem, warp * 16 + g, t);
+            if (t == key % 8 / 2) {
+#pragma unroll
+              for (int i = 0; i < kKeys / 8; ++i)
+                if (i == key / 8) {
+                  if (key & 1)
+                    s[i][1] += sum.x, s[i][3] += sum.y;
+                  else
+                    s[i][0] += sum.x, s[i][2] += sum.y;
+                }
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kKeys / 8; ++i) {
         const int key = key0 + i * 8 + 2 * t;
@@ -407,10 +463,10 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
         }
       }
     }
-    if (has_nan) {  // uniform in the CTA
+    if (has_apart) {  // uniform in the CTA
 #pragma unroll 1
       for (int key = 0; key < kKeys; ++key) {
-        const unsigned blocks = nan_v[buf * kKeys + key];
+        const unsigned blocks = marks[buf * C::kMarks * kKeys + key];
         if (!blocks) continue;
         float pk[2] = {0.f, 0.f};  // p of this key in this thread's rows
         const uint8_t *codes = nullptr;
@@ -420,10 +476,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
             if (i == key / 8) pk[0] = key & 1 ? s[i][1] : s[i][0], pk[1] = key & 1 ? s[i][3] : s[i][2];
           pk[0] = __shfl_sync(kAll, pk[0], (lane & ~3) | (key % 8 / 2));
           pk[1] = __shfl_sync(kAll, pk[1], (lane & ~3) | (key % 8 / 2));
-          const uint32_t index = static_cast<uint32_t>(kt) * kGroups + key / kMxGroup, col = by_page.div(index);
-          codes = p.value_pages +  // a marked key has a page
-                  ((static_cast<int64_t>(__ldg(table + col)) * p.num_kv_heads + kvh) * per_page + (index - col * per_page)) *
-                      (NB * kMxBytes);
+          codes = group_of(p.value_pages, kt, key);
         }
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
@@ -445,10 +498,10 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     }
     if (more) {
       place(w, buf ^ 1);
-      const bool mine = note_nan(w, buf ^ 1);
-      has_nan = __syncthreads_or(mine);
-      if (has_nan) {
-        mark_nan(w, buf ^ 1);
+      const bool mine = note_apart(w, buf ^ 1);
+      has_apart = __syncthreads_or(mine);
+      if (has_apart) {
+        mark_apart(w, buf ^ 1);
         __syncthreads();
       }
     }
