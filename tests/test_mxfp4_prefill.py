@@ -6,7 +6,7 @@ import torch
 
 import microinfer_b200 as mi
 from oracle import mxfp4_oracle as mo
-from tests.test_mxfp4 import PREFILL_STEP, _close, _cuda, _pages, _table
+from tests.test_mxfp4 import DTYPES, PREFILL_STEP, _close, _cuda, _pages, _prefill_case, _table
 
 gpu = pytest.mark.gpu
 LARGE = [140, 150, 1, 137, 144]  # with 8 kv heads of 128, 2 query heads each: 120 tiles of 128 rows
@@ -38,3 +38,31 @@ def test_prefill_keys_past_fp16(cuda_device, d, large):
     parts = [mo.attention(q[at[r]:at[r + 1]], mo.rows(kp, table[r], c), mo.rows(vp, table[r], c), d ** -0.5)
              for r, c in enumerate(ctxs)]
     _close(got, *[np.concatenate(x) for x in zip(*parts)], torch.float16, PREFILL_STEP[torch.float16])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+def test_gathered_scale_of_zero(cuda_device, name):
+    """Every key that a row sees weighs the same, masked ones nothing; rows before the first key are zeros."""
+    hkv, group, d = (8, 2, 128) if name != "f32" else (2, 2, 160)
+    got, free, want, dtype = _prefill_case(cuda_device, name, hkv, group, d, 16, LARGE, [140, 200, 9, 130, 300], scale=0.0)
+    for x in (got, free):
+        _close(x, *want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_16_bit_prefill_with_a_scale_of_zero(cuda_device, name):
+    dtype = DTYPES[name]
+    query, k, v = (torch.randn(200, h, 128, device=cuda_device).to(dtype) for h in (16, 8, 8))
+    cu = torch.tensor([0, 200], dtype=torch.int32, device=cuda_device)
+    want = (v.double().cumsum(0) / torch.arange(1, 201, device=cuda_device)[:, None, None]).repeat_interleave(2, 1)
+    # p is one for every key: what is left is the sum in fp32 and one rounding
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 200 * 2.0 ** -23 * v.double().abs().max()
+    got = mi.varlen_prefill(query, k, v, cu, cu, max_seqlen_q=200, scale=0.0)
+    assert bool(((got.double() - want).abs() <= bound).all())
+    pages_k, pages_v = (torch.cat([t, t[:8]]).view(13, 16, 8, 128) for t in (k, v))
+    table = torch.arange(13, dtype=torch.int32, device=cuda_device)[None]
+    got = mi.paged_prefill(query, pages_k, pages_v, cu, cu, table, max_seqlen_q=200, scale=0.0)
+    assert bool(((got.double() - want).abs() <= bound).all())
+    mi.check_device_status(cuda_device)
