@@ -478,6 +478,27 @@ MI_API int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_
                            void *stream);
 
 /*
+ * The same by way of rows: K and V of the contexts (kv_rows, their sum or a bound on it; rows past it are flagged)
+ * are decoded into the workspace and attended to as mi_varlen_prefill does, for chunks large enough for the tensor
+ * cores' dense kernel.  Sequences with blocks that do not go through it (a NaN of V, and in f16 a block past
+ * 65504) are then done over from the pages, so results are those of mi_paged_prefill_mxfp4; `out` must not
+ * overlap the query.  `max_context` bounds one context.
+ */
+MI_API size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t kv_rows,
+                                                       int32_t num_kv_heads, int32_t head_dim,
+                                                       int32_t dtype);
+MI_API int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *key_pages,
+                                    const void *value_pages, int64_t num_blocks,
+                                    int32_t block_size, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                    const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                    const int32_t *block_tables, int64_t block_table_stride,
+                                    int64_t num_seqs, int64_t num_tokens, int32_t max_seqlen_q,
+                                    int64_t max_context, int64_t kv_rows, float scale,
+                                    void *workspace, size_t workspace_bytes,
+                                    int32_t *dev_status, void *stream);
+
+/*
  * Bounded-wait self test: one thread spins on `flag` (device int32) until it
  * becomes non-zero or `timeout_ns` passes, then ORs MI_DEV_TIMEOUT into
  * dev_status if it ran out.  Exercises the same bounded-wait helper every

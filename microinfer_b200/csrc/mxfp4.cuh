@@ -12,6 +12,8 @@
 // 8 x 16-byte rows of an ldmatrix touch every shared-memory bank once.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mi {
@@ -49,6 +51,16 @@ __device__ __forceinline__ int64_t mx_group_offset(int64_t slot, int h, int bloc
 
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
+}
+
+// Blocks that 16-bit rows of type T cannot stand for in a product with zeros: NaN blocks of V (0 * NaN reaches rows that do
+// not see the key; one of K only meets its own scores), and those of K and V past fp16, which ends at
+// 65504 = 3.998 * 2^14.
+template <typename T>
+constexpr uint32_t mx_apart_from = std::is_same<T, __half>::value ? 127 + 14 : 255;
+template <typename T>
+__device__ __forceinline__ bool mx_apart(bool value, uint32_t byte) {
+  return byte >= mx_apart_from<T> && (value || (std::is_same<T, __half>::value && byte != 255u));
 }
 
 // Eight codes of a word, in element order, as four f16 pairs (exact).

@@ -155,8 +155,9 @@ __device__ __forceinline__ void write8(T *dst, const float (&x)[8]) {
   }
 }
 
-// grid (groups of 16 positions x kv heads, 8 warps to a CTA; sequences).
-template <typename T, int NB>
+// grid (groups of 16 positions x kv heads, 8 warps to a CTA; sequences).  REDO: rows for the dense prefill, which
+// notes the sequences that it cannot do.
+template <typename T, int NB, bool REDO>
 __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams p, const FastDiv by_heads,
                                                            const FastDiv by_page) {
   pdl_wait();
@@ -200,6 +201,12 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
       const int tok = half * 8 + (lane >> 2);
       const int64_t row = base + pos0 + tok;
       if (pos0 + tok >= ctx) continue;
+      if constexpr (REDO) {
+        bool apart = false;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) apart |= mx_apart<T>(false, ks[half][i]) || mx_apart<T>(true, vs[half][i]);
+        if (apart) p.redo[seq] = 1;
+      }
       if (row < 0 || row >= p.out_rows) {
         flag_status(p.status, MI_DEV_BAD_SLOT);
         continue;
@@ -238,15 +245,17 @@ cudaError_t launch_store_ti(const MxStoreParams &p, bool vec, cudaStream_t strea
   return launch_store_tin<T, I, 0>(p, vec, stream);
 }
 
-template <typename T>
+template <typename T, bool REDO>
 cudaError_t launch_gather_t(const MxGatherParams &p, int64_t num_seqs, int64_t max_context, cudaStream_t stream) {
   const int64_t tasks = (max_context + kMxGroup - 1) / kMxGroup * p.num_kv_heads;
   if (tasks >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>((tasks + 7) / 8), static_cast<unsigned>(num_seqs)), block(256);
   const FastDiv by_heads(p.num_kv_heads), by_page(p.block_size / kMxGroup);
-  if (p.head_dim == 128) return launch_pdl(mxfp4_gather_kernel<T, 4>, grid, block, 0, stream, p, by_heads, by_page);
-  if (p.head_dim == 64) return launch_pdl(mxfp4_gather_kernel<T, 2>, grid, block, 0, stream, p, by_heads, by_page);
-  return launch_pdl(mxfp4_gather_kernel<T, 0>, grid, block, 0, stream, p, by_heads, by_page);
+  if (p.head_dim == 128)
+    return launch_pdl(mxfp4_gather_kernel<T, 4, REDO>, grid, block, 0, stream, p, by_heads, by_page);
+  if constexpr (REDO) return cudaErrorInvalidValue;  // the dense kernel has one head_dim
+  if (p.head_dim == 64) return launch_pdl(mxfp4_gather_kernel<T, 2, false>, grid, block, 0, stream, p, by_heads, by_page);
+  return launch_pdl(mxfp4_gather_kernel<T, 0, false>, grid, block, 0, stream, p, by_heads, by_page);
 }
 
 template <typename T>
@@ -266,9 +275,12 @@ cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtyp
 
 cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
                                 cudaStream_t stream) {
-  if (dtype == MI_DTYPE_BFLOAT16) return launch_gather_t<__nv_bfloat16>(p, num_seqs, max_context, stream);
-  if (dtype == MI_DTYPE_FLOAT16) return launch_gather_t<__half>(p, num_seqs, max_context, stream);
-  return launch_gather_t<float>(p, num_seqs, max_context, stream);
+  if (p.redo != nullptr)
+    return dtype == MI_DTYPE_BFLOAT16 ? launch_gather_t<__nv_bfloat16, true>(p, num_seqs, max_context, stream)
+                                      : launch_gather_t<__half, true>(p, num_seqs, max_context, stream);
+  if (dtype == MI_DTYPE_BFLOAT16) return launch_gather_t<__nv_bfloat16, false>(p, num_seqs, max_context, stream);
+  if (dtype == MI_DTYPE_FLOAT16) return launch_gather_t<__half, false>(p, num_seqs, max_context, stream);
+  return launch_gather_t<float, false>(p, num_seqs, max_context, stream);
 }
 
 }  // namespace mi

@@ -272,4 +272,100 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
       launch_mxfp4_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, static_cast<cudaStream_t>(stream)));
 }
 
+// K and V of kv_rows rows, each from a multiple of 256 bytes, then a word per sequence.
+static size_t gathered_rows_bytes(int64_t kv_rows, int32_t num_kv_heads, int32_t head_dim, int32_t dtype) {
+  const size_t bytes = static_cast<size_t>(kv_rows) * num_kv_heads * head_dim * (dtype == MI_DTYPE_FLOAT32 ? 4 : 2);
+  return (bytes + 255) / 256 * 256;
+}
+
+size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t kv_rows, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t dtype) {
+  if (num_seqs <= 0 || kv_rows <= 0 || num_kv_heads <= 0 || head_dim <= 0 || !known_dtype(dtype)) return 0;
+  return 2 * gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype) + num_seqs * sizeof(int32_t);
+}
+
+int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *key_pages, const void *value_pages,
+                                    int64_t num_blocks, int32_t block_size, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                    const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                    const int32_t *block_tables, int64_t block_table_stride, int64_t num_seqs,
+                                    int64_t num_tokens, int32_t max_seqlen_q, int64_t max_context, int64_t kv_rows,
+                                    float scale, void *workspace, size_t workspace_bytes, int32_t *dev_status,
+                                    void *stream) {
+  if (!known_dtype(dtype)) return capi_fail(MI_ERR_INVALID, "unknown dtype");
+  if (const int s = check_cache(num_blocks, block_size, num_kv_heads, head_dim)) return s;
+  if (num_seqs < 0 || num_tokens < 0 || max_context < 0 || kv_rows < 0 || block_table_stride < 0)
+    return capi_fail(MI_ERR_INVALID, "negative sizes");
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads != 0)
+    return capi_fail(MI_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads");
+  if (num_seqs > 65535 || num_kv_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
+  if (num_seqs == 0 || num_tokens == 0) return MI_OK;
+  if (max_seqlen_q <= 0 || kv_rows == 0) return capi_fail(MI_ERR_INVALID, "max_seqlen_q and kv_rows must be positive");
+  if (!out || !query || !key_pages || !value_pages || !cu_seqlens_q || !cu_seqlens_k || !block_tables)
+    return capi_fail(MI_ERR_INVALID, "null pointer");
+  if (!aligned16(query) || !aligned16(out)) return capi_fail(MI_ERR_ALIGNMENT, "query and out must be 16-byte aligned");
+  const size_t rows = gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype);
+  if (workspace == nullptr ||
+      workspace_bytes < mi_paged_prefill_mxfp4_gathered_workspace_bytes(num_seqs, kv_rows, num_kv_heads, head_dim, dtype))
+    return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_prefill_mxfp4_gathered_workspace_bytes)");
+  if (!aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if (const int s = capi_select_device(key_pages)) return s;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char *keys = static_cast<char *>(workspace), *values = keys + rows;
+  // The tensor-core kernel multiplies what a row does not see by zero: sequences with blocks that this does not suit are
+  // noted by the gather and done over from the pages (their tables have to be within that kernel's limit).
+  const bool dense = mi_prefill_kernel_for(dtype, head_dim, num_q_heads, num_kv_heads, 0) == 2;
+  int32_t *redo = nullptr;
+  if (dense && max_seqlen_q <= (1 << 24) && block_table_stride <= (INT32_MAX - 256) / block_size) {
+    redo = reinterpret_cast<int32_t *>(values + rows);
+    if (const int s = capi_cuda_status(cudaMemsetAsync(redo, 0, num_seqs * sizeof(int32_t), st))) return s;
+  }
+  MxGatherParams g = {};
+  g.out_keys = keys;
+  g.out_values = values;
+  g.key_pages = static_cast<const uint8_t *>(key_pages);
+  g.value_pages = static_cast<const uint8_t *>(value_pages);
+  g.block_tables = block_tables;
+  g.cu_seqlens_k = cu_seqlens_k;
+  g.block_table_stride = block_table_stride;
+  g.num_blocks = num_blocks;
+  g.out_rows = kv_rows;
+  g.redo = redo;
+  g.block_size = block_size;
+  g.num_kv_heads = num_kv_heads;
+  g.head_dim = head_dim;
+  g.status = dev_status;
+  if (max_context > 0) {
+    if (max_context / kMxGroup + 1 >= (int64_t{1} << 31) / num_kv_heads)
+      return capi_fail(MI_ERR_UNSUPPORTED, "max_context too large for one call");
+    if (!aligned16(key_pages) || !aligned16(value_pages))
+      return capi_fail(MI_ERR_ALIGNMENT, "pages must be 16-byte aligned");
+    if (const int s = capi_cuda_status(launch_mxfp4_gather(g, dtype, num_seqs, max_context, st))) return s;
+  }
+  if (const int s = mi_varlen_prefill(out, query, keys, values, static_cast<int64_t>(num_kv_heads) * head_dim, num_q_heads,
+                                      num_kv_heads, head_dim, dtype, cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens,
+                                      kv_rows, max_seqlen_q, scale, dev_status, stream))
+    return s;
+  if (redo == nullptr) return MI_OK;
+  MxPrefillParams p = {};
+  p.out = out;
+  p.query = query;
+  p.key_pages = g.key_pages;
+  p.value_pages = g.value_pages;
+  p.block_tables = block_tables;
+  p.cu_seqlens_q = cu_seqlens_q;
+  p.cu_seqlens_k = cu_seqlens_k;
+  p.redo = redo;
+  p.bt_stride = block_table_stride;
+  p.num_blocks = num_blocks;
+  p.num_tokens = num_tokens;
+  p.num_splits = 1;
+  p.block_size = block_size;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.scale_log2 = scale * kLog2eHost;
+  p.status = dev_status;
+  return capi_cuda_status(launch_mxfp4_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, st));
+}
+
 }  // extern "C"

@@ -163,6 +163,7 @@ struct MxGatherParams {
   int64_t block_table_stride;
   int64_t num_blocks;
   int64_t out_rows;  // rows of out_keys / out_values; never written past
+  int32_t *redo;     // null, or a word per sequence, set where a block is not for the dense kernel (mxfp4.cuh)
   int32_t block_size;
   int32_t num_kv_heads;
   int32_t head_dim;
@@ -196,6 +197,7 @@ struct MxPrefillParams {
   const int32_t *cu_seqlens_q;
   const int32_t *cu_seqlens_k;
   float *workspace;  // num_splits > 1: [split][token][q head][2 + D]
+  const int32_t *redo;  // null, or a word per sequence: those without are left as they are
   int64_t bt_stride;
   int64_t num_blocks;
   int64_t num_tokens;

@@ -45,9 +45,8 @@ struct PfCfg {
   static constexpr bool kSplit = std::is_same<T, float>::value;
   using E = typename std::conditional<kSplit, __nv_bfloat16, T>::type;  // MMA operands
   static constexpr int kParts = kSplit ? 3 : 1;
-  // Scale bytes from here on are not for the MMA (of K in fp16 alone): fp16 ends at 65504 = 3.998 * 2^14.
   static constexpr bool kHalf = std::is_same<T, __half>::value;
-  static constexpr uint32_t kApart = kHalf ? 127 + 14 : 255;
+  static constexpr uint32_t kApart = mx_apart_from<T>;  // scale bytes from here on are not for the MMA (of K in fp16 alone)
   static constexpr int kMarks = kHalf ? 2 : 1;  // operands with such blocks: V, K
   static constexpr int D = NB * kMxBlock;
   static constexpr int kRowBytes = (NB + 1) / 2 * 128;  // rows of whole 128 bytes, for the swizzle
@@ -133,9 +132,10 @@ __device__ __noinline__ float2 apart_scores(const uint8_t *codes, unsigned block
 
 }  // namespace
 
+// 128 rows of one kv head against the keys of one split.
 template <typename T, int NB>
-__global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
-    mxfp4_prefill_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
+__device__ __forceinline__ void prefill_tile(const MxPrefillParams &p, const FastDiv &by_group, const FastDiv &by_page,
+                                             int seq, int kvh, int tile, int split) {
   using C = PfCfg<T, NB>;
   using E = typename C::E;
   constexpr int D = C::D, kParts = C::kParts;
@@ -144,11 +144,6 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   uint8_t *marks = tiles + 4 * C::kTile;  // [2][V, K][keys]: blocks that are not for the MMA, a bit each
   int *group_ok = reinterpret_cast<int *>(marks + 2 * C::kMarks * kKeys);  // [2][groups]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  pdl_wait();
-
-  const int seq = blockIdx.z, kvh = blockIdx.y;
-  const int tile = (gridDim.x - 1 - blockIdx.x) / p.num_splits;  // the last rows, with the most keys, first
-  const int split = (gridDim.x - 1 - blockIdx.x) % p.num_splits;
   const int G = p.num_q_heads / p.num_kv_heads;
   const int64_t q0 = p.cu_seqlens_q[seq];
   const int64_t q_len = p.cu_seqlens_q[seq + 1] - q0;
@@ -252,9 +247,6 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       w.scales[i] = from[NB * kMxBlockBytes + tok * NB + c.b] | 1u << 16;
     }
   };
-  auto is_apart = [](bool value, uint32_t byte) {  // a NaN of K only meets its own scores
-    return byte >= C::kApart && (value || (C::kHalf && byte != 255u));
-  };
   auto place = [&](const Words &w, int buf) {
 #pragma unroll
     for (int i = 0; i < C::kPer; ++i) {
@@ -263,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
       uint8_t *to = tiles + (buf * 2 + c.value) * C::kTile;
       const int key = c.group * kMxGroup + tok;
       const uint32_t byte = w.scales[i] & 255u;
-      const float f = is_apart(c.value, byte) ? 0.f : mx_scale(byte);
+      const float f = mx_apart<T>(c.value, byte) ? 0.f : mx_scale(byte);
       const uint32_t word[4] = {w.codes[i].x, w.codes[i].y, w.codes[i].z, w.codes[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -292,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
     for (int i = 0; i < C::kPer; ++i) {
       const Chunk c = chunk(i);
       const int key = c.group * kMxGroup + tok;
-      if (c.exists && is_apart(c.value, w.scales[i] & 255u))
+      if (c.exists && mx_apart<T>(c.value, w.scales[i] & 255u))
         atomicOr(reinterpret_cast<unsigned *>(marks + (buf * C::kMarks + !c.value) * kKeys) + key / 4,
                  1u << (key % 4 * 8 + c.b));
     }
@@ -538,6 +530,28 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
         *reinterpret_cast<float2 *>(st + 2 + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
     }
   }
+}
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
+    mxfp4_prefill_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
+  pdl_wait();
+  const int at = gridDim.x - 1 - blockIdx.x;  // the last rows, with the most keys, first
+  prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, at / p.num_splits, at % p.num_splits);
+  pdl_launch_dependents();
+}
+
+// After the dense kernel: the sequences of which the gather has noted that it cannot do them, over again.  Hardly ever any, so
+// a few CTAs look (a CTA to a tile would take 100 us to find nothing at 64 x 2048 tokens) and take all tiles if so.
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
+    mxfp4_prefill_redo_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
+  pdl_wait();
+  if (p.redo[blockIdx.z] != 0)
+    for (int tile = tiles - 1 - blockIdx.x; tile >= 0; tile -= gridDim.x) {
+      prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, tile, 0);
+      __syncthreads();  // every warp has read its rows of q
+    }
   pdl_launch_dependents();
 }
 
@@ -593,14 +607,30 @@ cudaError_t launch_pf(const MxPrefillParams &p, int64_t num_seqs, int64_t max_se
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int64_t tiles = (max_seqlen_q * G + kRows - 1) / kRows;
+  const FastDiv by_group(G), by_page(p.block_size / kMxGroup);
+  if constexpr (NB == 4 && !C::kSplit) {
+    if (p.redo != nullptr) {
+      auto redo = mxfp4_prefill_redo_kernel<T, NB>;
+      static bool redo_attr_set[64] = {};
+      if (dev >= 64 || !redo_attr_set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(redo, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) redo_attr_set[dev] = true;
+      }
+      int64_t ctas = 2 * sm_count_current() / (p.num_kv_heads * num_seqs);
+      ctas = ctas < 1 ? 1 : ctas > tiles ? tiles : ctas;
+      return launch_pdl(redo, dim3(static_cast<unsigned>(ctas), p.num_kv_heads, static_cast<unsigned>(num_seqs)),
+                        dim3(kThreads), C::kSmem, stream, p, by_group, by_page, static_cast<int>(tiles));
+    }
+  }
+  if (p.redo != nullptr) return cudaErrorInvalidValue;
   if (dev >= 64 || !attr_set[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_set[dev] = true;
   }
-  const int G = p.num_q_heads / p.num_kv_heads;
-  const int64_t tiles = (max_seqlen_q * G + kRows - 1) / kRows;
-  const FastDiv by_group(G), by_page(p.block_size / kMxGroup);
   cudaError_t e = launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.num_splits), p.num_kv_heads,
                                         static_cast<unsigned>(num_seqs)),
                              dim3(kThreads), C::kSmem, stream, p, by_group, by_page);

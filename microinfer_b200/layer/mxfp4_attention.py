@@ -22,7 +22,7 @@ from functools import lru_cache
 import torch
 
 from microinfer_b200 import _lib
-from microinfer_b200.layer.paged_attention import _idx, varlen_prefill
+from microinfer_b200.layer.paged_attention import _idx
 from microinfer_b200.worker.mxfp4_cache import page_dims
 
 
@@ -48,6 +48,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     if not t.is_contiguous():
         return t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors of as many bytes share any."""
+    return abs(a.data_ptr() - b.data_ptr()) < a.numel() * a.element_size()
 
 
 @lru_cache(maxsize=4096)
@@ -230,12 +235,20 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
             _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
         )
         return out
-    keys = torch.empty((rows, hkv, d), dtype=query.dtype, device=device)
-    values = torch.empty_like(keys)
-    _gather(keys, values, key_pages, value_pages, dims, block_tables, cu_seqlens_k, rows, most,
-            device)
-    return varlen_prefill(query, keys, values, cu_seqlens_q, cu_seqlens_k,
-                          max_seqlen_q=max_seqlen_q, scale=scale, out=out)
+    if out is None:
+        out = torch.empty_like(query)
+    elif _overlap(out, query):  # some rows may be done twice
+        query = query.clone()
+    need = _lib.load().mi_paged_prefill_mxfp4_gathered_workspace_bytes(requests, rows, hkv, d, dtype)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.call(
+        "mi_paged_prefill_mxfp4_gathered", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),
+        value_pages.data_ptr(), dims[0], bs, hq, hkv, d, dtype, cu_seqlens_q.data_ptr(),
+        cu_seqlens_k.data_ptr(), block_tables.data_ptr(), width, requests, tokens, int(max_seqlen_q),
+        most, rows, 1.0 / math.sqrt(d) if scale is None else float(scale), workspace.data_ptr(), need,
+        _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
+    )
+    return out
 
 
 def paged_attention_mxfp4_meta(query, key_pages, value_pages, metadata, *,

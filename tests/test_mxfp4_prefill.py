@@ -6,14 +6,14 @@ import torch
 
 import microinfer_b200 as mi
 from oracle import mxfp4_oracle as mo
-from tests.test_mxfp4 import DTYPES, PREFILL_STEP, _close, _cuda, _pages, _prefill_case, _table
+from tests.test_mxfp4 import DTYPES, PREFILL_STEP, _close, _close_or_past, _cuda, _pages, _prefill_case, _table
 
 gpu = pytest.mark.gpu
 LARGE = [140, 150, 1, 137, 144]  # with 8 kv heads of 128, 2 query heads each: 120 tiles of 128 rows
 
 
 @gpu
-@pytest.mark.parametrize("d,large", [(64, False), (96, False), (256, False), (128, False)])
+@pytest.mark.parametrize("d,large", [(64, False), (96, False), (256, False), (128, False), (128, True)])
 def test_prefill_keys_past_fp16(cuda_device, d, large):
     """Keys of 2^14 to 2^24, met by queries small enough for ordinary scores."""
     q_lens, ctxs = (LARGE, [140, 200, 9, 137, 300]) if large else ([86], [90])
@@ -65,4 +65,57 @@ def test_16_bit_prefill_with_a_scale_of_zero(cuda_device, name):
     table = torch.arange(13, dtype=torch.int32, device=cuda_device)[None]
     got = mi.paged_prefill(query, pages_k, pages_v, cu, cu, table, max_seqlen_q=200, scale=0.0)
     assert bool(((got.double() - want).abs() <= bound).all())
+    mi.check_device_status(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_gathered_nan_blocks_reach_only_rows_that_see_them(cuda_device, name):
+    def edit(kp, vp, table):
+        kc, kb = mo.unpack(kp)
+        vc, vb = mo.unpack(vp)
+        vb[table[0, 60 // 16], 60 % 16, 0, 1] = 255  # position 60 of 140, row 60
+        kb[table[1, 180 // 16], 180 % 16, 0, 0] = 255  # position 180 of 200, row 130 of 150
+        kp[:], vp[:] = mo.pack(kc, kb), mo.pack(vc, vb)
+
+    got, free, _, _ = _prefill_case(cuda_device, name, 8, 2, 128, 16, LARGE, [140, 200, 9, 137, 300], edit=edit)
+    for x in (got, free):
+        nan = torch.isnan(x).cpu()
+        assert bool(nan[60:140, :2, 32:64].all()) and int(nan[:140].sum()) == 80 * 2 * 32
+        assert bool(nan[140 + 130:290, :2].all()) and int(nan[140:290].sum()) == 20 * 2 * 128
+        assert not bool(nan[290:].any())
+
+
+@gpu
+def test_gathered_values_past_fp16(cuda_device):
+    def edit(kp, vp, table):
+        code, byte = mo.unpack(vp)
+        for i, pos in enumerate([5, 6, 17, 40, 63, 64, 70, 129]):
+            byte[table[0, pos // 16], pos % 16, 0, i % 4] = 127 + [14, 15, 20, 40][i % 4]
+        vp[:] = mo.pack(code, byte)
+
+    got, free, want, dtype = _prefill_case(cuda_device, "f16", 8, 2, 128, 16, LARGE, [140, 200, 9, 137, 300], edit=edit)
+    for x in (got, free):
+        _close_or_past(x, *want, dtype, PREFILL_STEP[dtype])
+    assert bool(torch.isfinite(got[:5]).all())
+
+
+@gpu
+@pytest.mark.parametrize("name,hkv,group,d,q_lens,ctxs", [
+    ("bf16", 8, 2, 128, LARGE, [140, 200, 9, 137, 300]), ("f16", 8, 4, 128, LARGE, [140, 200, 9, 137, 300]),
+    ("f32", 2, 2, 160, [40, 3], [50, 900]), ("bf16", 2, 4, 96, [40, 1], [50, 3000]), ("f32", 2, 4, 96, [1], [3000])])
+def test_results_over_the_query(cuda_device, name, hkv, group, d, q_lens, ctxs):
+    rng = np.random.default_rng(50)
+    dtype = DTYPES[name]
+    nb = sum(-(-c // 16) for c in ctxs)
+    kp, vp = _pages(rng, nb, 16, hkv, d)
+    table = _cuda(_table(rng, ctxs, nb, 16), cuda_device)
+    query = _cuda(rng.standard_normal((sum(q_lens), hkv * group, d)), cuda_device, dtype)
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=cuda_device) for x in (q_lens, ctxs))
+    args = (_cuda(kp, cuda_device), _cuda(vp, cuda_device), cu_q, cu_k, table)
+    want = mi.paged_prefill_mxfp4(query, *args, max_seqlen_q=max(q_lens))
+    for _ in range(3):
+        over = query.clone()
+        assert mi.paged_prefill_mxfp4(over, *args, max_seqlen_q=max(q_lens), out=over) is over
+        assert torch.equal(over, want)
     mi.check_device_status(cuda_device)
