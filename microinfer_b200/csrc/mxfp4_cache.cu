@@ -173,11 +173,23 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
   const int64_t col = by_page.div(g);  // groups of a page
   const int per_page = p.block_size / kMxGroup;
   const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
+  const int nb = blocks_of<NB>(p.head_dim);
   if (blk < 0 || blk >= p.num_blocks) {
     if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+    if constexpr (REDO) p.redo[seq] = 1;  // to be left out, as prefill from the pages does
+    if (!p.fill) return;
+    for (int tok = lane >> 2; tok < kMxGroup && pos0 + tok < ctx; tok += 8) {
+      const int64_t row = base + pos0 + tok;
+      if (row < 0 || row >= p.out_rows) continue;
+      const int64_t dst = (row * p.num_kv_heads + h) * p.head_dim + j * 8;
+      const float zeros[8] = {};
+      for (int b = 0; b < nb; ++b) {
+        write8(static_cast<T *>(p.out_keys) + dst + b * kMxBlock, zeros);
+        write8(static_cast<T *>(p.out_values) + dst + b * kMxBlock, zeros);
+      }
+    }
     return;
   }
-  const int nb = blocks_of<NB>(p.head_dim);
   const int64_t off = ((blk * p.num_kv_heads + h) * per_page + (g - col * per_page)) * (nb * kMxBytes);
   const uint8_t *kg = p.key_pages + off, *vg = p.value_pages + off;
   constexpr int kAhead = NB > 0 ? NB : 1;

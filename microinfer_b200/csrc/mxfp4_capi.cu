@@ -331,6 +331,7 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   g.num_blocks = num_blocks;
   g.out_rows = kv_rows;
   g.redo = redo;
+  g.fill = 1;
   g.block_size = block_size;
   g.num_kv_heads = num_kv_heads;
   g.head_dim = head_dim;

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import microinfer_b200 as mi
+from microinfer_b200 import _lib
 from oracle import mxfp4_oracle as mo
 from tests.test_mxfp4 import DTYPES, PREFILL_STEP, _close, _close_or_past, _cuda, _pages, _prefill_case, _table
 
@@ -119,3 +120,54 @@ def test_results_over_the_query(cuda_device, name, hkv, group, d, q_lens, ctxs):
         assert mi.paged_prefill_mxfp4(over, *args, max_seqlen_q=max(q_lens), out=over) is over
         assert torch.equal(over, want)
     mi.check_device_status(cuda_device)
+
+
+@gpu
+@pytest.mark.parametrize("name,hkv,d", [("bf16", 8, 128), ("f16", 8, 128), ("f32", 2, 160)])
+def test_gathered_bad_pages(cuda_device, name, hkv, d):
+    """Twice the same finite result with the allocator's memory full of NaN, and the other sequences untouched."""
+    rng = np.random.default_rng(40)
+    dtype = DTYPES[name]
+    q_lens, ctxs = LARGE, [140, 200, 9, 137, 300]
+    nb = sum(-(-c // 16) for c in ctxs)
+    kp, vp = _pages(rng, nb, 16, hkv, d)
+    table = _table(rng, ctxs, nb, 16)
+    broken = table.copy()
+    broken[1, 3], broken[4, 0], broken[4, 7] = nb + 5, -1, 1 << 30
+    query = _cuda(rng.standard_normal((sum(q_lens), 2 * hkv, d)), cuda_device, dtype)
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=cuda_device) for x in (q_lens, ctxs))
+    pages = _cuda(kp, cuda_device), _cuda(vp, cuda_device)
+
+    def call(t):
+        for n in (sum(ctxs) * hkv * d, 2 * sum(ctxs) * hkv * d + 4096):
+            for _ in range(3):
+                torch.full((n,), float("nan"), dtype=dtype, device=cuda_device)
+        return mi.paged_prefill_mxfp4(query, *pages, cu_q, cu_k, _cuda(t, cuda_device), max_seqlen_q=max(q_lens),
+                                      total_k=sum(ctxs))
+
+    good = call(table)
+    assert mi.read_device_status(cuda_device) == 0
+    got = call(broken)
+    assert mi.read_device_status(cuda_device) == _lib.DEV_BAD_BLOCK
+    again = call(broken)
+    mi.read_device_status(cuda_device)
+    assert bool(torch.isfinite(got).all()) and torch.equal(got, again)
+    at = np.cumsum([0, *q_lens])
+    for r in (0, 2, 3):
+        assert torch.equal(got[at[r]:at[r + 1]], good[at[r]:at[r + 1]])
+    # keys of pages that are none are left out; in fp32 above head_dim 128 they count as zeros
+    q = query.double().cpu().numpy()
+    for r, cols in ((1, [3]), (4, [0, 7])):
+        k, v = mo.rows(kp, table[r], ctxs[r]), mo.rows(vp, table[r], ctxs[r])
+        gone = np.isin(np.arange(ctxs[r]) // 16, cols)
+        k[gone], v[gone] = 0, 0
+        rows = q[at[r]:at[r + 1]]
+        x = np.einsum("qhd,khd->hqk", rows, k.repeat(2, 1)) * d ** -0.5
+        hidden = np.arange(ctxs[r])[None] > np.arange(ctxs[r] - len(rows), ctxs[r])[:, None]
+        x[:, hidden | gone if d == 128 else hidden] = -np.inf
+        p = np.exp(x - x.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        want = np.einsum("hqk,khd->qhd", p, v.repeat(2, 1))
+        weight = np.einsum("hqk,khd->qhd", p, np.abs(v).repeat(2, 1))
+        size = np.einsum("qhd,khd->qhk", np.abs(rows), np.abs(k).repeat(2, 1)).max(-1, keepdims=True) * d ** -0.5
+        _close(got[at[r]:at[r + 1]], want, weight, size, 0 * want, dtype, PREFILL_STEP[dtype])
