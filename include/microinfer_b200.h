@@ -483,7 +483,8 @@ MI_API int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_
  * cores' dense kernel.  Sequences with what does not go through it (a NaN of V, in f16 a block past 65504, a
  * page that is none) are then done over from the pages, so results are those of mi_paged_prefill_mxfp4; `out`
  * must not overlap the query.  In f32 above head_dim 128, which has no kernel for the pages, a page that is
- * none (MI_DEV_BAD_BLOCK) counts as zeros; elsewhere its keys are left out.  `max_context` bounds one context.
+ * none (MI_DEV_BAD_BLOCK) counts as zeros; elsewhere its keys are left out.  `max_context` bounds one context:
+ * what a longer one has past it is treated as pages that are none.
  */
 MI_API size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t kv_rows,
                                                        int32_t num_kv_heads, int32_t head_dim,

@@ -170,16 +170,10 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
   const int h = static_cast<int>(task - g * p.num_kv_heads);
   const int64_t pos0 = static_cast<int64_t>(g) * kMxGroup;
   if (pos0 >= ctx) return;
-  const int64_t col = by_page.div(g);  // groups of a page
-  const int per_page = p.block_size / kMxGroup;
-  const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
   const int nb = blocks_of<NB>(p.head_dim);
-  if (blk < 0 || blk >= p.num_blocks) {
-    if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
-    if constexpr (REDO) p.redo[seq] = 1;  // to be left out, as prefill from the pages does
-    if (!p.fill) return;
-    for (int tok = lane >> 2; tok < kMxGroup && pos0 + tok < ctx; tok += 8) {
-      const int64_t row = base + pos0 + tok;
+  auto zero_group = [&](int64_t from) {
+    for (int tok = lane >> 2; tok < kMxGroup && from + tok < ctx; tok += 8) {
+      const int64_t row = base + from + tok;
       if (row < 0 || row >= p.out_rows) continue;
       const int64_t dst = (row * p.num_kv_heads + h) * p.head_dim + j * 8;
       const float zeros[8] = {};
@@ -188,6 +182,21 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
         write8(static_cast<T *>(p.out_values) + dst + b * kMxBlock, zeros);
       }
     }
+  };
+  if (p.fill && ctx > static_cast<int64_t>(p.fill) * kMxGroup) {
+    if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+    if constexpr (REDO) p.redo[seq] = 1;
+    for (int64_t more = g + static_cast<int64_t>(p.fill); g < p.fill && more * kMxGroup < min(ctx, p.out_rows); more += p.fill)
+      zero_group(more * kMxGroup);
+  }
+  const int64_t col = by_page.div(g);  // groups of a page
+  const int per_page = p.block_size / kMxGroup;
+  const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
+  if (blk < 0 || blk >= p.num_blocks) {
+    if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
+    if constexpr (REDO) p.redo[seq] = 1;  // to be left out, as prefill from the pages does
+    if (!p.fill) return;
+    zero_group(pos0);
     return;
   }
   const int64_t off = ((blk * p.num_kv_heads + h) * per_page + (g - col * per_page)) * (nb * kMxBytes);

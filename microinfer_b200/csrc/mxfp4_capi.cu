@@ -300,10 +300,14 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
     return capi_fail(MI_ERR_INVALID, "num_q_heads must be divisible by num_kv_heads");
   if (num_seqs > 65535 || num_kv_heads > 65535) return capi_fail(MI_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
   if (num_seqs == 0 || num_tokens == 0) return MI_OK;
-  if (max_seqlen_q <= 0 || kv_rows == 0) return capi_fail(MI_ERR_INVALID, "max_seqlen_q and kv_rows must be positive");
+  if (max_seqlen_q <= 0 || kv_rows == 0 || max_context == 0)
+    return capi_fail(MI_ERR_INVALID, "max_seqlen_q, kv_rows and max_context must be positive");
+  if (max_context / kMxGroup + 1 >= (int64_t{1} << 31) / num_kv_heads)
+    return capi_fail(MI_ERR_UNSUPPORTED, "max_context too large for one call");
   if (!out || !query || !key_pages || !value_pages || !cu_seqlens_q || !cu_seqlens_k || !block_tables)
     return capi_fail(MI_ERR_INVALID, "null pointer");
-  if (!aligned16(query) || !aligned16(out)) return capi_fail(MI_ERR_ALIGNMENT, "query and out must be 16-byte aligned");
+  if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
+    return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
   const size_t rows = gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype);
   if (workspace == nullptr ||
       workspace_bytes < mi_paged_prefill_mxfp4_gathered_workspace_bytes(num_seqs, kv_rows, num_kv_heads, head_dim, dtype))
@@ -331,18 +335,12 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   g.num_blocks = num_blocks;
   g.out_rows = kv_rows;
   g.redo = redo;
-  g.fill = 1;
+  g.fill = static_cast<uint32_t>((max_context + kMxGroup - 1) / kMxGroup);
   g.block_size = block_size;
   g.num_kv_heads = num_kv_heads;
   g.head_dim = head_dim;
   g.status = dev_status;
-  if (max_context > 0) {
-    if (max_context / kMxGroup + 1 >= (int64_t{1} << 31) / num_kv_heads)
-      return capi_fail(MI_ERR_UNSUPPORTED, "max_context too large for one call");
-    if (!aligned16(key_pages) || !aligned16(value_pages))
-      return capi_fail(MI_ERR_ALIGNMENT, "pages must be 16-byte aligned");
-    if (const int s = capi_cuda_status(launch_mxfp4_gather(g, dtype, num_seqs, max_context, st))) return s;
-  }
+  if (const int s = capi_cuda_status(launch_mxfp4_gather(g, dtype, num_seqs, max_context, st))) return s;
   if (const int s = mi_varlen_prefill(out, query, keys, values, static_cast<int64_t>(num_kv_heads) * head_dim, num_q_heads,
                                       num_kv_heads, head_dim, dtype, cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens,
                                       kv_rows, max_seqlen_q, scale, dev_status, stream))

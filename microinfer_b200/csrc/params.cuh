@@ -164,7 +164,8 @@ struct MxGatherParams {
   int64_t num_blocks;
   int64_t out_rows;  // rows of out_keys / out_values; never written past
   int32_t *redo;     // null, or a word per sequence, set where a block is not for the dense kernel (mxfp4.cuh)
-  int32_t fill;      // whether rows of pages that are none are set to zero, not left as they are
+  uint32_t fill;     // 0: rows of pages that are none are left as they are; else the launch's groups of 16 positions, and
+                     // those rows are set to zero, as are a context's past the groups
   int32_t block_size;
   int32_t num_kv_heads;
   int32_t head_dim;

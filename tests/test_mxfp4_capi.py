@@ -56,3 +56,20 @@ def test_prefill_refuses_tables_whose_positions_pass_32_bits():
     assert prefill(16, (2 ** 31 - 16) // 16) == unsupported  # 2^31 - 16 positions
     assert prefill(1 << 20, 2047) == alignment
     assert prefill(16, 2 ** 60) == unsupported
+
+
+def test_gathered_prefill_refuses_bad_arguments():
+    lib = _lib.load()
+    p = np.zeros(64, dtype=np.uint8).ctypes.data
+
+    def prefill(dtype=2, bs=16, d=128, hq=4, n=1, tokens=1, q=1, most=16, rows=16, query=p, ws=p, nbytes=0):
+        return lib.mi_paged_prefill_mxfp4_gathered(p, query, p, p, 4, bs, hq, 2, d, dtype, p, p, p, 2, n, tokens, q, most, rows,
+                                                   0.1, ws, nbytes, None, None)
+
+    assert prefill(n=0) == 0 and prefill(tokens=0) == 0
+    for bad in (dict(dtype=9), dict(bs=8), dict(d=48), dict(hq=3), dict(n=-1), dict(n=70000), dict(q=0), dict(most=0), dict(rows=0),
+                dict(rows=-1), dict(query=None), dict(query=p | 1), dict(ws=None), dict(nbytes=100), dict(most=2 ** 40)):
+        assert prefill(**bad) < 0
+    size = lib.mi_paged_prefill_mxfp4_gathered_workspace_bytes
+    assert size(3, 10, 2, 128, 2) == 2 * 10 * 2 * 128 * 2 + 12
+    assert size(0, 10, 2, 128, 2) == 0 and size(3, 10, 2, 128, 9) == 0

@@ -171,3 +171,37 @@ def test_gathered_bad_pages(cuda_device, name, hkv, d):
         weight = np.einsum("hqk,khd->qhd", p, np.abs(v).repeat(2, 1))
         size = np.einsum("qhd,khd->qhk", np.abs(rows), np.abs(k).repeat(2, 1)).max(-1, keepdims=True) * d ** -0.5
         _close(got[at[r]:at[r + 1]], want, weight, size, 0 * want, dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name,hkv,d", [("bf16", 8, 128), ("f16", 8, 128), ("f32", 2, 160)])
+def test_gathered_context_past_the_table(cuda_device, name, hkv, d):
+    """A context longer than its block-table row is flagged; what it does see gives the same every time."""
+    rng = np.random.default_rng(41)
+    dtype = DTYPES[name]
+    q_lens, ctxs = LARGE, [140, 200, 9, 137, 300]
+    nb = sum(-(-c // 16) for c in ctxs)
+    kp, vp = _pages(rng, nb, 16, hkv, d)
+    table = _table(rng, ctxs, nb, 16)
+    query = _cuda(rng.standard_normal((sum(q_lens), 2 * hkv, d)), cuda_device, dtype)
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=cuda_device) for x in (q_lens, ctxs))
+    pages = _cuda(kp, cuda_device), _cuda(vp, cuda_device)
+
+    def call(width):
+        for n in (sum(ctxs) * hkv * d, 2 * sum(ctxs) * hkv * d + 4096):
+            for _ in range(3):
+                torch.full((n,), float("nan"), dtype=dtype, device=cuda_device)
+        return mi.paged_prefill_mxfp4(query, *pages, cu_q, cu_k, _cuda(table[:, :width], cuda_device), max_seqlen_q=max(q_lens))
+
+    good = call(table.shape[1])
+    assert mi.read_device_status(cuda_device) == 0
+    got = call(14)  # 224 positions
+    assert mi.read_device_status(cuda_device) & _lib.DEV_BAD_BLOCK
+    again = call(14)
+    mi.read_device_status(cuda_device)
+    assert bool(torch.isfinite(got).all()) and torch.equal(got, again)
+    end = sum(q_lens[:4])
+    assert torch.equal(got[:end], good[:end])
+    first = 224 - (300 - 144)  # rows of the last sequence that see nothing past the table
+    want = mo.attention(query[end:].double().cpu().numpy(), mo.rows(kp, table[4], 300), mo.rows(vp, table[4], 300), d ** -0.5)
+    _close(got[end:end + first], *[x[:first] for x in want], dtype, PREFILL_STEP[dtype])
