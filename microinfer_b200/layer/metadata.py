@@ -34,6 +34,7 @@ class AttentionMetadata:
     direct_prefill: bool = False
     validate_cache_write: bool = True
     _host: dict = field(default_factory=dict, repr=False, compare=False)
+    total_seqlen_k: int = 0  # sum of the contexts (prefill) or a bound on it; 0: not known
 
     @classmethod
     def build(cls, *, is_prefill: bool, block_tables=None, **fields) -> "AttentionMetadata":

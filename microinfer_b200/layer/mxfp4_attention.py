@@ -181,18 +181,20 @@ def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
 
 def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, *,
                         max_seqlen_q: int, total_k: int | None = None, scale: float | None = None,
-                        out: torch.Tensor | None = None) -> torch.Tensor:
+                        out: torch.Tensor | None = None,
+                        max_seqlen_k: int | None = None) -> torch.Tensor:
     """Causal chunked prefill from the 4-bit cache; also mixed batches.
 
     As ``paged_prefill``: request r's rows sit at the end of its context
     (``cu_seqlens_k`` is cumulative over contexts, the chunk included, which is
     already stored).  ``total_k`` is the sum of the contexts (or a bound on
     it) and sizes the workspace; without it the block table's capacity does.
+    ``max_seqlen_k`` (likewise a bound) is the longest of them.
     """
     if torch.compiler.is_compiling():  # an opaque node for torch.compile
         res = torch.ops.microinfer_b200.paged_prefill_mxfp4(
             query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables,
-            int(max_seqlen_q), total_k, scale)
+            int(max_seqlen_q), total_k, scale, max_seqlen_k)
         return res if out is None else out.copy_(res)
     dims = page_dims(key_pages, value_pages)
     _, bs, hkv, d = dims
@@ -209,16 +211,21 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
         raise ValueError("max_seqlen_q must be positive")
     if total_k is not None and total_k < 0:
         raise ValueError("total_k must be non-negative")
+    if max_seqlen_k is not None and max_seqlen_k < 0:
+        raise ValueError("max_seqlen_k must be non-negative")
     device = _lib.require_cuda(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables)
-    rows = requests * width * bs
+    most = width * bs  # keys of one request
+    if max_seqlen_k is not None:
+        most = min(most, int(max_seqlen_k))
+    rows = requests * most
     if total_k is not None:
         rows = min(rows, int(total_k))
+        most = min(most, rows)
     if rows == 0:  # no request can have a key
         return query.new_zeros(query.shape) if out is None else out.zero_()
     query, block_tables = _aligned(query), _idx(block_tables)
     cu_seqlens_q, cu_seqlens_k = _idx(cu_seqlens_q), _idx(cu_seqlens_k)
     tokens, hq, _ = query.shape
-    most = min(rows, width * bs)  # keys of one request
     dtype = _lib.dtype_code(query.dtype)
     if _reads_pages(dtype, hq, hkv, d, requests, int(max_seqlen_q), device.index or 0):
         if out is None:
@@ -272,7 +279,29 @@ def paged_attention_mxfp4_meta(query, key_pages, value_pages, metadata, *,
                            device=query.device)
         torch.cumsum(metadata.context_lens, 0, out=cu_k[1:])
     max_q = metadata.max_seqlen_q or max(metadata.q_lens_cpu, default=0)
-    most = metadata.max_seqlen_k
     return paged_prefill_mxfp4(query, key_pages, value_pages, cu_q, cu_k, block_tables,
-                               max_seqlen_q=max_q,
-                               total_k=most * block_tables.shape[0] if most else None, scale=scale)
+                               max_seqlen_q=max_q, total_k=_total_k(query, key_pages, metadata),
+                               scale=scale, max_seqlen_k=metadata.max_seqlen_k or None)
+
+
+# K and V rows of a gathered prefill that may be allocated for a bound on the contexts rather than their sum.
+_BOUND_BYTES = 256 << 20
+
+
+def _total_k(query, key_pages, metadata) -> int | None:
+    """The sum of the step's contexts, which sizes a gathered prefill, or a bound on it.
+
+    Metadata that does not say costs one copy of the lengths to the host per step, which is
+    not made where a bound will do (the longest context, or else the block table's width, for every
+    request) or the host does not know yet (in a capture, whose replays may have other lengths).
+    """
+    total = getattr(metadata, "total_seqlen_k", 0)
+    if total:
+        return total
+    requests, width = metadata.block_tables.shape
+    _, bs, hkv, d = page_dims(key_pages, key_pages)
+    bound = requests * (metadata.max_seqlen_k or width * bs)
+    if (2 * bound * hkv * d * query.element_size() <= _BOUND_BYTES or torch.compiler.is_compiling()
+            or (query.is_cuda and torch.cuda.is_current_stream_capturing())):
+        return bound
+    return sum(metadata.context_lens_cpu)

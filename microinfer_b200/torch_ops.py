@@ -138,13 +138,14 @@ def _(query, key_pages, value_pages, block_tables, context_lens, scale=None):
 def paged_prefill_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
                         cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
                         block_tables: torch.Tensor, max_seqlen_q: int,
-                        total_k: int | None = None, scale: float | None = None) -> torch.Tensor:
+                        total_k: int | None = None, scale: float | None = None,
+                        max_seqlen_k: int | None = None) -> torch.Tensor:
     return _mx.paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k,
                                    block_tables, max_seqlen_q=max_seqlen_q, total_k=total_k,
-                                   scale=scale)
+                                   scale=scale, max_seqlen_k=max_seqlen_k)
 
 
 @paged_prefill_mxfp4.register_fake
 def _(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, max_seqlen_q,
-      total_k=None, scale=None):
+      total_k=None, scale=None, max_seqlen_k=None):
     return query.new_empty(query.shape)  # contiguous, whatever the query's strides

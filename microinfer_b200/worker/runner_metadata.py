@@ -305,7 +305,7 @@ class DeviceRunnerMetadata:
         commits: list = []
         tokens = []
         seen = set()
-        width = max_q = max_k = 0
+        width = max_q = max_k = total_k = 0
         any_cached = False
         for i, seq in enumerate(seqs):
             start = int(seq.num_cached_tokens)
@@ -326,6 +326,7 @@ class DeviceRunnerMetadata:
             width = max(width, pages)
             max_q = max(max_q, end - start)
             max_k = max(max_k, end)
+            total_k += end
             any_cached = any_cached or start > 0
         ids = np.array(tokens, dtype=np.int64)
         if ids.size and (ids.min() < 0 or ids.max() > 2**31 - 1):
@@ -334,7 +335,7 @@ class DeviceRunnerMetadata:
             raise ValueError("too many scheduled tokens")
         return {"records": rec, "updates": updates.array(self.num_blocks),
                 "tokens": ids.astype(np.int32), "table_width": width if any_cached else 0,
-                "max_q": max_q, "max_k": max_k, "commits": commits}
+                "max_q": max_q, "max_k": max_k, "total_k": total_k, "commits": commits}
 
     def prepare_prefill(self, seqs, *, validate_cache_write: bool = False):
         """``ModelRunner.prepare_prefill``: the scheduled range
@@ -360,5 +361,6 @@ class DeviceRunnerMetadata:
         metadata = AttentionMetadata.build(
             is_prefill=True, cu_seqlens_q=cu[0], cu_seqlens_k=cu[1],
             max_seqlen_q=plan["max_q"], max_seqlen_k=plan["max_k"], slot_mapping=slots,
-            block_tables=bt, validate_cache_write=validate_cache_write)
+            block_tables=bt, validate_cache_write=validate_cache_write,
+            total_seqlen_k=plan["total_k"])
         return input_ids, positions, metadata
