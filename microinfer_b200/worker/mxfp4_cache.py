@@ -60,7 +60,9 @@ def store_kv_mxfp4(key_pages, value_pages, slots, keys, values):
     if heads != hkv or dim != d:
         raise ValueError("K/V heads do not match the cache")
     key_stride, value_stride = keys.stride(), values.stride()
-    if key_stride[1:] != (d, 1) or value_stride[1:] != (d, 1):
+    # the stride of a single head means nothing (a transpose of [1, T, D] is contiguous)
+    if (key_stride[2] != 1 or value_stride[2] != 1
+            or (hkv > 1 and (key_stride[1] != d or value_stride[1] != d))):
         raise ValueError("K/V inner dimensions must be contiguous")
     if keys.dtype != values.dtype:
         raise ValueError("K/V must share a dtype")
