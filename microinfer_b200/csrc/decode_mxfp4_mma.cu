@@ -582,9 +582,9 @@ struct MxWarp {
     }
   }
 
-  // One unit: K of its two groups at `base`, then V of both; `valid` of its 32 keys exist; `special`:
-  // that may be fewer than 32, or it is the `first` that the state meets.
-  __device__ __forceinline__ void process(uint32_t base, bool special, int valid, bool first) {
+  // One unit: K of its two groups at `base`, then V of both; `valid0` and `valid1` of their 16 keys exist; `special`:
+  // that may be fewer than 16, or it is the `first` that the state meets.
+  __device__ __forceinline__ void process(uint32_t base, bool special, int valid0, int valid1, bool first) {
     const uint32_t vbase = base + 2 * C::kGroup;
     float x[2][CT][2];
     scores(base, x);
@@ -599,8 +599,8 @@ struct MxWarp {
     if (special) {  // uniform
       if (first) {  // R_b starts at the largest scale here and two binades of room
         const uint32_t none[Q] = {};
-        mask_scales(w[0], valid, none);
-        mask_scales(w[1], valid - kMxGroup, none);
+        mask_scales(w[0], valid0, none);
+        mask_scales(w[1], valid1, none);
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
           const uint32_t top = __vmaxu4(over_keys(w[0][i]), over_keys(w[1][i]));
@@ -611,10 +611,10 @@ struct MxWarp {
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          if (j * kMxGroup + g >= valid) x[j][c][0] = -INFINITY;
-          if (j * kMxGroup + g + 8 >= valid) x[j][c][1] = -INFINITY;
+          if (g >= (j ? valid1 : valid0)) x[j][c][0] = -INFINITY;
+          if (g + 8 >= (j ? valid1 : valid0)) x[j][c][1] = -INFINITY;
         }
-        mask_scales(w[j], valid - j * kMxGroup, ref);  // whatever they are: their p is zero
+        mask_scales(w[j], j ? valid1 : valid0, ref);  // whatever they are: their p is zero
       }
     }
     // m follows the largest score, up to kLag binades behind it
@@ -662,7 +662,7 @@ struct MxWarp {
     const uint32_t far = distances(w[0], d[0]) | distances(w[1], d[1]);
     if (__any_sync(kAll, far != 0)) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) values_far(vbase + j * C::kGroup, p[j], valid - j * kMxGroup);
+      for (int j = 0; j < 2; ++j) values_far(vbase + j * C::kGroup, p[j], j ? valid1 : valid0);
     } else {
       values<false>(vbase, d[0], p[0]);
       values<false>(vbase + C::kGroup, d[1], p[1]);
@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
   constexpr int kEnds = 128;    // its last
   constexpr int kFirst = 256;   // the segment's first unit
   constexpr int kLast = 512;    // the segment's last
-  constexpr int kNoPage = 1024; // a page that is none: flagged, left out
+  constexpr int kNoPage = 1024; // its first group's page is none: flagged, left out (the second's is as if past the context)
   const int per_page = p.block_size / kMxGroup;
   int4 *table = unit_table + warp * 64;
   struct Unit {
@@ -895,7 +895,10 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
           where[j] = (page * p.num_kv_heads + kvh) * per_page + group - col * per_page;
         } else {
           flag_status(p.status, MI_DEV_BAD_BLOCK);
-          flags |= kNoPage;
+          if (j == 0)
+            flags |= kNoPage;
+          else
+            valid = kMxGroup;
         }
       }
       table[i & 63] = make_int4(where[0], where[1], valid | flags, r.seq * H + r.ht);
@@ -991,8 +994,9 @@ __global__ void __launch_bounds__(MxCfg<NB, CT, std::is_same<T, float>::value>::
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");  // this lane's copies of unit i
     __syncwarp();                                                         // every lane's
     const bool special = what != kUnit || fresh;
-    if (!(what & kNoPage)) {
-      st.process(smem_addr(ring) + stage * C::kStage, special, what & 63, fresh);
+    const int valid = what & 63, valid0 = what & kNoPage ? 0 : min(valid, kMxGroup), valid1 = valid - kMxGroup;
+    if (valid0 > 0 || valid1 > 0) {
+      st.process(smem_addr(ring) + stage * C::kStage, special, valid0, valid1, fresh);
       fresh = false;
     }
     __syncwarp();  // every lane has read the stage
