@@ -486,9 +486,9 @@ MI_API int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_
  * none (MI_DEV_BAD_BLOCK) counts as zeros; elsewhere its keys are left out.  `max_context` bounds one context:
  * what a longer one has past it is treated as pages that are none.
  */
-MI_API size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t kv_rows,
-                                                       int32_t num_kv_heads, int32_t head_dim,
-                                                       int32_t dtype);
+MI_API size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t max_context,
+                                                       int64_t kv_rows, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t dtype);
 MI_API int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *key_pages,
                                     const void *value_pages, int64_t num_blocks,
                                     int32_t block_size, int32_t num_q_heads,

@@ -107,7 +107,9 @@ SIGNATURES = {
         [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _I64,
          _I64, _F, _P, _SZ, _P, _P],
     ),
-    "mi_paged_prefill_mxfp4_gathered_workspace_bytes": (_SZ, [_I64, _I64, _I32, _I32, _I32]),
+    "mi_paged_prefill_mxfp4_gathered_workspace_bytes": (
+        _SZ, [_I64, _I64, _I64, _I32, _I32, _I32],
+    ),
     "mi_paged_prefill_mxfp4_gathered": (
         ctypes.c_int,
         [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _I32,

@@ -169,7 +169,14 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
   const uint32_t g = by_heads.div(task);
   const int h = static_cast<int>(task - g * p.num_kv_heads);
   const int64_t pos0 = static_cast<int64_t>(g) * kMxGroup;
-  if (pos0 >= ctx) return;
+  if (pos0 >= ctx || (p.fill && g >= p.fill)) return;
+  bool apart = false;  // REDO: this lane's blocks that are not for the dense kernel
+  auto note = [&] {    // before the warp returns
+    if constexpr (REDO) {
+      const bool any = __any_sync(0xffffffffu, apart);
+      if (lane == 0) p.redo[(static_cast<int64_t>(seq) * p.num_kv_heads + h) * p.redo_stride + g] = any;
+    }
+  };
   const int nb = blocks_of<NB>(p.head_dim);
   auto zero_group = [&](int64_t from) {
     for (int tok = lane >> 2; tok < kMxGroup && from + tok < ctx; tok += 8) {
@@ -185,8 +192,8 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
   };
   if (p.fill && ctx > static_cast<int64_t>(p.fill) * kMxGroup) {
     if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
-    if constexpr (REDO) p.redo[seq] = 1;
-    for (int64_t more = g + static_cast<int64_t>(p.fill); g < p.fill && more * kMxGroup < min(ctx, p.out_rows); more += p.fill)
+    apart = true;
+    for (int64_t more = g + static_cast<int64_t>(p.fill); more * kMxGroup < min(ctx, p.out_rows); more += p.fill)
       zero_group(more * kMxGroup);
   }
   const int64_t col = by_page.div(g);  // groups of a page
@@ -194,9 +201,9 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
   const int64_t blk = col < p.block_table_stride ? p.block_tables[seq * p.block_table_stride + col] : -1;
   if (blk < 0 || blk >= p.num_blocks) {
     if (lane == 0) flag_status(p.status, MI_DEV_BAD_BLOCK);
-    if constexpr (REDO) p.redo[seq] = 1;  // to be left out, as prefill from the pages does
-    if (!p.fill) return;
-    zero_group(pos0);
+    apart = true;  // to be left out, as prefill from the pages does
+    if (p.fill) zero_group(pos0);
+    note();
     return;
   }
   const int64_t off = ((blk * p.num_kv_heads + h) * per_page + (g - col * per_page)) * (nb * kMxBytes);
@@ -222,12 +229,9 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
       const int tok = half * 8 + (lane >> 2);
       const int64_t row = base + pos0 + tok;
       if (pos0 + tok >= ctx) continue;
-      if constexpr (REDO) {
-        bool apart = false;
+      if constexpr (REDO)
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) apart |= mx_apart<T>(false, ks[half][i]) || mx_apart<T>(true, vs[half][i]);
-        if (apart) p.redo[seq] = 1;
-      }
       if (row < 0 || row >= p.out_rows) {
         flag_status(p.status, MI_DEV_BAD_SLOT);
         continue;
@@ -243,6 +247,7 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
       }
     }
   }
+  note();
   pdl_launch_dependents();
 }
 

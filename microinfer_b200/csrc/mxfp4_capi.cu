@@ -272,16 +272,18 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
       launch_mxfp4_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, static_cast<cudaStream_t>(stream)));
 }
 
-// K and V of kv_rows rows, each from a multiple of 256 bytes, then a word per sequence.
+// K and V of kv_rows rows, each from a multiple of 256 bytes, then a byte per (sequence, kv head, group).
 static size_t gathered_rows_bytes(int64_t kv_rows, int32_t num_kv_heads, int32_t head_dim, int32_t dtype) {
   const size_t bytes = static_cast<size_t>(kv_rows) * num_kv_heads * head_dim * (dtype == MI_DTYPE_FLOAT32 ? 4 : 2);
   return (bytes + 255) / 256 * 256;
 }
 
-size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t kv_rows, int32_t num_kv_heads,
-                                                       int32_t head_dim, int32_t dtype) {
-  if (num_seqs <= 0 || kv_rows <= 0 || num_kv_heads <= 0 || head_dim <= 0 || !known_dtype(dtype)) return 0;
-  return 2 * gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype) + num_seqs * sizeof(int32_t);
+size_t mi_paged_prefill_mxfp4_gathered_workspace_bytes(int64_t num_seqs, int64_t max_context, int64_t kv_rows,
+                                                       int32_t num_kv_heads, int32_t head_dim, int32_t dtype) {
+  if (num_seqs <= 0 || max_context <= 0 || kv_rows <= 0 || num_kv_heads <= 0 || head_dim <= 0 || !known_dtype(dtype))
+    return 0;
+  return 2 * gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype) +
+         static_cast<size_t>(num_seqs) * num_kv_heads * ((max_context + kMxGroup - 1) / kMxGroup);
 }
 
 int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *key_pages, const void *value_pages,
@@ -310,7 +312,8 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
     return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
   const size_t rows = gathered_rows_bytes(kv_rows, num_kv_heads, head_dim, dtype);
   if (workspace == nullptr ||
-      workspace_bytes < mi_paged_prefill_mxfp4_gathered_workspace_bytes(num_seqs, kv_rows, num_kv_heads, head_dim, dtype))
+      workspace_bytes < mi_paged_prefill_mxfp4_gathered_workspace_bytes(num_seqs, max_context, kv_rows, num_kv_heads,
+                                                                        head_dim, dtype))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_prefill_mxfp4_gathered_workspace_bytes)");
   if (!aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
@@ -319,11 +322,10 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   // The tensor-core kernel multiplies what a row does not see by zero: sequences with blocks that this does not suit are
   // noted by the gather and done over from the pages (their tables have to be within that kernel's limit).
   const bool dense = mi_prefill_kernel_for(dtype, head_dim, num_q_heads, num_kv_heads, 0) == 2;
-  int32_t *redo = nullptr;
-  if (dense && max_seqlen_q <= (1 << 24) && block_table_stride <= (INT32_MAX - 256) / block_size) {
-    redo = reinterpret_cast<int32_t *>(values + rows);
-    if (const int s = capi_cuda_status(cudaMemsetAsync(redo, 0, num_seqs * sizeof(int32_t), st))) return s;
-  }
+  const int64_t groups = (max_context + kMxGroup - 1) / kMxGroup;
+  uint8_t *redo = nullptr;
+  if (dense && max_seqlen_q <= (1 << 24) && block_table_stride <= (INT32_MAX - 256) / block_size)
+    redo = reinterpret_cast<uint8_t *>(values + rows);
   MxGatherParams g = {};
   g.out_keys = keys;
   g.out_values = values;
@@ -335,7 +337,8 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   g.num_blocks = num_blocks;
   g.out_rows = kv_rows;
   g.redo = redo;
-  g.fill = static_cast<uint32_t>((max_context + kMxGroup - 1) / kMxGroup);
+  g.redo_stride = groups;
+  g.fill = static_cast<uint32_t>(groups);
   g.block_size = block_size;
   g.num_kv_heads = num_kv_heads;
   g.head_dim = head_dim;
@@ -355,6 +358,8 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   p.cu_seqlens_q = cu_seqlens_q;
   p.cu_seqlens_k = cu_seqlens_k;
   p.redo = redo;
+  p.redo_stride = groups;
+  p.redo_groups = static_cast<int32_t>(groups);
   p.bt_stride = block_table_stride;
   p.num_blocks = num_blocks;
   p.num_tokens = num_tokens;

@@ -163,7 +163,8 @@ struct MxGatherParams {
   int64_t block_table_stride;
   int64_t num_blocks;
   int64_t out_rows;  // rows of out_keys / out_values; never written past
-  int32_t *redo;     // null, or a word per sequence, set where a block is not for the dense kernel (mxfp4.cuh)
+  uint8_t *redo;     // null, or [seq][kv head][redo_stride], a byte per group: whether a block is not for the dense kernel
+  int64_t redo_stride;
   uint32_t fill;     // 0: rows of pages that are none are left as they are; else the launch's groups of 16 positions, and
                      // those rows are set to zero, as are a context's past the groups
   int32_t block_size;
@@ -199,7 +200,9 @@ struct MxPrefillParams {
   const int32_t *cu_seqlens_q;
   const int32_t *cu_seqlens_k;
   float *workspace;  // num_splits > 1: [split][token][q head][2 + D]
-  const int32_t *redo;  // null, or a word per sequence: those without are left as they are
+  const uint8_t *redo;  // null, or the gather's: sequences and kv heads without a set byte are left as they are
+  int64_t redo_stride;
+  int32_t redo_groups;  // that the gather has looked at, at most
   int64_t bt_stride;
   int64_t num_blocks;
   int64_t num_tokens;

@@ -541,13 +541,18 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
   pdl_launch_dependents();
 }
 
-// After the dense kernel: the sequences of which the gather has noted that it cannot do them, over again.  Hardly ever any, so
-// a few CTAs look (a CTA to a tile would take 100 us to find nothing at 64 x 2048 tokens) and take all tiles if so.
+// After the dense kernel: the sequences and kv heads of which the gather has noted that it cannot do them, over again.  Hardly
+// ever any, so a few CTAs look (a CTA to a tile would take 100 us to find nothing at 64 x 2048 tokens) and take all tiles if so.
 template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
     mxfp4_prefill_redo_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
   pdl_wait();
-  if (p.redo[blockIdx.z] != 0)
+  const int64_t ctx = static_cast<int64_t>(p.cu_seqlens_k[blockIdx.z + 1]) - p.cu_seqlens_k[blockIdx.z];
+  const int64_t groups = min((ctx + kMxGroup - 1) / kMxGroup, static_cast<int64_t>(p.redo_groups));
+  const uint8_t *noted = p.redo + (static_cast<int64_t>(blockIdx.z) * p.num_kv_heads + blockIdx.y) * p.redo_stride;
+  bool any = false;
+  for (int64_t i = threadIdx.x; i < groups; i += kThreads) any |= noted[i] != 0;
+  if (__syncthreads_or(any))
     for (int tile = tiles - 1 - blockIdx.x; tile >= 0; tile -= gridDim.x) {
       prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, tile, 0);
       __syncthreads();  // every warp has read its rows of q

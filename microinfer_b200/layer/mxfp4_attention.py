@@ -246,7 +246,7 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
         out = torch.empty_like(query)
     elif _overlap(out, query):  # some rows may be done twice
         query = query.clone()
-    need = _lib.load().mi_paged_prefill_mxfp4_gathered_workspace_bytes(requests, rows, hkv, d, dtype)
+    need = _lib.load().mi_paged_prefill_mxfp4_gathered_workspace_bytes(requests, most, rows, hkv, d, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.call(
         "mi_paged_prefill_mxfp4_gathered", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),

@@ -71,5 +71,5 @@ def test_gathered_prefill_refuses_bad_arguments():
                 dict(rows=-1), dict(query=None), dict(query=p | 1), dict(ws=None), dict(nbytes=100), dict(most=2 ** 40)):
         assert prefill(**bad) < 0
     size = lib.mi_paged_prefill_mxfp4_gathered_workspace_bytes
-    assert size(3, 10, 2, 128, 2) == 2 * 10 * 2 * 128 * 2 + 12
-    assert size(0, 10, 2, 128, 2) == 0 and size(3, 10, 2, 128, 9) == 0
+    assert size(3, 17, 10, 2, 128, 2) == 2 * 10 * 2 * 128 * 2 + 3 * 2 * 2
+    assert size(0, 17, 10, 2, 128, 2) == 0 and size(3, 17, 10, 2, 128, 9) == 0
