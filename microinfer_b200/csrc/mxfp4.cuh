@@ -41,14 +41,6 @@ struct FastDiv {
   }
 };
 
-// Byte offset of the group that holds `slot` (block * block_size + offset) of kv head h.
-__device__ __forceinline__ int64_t mx_group_offset(int64_t slot, int h, int block_size, int num_kv_heads,
-                                                   int head_dim) {
-  const int64_t block = slot / block_size;
-  const int group = static_cast<int>(slot - block * block_size) / kMxGroup;
-  return ((block * num_kv_heads + h) * (block_size / kMxGroup) + group) * mx_group_bytes(head_dim);
-}
-
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
 }
@@ -64,7 +56,9 @@ __device__ __forceinline__ bool mx_apart(bool value, uint32_t byte) {
 }
 
 // Eight codes of a word, in element order, as four f16 pairs (exact).
-// (Pass a word of memory: from a byte load, zero-extended, nvcc 12.9's conversions gave 0.)
+// All four bytes of the unpacked word are converted here: where the statement converts only one of them, nvcc
+// 12.9 gives 0 for every byte.  In this form all 256 bytes are right in every place, whichever results are used and
+// whether the word is loaded, masked or a byte extended by zeros.
 __device__ __forceinline__ void mx_codes_to_f16(uint32_t w, uint32_t (&r)[4]) {
   asm("{ .reg .b8 b0, b1, b2, b3;\n\t"
       "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
