@@ -15,7 +15,9 @@
 //     bits even 7 binades below R_b, and nothing above 2^-30 is lost, which a long context with
 //     one dominant key needs.  A group with a scale more than 7 binades below R_b, or above it
 //     (or zero, or NaN) takes a slower path that raises R_b or runs the products in windows of
-//     8 binades, so no spread of scales loses more;
+//     8 binades, so no spread of scales loses more.  R_b never falls within a segment: one token of V that is 2^6
+//     above all later ones keeps them on that path (32 x 8192: 60 us, then 92; a zero block in
+//     every group 119; scales over 23 binades 175);
 //   - q is multiplied by a power of two that puts its largest element into
 //     [2^14, 2^15) and converted to f16 (exact for bf16 down to 2^-28 of that element).
 // No code is moved between lanes or interleaved.  An ldmatrix of 8 keys x 16 bytes gives each lane 8
@@ -35,15 +37,18 @@
 // sequences load every SM alike.  A warp streams its range through a ring of its own, two units
 // deep, that runs across segment borders (139 KB in flight per SM with 16 warps at D = 128, 104 KB with 12).
 // Its lanes fill it with 16-byte cp.async; four bulk copies a unit, waited for on an
-// mbarrier, took 5 to 9% longer (96 x 8192, 32/8 heads of 128: 168 us, now 155).  Segments that lie within one
+// mbarrier, took 5 to 9% longer (96 x 8192, 32/8 heads of 128: 168 us against 155).  Segments that lie within one
 // warp's range are written at once; the parts of others are joined in shared
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
 // segment and the second launch has nothing to do.
 //
-// Measured (bf16, 32/8 heads): 96 x 8192, head_dim 128: 155 us, 5.5 TB/s (86% of the copy rate), 64% of the
-// ALU pipe's cycles, which the conversions, masks and shifts of the scales take; 32 x 8192, head_dim 256:
-// 104 us, 5.5 TB/s; 96: 58 us, 3.7 TB/s (its scales are read byte by byte); 1 x 131072, head_dim 128: 34.8 us,
+// Segments' results are means of V, divided by l before V's scale comes back, and are joined as means: nothing in
+// between is larger than V itself.
+//
+// Measured (bf16, 32/8 heads): 96 x 8192, head_dim 128: 157 us, 5.4 TB/s (84% of the copy rate), 64% of the
+// ALU pipe's cycles, which the conversions, masks and shifts of the scales take (fp32: 191 us); 32 x 8192, head_dim 256:
+// 107 us, 5.3 TB/s; 96: 56 us, 3.8 TB/s (its scales are read byte by byte); 1 x 131072, head_dim 128: 35.5 us,
 // of which 24 are the loop, the rest the start's dependent reads (lengths, table, pages) and the second launch.
 // 12 warps of three stages at head_dim 128: 168 us where 16 of two take 155; a third stage at 64 gains nothing.
 #include <type_traits>

@@ -10,15 +10,16 @@
 // 8 elements of every block of K and V before it uses any, two shuffles give a
 // block's a, and the tokens' codes of one block are 128 consecutive bytes, their scales 32 (at
 // D = 128) where the slots are consecutive.  Reads 2 or 4 bytes per element and writes 4.25
-// bits: HBM-bound on the read.  8000 tokens of 8 heads of 128 in bf16: 11.4 us, 3.6 TB/s (one wave of
-// warps; a plain copy of 33 MB reaches 2.8); 8 tokens: 2.0 us.
+// bits: HBM-bound on the read, where there is enough of it.  8000 tokens of 8 heads of 128 in bf16: 10.7 us,
+// 3.9 TB/s, fp32 15.0 us, 5.0 TB/s (every warp loads, encodes and writes once, with nothing to overlap; the plain
+// 16-bit store moves 34 MB at 4.6 TB/s); 64000 tokens 64.6 us, 5.1 TB/s, fp32 90.3 us, 6.6 TB/s; 8 tokens: 2.0 us.
 //
 // Gather: rows of each request in logical order, request-major, as
 // code * scale in the requested type (exact in fp32 and bf16 short of
 // overflow; fp16 rounds).  A warp takes a group of 16 positions of one kv head, four lanes to a token as
 // above; the heads of a group go to neighbouring warps, which write whole rows
 // together.  HBM-bound on the rows that it writes: 64 x 1152 rows of 8 heads of 128 to bf16 in 62 us,
-// 6.1 TB/s (95% of the copy rate).
+// 6.1 TB/s (95% of the copy rate); to fp32 163 us, 4.2 TB/s.
 #include <type_traits>
 
 #include "common.cuh"

@@ -17,10 +17,12 @@
 // are added in fp32, K's to the scores and V's to those rows.
 // Few rows over a long context are split over the keys; a second launch joins
 // the splits.
-// Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2313 us, 223 TFLOP/s; 8 x 250 on 2000, 16/8
-// heads of 64: 88 us, 174 TFLOP/s, of 256: 342 us, 180; fp32, of 128: 320 us, 96.  mma.sync itself would
-// bound this at about 560 TFLOP/s; what does is latency, 16 warps an SM (128 registers a thread) meeting at a
-// barrier per tile.  What it took, 2048 on 6144, 32/8 heads of 64: pages looked up a tile ahead (116 to 110 us at 8 x 250);
+// Sums of p V are divided by l at the end, p up to 8 (2^15 in fp16), so V has to stay below 2^127 / (8 * context).
+// Measured (bf16): 2048 tokens on 14336, 32/8 heads of 128: 2391 us, 216 TFLOP/s; 8 x 250 on 2000, 16/8
+// heads of 64: 93 us, 187 TFLOP/s, of 256: 361 us, 193; fp32, of 128: 362 us, 96.  mma.sync with its operands in
+// registers reaches 555 TFLOP/s; what bounds this is latency, 16 warps an SM (128 registers a thread) meeting at a
+// barrier per tile (tensor pipe 38% busy, issue slots 43%, 1.7 instructions a cycle, at 8 x 250, heads of 64).
+// What it took, 2048 on 6144, 32/8 heads of 64: pages looked up a tile ahead (116 to 110 us at 8 x 250);
 // a branch of its own for masked tiles (762 to 651); chunks of 16 bytes a thread, not words (595).
 // 32 rows a warp, which halves the reads of K and V fragments, leaves 8 warps and was slower (786 against 762).
 #include <type_traits>
@@ -536,7 +538,7 @@ template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
     mxfp4_prefill_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
   pdl_wait();
-  const int at = gridDim.x - 1 - blockIdx.x;  // the last rows, with the most keys, first
+  const unsigned at = gridDim.x - 1 - blockIdx.x;  // the last rows, with the most keys, first
   prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, at / p.num_splits, at % p.num_splits);
   pdl_launch_dependents();
 }

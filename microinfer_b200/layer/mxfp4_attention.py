@@ -5,11 +5,13 @@
 * ``gather_paged_kv_mxfp4``     rows in logical order, as ``gather_paged_kv``
 * ``paged_attention_mxfp4_meta``  dispatch on the step's metadata, as ``paged_attention_meta``
 
-Decode reads the codes and decodes them in registers.  Prefill of a large chunk decodes each
-context once into a workspace of the query's type and attends to that with the
-dense tensor-core kernel: a chunk of n tokens does 4 * n * Hq flops for each of the
-Hkv elements decoded, so the extra pass is a few percent.  Small chunks, and shapes that kernel does not
-take, are computed from the pages.
+Decode reads the codes and decodes them in registers.  Prefill has two ways.  Where there are tiles enough for
+the dense tensor-core kernel, each context is decoded once into a workspace of the query's type (3.76 times its
+pages in 16 bits) and that kernel attends to the rows: a chunk of n tokens does 4 * n * Hq flops for each of the
+Hkv elements decoded, so the extra pass is a few percent of a large chunk, and most of the call
+where every request has a few tokens.  Few tiles, and shapes that kernel does not take, are computed from the
+pages.  Both give the same result up to rounding: sequences with what the dense kernel cannot do
+(a NaN or, in fp16, a block past its range; a page that is none) are done over from the pages.
 Workspaces come from torch's allocator for the length of the call, so that calls on several
 streams, and captured graphs, each have their own.
 """
@@ -166,9 +168,13 @@ def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
     """Whether prefill reads the pages itself instead of gathering for the dense kernel.
 
     It does where the tcgen05 kernel does not take the shape (8 x 250 tokens on 2000, 16/8 heads of
-    256: 342 us, gathered 19103; 8 x 8 on nothing: 14 and 29), and where that would leave three
+    256: 361 us, gathered 19103; 8 x 8 on nothing: 14 and 29), and where that would leave three
     quarters of the SMs without a tile of 128 rows: reading the pages splits the keys
     (128 tokens on 16000, 32/8 heads of 128: 151 us, gathered 294; 256 tokens: 317 and 297).
+    Many requests of few tokens are many tiles, nearly empty in both kernels, and the dense one is faster on them
+    (64 x 4 on 8192, 32/8 heads of 128: 967 us, from the pages 1484).  The rule knows neither contexts nor
+    the real chunks: short contexts (4 x 64 on 64: 14 us from the pages, gathered 17) and one chunk among
+    decode rows (512 tokens and 63 rows on 8192: 1864, gathered 2452) go the slower way.
     """
     if dtype == _lib.dtype_code(torch.float32) and d > 128:  # q's three parts outgrow shared memory
         return False
