@@ -669,7 +669,7 @@ static int prefill_common(void *out, const void *query, const void *kbase, const
                           int32_t dtype, const int32_t *cu_q, const int32_t *cu_k,
                           const int32_t *block_tables, int64_t bt_stride, int64_t num_seqs,
                           int64_t num_tokens, int64_t num_kv_tokens, int32_t max_seqlen_q,
-                          float scale, int32_t *dev_status, void *stream, bool paged) {
+                          float scale, int32_t *dev_status, void *stream, bool paged, float p_lift = 0.f) {
   const int e = elem_size(dtype);
   if (e == 0) return fail(MI_ERR_INVALID, "unknown dtype");
   if (num_seqs < 0 || num_tokens < 0) return fail(MI_ERR_INVALID, "negative sizes");
@@ -706,6 +706,7 @@ static int prefill_common(void *out, const void *query, const void *kbase, const
   p.num_kv_heads = num_kv_heads;
   p.head_dim = head_dim;
   p.scale_log2 = scale * kLog2eHost;
+  p.p_lift = p_lift;
   p.status = dev_status;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int G = num_q_heads / num_kv_heads;
@@ -860,3 +861,18 @@ int mi_wait_flag_selftest(const int32_t *flag, int64_t timeout_ns, int32_t *dev_
 }
 
 }  // extern "C"
+
+namespace mi {
+
+// mi_varlen_prefill with p lifted (params.cuh).
+int capi_varlen_prefill_lifted(void *out, const void *query, const void *keys, const void *values,
+                               int64_t kv_token_stride, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t dtype, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                               int64_t num_seqs, int64_t num_tokens, int64_t num_kv_tokens, int32_t max_seqlen_q,
+                               float scale, float p_lift, int32_t *dev_status, void *stream) {
+  return prefill_common(out, query, keys, values, kv_token_stride, 0, 0, num_q_heads, num_kv_heads, head_dim, dtype,
+                        cu_seqlens_q, cu_seqlens_k, nullptr, 0, num_seqs, num_tokens, num_kv_tokens, max_seqlen_q,
+                        scale, dev_status, stream, false, p_lift);
+}
+
+}  // namespace mi

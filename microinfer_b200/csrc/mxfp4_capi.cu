@@ -12,6 +12,11 @@ namespace mi {
 int capi_fail(int code, const char *msg);
 int capi_select_device(const void *p);
 int capi_cuda_status(cudaError_t e);
+int capi_varlen_prefill_lifted(void *out, const void *query, const void *keys, const void *values,
+                               int64_t kv_token_stride, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t dtype, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                               int64_t num_seqs, int64_t num_tokens, int64_t num_kv_tokens, int32_t max_seqlen_q,
+                               float scale, float p_lift, int32_t *dev_status, void *stream);
 
 cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtype, bool vec,
                                cudaStream_t stream);
@@ -344,9 +349,10 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   g.head_dim = head_dim;
   g.status = dev_status;
   if (const int s = capi_cuda_status(launch_mxfp4_gather(g, dtype, num_seqs, max_context, st))) return s;
-  if (const int s = mi_varlen_prefill(out, query, keys, values, static_cast<int64_t>(num_kv_heads) * head_dim, num_q_heads,
-                                      num_kv_heads, head_dim, dtype, cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens,
-                                      kv_rows, max_seqlen_q, scale, dev_status, stream))
+  const float p_lift = dtype == MI_DTYPE_FLOAT16 ? 7.f : 0.f;  // small p keep their bits, as in the kernels on the pages
+  if (const int s = capi_varlen_prefill_lifted(
+          out, query, keys, values, static_cast<int64_t>(num_kv_heads) * head_dim, num_q_heads, num_kv_heads, head_dim, dtype,
+          cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens, kv_rows, max_seqlen_q, scale, p_lift, dev_status, stream))
     return s;
   if (redo == nullptr) return MI_OK;
   MxPrefillParams p = {};

@@ -70,6 +70,9 @@ struct AttnParams {
   // the decode kernel launched after it (mixed batches), and lets that launch
   // start as soon as all its CTAs are running.
   int32_t mixed_decode;
+  // The tensor-core prefill kernel holds p as 2^(x - m + p_lift), m up to 8 binades behind: up to 7 in fp16, whose
+  // small p otherwise lose bits from 2^-14 of the largest on.
+  float p_lift;
 };
 struct DecodeParams {
   void *out;

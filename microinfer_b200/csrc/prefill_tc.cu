@@ -47,6 +47,7 @@ struct __align__(64) PrefillTcParams {
   int32_t num_q_heads;
   int32_t paged;
   float scale_log2;
+  float p_lift;  // p is 2^(x - m + p_lift)
   int32_t *status;
   // Mixed batches: sequences with one query token are left to the decode kernel
   // launched right after this one, which may start once every CTA here has passed
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
         }
         // P = 2^(s * scale - m) as 16-bit pairs over the first 64 columns of S
         // (the row is already read back).
-        const float nb = m_new == -INFINITY ? 0.f : -m_new;  // masked: ex2(-inf) = 0
+        const float nb = m_new == -INFINITY ? 0.f : p.p_lift - m_new;  // masked: ex2(-inf) = 0
         const float2 sc2 = make_float2(sl2, sl2), nb2 = make_float2(nb, nb);
         float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -694,6 +695,7 @@ cudaError_t launch_prefill_tc(const AttnParams &a, int dtype, int G, int32_t max
   p.paged = paged ? 1 : 0;
   // A masked score is an infinity times the scale, so a scale of 0 is one that leaves every finite score at 0.
   p.scale_log2 = a.scale_log2 == 0.f ? 1e-30f : a.scale_log2;
+  p.p_lift = a.p_lift;
   p.status = a.status;
   p.skip_single = paged && a.mixed_decode ? 1 : 0;
   const int64_t n = a.num_seqs;

@@ -205,3 +205,33 @@ def test_gathered_context_past_the_table(cuda_device, name, hkv, d):
     first = 224 - (300 - 144)  # rows of the last sequence that see nothing past the table
     want = mo.attention(query[end:].double().cpu().numpy(), mo.rows(kp, table[4], 300), mo.rows(vp, table[4], 300), d ** -0.5)
     _close(got[end:end + first], *[x[:first] for x in want], dtype, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_gathered_keys_of_little_weight(cuda_device, name):
+    """One key takes nearly everything and its value is zero: the rest, each about 2^-20 of it, decides the result.
+    p is lifted by 2^7 in fp16, so half its smallest step is 2^-32 of the largest p, a key at most."""
+    dtype = DTYPES[name]
+    hkv, d, q_lens = 8, 128, LARGE
+    ctxs = [3000] * 5
+    rng = np.random.default_rng(80)
+    nb = 5 * 188
+    kc, kb = mo.encode(rng.standard_normal((nb, 16, hkv, d)) * 0.01)
+    vc, vb = mo.encode(rng.standard_normal((nb, 16, hkv, d)) + 1.0)
+    table = _table(rng, ctxs, nb, 16)
+    kc[table[:, 3], 5], kb[table[:, 3], 5] = 2, 127  # all 1.0
+    vc[table[:, 3], 5], vb[table[:, 3], 5] = 0, 0
+    kp, vp = mo.pack(kc, kb), mo.pack(vc, vb)
+    query = _cuda(np.full((sum(q_lens), 2 * hkv, d), 1.0), cuda_device, dtype)
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=cuda_device) for x in (q_lens, ctxs))
+    scale = 14.0 / d  # the sink is exp(14) = 2^20 above the others
+    got = mi.paged_prefill_mxfp4(query, _cuda(kp, cuda_device), _cuda(vp, cuda_device), cu_q, cu_k, _cuda(table, cuda_device),
+                                 max_seqlen_q=max(q_lens), total_k=sum(ctxs), scale=scale)
+    mi.check_device_status(cuda_device)
+    q, at = query.double().cpu().numpy(), np.cumsum([0, *q_lens])
+    parts = [mo.attention(q[at[r]:at[r + 1]], mo.rows(kp, table[r], c), mo.rows(vp, table[r], c), scale)
+             for r, c in enumerate(ctxs)]
+    want, weight, size, floor = (np.concatenate(x) for x in zip(*parts))
+    assert 0.0001 < np.abs(want).max() < 0.1
+    _close(got, want, weight, size, 4 * floor, dtype, PREFILL_STEP[dtype])
