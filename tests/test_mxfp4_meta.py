@@ -120,3 +120,37 @@ def test_a_captured_prefill_is_replayed_with_longer_contexts(cuda_device):
     parts = [mo.attention(q[at[r]:at[r + 1]], mo.rows(kp, table[r], c), mo.rows(vp, table[r], c), d ** -0.5)
              for r, c in enumerate(later)]
     _close(got, *[np.concatenate(x) for x in zip(*parts)], torch.bfloat16, PREFILL_STEP[torch.bfloat16])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hkv,d,bs", [(1, 64, 64), (2, 96, 16), (2, 256, 32)])
+def test_cached_attention_of_other_heads(cuda_device, dtype, hkv, d, bs):
+    """A chunk, one on its prefix and a token, through a bound layer; rows come as a transpose of heads first."""
+    from microinfer_b200.layer.cached_attention import CachedAttention
+
+    rng = np.random.default_rng(d)
+    pool = mi.MXFP4KVCache(2, 6, bs, hkv, d, device=cuda_device)
+    attn = CachedAttention()
+    attn.bind_cache(pool.layer(1))
+    table = [4, 1, 5, 0][:-(-34 // bs)]
+    tt = torch.tensor([table], dtype=torch.int32, device=cuda_device)
+    history, done = [np.zeros((0, hkv, d)) for _ in range(2)], 0
+    for n in (12, 21, 1):
+        q, k, v = (_cuda(rng.standard_normal((h, n, d)), cuda_device, dtype).transpose(0, 1) for h in (4 * hkv, hkv, hkv))
+        slots = [table[pos // bs] * bs + pos % bs for pos in range(done, done + n)]
+        done += n
+        history = [np.concatenate([old, mo.decode(*mo.encode(new.double().cpu().numpy()))]) for old, new in zip(history, (k, v))]
+        lens = torch.tensor([done], dtype=torch.int32, device=cuda_device)
+        fields = dict(slot_mapping=torch.tensor(slots, dtype=torch.int32, device=cuda_device), block_tables=tt)
+        if n > 1:
+            fields.update(cu_seqlens_q=torch.tensor([0, n], dtype=torch.int32, device=cuda_device),
+                          cu_seqlens_k=torch.tensor([0, done], dtype=torch.int32, device=cuda_device), max_seqlen_q=n,
+                          max_seqlen_k=done, total_seqlen_k=done)
+        else:
+            fields.update(context_lens=lens)
+        got = attn(q, k, v, mi.AttentionMetadata.build(is_prefill=n > 1, **fields))
+        want = mo.attention(q.double().cpu().numpy(), *history, d ** -0.5)
+        _close(got, *want, dtype, (PREFILL_STEP if n > 1 else DECODE_STEP)[dtype])
+    mi.check_device_status(cuda_device)
+    assert int(pool.keys[0].max()) == 0
