@@ -27,20 +27,6 @@ __host__ __device__ constexpr int mx_group_bytes(int head_dim) {
   return head_dim / kMxBlock * kMxBytes;
 }
 
-// n / d by a multiplication, n below 2^31.
-struct FastDiv {
-  uint32_t mul;
-  int shift;
-  explicit FastDiv(uint32_t d) {
-    shift = 31;
-    while ((uint64_t{1} << (shift - 31)) < d) ++shift;
-    mul = static_cast<uint32_t>(((uint64_t{1} << shift) + d - 1) / d);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    return static_cast<uint32_t>(static_cast<uint64_t>(n) * mul >> shift);
-  }
-};
-
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(byte << 23);
 }

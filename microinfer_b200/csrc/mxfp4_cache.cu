@@ -73,7 +73,7 @@ __device__ __forceinline__ int blocks_of(int head_dim) {
 
 // One warp per (8 tokens, kv head).  WIDE: slots past 32 bits.
 template <typename T, typename I, bool VEC, int NB, bool WIDE>
-__global__ void __launch_bounds__(128) mxfp4_store_kernel(const MxStoreParams p, const FastDiv by_heads,
+__global__ void __launch_bounds__(128) mxfp4_store_kernel(const CodedStoreParams p, const FastDiv by_heads,
                                                           const FastDiv by_block) {
   pdl_wait();
   const int lane = threadIdx.x & 31, j = lane & 3;
@@ -159,7 +159,7 @@ __device__ __forceinline__ void write8(T *dst, const float (&x)[8]) {
 // grid (groups of 16 positions x kv heads, 8 warps to a CTA; sequences).  REDO: rows for the dense prefill, which
 // notes the sequences that it cannot do.
 template <typename T, int NB, bool REDO>
-__global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams p, const FastDiv by_heads,
+__global__ void __launch_bounds__(256) mxfp4_gather_kernel(const CodedGatherParams p, const FastDiv by_heads,
                                                            const FastDiv by_page) {
   pdl_wait();
   const int seq = blockIdx.y;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256) mxfp4_gather_kernel(const MxGatherParams 
 }
 
 template <typename T, typename I, int NB>
-cudaError_t launch_store_tin(const MxStoreParams &p, bool vec, cudaStream_t stream) {
+cudaError_t launch_store_tin(const CodedStoreParams &p, bool vec, cudaStream_t stream) {
   const int64_t tasks = (p.num_tokens + 7) / 8 * p.num_kv_heads;
   if (tasks >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>((tasks + 3) / 4)), block(128);
@@ -266,14 +266,14 @@ cudaError_t launch_store_tin(const MxStoreParams &p, bool vec, cudaStream_t stre
 }
 
 template <typename T, typename I>
-cudaError_t launch_store_ti(const MxStoreParams &p, bool vec, cudaStream_t stream) {
+cudaError_t launch_store_ti(const CodedStoreParams &p, bool vec, cudaStream_t stream) {
   if (p.head_dim == 128) return launch_store_tin<T, I, 4>(p, vec, stream);
   if (p.head_dim == 64) return launch_store_tin<T, I, 2>(p, vec, stream);
   return launch_store_tin<T, I, 0>(p, vec, stream);
 }
 
 template <typename T, bool REDO>
-cudaError_t launch_gather_t(const MxGatherParams &p, int64_t num_seqs, int64_t max_context, cudaStream_t stream) {
+cudaError_t launch_gather_t(const CodedGatherParams &p, int64_t num_seqs, int64_t max_context, cudaStream_t stream) {
   const int64_t tasks = (max_context + kMxGroup - 1) / kMxGroup * p.num_kv_heads;
   if (tasks >= (int64_t{1} << 31)) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>((tasks + 7) / 8), static_cast<unsigned>(num_seqs)), block(256);
@@ -286,21 +286,21 @@ cudaError_t launch_gather_t(const MxGatherParams &p, int64_t num_seqs, int64_t m
 }
 
 template <typename T>
-cudaError_t launch_store_t(const MxStoreParams &p, int index_dtype, bool vec, cudaStream_t stream) {
+cudaError_t launch_store_t(const CodedStoreParams &p, int index_dtype, bool vec, cudaStream_t stream) {
   return index_dtype == MI_INDEX_INT32 ? launch_store_ti<T, int32_t>(p, vec, stream)
                                        : launch_store_ti<T, int64_t>(p, vec, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtype, bool vec,
+cudaError_t launch_mxfp4_store(const CodedStoreParams &p, int dtype, int index_dtype, bool vec,
                                cudaStream_t stream) {
   if (dtype == MI_DTYPE_BFLOAT16) return launch_store_t<__nv_bfloat16>(p, index_dtype, vec, stream);
   if (dtype == MI_DTYPE_FLOAT16) return launch_store_t<__half>(p, index_dtype, vec, stream);
   return launch_store_t<float>(p, index_dtype, vec, stream);
 }
 
-cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
+cudaError_t launch_mxfp4_gather(const CodedGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
                                 cudaStream_t stream) {
   if (p.redo != nullptr)
     return dtype == MI_DTYPE_BFLOAT16 ? launch_gather_t<__nv_bfloat16, true>(p, num_seqs, max_context, stream)

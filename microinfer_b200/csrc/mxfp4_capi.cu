@@ -18,11 +18,11 @@ int capi_varlen_prefill_lifted(void *out, const void *query, const void *keys, c
                                int64_t num_seqs, int64_t num_tokens, int64_t num_kv_tokens, int32_t max_seqlen_q,
                                float scale, float p_lift, int32_t *dev_status, void *stream);
 
-cudaError_t launch_mxfp4_store(const MxStoreParams &p, int dtype, int index_dtype, bool vec,
+cudaError_t launch_mxfp4_store(const CodedStoreParams &p, int dtype, int index_dtype, bool vec,
                                cudaStream_t stream);
-cudaError_t launch_mxfp4_gather(const MxGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
+cudaError_t launch_mxfp4_gather(const CodedGatherParams &p, int dtype, int64_t num_seqs, int64_t max_context,
                                 cudaStream_t stream);
-cudaError_t launch_mxfp4_decode(const MxDecodeParams &p, int dtype, cudaStream_t stream);
+cudaError_t launch_mxfp4_decode(const CodedDecodeParams &p, int dtype, cudaStream_t stream);
 bool mxfp4_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
                             int64_t capacity);
 size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity,
@@ -31,7 +31,7 @@ size_t mxfp4_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_head
 bool mxfp4_prefill_supported(int dtype, int head_dim);
 int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
                          int64_t capacity, int sms);
-cudaError_t launch_mxfp4_prefill(const MxPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
+cudaError_t launch_mxfp4_prefill(const CodedPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
                                  int64_t max_seqlen_q, cudaStream_t stream);
 
 }  // namespace mi
@@ -87,7 +87,7 @@ int mi_store_kv_mxfp4(void *key_pages, void *value_pages, int64_t num_blocks, in
     return capi_fail(MI_ERR_ALIGNMENT, "pages must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
   const int e = dtype == MI_DTYPE_FLOAT32 ? 4 : 2;
-  MxStoreParams p = {};
+  CodedStoreParams p = {};
   p.key_pages = static_cast<uint8_t *>(key_pages);
   p.value_pages = static_cast<uint8_t *>(value_pages);
   p.slots = slots;
@@ -124,7 +124,7 @@ int mi_gather_paged_kv_mxfp4(void *out_keys, void *out_values, const void *key_p
   if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(out_keys) || !aligned16(out_values))
     return capi_fail(MI_ERR_ALIGNMENT, "pages and outputs must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
-  MxGatherParams p = {};
+  CodedGatherParams p = {};
   p.out_keys = out_keys;
   p.out_values = out_values;
   p.key_pages = static_cast<const uint8_t *>(key_pages);
@@ -181,7 +181,7 @@ int mi_paged_decode_mxfp4(void *out, const void *query, const void *key_pages, c
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_decode_mxfp4_workspace_bytes)");
   if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  MxDecodeParams p = {};
+  CodedDecodeParams p = {};
   p.out = out;
   p.query = query;
   p.key_pages = static_cast<const uint8_t *>(key_pages);
@@ -255,7 +255,7 @@ int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_pages, 
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_prefill_mxfp4_workspace_bytes)");
   if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  MxPrefillParams p = {};
+  CodedPrefillParams p = {};
   p.out = out;
   p.query = query;
   p.key_pages = static_cast<const uint8_t *>(key_pages);
@@ -331,7 +331,7 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   uint8_t *redo = nullptr;
   if (dense && max_seqlen_q <= (1 << 24) && block_table_stride <= (INT32_MAX - 256) / block_size)
     redo = reinterpret_cast<uint8_t *>(values + rows);
-  MxGatherParams g = {};
+  CodedGatherParams g = {};
   g.out_keys = keys;
   g.out_values = values;
   g.key_pages = static_cast<const uint8_t *>(key_pages);
@@ -355,7 +355,7 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
           cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens, kv_rows, max_seqlen_q, scale, p_lift, dev_status, stream))
     return s;
   if (redo == nullptr) return MI_OK;
-  MxPrefillParams p = {};
+  CodedPrefillParams p = {};
   p.out = out;
   p.query = query;
   p.key_pages = g.key_pages;

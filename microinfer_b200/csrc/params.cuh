@@ -140,8 +140,8 @@ struct QkPrologueParams {
   int32_t *status;
 };
 
-// 4-bit paged cache (mxfp4.cuh): quantising store, dequantising gather, decode.
-struct MxStoreParams {
+// Quantised paged caches, 4 bits (mxfp4.cuh) and 8 (fp8.cuh): store, gather, decode, prefill.
+struct CodedStoreParams {
   uint8_t *key_pages;
   uint8_t *value_pages;
   const void *slots;
@@ -155,8 +155,10 @@ struct MxStoreParams {
   int32_t num_kv_heads;
   int32_t head_dim;
   int32_t *status;
+  int32_t *index;    // 8-bit: null, or an entry per slot of the pool (fp8_cache.cu)
+  int32_t wide_slots;  // 8-bit: slots are int64
 };
-struct MxGatherParams {
+struct CodedGatherParams {
   void *out_keys;
   void *out_values;
   const uint8_t *key_pages;
@@ -175,14 +177,14 @@ struct MxGatherParams {
   int32_t head_dim;
   int32_t *status;
 };
-struct MxDecodeParams {
+struct CodedDecodeParams {
   void *out;
   const void *query;
   const uint8_t *key_pages;
   const uint8_t *value_pages;
   const int32_t *block_tables;
   const int32_t *context_lens;
-  float *workspace;  // partial states, see decode_mxfp4_mma.cu
+  float *workspace;  // partial states, see decode_segments.cuh
   int64_t bt_stride;
   int64_t num_blocks;
   int64_t num_seqs;
@@ -194,7 +196,7 @@ struct MxDecodeParams {
   int32_t *status;
 };
 
-struct MxPrefillParams {
+struct CodedPrefillParams {
   void *out;
   const void *query;
   const uint8_t *key_pages;

@@ -136,7 +136,7 @@ __device__ __noinline__ float2 apart_scores(const uint8_t *codes, unsigned block
 
 // 128 rows of one kv head against the keys of one split.
 template <typename T, int NB>
-__device__ __forceinline__ void prefill_tile(const MxPrefillParams &p, const FastDiv &by_group, const FastDiv &by_page,
+__device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const FastDiv &by_group, const FastDiv &by_page,
                                              int seq, int kvh, int tile, int split) {
   using C = PfCfg<T, NB>;
   using E = typename C::E;
@@ -536,7 +536,7 @@ __device__ __forceinline__ void prefill_tile(const MxPrefillParams &p, const Fas
 
 template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
-    mxfp4_prefill_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
+    mxfp4_prefill_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
   pdl_wait();
   const unsigned at = gridDim.x - 1 - blockIdx.x;  // the last rows, with the most keys, first
   prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, at / p.num_splits, at % p.num_splits);
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 // ever any, so a few CTAs look (a CTA to a tile would take 100 us to find nothing at 64 x 2048 tokens) and take all tiles if so.
 template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 2 : 1)
-    mxfp4_prefill_redo_kernel(const MxPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
+    mxfp4_prefill_redo_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
   pdl_wait();
   const int64_t ctx = static_cast<int64_t>(p.cu_seqlens_k[blockIdx.z + 1]) - p.cu_seqlens_k[blockIdx.z];
   const int64_t groups = min((ctx + kMxGroup - 1) / kMxGroup, static_cast<int64_t>(p.redo_groups));
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, PfCfg<T, NB>::kSmem <= 100 * 1024 ? 
 
 // Join the splits: a warp to a row, the rows of the sequences only.
 template <typename T, int NB>
-__global__ void __launch_bounds__(kThreads) mxfp4_prefill_join_kernel(const MxPrefillParams p, const FastDiv by_group) {
+__global__ void __launch_bounds__(kThreads) mxfp4_prefill_join_kernel(const CodedPrefillParams p, const FastDiv by_group) {
   constexpr int D = NB * kMxBlock;
   pdl_wait();
   const int seq = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kThreads) mxfp4_prefill_join_kernel(const MxPr
 namespace {
 
 template <typename T, int NB>
-cudaError_t launch_pf(const MxPrefillParams &p, int64_t num_seqs, int64_t max_seqlen_q, cudaStream_t stream) {
+cudaError_t launch_pf(const CodedPrefillParams &p, int64_t num_seqs, int64_t max_seqlen_q, cudaStream_t stream) {
   using C = PfCfg<T, NB>;
   auto kern = mxfp4_prefill_kernel<T, NB>;
   static bool attr_set[64] = {};
@@ -650,7 +650,7 @@ cudaError_t launch_pf(const MxPrefillParams &p, int64_t num_seqs, int64_t max_se
 }
 
 template <typename T>
-cudaError_t launch_pf_t(const MxPrefillParams &p, int head_dim, int64_t num_seqs, int64_t max_seqlen_q,
+cudaError_t launch_pf_t(const CodedPrefillParams &p, int head_dim, int64_t num_seqs, int64_t max_seqlen_q,
                         cudaStream_t stream) {
   switch (head_dim / kMxBlock) {
     case 1: return launch_pf<T, 1>(p, num_seqs, max_seqlen_q, stream);
@@ -688,7 +688,7 @@ int mxfp4_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-cudaError_t launch_mxfp4_prefill(const MxPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
+cudaError_t launch_mxfp4_prefill(const CodedPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
                                  int64_t max_seqlen_q, cudaStream_t stream) {
   if (dtype == MI_DTYPE_BFLOAT16) return launch_pf_t<__nv_bfloat16>(p, head_dim, num_seqs, max_seqlen_q, stream);
   if (dtype == MI_DTYPE_FLOAT16) return launch_pf_t<__half>(p, head_dim, num_seqs, max_seqlen_q, stream);
