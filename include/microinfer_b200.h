@@ -501,6 +501,125 @@ MI_API int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const v
                                     int32_t *dev_status, void *stream);
 
 /*
+ * 8-bit paged KV cache.  K and V are held in 8-bit floating point (e4m3: sign, 4 bits of
+ * exponent, 3 of mantissa; largest 448, smallest 2^-9, 0x7f and 0xff not a number) with one
+ * power-of-two scale for every block of 16 tokens and kv head.  key_pages / value_pages are bytes
+ *   [num_blocks][num_kv_heads][mi_fp8_page_bytes(block_size, head_dim)];
+ * a page holds, for every 16 tokens, a group of 16 * head_dim + 16 bytes: the codes in parts of 64
+ * dims (w = 64; a last part of w = 32 where head_dim is an odd multiple of 32),
+ *   K  [16 tokens][w]
+ *   V  [2 halves][8][4 pairs][w / 8 dims][2 tokens], token = 8 half + 2 pair + last index,
+ *                                                    dim = w / 8 * second index + fourth
+ * then the scale byte b (2^(b - 127), 0 for zero) and 15 bytes that are zero.
+ * block_size must be a multiple of 16, head_dim a multiple of 32 up to 256
+ * (MI_ERR_UNSUPPORTED otherwise); pages are 16-byte aligned.  Zero-filled pages hold
+ * zeros.  mi_copy_blocks copies them as it copies others (block_bytes =
+ * num_kv_heads * mi_fp8_page_bytes).  The reference has no quantised cache.
+ */
+
+/* Bytes of one kv head of one page, or a negative status. */
+MI_API int64_t mi_fp8_page_bytes(int32_t block_size, int32_t head_dim);
+
+/*
+ * Quantising store: token t's rows (any token stride, in elements; each
+ * [num_kv_heads, head_dim] row contiguous; f32/f16/bf16) to slot
+ * slots[t] = block * block_size + offset, -1 writes nothing, in any order.  The tokens of a call that
+ * fall into one group are quantised together: with a their largest finite magnitude they need the byte
+ * 0 if a = 0, else e + 127, e least with a <= 448 * 2^e, held between 1 and 246.  A call that writes the
+ * group's first slot sets its byte to that; any other raises it to that at most, and where it rises
+ * the group's other codes are rounded to the new scale.  Codes round to nearest, ties to even, saturating
+ * at 448; elements that are not finite become NaN.  Slots must be unique within a call; those
+ * outside the pool are skipped (MI_DEV_BAD_SLOT).  The workspace (num_blocks * block_size entries for
+ * long calls, none for short ones) holds for the duration of the call which token goes to which slot
+ * and needs no initial value; calls that can run at the same time need one each.
+ */
+MI_API size_t mi_store_kv_fp8_workspace_bytes(int64_t num_tokens, int64_t num_blocks,
+                                       int32_t block_size);
+MI_API int mi_store_kv_fp8(void *key_pages, void *value_pages, int64_t num_blocks,
+                    int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                    const void *slots, int32_t index_dtype, const void *keys,
+                    const void *values, int32_t dtype, int64_t key_token_stride,
+                    int64_t value_token_stride, int64_t num_tokens, void *workspace,
+                    size_t workspace_bytes, int32_t *dev_status, void *stream);
+
+/*
+ * Dequantising block-table gather: rows of logical position t of sequence s to
+ * out[cu_seqlens_k[s] + t] in `dtype`, for t < context_s.  `max_context`
+ * bounds the launch shape, `out_rows` is the row capacity of the outputs (never
+ * written past).  Outputs are contiguous and 16-byte aligned.
+ */
+MI_API int mi_gather_paged_kv_fp8(void *out_keys, void *out_values, const void *key_pages,
+                             const void *value_pages, int64_t num_blocks,
+                             int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t dtype, const int32_t *block_tables,
+                             int64_t block_table_stride, const int32_t *cu_seqlens_k,
+                             int64_t num_seqs, int64_t out_rows, int64_t max_context,
+                             int32_t *dev_status, void *stream);
+
+/*
+ * Paged decode over the 8-bit cache: out[s, h] = softmax(scale * K_s q[s, h]) V_s
+ * over context_lens[s] positions, GQA with any group; a sequence without
+ * keys gives zeros.  query / out are contiguous [num_seqs, num_q_heads, head_dim]
+ * in `dtype`, 16-byte aligned.  The workspace holds partial states for the
+ * duration of the call and needs no initial value; calls that can run at the
+ * same time need one each.
+ */
+MI_API size_t mi_paged_decode_fp8_workspace_bytes(int64_t num_seqs, int64_t num_blocks,
+                                             int32_t block_size, int32_t num_q_heads,
+                                             int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t dtype, int64_t block_table_stride,
+                                             int device);
+MI_API int mi_paged_decode_fp8(void *out, const void *query, const void *key_pages,
+                          const void *value_pages, int64_t num_blocks, int32_t block_size,
+                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t dtype, const int32_t *block_tables,
+                          int64_t block_table_stride, const int32_t *context_lens,
+                          int64_t num_seqs, float scale, void *workspace,
+                          size_t workspace_bytes, int32_t *dev_status, void *stream);
+
+/*
+ * Causal chunked prefill from the 8-bit cache (also mixed batches): rows as
+ * mi_paged_prefill, any type, GQA group and head_dim.  `max_seqlen_q`
+ * bounds the launch shape, `max_context` (a bound on the contexts, or less) the split over the keys
+ * of few rows, whose states take the workspace for the duration of the call.
+ */
+MI_API size_t mi_paged_prefill_fp8_workspace_bytes(int64_t num_seqs, int64_t num_tokens,
+                                              int64_t max_seqlen_q, int32_t num_q_heads,
+                                              int32_t num_kv_heads, int32_t head_dim,
+                                              int64_t max_context, int device);
+MI_API int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pages,
+                           const void *value_pages, int64_t num_blocks, int32_t block_size,
+                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t dtype, const int32_t *cu_seqlens_q,
+                           const int32_t *cu_seqlens_k, const int32_t *block_tables,
+                           int64_t block_table_stride, int64_t num_seqs, int64_t num_tokens,
+                           int64_t max_seqlen_q, int64_t max_context, float scale,
+                           void *workspace, size_t workspace_bytes, int32_t *dev_status,
+                           void *stream);
+
+/*
+ * The same by way of rows, for chunks large enough for the tensor cores' dense kernel and shapes that it takes
+ * (MI_ERR_UNSUPPORTED otherwise): K and V of the contexts (kv_rows, their sum or a bound on it; rows past it are
+ * flagged) are decoded into the workspace and attended to as mi_varlen_prefill does.  Sequences with what does not go
+ * through it (a NaN of V, in f16 a value past 65504, a page that is none) are then done over from the
+ * pages, so results are those of mi_paged_prefill_fp8; `out` must not overlap the query.  `max_context` bounds one
+ * context: what a longer one has past it is treated as pages that are none.
+ */
+MI_API size_t mi_paged_prefill_fp8_gathered_workspace_bytes(int64_t num_seqs, int64_t max_context,
+                                                       int64_t kv_rows, int32_t num_kv_heads,
+                                                       int32_t head_dim, int32_t dtype);
+MI_API int mi_paged_prefill_fp8_gathered(void *out, const void *query, const void *key_pages,
+                                    const void *value_pages, int64_t num_blocks,
+                                    int32_t block_size, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                    const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
+                                    const int32_t *block_tables, int64_t block_table_stride,
+                                    int64_t num_seqs, int64_t num_tokens, int32_t max_seqlen_q,
+                                    int64_t max_context, int64_t kv_rows, float scale,
+                                    void *workspace, size_t workspace_bytes,
+                                    int32_t *dev_status, void *stream);
+
+/*
  * Bounded-wait self test: one thread spins on `flag` (device int32) until it
  * becomes non-zero or `timeout_ns` passes, then ORs MI_DEV_TIMEOUT into
  * dev_status if it ran out.  Exercises the same bounded-wait helper every

@@ -115,6 +115,40 @@ SIGNATURES = {
         [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _I32,
          _I64, _I64, _F, _P, _SZ, _P, _P],
     ),
+    "mi_fp8_page_bytes": (_I64, [_I32, _I32]),
+    "mi_store_kv_fp8_workspace_bytes": (_SZ, [_I64, _I64, _I32]),
+    "mi_store_kv_fp8": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I32, _I32, _I32, _P, _I32, _P, _P, _I32, _I64, _I64, _I64, _P, _SZ, _P, _P],
+    ),
+    "mi_gather_paged_kv_fp8": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P, _I64, _I64, _I64, _P, _P],
+    ),
+    "mi_paged_decode_fp8_workspace_bytes": (
+        _SZ, [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, ctypes.c_int],
+    ),
+    "mi_paged_decode_fp8": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P, _I64, _F, _P, _SZ, _P,
+         _P],
+    ),
+    "mi_paged_prefill_fp8_workspace_bytes": (
+        _SZ, [_I64, _I64, _I64, _I32, _I32, _I32, _I64, ctypes.c_int],
+    ),
+    "mi_paged_prefill_fp8": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _I64,
+         _I64, _F, _P, _SZ, _P, _P],
+    ),
+    "mi_paged_prefill_fp8_gathered_workspace_bytes": (
+        _SZ, [_I64, _I64, _I64, _I32, _I32, _I32],
+    ),
+    "mi_paged_prefill_fp8_gathered": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _I64, _I64, _I32,
+         _I64, _I64, _F, _P, _SZ, _P, _P],
+    ),
     "mi_copy_blocks": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P]),
     "mi_wait_flag_selftest": (ctypes.c_int, [_P, _I64, _P, _P]),
     "mi_build_decode_metadata": (

@@ -6,8 +6,8 @@ attend.  Prefill without a block table ("direct", no cached prefix) attends
 to this step's contiguous K/V with the dense varlen kernel, which replaces the
 reference's FlashAttention varlen / per-request SDPA paths (:17-55).
 
-A layer of the 4-bit pool (``LayerMXFP4Cache``) binds like any other: its store
-quantises, and paged attention reads the codes; direct prefill attends to this
+A layer of the 4-bit or 8-bit pool (``LayerMXFP4Cache``, ``LayerFP8Cache``) binds like any other: its
+store quantises, and paged attention reads the codes; direct prefill attends to this
 step's K/V as they are.
 """
 
@@ -16,12 +16,14 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from microinfer_b200.layer.fp8_attention import paged_attention_fp8_meta
 from microinfer_b200.layer.mxfp4_attention import paged_attention_mxfp4_meta
 from microinfer_b200.layer.paged_attention import (
     paged_attention_meta,
     paged_decode_store,
     varlen_prefill,
 )
+from microinfer_b200.worker.fp8_cache import LayerFP8Cache
 from microinfer_b200.worker.kv_cache import LayerKVCache
 from microinfer_b200.worker.mxfp4_cache import LayerMXFP4Cache
 
@@ -29,9 +31,9 @@ from microinfer_b200.worker.mxfp4_cache import LayerMXFP4Cache
 class CachedAttention(nn.Module):
     def __init__(self):
         super().__init__()
-        self.cache: LayerKVCache | LayerMXFP4Cache | None = None
+        self.cache: LayerKVCache | LayerMXFP4Cache | LayerFP8Cache | None = None
 
-    def bind_cache(self, cache: LayerKVCache | LayerMXFP4Cache):
+    def bind_cache(self, cache: LayerKVCache | LayerMXFP4Cache | LayerFP8Cache):
         self.cache = cache
 
     def forward(self, q, k, v, metadata):
@@ -43,8 +45,8 @@ class CachedAttention(nn.Module):
         if cache is not None:
             if metadata.slot_mapping is None:
                 raise ValueError("bound cache requires slot_mapping")
-            if (not isinstance(cache, LayerMXFP4Cache) and metadata.is_decode and not metadata.validate_cache_write
-                    and metadata.context_lens is not None):
+            if (not isinstance(cache, (LayerMXFP4Cache, LayerFP8Cache)) and metadata.is_decode
+                    and not metadata.validate_cache_write and metadata.context_lens is not None):
                 # One launch: store this step's K/V, then decode over the cache.
                 return paged_decode_store(q, cache.keys, cache.values, metadata.block_tables,
                                           metadata.context_lens, k, v, metadata.slot_mapping)
@@ -54,6 +56,8 @@ class CachedAttention(nn.Module):
                 cache.write_slots(metadata.slot_mapping, k, v)
         if not direct and isinstance(cache, LayerMXFP4Cache):
             return paged_attention_mxfp4_meta(q, cache.keys, cache.values, metadata)
+        if not direct and isinstance(cache, LayerFP8Cache):
+            return paged_attention_fp8_meta(q, cache.keys, cache.values, metadata)
         if not direct:
             return paged_attention_meta(q, cache.keys, cache.values, metadata)
         if q.shape[1] % k.shape[1]:

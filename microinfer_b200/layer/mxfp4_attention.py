@@ -267,14 +267,19 @@ def paged_prefill_mxfp4(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_
 def paged_attention_mxfp4_meta(query, key_pages, value_pages, metadata, *,
                                scale: float | None = None) -> torch.Tensor:
     """Backend dispatch on validated metadata, as ``paged_attention_meta`` over the 4-bit cache."""
+    return coded_attention_meta(query, key_pages, value_pages, metadata, scale, paged_decode_mxfp4,
+                                paged_prefill_mxfp4, page_dims)
+
+
+def coded_attention_meta(query, key_pages, value_pages, metadata, scale, decode, prefill, dims):
+    """``decode`` or ``prefill`` over quantised pages, whose ``dims`` are as ``page_dims``', by the step's metadata."""
     if query.shape[0] == 0:
         return torch.empty_like(query)
     block_tables = metadata.block_tables
     if block_tables is None:
         raise ValueError("paged attention needs metadata.block_tables")
     if metadata.is_decode and metadata.context_lens is not None:
-        return paged_decode_mxfp4(query, key_pages, value_pages, block_tables,
-                                  metadata.context_lens, scale=scale)
+        return decode(query, key_pages, value_pages, block_tables, metadata.context_lens, scale=scale)
     cu_q, cu_k = metadata.cu_seqlens_q, metadata.cu_seqlens_k
     if cu_q is None:
         cu_q = torch.tensor(metadata.cu_q_cpu, dtype=torch.int32, device=query.device)
@@ -285,16 +290,16 @@ def paged_attention_mxfp4_meta(query, key_pages, value_pages, metadata, *,
                            device=query.device)
         torch.cumsum(metadata.context_lens, 0, out=cu_k[1:])
     max_q = metadata.max_seqlen_q or max(metadata.q_lens_cpu, default=0)
-    return paged_prefill_mxfp4(query, key_pages, value_pages, cu_q, cu_k, block_tables,
-                               max_seqlen_q=max_q, total_k=_total_k(query, key_pages, metadata),
-                               scale=scale, max_seqlen_k=metadata.max_seqlen_k or None)
+    return prefill(query, key_pages, value_pages, cu_q, cu_k, block_tables, max_seqlen_q=max_q,
+                   total_k=_total_k(query, dims(key_pages, value_pages), metadata), scale=scale,
+                   max_seqlen_k=metadata.max_seqlen_k or None)
 
 
 # K and V rows of a gathered prefill that may be allocated for a bound on the contexts rather than their sum.
 _BOUND_BYTES = 256 << 20
 
 
-def _total_k(query, key_pages, metadata) -> int | None:
+def _total_k(query, dims, metadata) -> int | None:
     """The sum of the step's contexts, which sizes a gathered prefill, or a bound on it.
 
     Metadata that does not say costs one copy of the lengths to the host per step, which is
@@ -305,7 +310,7 @@ def _total_k(query, key_pages, metadata) -> int | None:
     if total:
         return total
     requests, width = metadata.block_tables.shape
-    _, bs, hkv, d = page_dims(key_pages, key_pages)
+    _, bs, hkv, d = dims
     bound = requests * (metadata.max_seqlen_k or width * bs)
     if (2 * bound * hkv * d * query.element_size() <= _BOUND_BYTES or torch.compiler.is_compiling()
             or (query.is_cuda and torch.cuda.is_current_stream_capturing())):

@@ -15,9 +15,11 @@ from __future__ import annotations
 
 import torch
 
+from microinfer_b200.layer import fp8_attention as _f8
 from microinfer_b200.layer import mxfp4_attention as _mx
 from microinfer_b200.layer import paged_attention as _pa
 from microinfer_b200.layer import prologue as _pro
+from microinfer_b200.worker import fp8_cache as _f8c
 from microinfer_b200.worker import kv_store as _store
 from microinfer_b200.worker import mxfp4_cache as _mxc
 
@@ -146,6 +148,47 @@ def paged_prefill_mxfp4(query: torch.Tensor, key_pages: torch.Tensor, value_page
 
 
 @paged_prefill_mxfp4.register_fake
+def _(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, max_seqlen_q,
+      total_k=None, scale=None, max_seqlen_k=None):
+    return query.new_empty(query.shape)  # contiguous, whatever the query's strides
+
+
+@torch.library.custom_op(f"{_NS}::store_kv_fp8", mutates_args=("key_pages", "value_pages"))
+def store_kv_fp8(key_pages: torch.Tensor, value_pages: torch.Tensor, slots: torch.Tensor,
+                 keys: torch.Tensor, values: torch.Tensor) -> None:
+    _f8c.store_kv_fp8(key_pages, value_pages, slots, keys, values)
+
+
+@store_kv_fp8.register_fake
+def _(key_pages, value_pages, slots, keys, values):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::paged_decode_fp8", mutates_args=())
+def paged_decode_fp8(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                     block_tables: torch.Tensor, context_lens: torch.Tensor,
+                     scale: float | None = None) -> torch.Tensor:
+    return _f8.paged_decode_fp8(query, key_pages, value_pages, block_tables, context_lens,
+                                scale=scale)
+
+
+@paged_decode_fp8.register_fake
+def _(query, key_pages, value_pages, block_tables, context_lens, scale=None):
+    return query.new_empty(query.shape)  # contiguous, whatever the query's strides
+
+
+@torch.library.custom_op(f"{_NS}::paged_prefill_fp8", mutates_args=())
+def paged_prefill_fp8(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                      cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                      block_tables: torch.Tensor, max_seqlen_q: int,
+                      total_k: int | None = None, scale: float | None = None,
+                      max_seqlen_k: int | None = None) -> torch.Tensor:
+    return _f8.paged_prefill_fp8(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k,
+                                 block_tables, max_seqlen_q=max_seqlen_q, total_k=total_k,
+                                 scale=scale, max_seqlen_k=max_seqlen_k)
+
+
+@paged_prefill_fp8.register_fake
 def _(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, max_seqlen_q,
       total_k=None, scale=None, max_seqlen_k=None):
     return query.new_empty(query.shape)  # contiguous, whatever the query's strides
