@@ -29,23 +29,24 @@ namespace {
 
 constexpr float kLift = 12.f;  // p is held as 2^(x - m + kLift)
 constexpr float kLag = 3.f;    // m may be this far behind: p <= 2^15
+constexpr float kExact = 0x1p20f;  // m up to here is off by 2^-4 at most
 constexpr int kNear = 7;       // binades below R that p takes in
 constexpr int kFactorMax = 94; // largest exponent of a score's first factor: sums of products are below 2^32, and the
                                // scale's mantissa below 2
 
-// NB blocks of 32 dims, CT column tiles of 8 columns (8 query heads, fp32 4).  As many warps as shared memory holds with
-// rings of two units.
+// Heads of a segment (CT column tiles of 8 columns: 8 query heads, fp32 4), and warps of a CTA: as many as shared memory
+// holds with rings of two units.
+constexpr int f8_heads(int columns, bool split) { return columns * (split ? 4 : 8); }
+constexpr int f8_warps(int head_dim, int columns, bool split) {
+  const int heads = f8_heads(columns, split);
+  const int per_warp = 2 * 4 * f8_group_bytes(head_dim) + heads * (head_dim + 2) * 4 + 64 * 16 + 2 * 8 + 24 + 2 * heads * 12;
+  const int fit = (227 * 1024 - (kMaxSeqs + 1) * 4 - 16) / per_warp;
+  return fit > 16 ? 16 : fit;
+}
+constexpr int kF8Slack = 3;  // units per warp that keeping a segment in one CTA may cost: the second launch costs as much
+// NB blocks of 32 dims.  q's fragments stay in registers.
 template <int NB, int CT, bool SPLIT>
-struct F8Shape {
-  static constexpr int kHeads = CT * (SPLIT ? 4 : 8);
-  static constexpr int kQuery = CT * NB * 512;
-  static constexpr int kPerWarp = 2 * 4 * f8_group_bytes(NB * 32) + kHeads * (NB * 32 + 2) * 4 + 64 * 16 + kQuery + 24 + 2 * kHeads * 12;
-  static constexpr int kFit = (227 * 1024 - (kMaxSeqs + 1) * 4 - 16) / kPerWarp;
-  static constexpr int kWarps = kFit > 16 ? 16 : kFit;
-};
-template <int NB, int CT, bool SPLIT>
-using F8Cfg = SegCfg<NB * 32, F8Shape<NB, CT, SPLIT>::kWarps, 2, F8Shape<NB, CT, SPLIT>::kHeads, f8_group_bytes(NB * 32),
-                     F8Shape<NB, CT, SPLIT>::kQuery>;
+using F8Cfg = SegCfg<NB * 32, f8_warps(NB * 32, CT, SPLIT), 2, f8_heads(CT, SPLIT), f8_group_bytes(NB * 32), 0>;
 
 __device__ __forceinline__ uint32_t lds8(uint32_t addr) {
   uint32_t r;
@@ -71,6 +72,8 @@ __device__ __forceinline__ void sts(uint32_t addr, const uint32_t (&w)[4]) {
 template <typename T, int NB, int CT>
 struct F8Warp {
   using Elem_ = T;
+  static constexpr int kSlack = kF8Slack;
+  static constexpr bool kBulk = true;
   static constexpr bool kSplit = std::is_same<T, float>::value;
   using C = F8Cfg<NB, CT, kSplit>;
   static constexpr int D = C::D;
@@ -79,18 +82,17 @@ struct F8Warp {
   static constexpr int kCodes = kF8Group * D;   // bytes of a group's codes
   static constexpr int kFull = NB / 2;          // parts of 64 dims
   static constexpr int kOut = 2 * NB;           // 16-dim tiles of O: part p's are 4p to 4p + 3, a last part of 32 has two
-  uint32_t q;             // shared address of this lane's B fragments of q: 4 words per 32 dims, 512 bytes between
-  int re[CT][kCols];      // exponent that takes a sum of products to the log2 domain, without K's scale
+  uint32_t q[CT][NB][4];  // this lane's B fragments of q
+  float unit[CT][kCols];  // takes a sum of products to the log2 domain, but for K's scale: 2^power * mantissa
+  int power[CT][kCols];
+  int top_byte[CT][kCols];  // of K's scales that may multiply it
   float mantissa;         // of the softmax's scale
   float o[CT][kOut][4];   // columns 2t and 2t + 1, dims 2i and 2i + 1 of the lane's in the part, times 2^(R - 127)
   float m[CT][kCols], l[CT][kCols];  // l: this lane's keys only
   int ref;                // R
   int lane, g, t;
 
-  __device__ __forceinline__ void setup(uint32_t query_smem) {
-    lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    q = query_smem + lane * 16;
-  }
+  __device__ __forceinline__ void setup(uint32_t) { lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3; }
 
   __device__ __forceinline__ void reset() {
     ref = 0;
@@ -125,13 +127,12 @@ struct F8Warp {
   }
   // ... as f16 fragments.
   __device__ __forceinline__ void set_query(const Raw &raw, float scale_log2) {
-    const uint32_t bits = __float_as_uint(scale_log2);
-    int scale_exp = static_cast<int>(bits >> 23 & 255u) - 127;
-    mantissa = __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
-    if ((bits & 0x7fffffffu) < 0x00800000u || (bits & 0x7f800000u) == 0x7f800000u) {  // 0, below normal, not finite
-      scale_exp = 0;
-      mantissa = scale_log2;
-    }
+    // the scale's sign goes into q, so that the largest product is the largest score; a scale of 0 becomes one that leaves
+    // every score at 0
+    const float scale = fmaxf(fabsf(scale_log2), 1e-30f);
+    const bool whole = scale < INFINITY;
+    const int scale_exp = whole ? static_cast<int>(__float_as_uint(scale) >> 23) - 127 : 0;
+    mantissa = whole ? __uint_as_float((__float_as_uint(scale) & 0x7fffffu) | 0x3f800000u) : scale;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float x[NB][8];
@@ -159,7 +160,7 @@ struct F8Warp {
       int e = 14 - (static_cast<int>(top >> 23) - 127);  // largest element to [2^14, 2^15)
       if (top >= 0x7f800000u) e = 0;                     // not finite: as it is
       e = min(e, 126);
-      const float f = exp2i(e);
+      const float f = exp2i(e) * (scale_log2 < 0.f ? -1.f : 1.f);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -167,15 +168,17 @@ struct F8Warp {
           x[b][i] *= f;
           if (kSplit && (g & 1)) x[b][i] -= __half2float(__float2half_rn(x[b][i]));  // what the other column leaves
         }
-        // read by this lane alone
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q + (c * NB + b) * 512),
-                     "r"(pack_f16(x[b][0], x[b][1])), "r"(pack_f16(x[b][2], x[b][3])),
-                     "r"(pack_f16(x[b][4], x[b][5])), "r"(pack_f16(x[b][6], x[b][7]))
-                     : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[c][b][i] = pack_f16(x[b][2 * i], x[b][2 * i + 1]);
       }
 #pragma unroll
-      for (int u = 0; u < kCols; ++u)  // a lane of this query head: its column is 2t + u
-        re[c][u] = scale_exp - __shfl_sync(kAll, e, 4 * (2 * t + u));
+      for (int u = 0; u < kCols; ++u) {  // a lane of this query head: its column is 2t + u
+        const int e2 = scale_exp - __shfl_sync(kAll, e, 4 * (2 * t + u));
+        power[c][u] = e2;
+        const bool normal = e2 >= -126 && e2 <= kFactorMax;
+        unit[c][u] = __uint_as_float(static_cast<uint32_t>((normal ? e2 : 0) + 127) << 23) * mantissa;
+        top_byte[c][u] = normal ? kFactorMax + 127 - e2 : -1;
+      }
     }
   }
 
@@ -191,9 +194,6 @@ struct F8Warp {
     }
 #pragma unroll
     for (int b = 0; b < W / 2; ++b) {
-      uint32_t f[CT][4];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) lds<4>(q + (c * NB + 2 * part + b) * 512, f[c]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -202,13 +202,14 @@ struct F8Warp {
           f8_to_f16(lo[j][2 * b + i], a[0], a[2]);
           f8_to_f16(hi[j][2 * b + i], a[1], a[3]);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) mma_f16(d[j][c], a[0], a[1], a[2], a[3], f[c][2 * i], f[c][2 * i + 1]);
+          for (int c = 0; c < CT; ++c) mma_f16(d[j][c], a[0], a[1], a[2], a[3], q[c][2 * part + b][2 * i], q[c][2 * part + b][2 * i + 1]);
         }
     }
   }
 
-  // Scores of a unit's 32 keys, log2 domain: x[j][c][r][u], key g + 8r of group j, query head kCols * t + u of tile c.
-  __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[2][CT][2][kCols]) const {
+  // Sums of products of a unit's 32 keys: x[j][c][r][u], key g + 8r of group j, query head kCols * t + u of tile c; and the
+  // factors that make them scores in the log2 domain.
+  __device__ __forceinline__ void scores(uint32_t kbase, float (&x)[2][CT][2][kCols], float (&factor)[2][CT][kCols]) const {
     float d[2][CT][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -224,15 +225,15 @@ struct F8Warp {
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int u = 0; u < kCols; ++u) {
-          const int e = static_cast<int>(byte[j]) - 127 + re[c][u];
-          const int near = max(-126, min(kFactorMax, e));  // further down every score is 0
-          const float f = __uint_as_float(static_cast<uint32_t>(near + 127) << 23) * mantissa;
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            x[j][c][r][u] = (kSplit ? d[j][c][2 * r] + d[j][c][2 * r + 1] : d[j][c][2 * r + u]) * f;
-          if (e > kFactorMax) {
-            const float more = exp2i(e - kFactorMax);
-            x[j][c][0][u] *= more, x[j][c][1][u] *= more;
+          x[j][c][0][u] = kSplit ? d[j][c][0] + d[j][c][1] : d[j][c][u];
+          x[j][c][1][u] = kSplit ? d[j][c][2] + d[j][c][3] : d[j][c][2 + u];
+          // further down every score is 0; not 0 itself, which a masked score would make a NaN
+          factor[j][c][u] = fmaxf(f8_scale(byte[j]) * unit[c][u], 0x1p-126f);
+          if (static_cast<int>(byte[j]) > top_byte[c][u]) {  // hardly ever
+            const int e = static_cast<int>(byte[j]) - 127 + power[c][u], near = max(-126, min(kFactorMax, e));
+            factor[j][c][u] = __uint_as_float(static_cast<uint32_t>(near + 127) << 23) * mantissa;
+            const float f = exp2i(max(0, e - kFactorMax));
+            x[j][c][0][u] *= f, x[j][c][1][u] *= f;
           }
         }
   }
@@ -293,8 +294,8 @@ struct F8Warp {
   // that may be fewer than 16, or it is the `first` that the state meets.
   __device__ __forceinline__ void process(uint32_t base, bool special, int valid0, int valid1, bool first) {
     const uint32_t vbase = base + 2 * C::kGroup;
-    float x[2][CT][2][kCols];
-    scores(base, x);
+    float x[2][CT][2][kCols], factor[2][CT][kCols];
+    scores(base, x, factor);
     int byte[2] = {static_cast<int>(lds8(vbase + kCodes)), static_cast<int>(lds8(vbase + C::kGroup + kCodes))};
     if (special) {  // uniform
 #pragma unroll
@@ -309,6 +310,7 @@ struct F8Warp {
             if (g + 8 >= valid) x[j][c][1][u] = -INFINITY;
           }
         clear_values(vbase + j * C::kGroup, valid);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the copies that overwrite it
         if (valid <= 0) byte[j] = 0;
       }
       if (first) ref = max(byte[0], byte[1]) + 2;  // two binades of room
@@ -320,7 +322,8 @@ struct F8Warp {
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int u = 0; u < kCols; ++u) {
-        top[c][u] = fmaxf(fmaxf(x[0][c][0][u], x[0][c][1][u]), fmaxf(x[1][c][0][u], x[1][c][1][u]));
+        top[c][u] = fmaxf(fmaxf(x[0][c][0][u], x[0][c][1][u]) * factor[0][c][u],
+                          fmaxf(x[1][c][0][u], x[1][c][1][u]) * factor[1][c][u]);
         behind |= top[c][u] > m[c][u] + kLag;
       }
     if (__any_sync(kAll, behind)) {
@@ -363,6 +366,23 @@ struct F8Warp {
     uint32_t p[2][CT][2];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
+      float lift[kCols];
+      bool large = false;
+#pragma unroll
+      for (int u = 0; u < kCols; ++u) {
+        lift[u] = kLift - m[c][u];
+        large |= fabsf(m[c][u]) > kExact;
+      }
+      if (large) {  // m rounds away more than p may be off by: the products round as it did, and m goes at once
+#pragma unroll
+        for (int u = 0; u < kCols; ++u) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i / 2][c][i % 2][u] = __fmul_rn(x[i / 2][c][i % 2][u], factor[i / 2][c][u]) - m[c][u];
+          factor[0][c][u] = factor[1][c][u] = 1.f;
+          lift[u] = kLift;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -370,7 +390,7 @@ struct F8Warp {
           float w[2];
 #pragma unroll
           for (int u = 0; u < kCols; ++u) {
-            w[u] = fast_exp2((x[j][c][r][u] - m[c][u]) + kLift);  // in this order: at most 2^15 however large the scores
+            w[u] = fast_exp2(fmaf(x[j][c][r][u], factor[j][c][u], lift[u]));
             l[c][u] += w[u];
             w[u] *= near[j];
           }
@@ -482,19 +502,17 @@ cudaError_t launch_f8(const CodedDecodeParams &p, int tiles, bool join, int ctas
                                             join, ctas, stream);
 }
 
-// Query heads of a column tile, column tiles of a segment (two rings' worth of sums do not fit past D = 128), and segments
-// of a kv head.
-int f8_tile_heads(int dtype) { return dtype == MI_DTYPE_FLOAT32 ? 4 : 8; }
-int f8_columns(int group, int head_dim, int dtype) { return group <= f8_tile_heads(dtype) || head_dim > 128 ? 1 : 2; }
-int f8_tiles(int group, int head_dim, int dtype) {
-  const int heads = f8_tile_heads(dtype) * f8_columns(group, head_dim, dtype);
+// Column tiles of a segment (two rings' worth of sums do not fit past D = 128), and segments of a kv head.
+int f8_columns(int group, int head_dim, bool split) { return group <= f8_heads(1, split) || head_dim > 128 ? 1 : 2; }
+int f8_tiles(int group, int head_dim, bool split) {
+  const int heads = f8_heads(f8_columns(group, head_dim, split), split);
   return (group + heads - 1) / heads;
 }
 
-bool f8_joins(int64_t segments, int head_dim, int64_t capacity, int sms) {
-  constexpr int kWide = F8Shape<8, 1, false>::kWarps, kOther = F8Shape<4, 2, false>::kWarps;  // the fewest
-  static_assert(kWide <= F8Shape<8, 1, true>::kWarps && kOther <= F8Shape<4, 2, true>::kWarps, "of both types");
-  return segments_join(segments, capacity, head_dim > 128 ? kWide : kOther, sms);
+bool f8_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, bool split, int64_t capacity, int sms) {
+  const int group = num_q_heads / num_kv_heads;
+  return segments_join(num_seqs * num_kv_heads * f8_tiles(group, head_dim, split), capacity,
+                       kF8Slack * f8_warps(head_dim, f8_columns(group, head_dim, split), split), sms);
 }
 
 template <typename T>
@@ -520,23 +538,25 @@ cudaError_t launch_f8_t(const CodedDecodeParams &p, int tiles, int columns, bool
 
 bool fp8_decode_supported(int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t num_blocks, int block_size,
                           int64_t capacity) {
-  return segments_supported(static_cast<int64_t>(num_kv_heads) * f8_tiles(num_q_heads / num_kv_heads, head_dim, dtype),
-                            num_kv_heads, num_blocks, block_size, capacity);
+  const int tiles = f8_tiles(num_q_heads / num_kv_heads, head_dim, dtype == MI_DTYPE_FLOAT32);
+  return segments_supported(static_cast<int64_t>(num_kv_heads) * tiles, num_kv_heads, num_blocks, block_size, capacity);
 }
 
 size_t fp8_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                             int64_t capacity, int sms) {
-  const int group = num_q_heads / num_kv_heads;
+  const bool split = dtype == MI_DTYPE_FLOAT32;
   sms = segment_ctas(sms);
-  if (!f8_joins(num_seqs * num_kv_heads * f8_tiles(group, head_dim, dtype), head_dim, capacity, sms)) return 0;
-  return segment_workspace(f8_tile_heads(dtype) * f8_columns(group, head_dim, dtype), head_dim, sms);
+  if (!f8_joins(num_seqs, num_q_heads, num_kv_heads, head_dim, split, capacity, sms)) return 0;
+  return segment_workspace(f8_heads(f8_columns(num_q_heads / num_kv_heads, head_dim, split), split), head_dim, sms);
 }
 
 cudaError_t launch_fp8_decode(const CodedDecodeParams &p, int dtype, cudaStream_t stream) {
   const int group = p.num_q_heads / p.num_kv_heads;
-  const int tiles = f8_tiles(group, p.head_dim, dtype), columns = f8_columns(group, p.head_dim, dtype);
+  const bool split = dtype == MI_DTYPE_FLOAT32;
+  const int tiles = f8_tiles(group, p.head_dim, split), columns = f8_columns(group, p.head_dim, split);
   const int sms = segment_ctas(sm_count_current());
-  const bool join = f8_joins(p.num_seqs * p.num_kv_heads * tiles, p.head_dim, p.bt_stride * p.block_size, sms);
+  const bool join =
+      f8_joins(p.num_seqs, p.num_q_heads, p.num_kv_heads, p.head_dim, split, p.bt_stride * p.block_size, sms);
   return launch_segment_slices(p, tiles, dtype, [&](const CodedDecodeParams &q) {
     return dtype == MI_DTYPE_BFLOAT16 ? launch_f8_t<__nv_bfloat16>(q, tiles, columns, join, sms, stream)
            : dtype == MI_DTYPE_FLOAT16  ? launch_f8_t<__half>(q, tiles, columns, join, sms, stream)

@@ -170,6 +170,8 @@ template <typename T, int NB, int CT>
 struct MxWarp {
   static constexpr bool kSplit = std::is_same<T, float>::value;
   using Elem_ = T;
+  static constexpr int kSlack = 1;
+  static constexpr bool kBulk = false;
   using C = MxCfg<NB, CT, kSplit>;
   static constexpr int D = C::D;
   static constexpr int kParts = kSplit ? 2 : 1;  // f16 parts of p
@@ -679,6 +681,7 @@ int mma_tiles(int num_q_heads, int num_kv_heads, int head_dim) {
 
 bool mma_joins(int64_t num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int64_t capacity, int sms) {
   const int64_t segments = num_seqs * num_kv_heads * mma_tiles(num_q_heads, num_kv_heads, head_dim);
+  // the fewest warps of a CTA, at a slack of one unit each
   return segments_join(segments, capacity, head_dim > 128 ? MxCfg<8, 1, true>::kWarps : MxCfg<4, 2, true>::kWarps, sms);
 }
 

@@ -5,6 +5,8 @@
 // (a sequence, kv head and up to C::kHeads of its query heads):
 //   W::C                      SegCfg of the format and shape
 //   W::Elem_                  type of query and out
+//   W::kSlack                 units per warp that keeping a segment in one CTA may cost
+//   W::kBulk                  whether a lane fills the ring by bulk copies, or all by 16-byte ones
 //   setup(shared address of C::kQuery bytes), fetch_query(), set_query(), reset()
 //   process(base, special, valid0, valid1, first): one unit of 32 keys, K of its two groups at `base`, then V of both
 //   finish(), write_out(), write_state(): the mean of V over the keys seen, and m and l
@@ -12,7 +14,7 @@
 // Work: the units of 32 keys of all segments, in that order, are one list that is cut into equal ranges, one per
 // warp (one CTA to an SM), so ragged batches and single long
 // sequences load every SM alike.  A warp streams its range through a ring of its own, a few units
-// deep, that runs across segment borders.  Its lanes fill it with 16-byte cp.async.  Segments that lie within one
+// deep, that runs across segment borders.  Segments that lie within one
 // warp's range are written at once; the parts of others are joined in shared
 // memory, and those that cross CTAs by a second launch, whose order is fixed.
 // When every segment fits a CTA at hardly more work per warp, each CTA takes one
@@ -36,7 +38,6 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr int kSegGroup = 16;           // tokens of a group
 constexpr int kUnit = 2 * kSegGroup;    // keys of a unit of work
 constexpr int kMaxSeqs = 2048;          // sequences of one launch (prefix sums in shared memory)
-constexpr int kAlignedSlack = 1;        // units per warp that keeping a segment in one CTA may cost
 
 // Shared memory of a CTA of WARPS warps, each with a ring of STAGES units of GROUP-byte groups and QUERY bytes for q.
 template <int D_, int WARPS, int STAGES, int HEADS, int GROUP, int QUERY>
@@ -54,9 +55,10 @@ struct SegCfg {
   static constexpr int kSmemUnits = kWarps * 64 * 16;     // two batches of 32 units per warp
   static constexpr int kQuery = QUERY;                    // q's fragments, per warp
   static constexpr int kSmemQuery = kWarps * kQuery;
+  static constexpr int kSmemBars = kWarps * kStages * 8;  // bulk copies: a barrier to a stage
   static constexpr int kSmemPrefix = (kMaxSeqs + 1) * 4;
   static constexpr int kSmemMisc = 6 * kWarps * 4 + 2 * kWarps * kHeads * 12 + 16;
-  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemQuery + kSmemPrefix +
+  static constexpr int kSmem = kSmemRing + kSmemHeads + kSmemUnits + kSmemQuery + kSmemBars + kSmemPrefix +
                                kSmemMisc;
   static_assert(kState * 4 <= kRing, "a warp's last part goes into its own ring");
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -122,8 +124,10 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
   extern __shared__ __align__(128) uint8_t smem[];
   float *heads_smem = reinterpret_cast<float *>(smem + C::kSmemRing);
   int4 *unit_table = reinterpret_cast<int4 *>(smem + C::kSmemRing + C::kSmemHeads);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery) +
+                   (threadIdx.x >> 5) * C::kStages;
   int *prefix =
-      reinterpret_cast<int *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery);  // units of a segment before sequence s
+      reinterpret_cast<int *>(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + C::kSmemQuery + C::kSmemBars);  // units of a segment before sequence s
   int *part_seg = prefix + kMaxSeqs + 1;   // [2 * kWarps]: first and last part of each warp, -1: none
   int *part_flags = part_seg + 2 * kWarps;  // 1: has the segment's first group, 2: its last
   int *scan = part_flags + 2 * kWarps;      // [2 * kWarps]
@@ -137,6 +141,14 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
   const int G = p.num_q_heads / p.num_kv_heads;
   const int tiles = plan.tiles, H = p.num_kv_heads * tiles;  // segments of a sequence
 
+  if constexpr (W::kBulk) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  }
   pdl_wait();
 
   // ---- units of each sequence, their prefix sums and largest ----
@@ -214,7 +226,7 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
   const uint32_t share = plan.by_ctas.div(total), over = total - share * gridDim.x;  // `over` CTAs take one more
   uint32_t u0, cta_units;
   if (static_cast<uint32_t>(n) * H <= gridDim.x &&
-      static_cast<uint32_t>(c_max) <= share + (over != 0) + kAlignedSlack * kWarps) {
+      static_cast<uint32_t>(c_max) <= share + (over != 0) + W::kSlack * kWarps) {
     const int s = static_cast<int>(plan.by_segments.div(blockIdx.x));  // one segment to a CTA
     cta_units = s < n ? prefix[s + 1] - prefix[s] : 0;
     u0 = s < n ? static_cast<uint32_t>(prefix[s]) * H + (blockIdx.x - s * H) * cta_units : 0;
@@ -304,6 +316,17 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
   };
   auto issue = [&](int i, int at) {
     const int2 where = *reinterpret_cast<const int2 *>(table + (i & 63));
+    if constexpr (W::kBulk) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bars + at, C::kStage);
+#pragma unroll
+        for (int run = 0; run < 4; ++run)
+          bulk_g2s(ring + at * C::kStage + run * C::kGroup,
+                   (run & 2 ? p.value_pages : p.key_pages) + static_cast<int64_t>(run & 1 ? where.y : where.x) * C::kGroup,
+                   C::kGroup, bars + at);
+      }
+      return;
+    }
     const uint32_t to = my_place + at * C::kStage;
 #pragma unroll
     for (int run = 0; run < 4; ++run) {
@@ -316,7 +339,19 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
       copy16(my_left_place + at * C::kStage,
              my_left + static_cast<int64_t>(left_run & 1 ? where.y : where.x) * C::kGroup);
   };
-  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  auto commit = [] {
+    if constexpr (!W::kBulk) asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // Whether unit i has come to stage `at` (else the status says so).
+  auto arrived = [&](int i, int at) {
+    if constexpr (W::kBulk) {
+      return mbar_wait_bounded(bars + at, i / kStages & 1, p.status);
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");  // this lane's copies
+      __syncwarp();                                                         // every lane's
+      return true;
+    }
+  };
 
   W st;
   st.setup(smem_addr(smem + C::kSmemRing + C::kSmemHeads + C::kSmemUnits + warp * C::kQuery));
@@ -377,8 +412,10 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
       st.reset();
       fresh = true;
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");  // this lane's copies of unit i
-    __syncwarp();                                                         // every lane's
+    if (!arrived(i, stage)) {
+      for (int k = i + 1; k < min(units, i + kStages); ++k) arrived(k, k % kStages);  // nothing is on its way at the end
+      break;
+    }
     const bool special = what != kUnit || fresh;
     const int valid = what & 63, valid0 = what & kNoPage ? 0 : min(valid, kSegGroup), valid1 = valid - kSegGroup;
     if (valid0 > 0 || valid1 > 0) {
@@ -602,9 +639,9 @@ cudaError_t launch_segments(void (*kern)(CodedDecodeParams, SegPlan), void (*joi
 int segment_ctas(int sms) { return sms < kMaxCtas ? sms : kMaxCtas; }
 
 // Whether some lengths that the table can hold need the second launch: not when
-// every segment has a CTA and a full table is no more than the slack per warp (`warps`: the fewest of a CTA).
-bool segments_join(int64_t segments, int64_t capacity, int warps, int sms) {
-  return segments > sms || capacity > static_cast<int64_t>(kAlignedSlack) * warps * kUnit;
+// every segment has a CTA and a full table is no more than `aligned` units.
+bool segments_join(int64_t segments, int64_t capacity, int aligned, int sms) {
+  return segments > sms || capacity > static_cast<int64_t>(aligned) * kUnit;
 }
 
 size_t segment_workspace(int heads, int head_dim, int sms) {
