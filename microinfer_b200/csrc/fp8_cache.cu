@@ -85,11 +85,19 @@ __device__ __forceinline__ void separate(uint4 v, uint2 &a, uint2 &b) {
   a = make_uint2(__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.z, v.w, 0x6420));
   b = make_uint2(__byte_perm(v.x, v.y, 0x7531), __byte_perm(v.z, v.w, 0x7531));
 }
+// WHOLE: the 16 bytes of 8 dims of a pair lie together.
+template <bool WHOLE>
 __device__ __forceinline__ uint4 read_pair(const uint8_t *at, int split) {
+  if constexpr (WHOLE) return *reinterpret_cast<const uint4 *>(at);
   const uint2 lo = *reinterpret_cast<const uint2 *>(at), hi = *reinterpret_cast<const uint2 *>(at + split);
   return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
+template <bool WHOLE>
 __device__ __forceinline__ void write_pair(uint8_t *at, int split, uint4 v) {
+  if constexpr (WHOLE) {
+    *reinterpret_cast<uint4 *>(at) = v;
+    return;
+  }
   *reinterpret_cast<uint2 *>(at) = make_uint2(v.x, v.y);
   *reinterpret_cast<uint2 *>(at + split) = make_uint2(v.z, v.w);
 }
@@ -115,6 +123,7 @@ __device__ __forceinline__ void store_group(const CodedStoreParams &p, uint8_t *
   const bool fresh = member[0] >= 0;
   const uint32_t old = fresh ? 0u : group[kF8Group * D];
   constexpr int kHeld = NB > 0 ? NB : 1;
+  constexpr bool kWhole = NB > 0 && NB % 2 == 0;
   Raw8<T> x[kHeld][2];
   // item i of a lane: 8 dims of a pair of tokens
   auto pair_of = [&](int i) { return (i * 32 + lane) / octets; };
@@ -127,38 +136,48 @@ __device__ __forceinline__ void store_group(const CodedStoreParams &p, uint8_t *
       if (t >= 0) load8<T, VEC>(rows + t * stride + octet_of(i) * 8, v[k]);
     }
   };
-  uint32_t top = 0, finite = 0;  // largest magnitude as bits (NaN above infinity), and the largest finite one
-  auto look = [&](const Raw8<T> (&v)[2], bool all) {
+  // Largest magnitude as bits of T, which order like the values with NaN above infinity; 16-bit ones two to a word, never
+  // unpacked for it.  Where something is not finite, once more without that.
+  constexpr uint32_t kMask = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+  constexpr uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  uint32_t top = 0;
+  auto larger = [](uint32_t u, uint32_t v) { return sizeof(T) == 2 ? __vmaxu2(u, v) : max(u, v); };
+  auto look = [&](const Raw8<T> (&v)[2], bool finite) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float f[8];
-      unpack8(v[k], f);
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const uint32_t bits = __float_as_uint(f[u]) & 0x7fffffffu;
-        top = max(top, bits);
-        if (!all) finite = max(finite, bits < 0x7f800000u ? bits : 0u);
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+        const uint32_t w[4] = {v[k].v[i].x, v[k].v[i].y, v[k].v[i].z, v[k].v[i].w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint32_t bits = w[u] & kMask;
+          if (finite) bits &= sizeof(T) == 2 ? __vcmpltu2(bits, kInf) : bits < kInf ? ~0u : 0u;
+          top = larger(top, bits);
+        }
       }
-    }
   };
   if constexpr (NB > 0) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) read(i, x[i]);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) look(x[i], true);
-    if (__any_sync(kAll, top >= 0x7f800000u)) {
+    for (int i = 0; i < NB; ++i) look(x[i], false);
+    const bool all = sizeof(T) == 2 ? __vcmpltu2(top, kInf) == ~0u : top < kInf;
+    if (__any_sync(kAll, !all)) {
+      top = 0;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) look(x[i], false);
-    } else {
-      finite = top;
+      for (int i = 0; i < NB; ++i) look(x[i], true);
     }
   } else {
     for (int i = 0; i < items; ++i) {
       read(i, x[0]);
-      look(x[0], false);
+      look(x[0], true);
     }
   }
-  const uint32_t need = f8_byte_for(__reduce_max_sync(kAll, finite));
+  if constexpr (sizeof(T) == 2) {
+    const uint16_t most = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
+    top = __float_as_uint(Elem<T>::to_float(*reinterpret_cast<const T *>(&most)));
+  }
+  const uint32_t need = f8_byte_for(__reduce_max_sync(kAll, top));
   const uint32_t byte = max(need, old);
   const bool grown = !fresh && byte > old;
   const float inverse = byte == 0 ? 1.f : __uint_as_float((254u - byte) << 23);
@@ -180,14 +199,14 @@ __device__ __forceinline__ void store_group(const CodedStoreParams &p, uint8_t *
       uint8_t *to = group + at.v + (pair >> 2) * at.half + (pair & 3) * at.pair;
       if (!(in[0] && in[1])) {
         uint2 was[2];
-        separate(read_pair(to, at.split), was[0], was[1]);
+        separate(read_pair<kWhole>(to, at.split), was[0], was[1]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (in[k]) continue;
           w[k] = grown ? make_uint2(rescale4(was[k].x, factor), rescale4(was[k].y, factor)) : was[k];
         }
       }
-      write_pair(to, at.split, interleave(w[0], w[1]));
+      write_pair<kWhole>(to, at.split, interleave(w[0], w[1]));
     } else {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -216,12 +235,24 @@ __device__ __forceinline__ void store_group(const CodedStoreParams &p, uint8_t *
 
 // A CTA per token (SCAN) or per chunk of tokens, and 8 of the kv heads' operands, one to a warp.
 template <typename T, bool VEC, int NB, bool SCAN>
-__global__ void __launch_bounds__(256) fp8_store_kernel(const CodedStoreParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) fp8_store_kernel(const CodedStoreParams p) {
   constexpr int kTokens = SCAN ? 1 : kChunk;
   __shared__ int32_t member[kTokens][kF8Group];
   __shared__ int64_t owned[kTokens];  // groups of the pool
   __shared__ int num_owned;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int operand = blockIdx.y * 8 + warp, head = operand >> 1;
+  // The chunk's rows are on their way into L2 while it finds out where they go.
+  if (head < p.num_kv_heads) {
+    constexpr int kLine = 128;
+    const int row_bytes = p.head_dim * static_cast<int>(sizeof(T)), lines = (row_bytes + kLine - 1) / kLine;
+    for (int i = lane; i < kTokens * lines; i += 32) {
+      const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + i / lines;
+      const char *row = reinterpret_cast<const char *>(static_cast<const T *>(operand & 1 ? p.values : p.keys) +
+                                                       t * (operand & 1 ? p.value_stride : p.key_stride) + head * p.head_dim);
+      if (t < p.num_tokens) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i % lines * kLine));
+    }
+  }
   pdl_wait();
   if constexpr (SCAN) {
     const int64_t t = blockIdx.x;
@@ -254,7 +285,10 @@ __global__ void __launch_bounds__(256) fp8_store_kernel(const CodedStoreParams p
       if (good) {
         const int64_t first = slot - slot % kF8Group;
 #pragma unroll
-        for (int j = 0; j < kF8Group; ++j) entry[j] = __ldcg(p.index + first + j);
+        for (int j = 0; j < kF8Group; j += 4) {
+          const int4 v = __ldcg(reinterpret_cast<const int4 *>(p.index + first + j));
+          entry[j] = v.x, entry[j + 1] = v.y, entry[j + 2] = v.z, entry[j + 3] = v.w;
+        }
         int32_t least = INT32_MAX;
 #pragma unroll
         for (int j = 0; j < kF8Group; ++j) {
@@ -276,7 +310,6 @@ __global__ void __launch_bounds__(256) fp8_store_kernel(const CodedStoreParams p
     __syncthreads();
   }
   const int per_page = p.block_size / kF8Group, bytes = f8_group_bytes(p.head_dim);
-  const int operand = blockIdx.y * 8 + warp, head = operand >> 1;
   if (head < p.num_kv_heads)
     for (int i = 0; i < num_owned; ++i) {
       const int64_t page = owned[i] / per_page;
@@ -362,6 +395,7 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const CodedGatherParams
   const float ks = f8_scale(kbyte), vs = f8_scale(vbyte);
   const bool far = REDO && std::is_same<T, __half>::value && max(kbyte, vbyte) >= 127u + 8u;  // 448 * 2^7 < 65504
   constexpr int kHeld = NB > 0 ? NB : 1;
+  constexpr bool kWhole = NB > 0 && NB % 2 == 0;
   for (int i0 = 0; i0 < items; i0 += kHeld) {
     uint2 kw[kHeld][2];
     uint4 vw[kHeld];
@@ -372,7 +406,7 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const CodedGatherParams
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         kw[u][k] = __ldg(reinterpret_cast<const uint2 *>(kg + at.k + (2 * pair + k) * at.row));
-      vw[u] = read_pair(vg + at.v + (pair >> 2) * at.half + (pair & 3) * at.pair, at.split);
+      vw[u] = read_pair<kWhole>(vg + at.v + (pair >> 2) * at.half + (pair & 3) * at.pair, at.split);
     }
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
