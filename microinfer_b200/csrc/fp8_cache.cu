@@ -29,7 +29,7 @@ namespace mi {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
-constexpr int kChunk = 16;       // tokens of a CTA that finds groups by the index
+constexpr int kChunk = 256;      // tokens of a CTA that finds groups by the index, at most
 constexpr int kScanTokens = 512; // calls up to this long look through the slots instead
 
 // Eight elements of a row as they are in memory.
@@ -233,31 +233,35 @@ __device__ __forceinline__ void store_group(const CodedStoreParams &p, uint8_t *
   if (lane == 0 && (fresh || grown)) group[kF8Group * D] = static_cast<uint8_t>(byte);
 }
 
-// A CTA per token (SCAN) or per chunk of tokens, and 8 of the kv heads' operands, one to a warp.
+// 128-byte lines of one operand's row of a head, into L2.
+template <typename T>
+__device__ __forceinline__ void prefetch_row(const T *row, int head_dim, int part, int parts) {
+  const char *from = reinterpret_cast<const char *>(row);
+  for (int at = part * 128; at < head_dim * static_cast<int>(sizeof(T)); at += parts * 128)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
+}
+
+// A CTA takes one token (SCAN) or `chunk` of them, at most kChunk, and 8 of the kv heads' operands, one to a warp.  Rows are on their
+// way into L2 while the CTA finds out where the first of them go, and while the group before theirs is worked on.
 template <typename T, bool VEC, int NB, bool SCAN>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) fp8_store_kernel(const CodedStoreParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) fp8_store_kernel(const CodedStoreParams p, int chunk) {
   constexpr int kTokens = SCAN ? 1 : kChunk;
   __shared__ int32_t member[kTokens][kF8Group];
   __shared__ int64_t owned[kTokens];  // groups of the pool
   __shared__ int num_owned;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int operand = blockIdx.y * 8 + warp, head = operand >> 1;
-  // The chunk's rows are on their way into L2 while it finds out where they go.
+  const T *rows = static_cast<const T *>(operand & 1 ? p.values : p.keys) + head * p.head_dim;
+  const int64_t stride = operand & 1 ? p.value_stride : p.key_stride;
+  const int64_t first = SCAN ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * chunk;
   if (head < p.num_kv_heads) {
-    constexpr int kLine = 128;
-    const int row_bytes = p.head_dim * static_cast<int>(sizeof(T)), lines = (row_bytes + kLine - 1) / kLine;
-    for (int i = lane; i < kTokens * lines; i += 32) {
-      const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokens + i / lines;
-      const char *row = reinterpret_cast<const char *>(static_cast<const T *>(operand & 1 ? p.values : p.keys) +
-                                                       t * (operand & 1 ? p.value_stride : p.key_stride) + head * p.head_dim);
-      if (t < p.num_tokens) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i % lines * kLine));
-    }
+    const int64_t t = first + (lane >> 1);
+    if (t < p.num_tokens && (!SCAN || lane < 2)) prefetch_row(rows + t * stride, p.head_dim, lane & 1, 2);
   }
   pdl_wait();
   if constexpr (SCAN) {
-    const int64_t t = blockIdx.x;
     if (threadIdx.x < kF8Group) member[0][threadIdx.x] = -1;
-    const int64_t slot = slot_at(p, t);
+    const int64_t slot = slot_at(p, first);
     const bool good = slot >= 0 && slot < p.num_slots;
     if (!good && slot != -1 && threadIdx.x == 0) flag_status(p.status, MI_DEV_BAD_SLOT);
     __syncthreads();
@@ -267,51 +271,49 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) fp8_store_kernel(
         const int64_t s = slot_at(p, i);
         if (s >= 0 && s / kF8Group == slot / kF8Group) {
           atomicMax(&member[0][s % kF8Group], i);
-          earlier |= i < t;
+          earlier |= i < first;
         }
       }
     if (__syncthreads_or(earlier) || !good) return;
     if (threadIdx.x == 0) num_owned = 1, owned[0] = slot / kF8Group;
-    __syncthreads();
   } else {
-    if (warp == 0) {
-      const int64_t t = static_cast<int64_t>(blockIdx.x) * kChunk + lane;
-      const bool mine = lane < kChunk && t < p.num_tokens;
-      const int64_t slot = mine ? slot_at(p, t) : -1;
-      const bool good = slot >= 0 && slot < p.num_slots;
-      if (!good && slot != -1) flag_status(p.status, MI_DEV_BAD_SLOT);
-      int32_t entry[kF8Group];
-      bool owner = false;
-      if (good) {
-        const int64_t first = slot - slot % kF8Group;
+    if (threadIdx.x == 0) num_owned = 0;
+    __syncthreads();
+    const int64_t t = first + threadIdx.x;
+    const bool mine = threadIdx.x < chunk && t < p.num_tokens;
+    const int64_t slot = mine ? slot_at(p, t) : -1;
+    const bool good = slot >= 0 && slot < p.num_slots;
+    if (!good && slot != -1) flag_status(p.status, MI_DEV_BAD_SLOT);
+    if (good) {
+      const int64_t base = slot - slot % kF8Group;
+      int32_t entry[kF8Group], least = INT32_MAX;
 #pragma unroll
-        for (int j = 0; j < kF8Group; j += 4) {
-          const int4 v = __ldcg(reinterpret_cast<const int4 *>(p.index + first + j));
-          entry[j] = v.x, entry[j + 1] = v.y, entry[j + 2] = v.z, entry[j + 3] = v.w;
-        }
-        int32_t least = INT32_MAX;
-#pragma unroll
-        for (int j = 0; j < kF8Group; ++j) {
-          const bool there = entry[j] >= 0 && entry[j] < p.num_tokens && slot_at(p, entry[j]) == first + j;
-          entry[j] = there ? entry[j] : -1;
-          if (there) least = min(least, entry[j]);
-        }
-        owner = least == t;
+      for (int j = 0; j < kF8Group; j += 4) {
+        const int4 v = __ldcg(reinterpret_cast<const int4 *>(p.index + base + j));
+        entry[j] = v.x, entry[j + 1] = v.y, entry[j + 2] = v.z, entry[j + 3] = v.w;
       }
-      const unsigned owners = __ballot_sync(kAll, owner);
-      if (owner) {
-        const int at = __popc(owners & ((1u << lane) - 1u));
+#pragma unroll
+      for (int j = 0; j < kF8Group; ++j) {
+        const bool there = entry[j] >= 0 && entry[j] < p.num_tokens && slot_at(p, entry[j]) == base + j;
+        entry[j] = there ? entry[j] : -1;
+        if (there) least = min(least, entry[j]);
+      }
+      if (least == t) {  // the group's first token
+        const int at = atomicAdd(&num_owned, 1);
         owned[at] = slot / kF8Group;
 #pragma unroll
         for (int j = 0; j < kF8Group; ++j) member[at][j] = entry[j];
       }
-      if (lane == 0) num_owned = __popc(owners);
     }
-    __syncthreads();
   }
+  __syncthreads();
   const int per_page = p.block_size / kF8Group, bytes = f8_group_bytes(p.head_dim);
   if (head < p.num_kv_heads)
     for (int i = 0; i < num_owned; ++i) {
+      if (i + 1 < num_owned) {
+        const int t = member[i + 1][lane >> 1];
+        if (t >= 0) prefetch_row(rows + t * stride, p.head_dim, lane & 1, 2);
+      }
       const int64_t page = owned[i] / per_page;
       const int64_t at = ((page * p.num_kv_heads + head) * per_page + (owned[i] - page * per_page)) * bytes;
       if (operand & 1)
@@ -451,12 +453,19 @@ cudaError_t launch_store_nb(const CodedStoreParams &p, cudaStream_t stream) {
   const unsigned operands = static_cast<unsigned>((2 * p.num_kv_heads + 7) / 8);
   if (p.index == nullptr)
     return launch_pdl(fp8_store_kernel<T, VEC, NB, true>, dim3(static_cast<unsigned>(p.num_tokens), operands), block, 0,
-                      stream, p);
+                      stream, p, 1);
   const cudaError_t e = launch_pdl(fp8_index_kernel, dim3(static_cast<unsigned>((p.num_tokens + 255) / 256)), dim3(256), 0,
                                    stream, p);
   if (e != cudaSuccess) return e;
+  // One round of CTAs, as far as it goes: finding the groups is paid once by each (about 2 us).
+  const int64_t ctas = (sizeof(T) == 2 ? 4 : 2) * static_cast<int64_t>(sm_count_current()) / operands;
+  int64_t chunk = (p.num_tokens + (ctas > 0 ? ctas : 1) - 1) / (ctas > 0 ? ctas : 1);
+  chunk = (chunk + kF8Group - 1) / kF8Group * kF8Group;
+  if (chunk > kChunk) chunk = kChunk;
+  if (chunk > static_cast<int64_t>(block.x)) chunk = block.x;  // a thread to a token
   return launch_pdl(fp8_store_kernel<T, VEC, NB, false>,
-                    dim3(static_cast<unsigned>((p.num_tokens + kChunk - 1) / kChunk), operands), block, 0, stream, p);
+                    dim3(static_cast<unsigned>((p.num_tokens + chunk - 1) / chunk), operands), block, 0, stream, p,
+                    static_cast<int>(chunk));
 }
 
 template <typename T, bool VEC>
