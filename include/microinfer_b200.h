@@ -580,13 +580,14 @@ MI_API int mi_paged_decode_fp8(void *out, const void *query, const void *key_pag
 /*
  * Causal chunked prefill from the 8-bit cache (also mixed batches): rows as
  * mi_paged_prefill, any type, GQA group and head_dim.  `max_seqlen_q`
- * bounds the launch shape, `max_context` (a bound on the contexts, or less) the split over the keys
- * of few rows, whose states take the workspace for the duration of the call.
+ * bounds the longest chunk; with it `max_context` (a bound on the contexts, or less) decides on the kernel and on splits
+ * over the keys, whose partial results take the workspace for the duration of the call.  `out` must not overlap the query.
  */
 MI_API size_t mi_paged_prefill_fp8_workspace_bytes(int64_t num_seqs, int64_t num_tokens,
-                                              int64_t max_seqlen_q, int32_t num_q_heads,
-                                              int32_t num_kv_heads, int32_t head_dim,
-                                              int64_t max_context, int device);
+                                            int64_t max_seqlen_q, int64_t num_blocks,
+                                            int32_t block_size, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                            int64_t max_context, int device);
 MI_API int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pages,
                            const void *value_pages, int64_t num_blocks, int32_t block_size,
                            int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,

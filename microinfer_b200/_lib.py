@@ -134,7 +134,7 @@ SIGNATURES = {
          _P],
     ),
     "mi_paged_prefill_fp8_workspace_bytes": (
-        _SZ, [_I64, _I64, _I64, _I32, _I32, _I32, _I64, ctypes.c_int],
+        _SZ, [_I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I64, ctypes.c_int],
     ),
     "mi_paged_prefill_fp8": (
         ctypes.c_int,

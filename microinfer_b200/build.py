@@ -23,7 +23,8 @@ BUILD_DIR = PKG_DIR.parent / "_build"
 SOURCES = ["capi.cu", "copy_kernels.cu", "attention.cu", "decode.cu",
            "decode_mma.cu", "prefill_tc.cu", "decode_noalloc.cu", "qk_prologue.cu", "runner_meta.cu",
            "mxfp4_cache.cu", "decode_mxfp4_mma.cu", "prefill_mxfp4.cu",
-           "mxfp4_capi.cu", "fp8_cache.cu", "decode_fp8.cu", "prefill_fp8.cu", "fp8_capi.cu"]
+           "mxfp4_capi.cu", "fp8_cache.cu", "decode_fp8.cu", "prefill_fp8.cu",
+           "prefill_fp8_tc.cu", "fp8_capi.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3",

@@ -6,6 +6,7 @@
 #include "launch.cuh"
 #include "fp8.cuh"
 #include "params.cuh"
+#include "prefill_fp8.cuh"
 
 namespace mi {
 
@@ -31,7 +32,13 @@ size_t fp8_decode_workspace(int64_t num_seqs, int num_q_heads, int num_kv_heads,
 int fp8_prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int num_q_heads, int num_kv_heads,
                          int64_t capacity, int sms);
 cudaError_t launch_fp8_prefill(const CodedPrefillParams &p, int dtype, int head_dim, int64_t num_seqs,
-                                 int64_t max_seqlen_q, cudaStream_t stream);
+                               int64_t max_seqlen_q, cudaStream_t stream);
+bool fp8_prefill_tc_takes(int dtype, int head_dim, int64_t num_blocks, int block_size, int num_q_heads, int num_kv_heads,
+                          int64_t num_seqs, int64_t max_seqlen_q, int64_t max_context, int sms);
+size_t fp8_prefill_tc_workspace(int head_dim, int sms);
+cudaError_t launch_fp8_prefill_tc(const CodedPrefillParams &p, int dtype, int head_dim, cudaStream_t stream);
+cudaError_t launch_fp8_prefill_redo(const CodedPrefillParams &p, int dtype, int head_dim, cudaStream_t stream);
+cudaError_t launch_fp8_prefill_redo_gathered(const CodedPrefillParams &p, int dtype, int64_t max_seqlen_q, cudaStream_t stream);
 
 }  // namespace mi
 
@@ -213,25 +220,24 @@ int mi_paged_decode_fp8(void *out, const void *query, const void *key_pages, con
   return capi_cuda_status(launch_fp8_decode(p, dtype, static_cast<cudaStream_t>(stream)));
 }
 
-static int prefill_splits(int64_t num_seqs, int64_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
-                          int64_t max_context, int sms) {
-  return fp8_prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context, sms);
-}
-
 static size_t prefill_workspace(int splits, int64_t num_tokens, int32_t num_q_heads, int32_t head_dim) {
   return splits <= 1 ? 0
                      : static_cast<size_t>(splits) * num_tokens * num_q_heads * (head_dim + 2) * sizeof(float);
 }
 
 size_t mi_paged_prefill_fp8_workspace_bytes(int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen_q,
-                                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                                              int64_t max_context, int device) {
+                                            int64_t num_blocks, int32_t block_size, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int64_t max_context,
+                                            int device) {
   if (num_seqs <= 0 || num_tokens <= 0 || max_seqlen_q <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
-      num_q_heads % num_kv_heads != 0 || head_dim <= 0 || max_context < 0)
+      num_q_heads % num_kv_heads != 0 || max_context < 0 || !known_dtype(dtype) ||
+      check_cache(num_blocks, block_size, num_kv_heads, head_dim) != MI_OK)
     return 0;
-  const int splits = prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context,
-                                    sm_count_of(device < 0 ? 0 : device));
-  return prefill_workspace(splits, num_tokens, num_q_heads, head_dim);
+  const int sms = sm_count_of(device < 0 ? 0 : device);
+  if (fp8_prefill_tc_takes(dtype, head_dim, num_blocks, block_size, num_q_heads, num_kv_heads, num_seqs, max_seqlen_q, max_context, sms))
+    return fp8_prefill_tc_workspace(head_dim, sms);
+  return prefill_workspace(fp8_prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context, sms),
+                           num_tokens, num_q_heads, head_dim);
 }
 
 int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pages, const void *value_pages,
@@ -259,9 +265,11 @@ int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pages, co
   if (!aligned16(key_pages) || !aligned16(value_pages) || !aligned16(query) || !aligned16(out))
     return capi_fail(MI_ERR_ALIGNMENT, "pages, query and out must be 16-byte aligned");
   if (const int s = capi_select_device(key_pages)) return s;
-  const int splits = prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context,
-                                    sm_count_current());
-  const size_t need = prefill_workspace(splits, num_tokens, num_q_heads, head_dim);
+  const bool tc = fp8_prefill_tc_takes(dtype, head_dim, num_blocks, block_size, num_q_heads, num_kv_heads, num_seqs, max_seqlen_q,
+                                       max_context, sm_count_current());
+  const int splits = tc ? 1 : fp8_prefill_splits(num_seqs, max_seqlen_q, num_q_heads, num_kv_heads, max_context, sm_count_current());
+  const size_t need = tc ? fp8_prefill_tc_workspace(head_dim, sm_count_current())
+                         : prefill_workspace(splits, num_tokens, num_q_heads, head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return capi_fail(MI_ERR_INVALID, "workspace too small (see mi_paged_prefill_fp8_workspace_bytes)");
   if (need > 0 && !aligned16(workspace)) return capi_fail(MI_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
@@ -283,8 +291,18 @@ int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pages, co
   p.num_kv_heads = num_kv_heads;
   p.scale_log2 = scale * kLog2eHost;
   p.status = dev_status;
-  return capi_cuda_status(
-      launch_fp8_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, static_cast<cudaStream_t>(stream)));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!tc) return capi_cuda_status(launch_fp8_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, st));
+  for (int64_t s = 0; s < num_seqs; s += kF8MaxSeqs) {
+    CodedPrefillParams q = p;
+    q.num_seqs = num_seqs - s < kF8MaxSeqs ? num_seqs - s : kF8MaxSeqs;
+    q.cu_seqlens_q = cu_seqlens_q + s;
+    q.cu_seqlens_k = cu_seqlens_k + s;
+    q.block_tables = block_tables + s * block_table_stride;
+    if (const int e = capi_cuda_status(launch_fp8_prefill_tc(q, dtype, head_dim, st))) return e;
+    if (const int e = capi_cuda_status(launch_fp8_prefill_redo(q, dtype, head_dim, st))) return e;
+  }
+  return MI_OK;
 }
 
 // K and V of kv_rows rows, each from a multiple of 256 bytes, then a byte per (sequence, kv head, group).
@@ -381,13 +399,14 @@ int mi_paged_prefill_fp8_gathered(void *out, const void *query, const void *key_
   p.bt_stride = block_table_stride;
   p.num_blocks = num_blocks;
   p.num_tokens = num_tokens;
+  p.num_seqs = num_seqs;
   p.num_splits = 1;
   p.block_size = block_size;
   p.num_q_heads = num_q_heads;
   p.num_kv_heads = num_kv_heads;
   p.scale_log2 = scale * kLog2eHost;
   p.status = dev_status;
-  return capi_cuda_status(launch_fp8_prefill(p, dtype, head_dim, num_seqs, max_seqlen_q, st));
+  return capi_cuda_status(launch_fp8_prefill_redo_gathered(p, dtype, max_seqlen_q, st));
 }
 
 }  // extern "C"

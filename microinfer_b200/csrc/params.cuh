@@ -211,6 +211,7 @@ struct CodedPrefillParams {
   int64_t bt_stride;
   int64_t num_blocks;
   int64_t num_tokens;
+  int64_t num_seqs;  // 8-bit
   int32_t num_splits;
   int32_t block_size;
   int32_t num_q_heads;

@@ -1,6 +1,5 @@
-// Causal chunked prefill straight from the 8-bit cache (layout: fp8.cuh) on the warp-level tensor cores, for what the dense
-// tcgen05 kernel behind the gather does not take (head_dim other than 128, fp32, other groups) and for chunks too small
-// to fill it.
+// Causal chunked prefill straight from the 8-bit cache (layout: fp8.cuh) on the warp-level tensor cores, for what the tcgen05
+// kernels do not take (fp32, head_dims other than 64 and 128), for little work, and for what they leave to be done over.
 //
 // A CTA takes 128 rows of one kv head, a row being (token, query head of the group), so any group
 // fills the tiles; 8 warps of 16 rows.  It walks the keys 64 at a time: the codes of the next tile are on their
@@ -16,12 +15,17 @@
 // further below (or a zero one) take their groups one by one and add them in fp32; a group above raises R.
 // NaN of V are held as zeros and set in the rows that see the key, so they never reach rows before it.
 // Few rows over a long context are split over the keys; a second launch joins the splits, as means of V.
+//
+// Measured (cold L2): 1 x 64 rows on 64 keys 12 us (head_dim 64) and 16 us (128), 16 x 64 on 64 the same, 1 x 512 on 512 30 to 34.
+// Larger calls it does at 170 to 190 TFLOP/s of head_dim 64, half of what the tcgen05 kernel does: the exponentials and the decoding
+// share the issue slots of the warps that also feed the MMAs.
 #include <type_traits>
 
 #include "common.cuh"
 #include "fp8.cuh"
 #include "launch.cuh"
 #include "params.cuh"
+#include "prefill_fp8.cuh"
 
 namespace mi {
 
@@ -49,7 +53,7 @@ struct P8Cfg {
   static constexpr int kChunks = 2 * kGroups * D;       // 16-byte chunks of codes of a tile, K and V
   static constexpr int kPer = (kChunks + kThreads - 1) / kThreads;  // of those per thread
   static constexpr int kRaw = kPer * kThreads * 16;     // codes on their way
-  static constexpr int kMisc = kRows * 4 + 2 * (2 * kGroups * 4 + kKeys);
+  static constexpr int kMisc = kRows * 4 + 2 * (2 * kGroups * 4 + kGroups * 8 + kKeys);
   static constexpr int kSmem = kParts * kQuery + 4 * kTile + kRaw + kMisc;
   static constexpr int kCtas = kSmem <= 113 * 1024 ? 2 : 1;  // of an SM
   static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
@@ -111,7 +115,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
   uint8_t *raw = tiles + 4 * C::kTile;         // codes of the next tile, each thread's its own
   int *row_exp = reinterpret_cast<int *>(raw + C::kRaw);  // [rows]: exponent that a row's products want, without K's scale
   int *bytes = row_exp + kRows;                // [2][K, V][groups]: scale bytes, -1 where the page is none (V's past the keys too)
-  uint8_t *marks = reinterpret_cast<uint8_t *>(bytes + 4 * kGroups);  // [2][keys]: blocks of 32 dims of V with a NaN, a bit each
+  int64_t *where = reinterpret_cast<int64_t *>(bytes + 4 * kGroups);  // [2][groups]: places in the pools, -1 past the keys, -2: the page is none
+  uint8_t *marks = reinterpret_cast<uint8_t *>(where + 2 * kGroups);  // [2][keys]: blocks of 32 dims of V with a NaN, a bit each
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = p.num_q_heads / p.num_kv_heads;
   const int64_t q0 = p.cu_seqlens_q[seq];
@@ -154,36 +159,41 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
   };
   const int per_page = p.block_size / kF8Group;
   const int32_t *table = p.block_tables + seq * p.bt_stride;
-  // Group `index` of the context: its place in the pools, -1 past the keys, -2 where its page is none.
-  auto look_up = [&](uint32_t index) -> int64_t {
-    if (static_cast<int64_t>(index) * kF8Group >= keys) return -1;
-    const uint32_t col = by_page.div(index);
-    const int page = __ldg(table + col);
-    if (page < 0 || page >= p.num_blocks) return -2;
-    return (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page + (index - col * per_page);
+  // Group `index` of the context: its place in the pools from the page that the table names.
+  auto page_of = [&](uint32_t index) {
+    return static_cast<int64_t>(index) * kF8Group < keys ? __ldg(table + by_page.div(index)) : INT32_MIN;
   };
-  // Pages are looked up a tile before their codes are asked for.
-  int64_t where[C::kPer], my_scale_at = -1;  // my_scale_at: threads up to 2 * kGroups bring a scale each
-  auto look_ahead = [&](int kt) {
-#pragma unroll
-    for (int n = 0; n < C::kPer; ++n) where[n] = chunk(n).exists ? look_up(static_cast<uint32_t>(kt) * kGroups + chunk(n).group) : -1;
-    if (threadIdx.x < 2 * kGroups) my_scale_at = look_up(static_cast<uint32_t>(kt) * kGroups + threadIdx.x % kGroups);
+  auto place_of = [&](uint32_t index, int page) -> int64_t {
+    if (page == INT32_MIN && static_cast<int64_t>(index) * kF8Group >= keys) return -1;
+    if (page < 0 || page >= p.num_blocks) return -2;
+    return (static_cast<int64_t>(page) * p.num_kv_heads + kvh) * per_page + (index - by_page.div(index) * per_page);
+  };
+  // The pages of a tile's groups are looked up by a thread each, two tiles ahead of the products and one of the copies.
+  int my_page = INT32_MIN;
+  auto look_up = [&](int kt) {
+    if (threadIdx.x < kGroups) my_page = page_of(static_cast<uint32_t>(kt) * kGroups + threadIdx.x);
+  };
+  auto looked_up = [&](int kt) {
+    if (threadIdx.x < kGroups)
+      where[(kt & 1) * kGroups + threadIdx.x] = place_of(static_cast<uint32_t>(kt) * kGroups + threadIdx.x, my_page);
   };
   const uint32_t my_raw = smem_addr(raw) + threadIdx.x * 16;
-  int my_scale = 0;
-  auto fetch = [&] {
+  int my_scale = 0;  // of the first threads, a group each of K, then of V
+  auto fetch = [&](int kt) {
 #pragma unroll
     for (int n = 0; n < C::kPer; ++n) {
       const Chunk c = chunk(n);
-      const uint8_t *from = (c.value ? p.value_pages : p.key_pages) + max(where[n], int64_t{0}) * f8_group_bytes(D) + c.i * 16;
-      const int size = where[n] < 0 ? 0 : 16;  // keys that do not exist: zeros
+      const int64_t place = c.exists ? where[(kt & 1) * kGroups + c.group] : -1;
+      const uint8_t *from = (c.value ? p.value_pages : p.key_pages) + max(place, int64_t{0}) * f8_group_bytes(D) + c.i * 16;
+      const int size = place < 0 ? 0 : 16;  // keys that do not exist: zeros
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(my_raw + n * kThreads * 16), "l"(from), "r"(size)
                    : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     if (threadIdx.x < 2 * kGroups) {
+      const int64_t place = where[(kt & 1) * kGroups + threadIdx.x % kGroups];
       const uint8_t *pool = threadIdx.x < kGroups ? p.key_pages : p.value_pages;
-      my_scale = my_scale_at < 0 ? (my_scale_at == -2 || threadIdx.x >= kGroups ? -1 : 0) : pool[my_scale_at * f8_group_bytes(D) + kF8Group * D];
+      my_scale = place < 0 ? (place == -2 || threadIdx.x >= kGroups ? -1 : 0) : pool[place * f8_group_bytes(D) + kF8Group * D];
     }
   };
   // This thread's chunks as f16 rows of buffer `buf`; whether V has a NaN among them.
@@ -266,6 +276,7 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
     }
   };
   auto arrive = [&](int buf, int kt) -> bool {
+    looked_up(kt + 1);
     const bool mine = place(buf);
     const bool any = __syncthreads_or(mine);
     if (any) {
@@ -276,9 +287,11 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
   };
 
   if (k_begin < k_end) {
-    look_ahead(k_begin);
-    fetch();
-    look_ahead(k_begin + 1);
+    look_up(k_begin);
+    looked_up(k_begin);
+    look_up(k_begin + 1);
+    __syncthreads();
+    fetch(k_begin);
   }
 
   // ---- q into shared memory, as `kParts` operands: four lanes to a row, 8 of every 32 dims each ----
@@ -364,8 +377,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
     const int buf = (kt - k_begin) & 1;
     const bool more = kt + 1 < k_end;
     if (more) {
-      fetch();
-      look_ahead(kt + 2);
+      fetch(kt + 1);
+      look_up(kt + 2);
     }
     const uint32_t k_base = t_base + buf * 2 * C::kTile + k_lane;
     const uint32_t v_base = t_base + buf * 2 * C::kTile + C::kTile + v_lane;
@@ -545,7 +558,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
       for (int key = 0; key < kKeys; ++key) {
         const unsigned blocks = marks[buf * kKeys + key];
         if (!blocks) continue;
-        const uint8_t *codes = p.value_pages + look_up(static_cast<uint32_t>(kt) * kGroups + key / kF8Group) * f8_group_bytes(D);
+        const uint32_t index = static_cast<uint32_t>(kt) * kGroups + key / kF8Group;
+        const uint8_t *codes = p.value_pages + place_of(index, page_of(index)) * f8_group_bytes(D);  // it has a page
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
           if (!(blocks >> (n / 4) & 1u)) continue;
@@ -609,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, P8Cfg<T, NB>::kCtas)
 // ever any, so a few CTAs look and take all tiles if so.
 template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, P8Cfg<T, NB>::kCtas)
-    fp8_prefill_redo_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
+    fp8_prefill_redo_gathered_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page, int tiles) {
   pdl_wait();
   const int64_t ctx = static_cast<int64_t>(p.cu_seqlens_k[blockIdx.z + 1]) - p.cu_seqlens_k[blockIdx.z];
   const int64_t groups = min((ctx + kF8Group - 1) / kF8Group, static_cast<int64_t>(p.redo_groups));
@@ -621,6 +635,40 @@ __global__ void __launch_bounds__(kThreads, P8Cfg<T, NB>::kCtas)
       prefill_tile<T, NB>(p, by_group, by_page, blockIdx.z, blockIdx.y, tile, 0);
       __syncthreads();  // every warp has read what the next tile overwrites
     }
+  pdl_launch_dependents();
+}
+
+// After the tcgen05 kernel: the sequences and kv heads in whose CTAs it met what it cannot do, over again.  Hardly ever any.
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_prefill_redo_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page, int ctas) {
+  __shared__ int64_t prefix[kF8MaxSeqs + 1], scratch[32];
+  pdl_wait();
+  const uint8_t *odd = f8_odd(p, NB * 32, ctas);
+  bool any = false;
+  for (int i = threadIdx.x; i < ctas * 8; i += kThreads) any |= odd[i] != 0;
+  if (!__syncthreads_or(any)) {
+    pdl_launch_dependents();
+    return;
+  }
+  const F8Work work = f8_work(p, by_group, prefix, scratch, ctas);
+  for (int seq = 0; seq < p.num_seqs; ++seq) {
+    const int64_t cost = (prefix[seq + 1] - prefix[seq]) / p.num_kv_heads;
+    if (cost == 0) continue;
+    F8Seq q;
+    q.load(p, seq);
+    for (int kvh = 0; kvh < p.num_kv_heads; ++kvh) {
+      const int64_t from = prefix[seq] + kvh * cost;
+      const int first = static_cast<int>(from / work.share), last = static_cast<int>((from + cost - 1) / work.share);
+      any = false;
+      for (int i = first * 8 + threadIdx.x; i < (last + 1) * 8; i += kThreads) any |= odd[i] != 0;
+      if (!__syncthreads_or(any)) continue;
+      for (int tile = blockIdx.x; tile < (q.rows + kRows - 1) / kRows; tile += gridDim.x) {
+        prefill_tile<T, NB>(p, by_group, by_page, seq, kvh, tile, 0);
+        __syncthreads();  // every warp has read what the next tile overwrites
+      }
+    }
+  }
   pdl_launch_dependents();
 }
 
@@ -680,22 +728,6 @@ cudaError_t launch_p8(const CodedPrefillParams &p, int64_t num_seqs, int64_t max
   const int G = p.num_q_heads / p.num_kv_heads;
   const int64_t tiles = (max_seqlen_q * G + kRows - 1) / kRows;
   const FastDiv by_group(G), by_page(p.block_size / kF8Group);
-  if constexpr (NB == 4 && !C::kSplit) {
-    if (p.redo != nullptr) {
-      auto redo = fp8_prefill_redo_kernel<T, NB>;
-      static bool redo_attr_set[64] = {};
-      if (dev >= 64 || !redo_attr_set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(redo, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-        if (e != cudaSuccess) return e;
-        if (dev < 64) redo_attr_set[dev] = true;
-      }
-      int64_t ctas = 2 * sm_count_current() / (p.num_kv_heads * num_seqs);
-      ctas = ctas < 1 ? 1 : ctas > tiles ? tiles : ctas;
-      return launch_pdl(redo, dim3(static_cast<unsigned>(ctas), p.num_kv_heads, static_cast<unsigned>(num_seqs)),
-                        dim3(kThreads), C::kSmem, stream, p, by_group, by_page, static_cast<int>(tiles));
-    }
-  }
-  if (p.redo != nullptr) return cudaErrorInvalidValue;
   if (dev >= 64 || !attr_set[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return e;
@@ -728,6 +760,43 @@ cudaError_t launch_p8_t(const CodedPrefillParams &p, int head_dim, int64_t num_s
   return cudaErrorInvalidValue;
 }
 
+template <typename T, int NB>
+cudaError_t launch_redo(const CodedPrefillParams &p, cudaStream_t stream) {
+  using C = P8Cfg<T, NB>;
+  auto kern = fp8_prefill_redo_kernel<T, NB>;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  const int ctas = sm_count_current();
+  return launch_pdl(kern, dim3(ctas), dim3(kThreads), C::kSmem, stream, p, FastDiv(p.num_q_heads / p.num_kv_heads),
+                    FastDiv(p.block_size / kF8Group), ctas);
+}
+
+template <typename T>
+cudaError_t launch_redo_gathered(const CodedPrefillParams &p, int64_t max_seqlen_q, cudaStream_t stream) {
+  using C = P8Cfg<T, 4>;  // the dense kernel has one head_dim
+  auto kern = fp8_prefill_redo_gathered_kernel<T, 4>;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  const int64_t tiles = (max_seqlen_q * (p.num_q_heads / p.num_kv_heads) + kRows - 1) / kRows;
+  int64_t ctas = 2 * sm_count_current() / (p.num_kv_heads * p.num_seqs);
+  ctas = ctas < 1 ? 1 : ctas > tiles ? tiles : ctas;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(ctas), p.num_kv_heads, static_cast<unsigned>(p.num_seqs)), dim3(kThreads),
+                    C::kSmem, stream, p, FastDiv(p.num_q_heads / p.num_kv_heads), FastDiv(p.block_size / kF8Group),
+                    static_cast<int>(tiles));
+}
+
 }  // namespace
 
 // Splits over the keys: enough CTAs for two per SM, each split at least 256 keys of a full table.
@@ -747,6 +816,17 @@ cudaError_t launch_fp8_prefill(const CodedPrefillParams &p, int dtype, int head_
   if (dtype == MI_DTYPE_BFLOAT16) return launch_p8_t<__nv_bfloat16>(p, head_dim, num_seqs, max_seqlen_q, stream);
   if (dtype == MI_DTYPE_FLOAT16) return launch_p8_t<__half>(p, head_dim, num_seqs, max_seqlen_q, stream);
   return launch_p8_t<float>(p, head_dim, num_seqs, max_seqlen_q, stream);
+}
+
+cudaError_t launch_fp8_prefill_redo(const CodedPrefillParams &p, int dtype, int head_dim, cudaStream_t stream) {
+  if (dtype == MI_DTYPE_BFLOAT16)
+    return head_dim == 64 ? launch_redo<__nv_bfloat16, 2>(p, stream) : launch_redo<__nv_bfloat16, 4>(p, stream);
+  return head_dim == 64 ? launch_redo<__half, 2>(p, stream) : launch_redo<__half, 4>(p, stream);
+}
+
+cudaError_t launch_fp8_prefill_redo_gathered(const CodedPrefillParams &p, int dtype, int64_t max_seqlen_q, cudaStream_t stream) {
+  return dtype == MI_DTYPE_BFLOAT16 ? launch_redo_gathered<__nv_bfloat16>(p, max_seqlen_q, stream)
+                                    : launch_redo_gathered<__half>(p, max_seqlen_q, stream);
 }
 
 }  // namespace mi

@@ -5,11 +5,13 @@
 * ``gather_paged_kv_fp8``     rows in logical order, as ``gather_paged_kv``
 * ``paged_attention_fp8_meta``  dispatch on the step's metadata, as ``paged_attention_meta``
 
-Decode reads the codes and decodes them in registers.  Prefill has two ways.  Where there are tiles enough for
-the dense tensor-core kernel, each context is decoded once into a workspace of the query's type (twice its
-pages) and that kernel attends to the rows.  Few tiles, and shapes that kernel does not take, are computed from the
-pages.  Both give the same result up to rounding: sequences with what the dense kernel cannot do
-(a NaN of V or, in fp16, a value past its range; a page that is none) are done over from the pages.
+Decode reads the codes and decodes them in registers.  Prefill has three ways.  Where many rows share the keys of a
+shape that the dense tensor-core kernel takes, each context is decoded once into a workspace of the query's
+type (twice its pages) and that kernel attends to the rows.  Elsewhere the pages are read: by a tcgen05 kernel (16-bit
+queries, head_dim 64 and 128), or by one on the warp-level tensor cores for little work and everything
+else.  All give the same result up to rounding: what the tensor-core kernels cannot do (a NaN of V,
+scales too far apart, in fp16 a value past its range) is done over by the third.  The choice goes by the shapes and the bounds
+``max_seqlen_q``, ``max_seqlen_k`` and ``total_k``, never by what the tensors hold.
 Workspaces come from torch's allocator for the length of the call, so that calls on several
 streams, and captured graphs, each have their own.
 """
@@ -134,16 +136,23 @@ def _prefill_workspace_bytes(*shape):
 
 
 @lru_cache(maxsize=4096)
-def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, device):
-    """Whether prefill reads the pages itself instead of gathering for the dense kernel: where the tcgen05 kernel does
-    not take the shape, and where that would leave three quarters of the SMs without a tile of 128 rows
-    (reading the pages splits the keys).
+def _reads_pages(dtype, hq, hkv, d, requests, max_seqlen_q, most, device):
+    """Whether prefill reads the pages itself instead of gathering for the dense kernel.
+
+    Where the dense kernel does not take the shape; for little work, up to 5 tiles of 128 rows x 128 keys for every two SMs
+    (16 to 42 us where two kernels more take 28 to 44); from 3000 keys where its tiles of 128
+    rows do not fill the SMs (reading the pages splits the keys: 1 x 256 rows on 16000, 32 heads on 8, 142 us where the dense way
+    takes 314), or a sequence has at most 256 rows of a kv head to gather its keys for (16 x 64 on 8000: 251, 296).
+    Else the rows are worth decoding once: 1 x 4096 takes 236 us there and 312 from the pages, 4 x 1024 on 4000 314 and 431.
     """
     lib = _lib.load()
     if lib.mi_prefill_kernel_for(dtype, d, hq, hkv, 0) != 2:
         return True
-    tiles = requests * hkv * -(-max_seqlen_q * (hq // hkv) // 128)
-    return 4 * tiles <= lib.mi_device_sm_count(device)
+    sms, rows = lib.mi_device_sm_count(device), max_seqlen_q * (hq // hkv)
+    tiles = requests * hkv * -(-rows // 128)
+    if 2 * tiles * -(-most // 128) <= 5 * sms:
+        return True
+    return most >= 3000 and (tiles <= sms or rows <= 256)
 
 
 def paged_prefill_fp8(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k, block_tables, *,
@@ -194,11 +203,13 @@ def paged_prefill_fp8(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k,
     cu_seqlens_q, cu_seqlens_k = _idx(cu_seqlens_q), _idx(cu_seqlens_k)
     tokens, hq, _ = query.shape
     dtype = _lib.dtype_code(query.dtype)
-    if _reads_pages(dtype, hq, hkv, d, requests, int(max_seqlen_q), device.index or 0):
-        if out is None:
-            out = torch.empty_like(query)
-        shape = (requests, tokens, int(max_seqlen_q), hq, hkv, d, most, device.index or 0)
-        need = _prefill_workspace_bytes(*shape)
+    if out is None:
+        out = torch.empty_like(query)
+    elif _overlap(out, query):  # some rows may be done twice
+        query = query.clone()
+    if _reads_pages(dtype, hq, hkv, d, requests, int(max_seqlen_q), most, device.index or 0):
+        need = _prefill_workspace_bytes(requests, tokens, int(max_seqlen_q), dims[0], bs, hq, hkv, d, dtype, most,
+                                        device.index or 0)
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         _lib.call(
             "mi_paged_prefill_fp8", out.data_ptr(), query.data_ptr(), key_pages.data_ptr(),
@@ -209,10 +220,6 @@ def paged_prefill_fp8(query, key_pages, value_pages, cu_seqlens_q, cu_seqlens_k,
             _lib.status_buffer(device).data_ptr(), _lib.stream_of(device),
         )
         return out
-    if out is None:
-        out = torch.empty_like(query)
-    elif _overlap(out, query):  # some rows may be done twice
-        query = query.clone()
     need = _lib.load().mi_paged_prefill_fp8_gathered_workspace_bytes(requests, most, rows, hkv, d, dtype)
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _lib.call(

@@ -11,7 +11,8 @@ with u half a step of the output type and c from the kernels' roundings:
 floor: f16 ends.  p times 2^12 times 2^(byte - R) with R at most 2 above the largest byte of V's scales
   loses at most half of 2^-24 a key, which is 2^-37 of the sum of p (at least 2^12) times the largest magnitude of
   a code, 448 * 2^(R - 127) <= 8 * 224 * 2^(largest byte - 127): 2^-34 of the oracle's floor.  The dense kernel of fp16
-  prefill lifts p by 2^7 only and has no R: half of 2^-24 of 2^7, times 448 * 2^(byte - 127): 2^-31 of it.
+  prefill lifts p by 2^7 only and has no R: half of 2^-24 of 2^7, times 448 * 2^(byte - 127): 2^-31 of it; the tcgen05
+  kernel by 2^11: 2^-33 (of keys 2^25 below the largest, which the cases held to 2^-34 do not have).
 """
 
 import numpy as np

@@ -188,6 +188,11 @@ def test_c_entries_refuse_bad_arguments():
                       (dict(rows=0), b"positive"), (dict(size=64), b"workspace"), (dict(ws=None), b"workspace"),
                       (dict(hq=12), b"divisible"), (dict(stride=(1 << 27) + 1), b"too long")):
         assert gathered(**bad) < 0 and word in lib.mi_last_error(), bad
+    need = lib.mi_paged_prefill_fp8_workspace_bytes
+    assert need(1, 4096, 4096, 512, 16, 4, 2, 128, 2, 8192, 0) == 148 * (2 * 256 * 130 * 4 + 16 + 8)  # 148 SMs without a device
+    assert need(1, 4096, 4096, 512, 16, 4, 2, 128, 0, 256, 0) == 0  # too few keys to split
+    assert need(1, 4, 4, 4, 16, 4, 2, 128, 2, 16, 0) == 0  # little work: the other kernel, not split
+    assert need(1, 4, 4, 4, 8, 4, 2, 128, 2, 16, 0) == 0
 
 
 # ---------------------------------------------------------------------------
