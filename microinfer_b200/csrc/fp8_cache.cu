@@ -9,7 +9,7 @@
 // Which tokens share a group is not in the order of the slots (a batch's rows may come in any), and a group must have one
 // writer.  The first token of a group in the call's order is its owner.  Short calls: a CTA per token, whose threads look through
 // all slots for the token's group.  Longer ones: a launch before it writes each token's number to index[slot],
-// and a CTA per 16 tokens reads the 16 entries of each of their groups; the index needs no initial value, since an
+// and a CTA of up to 256 tokens reads the 16 entries of each of their groups; the index needs no initial value, since an
 // entry i is this call's where slots[i] is the slot again.
 // An owner's rows are read at once (8 16-byte loads a lane at head_dim 128 in 16 bits): the maximum goes through five
 // shuffles and the codes are written from registers, whole 32-byte sectors of K and V.
