@@ -17,6 +17,10 @@
 // Gather: rows of each request in logical order, request-major, as code * scale in the requested type (exact in fp32 and
 // bf16; fp16 rounds).  A warp takes a group of 16 positions of one kv head and writes 16 bytes a lane, whole rows together.
 // HBM-bound on the rows that it writes.
+//
+// Measured, 8 heads of 128: store of 32 tokens 4.6 us, 8000 in bf16 18 and in fp32 29, 64000 in bf16 75 (5.3 TB/s, 80% of a copy; issue
+// slots 62%, ALU 50%); scan and index, us: 300 tokens 8 : 11, 1000 14 : 13,
+// 2000 22 : 13; where each token has a group of its own 300 12 : 15, 1000 25 : 26, 2000 45 : 38.  Gather of 48 x 1500 to bf16 69 us (5.6 TB/s).
 #include <type_traits>
 
 #include "common.cuh"
@@ -30,7 +34,7 @@ namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
 constexpr int kChunk = 256;      // tokens of a CTA that finds groups by the index, at most
-constexpr int kScanTokens = 512; // calls up to this long look through the slots instead
+constexpr int kScanTokens = 512; // calls up to this long look through the slots instead, without an index
 
 // Eight elements of a row as they are in memory.
 template <typename T>
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) fp8_store_kernel(
   const int64_t first = SCAN ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * chunk;
   if (head < p.num_kv_heads) {
     const int64_t t = first + (lane >> 1);
-    if (t < p.num_tokens && (!SCAN || lane < 2)) prefetch_row(rows + t * stride, p.head_dim, lane & 1, 2);
+    if (t < p.num_tokens && (lane >> 1) < chunk) prefetch_row(rows + t * stride, p.head_dim, lane & 1, 2);
   }
   pdl_wait();
   if constexpr (SCAN) {
@@ -460,7 +464,9 @@ cudaError_t launch_store_nb(const CodedStoreParams &p, cudaStream_t stream) {
   // One round of CTAs, as far as it goes: finding the groups is paid once by each (about 2 us).
   const int64_t ctas = (sizeof(T) == 2 ? 4 : 2) * static_cast<int64_t>(sm_count_current()) / operands;
   int64_t chunk = (p.num_tokens + (ctas > 0 ? ctas : 1) - 1) / (ctas > 0 ? ctas : 1);
-  chunk = (chunk + kF8Group - 1) / kF8Group * kF8Group;
+  // Below a group's tokens as it is: where each token has a group of its own (a decode step of many sequences) a CTA's
+  // are worked on one after the other.
+  if (chunk > kF8Group) chunk = (chunk + kF8Group - 1) / kF8Group * kF8Group;
   if (chunk > kChunk) chunk = kChunk;
   if (chunk > static_cast<int64_t>(block.x)) chunk = block.x;  // a thread to a token
   return launch_pdl(fp8_store_kernel<T, VEC, NB, false>,

@@ -47,7 +47,8 @@ struct F8Seq {
     q0 = p.cu_seqlens_q[seq];
     const int64_t q_len = max(int64_t{0}, static_cast<int64_t>(p.cu_seqlens_q[seq + 1]) - q0);
     const int64_t ctx = static_cast<int64_t>(p.cu_seqlens_k[seq + 1]) - p.cu_seqlens_k[seq];
-    rows = static_cast<int>(min(q_len * (p.num_q_heads / p.num_kv_heads), int64_t{INT32_MAX} - 512));
+    // lengths that cannot be are work for the tokens that there are and one, which is flagged
+    rows = static_cast<int>(min(min(q_len, p.num_tokens + 1) * (p.num_q_heads / p.num_kv_heads), int64_t{INT32_MAX} - 512));
     prefix = static_cast<int>(ctx - q_len);
     keys = static_cast<int>(max(int64_t{0}, min(ctx, p.bt_stride * p.block_size)));
   }
