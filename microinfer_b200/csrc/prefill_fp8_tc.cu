@@ -25,7 +25,7 @@
 // Every wait is bounded; a timeout flags MI_DEV_TIMEOUT, unwinds every role, waits for the MMAs, frees TMEM and returns.
 //
 // What it leaves to the kernel on the warp-level tensor cores, launched behind it for those sequences and heads alone ("odd"): a NaN
-// of V (0 * NaN reaches rows that do not see its key), scales of V more than 14 binades apart, scores past 2^20 or
+// of V (0 * NaN reaches rows that do not see its key; one in a group of scale 0 is looked for by the loader), scales of V more than 14 binades apart, scores past 2^20 or
 // whose factor leaves fp32's range.  Without any it returns at once.
 //
 // Measured (cold L2): head_dim 64, 32 heads on 8: 1 x 256 rows on 16000 keys 110 us, 1 x 2048 on 6144 316 us (380 TFLOP/s; the warp-level
@@ -96,7 +96,7 @@ enum {
   B_INFO = 33,    // two words: what the loader says of the tile of K and of V
   B_COUNT = 34
 };
-static_assert(B_COUNT * 8 + 8 <= 288 && kItems == 4, "their place in shared memory");
+static_assert(B_COUNT * 8 + 12 <= 288 && kItems == 4, "their place in shared memory");
 constexpr uint32_t kNoMore = 1u << 31;  // of K's word: there is no tile; else bits 0-7 the groups that exist, 8-15 those whose
                                         // V is zero, 16-20 the keys of the last group that exists
 
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t *bar = reinterpret_cast<uint64_t *>(smem + C::kOffMisc);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + B_COUNT);
-  int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1);
+  int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1), *nan_flag = abort_flag + 1;
   constexpr int kScaleRing = C::kScaleRing;
   uint8_t *scales = smem + C::kOffScales;  // ring: K's bytes of 8 groups, V's, then a bit for each whose page is none
   F8Item *item_ring = reinterpret_cast<F8Item *>(smem + C::kOffItems);
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int o = 0; o < 2; ++o) mbar_init(&bar[B_RAWFULL + o], 1), mbar_init(&bar[B_RAWEMPTY + o], kDecoders);
     for (int i = 0; i < kItems; ++i) mbar_init(&bar[B_ITEMFULL + i], 1), mbar_init(&bar[B_ITEMEMPTY + i], 256 + 2);
     mbar_init(&bar[B_FIN], 2);
-    *abort_flag = 0;
+    *abort_flag = *nan_flag = 0;
     fence_mbar_init();
   }
   if (warp == 12) tc::tmem_alloc(tmem_slot, 512);
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int q = 2 * h + i, vb = byte_of(q < 4 ? sb.z : sb.w, q & 3);
-            const int below = vb == 0 ? 0 : max(vb - ref, -100);  // of scale 0: its codes are zeros
+            const int below = vb == 0 ? 0 : max(vb - ref, -100);  // of scale 0: decoded to zeros
             lowest = min(lowest, below);
             const float f = factor(q), nq = nb + static_cast<float>(below);
             const float2 f2 = make_float2(f, f), n2 = make_float2(nq, nq);
@@ -424,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       it = next;
     }
     if (!ok && lane == 0) *(volatile int *)abort_flag = 1;
+    odd |= *(volatile const int *)nan_flag != 0;  // of this CTA's tiles, which have all come by way of the loader
     const bool any = __any_sync(kAll, odd);
     if (lane == 0) f8_odd(p, D, gridDim.x)[blockIdx.x * 8 + warp] = any;
     if (threadIdx.x == 0) f8_meta(p, D, gridDim.x)[blockIdx.x] = meta;
@@ -625,6 +626,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           // keys of the last group that exists (later ones may have no page; theirs are zeros in any case)
           const int last = 31 - __clz(static_cast<int>(exists));
           const int in_last = exists ? min(kF8Group, it.keys - (j * 8 + last) * kF8Group) : 0;
+          // Groups of V of scale 0 are decoded to zeros.  What the store makes of a group without a finite element but zeros is one,
+          // with NaN codes: looked for here, where it costs the tile nothing (in the decoding warps 3 to 7 us of 75).
+          for (unsigned left = zero & exists; left; left &= left - 1) {
+            const int group = __ffs(static_cast<int>(left)) - 1;
+            const int from = __shfl_sync(kAll, place, group), tokens = group == last ? in_last : kF8Group;
+            const uint4 *codes = reinterpret_cast<const uint4 *>(p.value_pages + static_cast<int64_t>(from) * C::kGroup);
+            bool nan = false;
+#pragma unroll
+            for (int i = lane; i < D; i += 32) {
+              const uint4 w = __ldg(codes + i);
+              const int tok = i % 64 / 32 * 8 + i % 4 * 2;  // 8 dims of it and the next
+              const uint32_t keep = (tok < tokens ? 0x00ff00ffu : 0u) | (tok + 1 < tokens ? 0xff00ff00u : 0u);
+              nan |= f8_any_nan(w.x & keep) || f8_any_nan(w.y & keep) || f8_any_nan(w.z & keep) || f8_any_nan(w.w & keep);
+            }
+            if (nan) *(volatile int *)nan_flag = 1;
+          }
 #pragma unroll
           for (int o = 0; o < 2; ++o) {  // K, V
             if (!__all_sync(kAll, mbar_wait_bounded(&bar[B_RAWEMPTY + o], (tiles & 1) ^ 1, p.status) && !aborted(abort_flag))) {

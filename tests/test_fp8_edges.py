@@ -1,0 +1,93 @@
+"""Attention over the 8-bit cache where its ways of computing could part: values that are nowhere finite, groups of scale 0,
+scales and scores at the ends of the range (bounds: fp8_support.py).  Prefill's cases run in each of its ways."""
+
+import numpy as np
+import pytest
+import torch
+
+import microinfer_b200 as mi
+from oracle import fp8_oracle as fo
+from tests.fp8_support import DECODE_STEP, DTYPES, PREFILL_STEP, close, cuda, pages, prefill_case, table_of
+from tests.test_fp8_attention import DENSE_LOST, _place, _set_byte, _set_code
+from tests.test_fp8_prefill_ways import way  # noqa: F401  (a fixture)
+
+gpu = pytest.mark.gpu
+
+
+def _same(got, want, step, lost=DENSE_LOST):
+    """NaN exactly where the formula has it, and the bound elsewhere."""
+    nan = np.isnan(want[0])
+    assert np.array_equal(torch.isnan(got).cpu().numpy(), nan)
+    got = torch.where(torch.from_numpy(nan).to(got.device), torch.zeros_like(got), got)
+    close(got, np.where(nan, 0.0, want[0]), *want[1:], step, lost=lost)
+
+
+def _attend(device, query, kp, vp, tables, q_lens, ctxs, scale, decode=False):
+    """The operators' result and the formula's."""
+    cu_q, cu_k = (torch.tensor([0, *np.cumsum(x)], dtype=torch.int32, device=device) for x in (q_lens, ctxs))
+    pool = cuda(kp, device), cuda(vp, device)
+    table = cuda(np.asarray(tables, dtype=np.int32), device)
+    if decode:
+        got = mi.paged_decode_fp8(query, *pool, table, torch.tensor(ctxs, dtype=torch.int32, device=device), scale=scale)
+    else:
+        got = mi.paged_prefill_fp8(query, *pool, cu_q, cu_k, table, max_seqlen_q=max(q_lens), total_k=sum(ctxs), scale=scale)
+    mi.check_device_status(device)
+    q = query.double().cpu().numpy()
+    at = np.cumsum([0, *q_lens])
+    parts = [fo.attention(q[at[r]:at[r + 1]], kp, vp, tables[r], c, scale) for r, c in enumerate(ctxs)]
+    return got, [np.concatenate(x) for x in zip(*parts)]
+
+
+# ---------------------------------------------------------------------------
+# values that are nowhere finite: their group's scale is 0
+# ---------------------------------------------------------------------------
+def _stored_rows_that_are_not_finite(device, dtype, d):
+    """Pages as the store leaves them of rows of V without a finite element (but zeros), and tables and contexts."""
+    rng = np.random.default_rng(d)
+    hkv = 2
+    kt = torch.zeros(14, hkv, 1, 16 * d + 16, dtype=torch.uint8, device=device)
+    vt = torch.zeros_like(kt)
+    tables = [[3, 1, 0, 5, 9, 7], [2, 4, 13], [6, -1, -1], [8, 10, 11]]
+    tables = [t + [-1] * (6 - len(t)) for t in tables]
+    q_lens, ctxs = [40, 33, 1, 40], [90, 33, 1, 40]
+    k, v = (rng.standard_normal((sum(ctxs), hkv, d)) for _ in range(2))
+    v[64:80, 0] = np.nan            # sequence 0: a whole group of head 0, beside finite ones
+    v[16:32, 1] = 0.0               # zeros with one NaN among them, of head 1
+    v[20, 1, 3] = np.inf
+    v[90 + 32, :] = -np.inf         # sequence 1: the last group is one token
+    v[90 + 33, 1] = np.nan          # sequence 2: the only key
+    slots = np.concatenate([np.asarray(t)[np.arange(c) // 16] * 16 + np.arange(c) % 16 for t, c in zip(tables, ctxs)])
+    mi.store_kv_fp8(kt, vt, cuda(slots, device), cuda(k, device, dtype), cuda(v, device, dtype))
+    assert [int(vt[b, h, 0, 16 * d]) for b, h in ((9, 0), (1, 1), (13, 0), (13, 1), (6, 1))] == [0] * 5
+    return kt.cpu().numpy(), vt.cpu().numpy(), tables, q_lens, ctxs
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefill_of_values_that_are_nowhere_finite(cuda_device, way, name, d):  # noqa: F811
+    """They are NaN in the rows that see them, and only there, though their group's scale is 0."""
+    dtype = DTYPES[name]
+    kp, vp, tables, q_lens, ctxs = _stored_rows_that_are_not_finite(cuda_device, dtype, d)
+    query = cuda(np.random.default_rng(1).standard_normal((sum(q_lens), 4, d)), cuda_device, dtype)
+    got, want = _attend(cuda_device, query, kp, vp, tables, q_lens, ctxs, d ** -0.5)
+    nan = np.isnan(want[0])
+    assert nan[:40, 2:, 3].all() and not nan[:14, :2].any() and nan[14:40, :2].all()
+    assert nan[72].all() and not nan[40:72].any() and nan[73, 2:].all() and not nan[74:].any()
+    _same(got, want, PREFILL_STEP[dtype])
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("decode", [False, True])
+def test_values_that_are_nowhere_finite(cuda_device, name, d, decode):
+    """The same in decode, and in prefill of every type by the way that it chooses."""
+    dtype = DTYPES[name]
+    kp, vp, tables, q_lens, ctxs = _stored_rows_that_are_not_finite(cuda_device, dtype, d)
+    if decode:
+        q_lens = [1] * 4
+    query = cuda(np.random.default_rng(2).standard_normal((sum(q_lens), 4, d)), cuda_device, dtype)
+    got, want = _attend(cuda_device, query, kp, vp, tables, q_lens, ctxs, d ** -0.5, decode)
+    assert np.isnan(want[0]).any()
+    _same(got, want, (DECODE_STEP if decode else PREFILL_STEP)[dtype])
