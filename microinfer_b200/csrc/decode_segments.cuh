@@ -80,6 +80,19 @@ struct SegMeta {
   int32_t segment, parts;
 };
 
+// Where a CTA's join puts what its parts of a segment hold together, by their flags (1: the segment's first unit, 2: its last):
+// into the result, or into one of the CTA's two states, which a call has only where a second launch was planned.  Without them
+// every segment is whole, unless a wait gave up and its part is missing (the status says so): then there is nowhere to write.
+enum class SegDest { kOut, kEarlier, kGoesOn, kNowhere };
+__host__ __device__ constexpr SegDest segment_dest(int flags, bool states) {
+  return flags == 3 ? SegDest::kOut : !states ? SegDest::kNowhere : (flags & 1) != 0 ? SegDest::kGoesOn : SegDest::kEarlier;
+}
+static_assert(segment_dest(3, false) == SegDest::kOut && segment_dest(3, true) == SegDest::kOut);
+static_assert(segment_dest(0, false) == SegDest::kNowhere && segment_dest(1, false) == SegDest::kNowhere &&
+              segment_dest(2, false) == SegDest::kNowhere);
+static_assert(segment_dest(0, true) == SegDest::kEarlier && segment_dest(2, true) == SegDest::kEarlier &&
+              segment_dest(1, true) == SegDest::kGoesOn);
+
 __device__ __forceinline__ uint32_t movm(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -342,10 +355,11 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
   auto commit = [] {
     if constexpr (!W::kBulk) asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // Whether unit i has come to stage `at` (else the status says so).
+  // Whether unit i has come to stage `at` (else the status says so), the same for every lane: one whose wait gave up takes the
+  // others with it.
   auto arrived = [&](int i, int at) {
     if constexpr (W::kBulk) {
-      return mbar_wait_bounded(bars + at, i / kStages & 1, p.status);
+      return __all_sync(kAll, mbar_wait_bounded(bars + at, i / kStages & 1, p.status)) != 0;
     } else {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");  // this lane's copies
       __syncwarp();                                                         // every lane's
@@ -482,8 +496,10 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
       meta.segment = segment;
       meta.parts = static_cast<int>(cta - blockIdx.x) + 1;
     }
-    has_head |= !(flags & 1);
-    float *state = flags & 1 ? ws + C::kState : ws;
+    const SegDest dest = segment_dest(flags, p.workspace != nullptr);
+    if (dest == SegDest::kNowhere) continue;
+    has_head |= dest == SegDest::kEarlier;
+    float *state = dest == SegDest::kGoesOn ? ws + C::kState : ws;
     T *out = static_cast<T *>(p.out) + row * D;
     for (int e = threadIdx.x; e < heads * D; e += blockDim.x) {
       const int h = e / D;
@@ -491,7 +507,7 @@ __device__ __forceinline__ void decode_segments(const CodedDecodeParams &p, cons
 #pragma unroll 4
       for (int j = j0; j < j1; ++j)
         A = fmaf(factor[j * C::kHeads + h], reinterpret_cast<const float *>(smem)[part_at[j] + e], A);
-      if (flags == 3) {
+      if (dest == SegDest::kOut) {
         out[e] = Elem<T>::from_float(A);
       } else {
         state[e] = A;
