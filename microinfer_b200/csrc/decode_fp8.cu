@@ -232,7 +232,7 @@ struct F8Warp {
           // further down every score is 0; not 0 itself, which a masked score would make a NaN
           factor[j][c][u] = fmaxf(f8_scale(byte[j]) * unit[c][u], 0x1p-126f);
           if (static_cast<int>(byte[j]) > top_byte[c][u]) {  // hardly ever
-            const int e = static_cast<int>(byte[j]) - 127 + power[c][u], near = max(-126, min(kFactorMax, e));
+            const int e = byte[j] == 0 ? -126 : static_cast<int>(byte[j]) - 127 + power[c][u], near = max(-126, min(kFactorMax, e));
             factor[j][c][u] = __uint_as_float(static_cast<uint32_t>(near + 127) << 23) * mantissa;
             const float f = exp2i(max(0, e - kFactorMax));
             x[j][c][0][u] *= f, x[j][c][1][u] *= f;

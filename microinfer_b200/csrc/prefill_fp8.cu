@@ -425,13 +425,13 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
     }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) vb[i] = vb[i] < 0 ? ref : vb[i];  // its keys have no p
-    const bool far_values = ref - v_low > kNear;  // uniform in the CTA; zero groups among them
+    const bool far_values = v_low == 0 || ref - v_low > kNear;  // uniform in the CTA; a byte of 0 is no exponent
     float factor[kGroups][2];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int e = max(-126, min(kFactorMax, kb[i] - 127 + rexp[u]));  // further down every score is 0
+        const int e = kb[i] == 0 ? -126 : max(-126, min(kFactorMax, kb[i] - 127 + rexp[u]));  // further down every score is 0
         factor[i][u] = __uint_as_float(static_cast<uint32_t>(e + 127) << 23) * mantissa;
       }
     if (__any_sync(kAll, far_scores)) {
@@ -439,7 +439,7 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
       for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const int e = kb[i / 2] - 127 + rexp[u >> 1] - kFactorMax;
+          const int e = kb[i / 2] == 0 ? 0 : kb[i / 2] - 127 + rexp[u >> 1] - kFactorMax;
           if (e > 0) s[i][u] *= exp2i(e);
         }
     }

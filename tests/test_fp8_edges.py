@@ -91,3 +91,37 @@ def test_values_that_are_nowhere_finite(cuda_device, name, d, decode):
     got, want = _attend(cuda_device, query, kp, vp, tables, q_lens, ctxs, d ** -0.5, decode)
     assert np.isnan(want[0]).any()
     _same(got, want, (DECODE_STEP if decode else PREFILL_STEP)[dtype])
+
+
+# ---------------------------------------------------------------------------
+# groups of scale 0 are zeros, whatever their codes
+# ---------------------------------------------------------------------------
+def _zero_groups(device, name, d, operand, decode):
+    rng = np.random.default_rng(d)
+    dtype = DTYPES[name]
+    kp, vp = pages(rng, 6, 16, 1, d)
+    (kp if operand == "keys" else vp)[..., 16 * d] = 0
+    ctxs, q_lens = [70], [1 if decode else 20]
+    # queries so large that 2^-127, taken for 0, would give scores
+    query = rng.standard_normal((sum(q_lens), 4, d)) * (1.0 if operand == "values" or name == "f16" else 2.0 ** 120)
+    got, want = _attend(device, cuda(query, device, dtype), kp, vp, [[0, 1, 2, 3, 4, 5]], q_lens, ctxs, 1.0, decode)
+    if operand == "values":
+        assert bool((got == 0).all())
+    else:  # the mean of V
+        close(got, *want, (DECODE_STEP if decode else PREFILL_STEP)[dtype], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("operand", ["keys", "values"])
+def test_prefill_over_groups_of_scale_zero(cuda_device, way, name, d, operand):  # noqa: F811
+    _zero_groups(cuda_device, name, d, operand, False)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("operand", ["keys", "values"])
+@pytest.mark.parametrize("d,decode", [(64, True), (96, True), (96, False), (128, False)])
+def test_attention_over_groups_of_scale_zero(cuda_device, name, operand, d, decode):
+    _zero_groups(cuda_device, name, d, operand, decode)
