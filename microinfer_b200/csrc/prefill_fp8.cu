@@ -479,7 +479,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
 #pragma unroll
       for (int i = 0; i < kKeys / 8; ++i)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) s[i][u] = m[u >> 1] == -INFINITY ? -INFINITY : __fmul_rn(s[i][u], factor[i / 2][u >> 1]) - m[u >> 1];
+        for (int u = 0; u < 4; ++u)  // a row without an m has masked scores and NaN, which stay
+          s[i][u] = __fmul_rn(s[i][u], factor[i / 2][u >> 1]) - (m[u >> 1] == -INFINITY ? 0.f : m[u >> 1]);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) factor[i][0] = factor[i][1] = 1.f;
 #pragma unroll

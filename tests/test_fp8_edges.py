@@ -125,3 +125,40 @@ def test_prefill_over_groups_of_scale_zero(cuda_device, way, name, d, operand): 
 @pytest.mark.parametrize("d,decode", [(64, True), (96, True), (96, False), (128, False)])
 def test_attention_over_groups_of_scale_zero(cuda_device, name, operand, d, decode):
     _zero_groups(cuda_device, name, d, operand, decode)
+
+
+# ---------------------------------------------------------------------------
+# NaN beside large scores
+# ---------------------------------------------------------------------------
+def _nan_beside_large_scores(device, name, where):
+    """Chunks of 16 rows (one warp's) whose row 5 has scores past 2^21, with a NaN in row 9 of q or in key 0."""
+    rng = np.random.default_rng(16)
+    dtype, d = DTYPES[name], 64
+    kp, vp = pages(rng, 4, 16, 1, d)
+    if where == "key":
+        _set_code(kp, False, (0, 0, 0), 0, 11, 127)
+    query = rng.standard_normal((16, 1, d)) * 2.0 ** -12
+    query[5] = np.sign(query[5]) * 2.0 ** 10
+    if where == "query":
+        query[9, 0, 3] = np.nan
+    got, want = _attend(device, cuda(query, device, dtype), kp, vp, [[0, 1]], [16], [16], 2.0 ** 12)
+    if where == "key":  # every row sees it
+        assert bool(torch.isnan(got).all())
+        return
+    assert bool(torch.isnan(got[9]).all())
+    keep = [i for i in range(16) if i not in (5, 9)]  # row 5's one key is as good as any here
+    assert bool(torch.isfinite(got[5]).all())
+    close(got[keep], *(x[keep] for x in want), PREFILL_STEP[dtype], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("where", ["query", "key"])
+def test_prefill_of_nan_beside_large_scores(cuda_device, way, name, where):  # noqa: F811
+    _nan_beside_large_scores(cuda_device, name, where)
+
+
+@gpu
+@pytest.mark.parametrize("where", ["query", "key"])
+def test_prefill_of_nan_beside_large_scores_in_fp32(cuda_device, where):
+    _nan_beside_large_scores(cuda_device, "f32", where)
