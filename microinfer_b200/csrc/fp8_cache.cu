@@ -343,8 +343,8 @@ __device__ __forceinline__ void write8(T *dst, const float (&x)[8]) {
 }
 
 // grid (groups of 16 positions x kv heads, 8 warps to a CTA; sequences).  REDO: rows for the dense prefill, which cannot
-// do NaN of V (0 * NaN reaches rows that do not see the key; one of K only meets its own scores) nor values past fp16:
-// the sequences and heads that have some are noted.
+// do NaN of V (0 * NaN reaches rows that do not see the key; one of K only meets its own scores) nor values at the ends of
+// the range: the sequences and heads that have some are noted.
 template <typename T, int NB, bool REDO>
 __global__ void __launch_bounds__(256) fp8_gather_kernel(const CodedGatherParams p, const FastDiv by_heads,
                                                          const FastDiv by_page) {
@@ -399,7 +399,13 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const CodedGatherParams
   const uint8_t *kg = p.key_pages + off, *vg = p.value_pages + off;
   const uint32_t kbyte = __ldg(kg + kF8Group * D), vbyte = __ldg(vg + kF8Group * D);
   const float ks = f8_scale(kbyte), vs = f8_scale(vbyte);
-  const bool far = REDO && std::is_same<T, __half>::value && max(kbyte, vbyte) >= 127u + 8u;  // 448 * 2^7 < 65504
+  // What the dense kernel does not hold.  fp16: values past its range, and of K those that lose bits below its smallest step (of V
+  // they are as small in the result).  bf16, whose sums of products meet the softmax's scale behind them: K
+  // beyond 2^-64 to 2^64, V above it, whose sums over a long context leave fp32's range.
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  const bool far = REDO && kHalf && max(kbyte, vbyte) >= 127u + 8u;         // 448 * 2^7 < 65504
+  const bool low = REDO && kHalf && kbyte != 0 && kbyte < 127u + 9u - 24u;  // codes are multiples of 2^-9
+  if (REDO && !kHalf) apart |= max(kbyte, vbyte) > 127u + 64u || (kbyte != 0 && kbyte < 127u - 64u);
   constexpr int kHeld = NB > 0 ? NB : 1;
   constexpr bool kWhole = NB > 0 && NB % 2 == 0;
   for (int i0 = 0; i0 < items; i0 += kHeld) {
@@ -443,6 +449,9 @@ __global__ void __launch_bounds__(256) fp8_gather_kernel(const CodedGatherParams
           if (far)
 #pragma unroll
             for (int n = 0; n < 8; ++n) apart |= fmaxf(fabsf(x[n]), fabsf(y[n])) > 65504.f;  // the next one is 65536
+          if (low)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) apart |= __half2float(__float2half_rn(x[n])) != x[n];
         }
       }
     }

@@ -162,3 +162,51 @@ def test_prefill_of_nan_beside_large_scores(cuda_device, way, name, where):  # n
 @pytest.mark.parametrize("where", ["query", "key"])
 def test_prefill_of_nan_beside_large_scores_in_fp32(cuda_device, where):
     _nan_beside_large_scores(cuda_device, "f32", where)
+
+
+# ---------------------------------------------------------------------------
+# the ends of the range in each way of prefill, at the dense kernel's head_dim
+# ---------------------------------------------------------------------------
+def _range_case(device, name, d, k_byte, q_power, v_byte, scale, decode=False):
+    rng = np.random.default_rng(abs(q_power) + k_byte)
+    kb = np.clip(k_byte - rng.integers(0, 3, (5, 1, 1)), 1, 246).astype(np.uint8)
+    vb = np.clip(v_byte - rng.integers(0, 3, (5, 1, 1)), 1, 246).astype(np.uint8)
+    kp = fo.pack(fo.codes_of(30 * rng.standard_normal((5, 16, 1, d))), kb, False)
+    vp = fo.pack(fo.codes_of(30 * rng.standard_normal((5, 16, 1, d))), vb, True)
+    n = 1 if decode else 3
+    query = cuda(rng.standard_normal((n, 2, d)) * 2.0 ** q_power, device, DTYPES[name])
+    return _attend(device, query, kp, vp, [[0, 1, 2, 3, 4]], [n], [70], float(np.float32(scale)), decode)
+
+
+@gpu
+@pytest.mark.parametrize("name,k_byte,q_power,v_byte", [
+    ("bf16", 246, -100, 246), ("bf16", 1, 90, 1), ("bf16", 246, 0, 127), ("bf16", 127, -120, 200), ("bf16", 20, 20, 10),
+    ("bf16", 230, 10, 60), ("f16", 246, -14, 130), ("f16", 105, 8, 127), ("f16", 20, 8, 118), ("f16", 111, 10, 120)])
+def test_prefill_over_the_whole_range_of_scales(cuda_device, way, name, k_byte, q_power, v_byte):  # noqa: F811
+    scale = 2.0 ** np.clip(127 - k_byte - q_power - 6, -100, 100)  # scores of about 1
+    got, want = _range_case(cuda_device, name, 128, k_byte, q_power, v_byte, scale)
+    close(got, *want, PREFILL_STEP[DTYPES[name]], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("v_byte", [246, 190])
+def test_prefill_of_large_values_over_a_long_context(cuda_device, way, v_byte):  # noqa: F811
+    """Sums of p v are past fp32's range, their mean is not."""
+    rng = np.random.default_rng(v_byte)
+    d, ctx = 128, 3000
+    nb = -(-ctx // 16)
+    kp, vp = pages(rng, nb, 16, 1, d)
+    codes = fo.codes_of(30 * np.abs(rng.standard_normal((nb, 16, 1, d))))
+    vp = fo.pack(codes, np.full((nb, 1, 1), v_byte, dtype=np.uint8), True)
+    query = cuda(rng.standard_normal((40, 2, d)), cuda_device, torch.bfloat16)
+    got, want = _attend(cuda_device, query, kp, vp, [np.arange(nb)], [40], [ctx], d ** -0.5)
+    close(got, *want, PREFILL_STEP[torch.bfloat16], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("spread,scale", [(0.5, 2.0), (0.5, 0.0), (0.5, -0.3), (5.0, None), (0.5, 2.0 ** -40)])
+def test_prefill_scales(cuda_device, way, name, spread, scale):  # noqa: F811
+    got, free, want = prefill_case(cuda_device, name, 2, 4, 128, 16, [50, 20], [70, 150], scale=scale, spread=spread)
+    for x in (got, free):
+        close(x, *want, PREFILL_STEP[DTYPES[name]], lost=DENSE_LOST)
