@@ -129,12 +129,8 @@ struct F8Warp {
   }
   // ... as f16 fragments.
   __device__ __forceinline__ void set_query(const Raw &raw, float scale_log2) {
-    // the scale's sign goes into q, so that the largest product is the largest score; a scale of 0 becomes one that leaves
-    // every score at 0
-    const float scale = fmaxf(fabsf(scale_log2), 1e-30f);
-    const bool whole = scale < INFINITY;
-    const int scale_exp = whole ? static_cast<int>(__float_as_uint(scale) >> 23) - 127 : 0;
-    mantissa = whole ? __uint_as_float((__float_as_uint(scale) & 0x7fffffu) | 0x3f800000u) : scale;
+    const F8Scale scale = f8_softmax_scale(scale_log2);
+    mantissa = scale.mantissa;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       float x[NB][8];
@@ -160,9 +156,9 @@ struct F8Warp {
       top = max(top, __shfl_xor_sync(kAll, top, 1));
       top = max(top, __shfl_xor_sync(kAll, top, 2));
       int e = 14 - (static_cast<int>(top >> 23) - 127);  // largest element to [2^14, 2^15)
-      if (top >= 0x7f800000u) e = 0;                     // not finite: as it is
+      if (top >= 0x7f800000u || top == 0 || scale.sign == 0.f) e = 0;  // not finite: as it is; nor do zeros need a power
       e = min(e, 126);
-      const float f = exp2i(e) * (scale_log2 < 0.f ? -1.f : 1.f);
+      const float f = exp2i(e) * scale.sign;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -175,7 +171,7 @@ struct F8Warp {
       }
 #pragma unroll
       for (int u = 0; u < kCols; ++u) {  // a lane of this query head: its column is 2t + u
-        const int e2 = scale_exp - __shfl_sync(kAll, e, 4 * (2 * t + u));
+        const int e2 = scale.exponent - __shfl_sync(kAll, e, 4 * (2 * t + u));
         power[c][u] = e2;
         const bool normal = e2 >= -126 && e2 <= kFactorMax;
         unit[c][u] = __uint_as_float(static_cast<uint32_t>((normal ? e2 : 0) + 127) << 23) * mantissa;

@@ -81,6 +81,27 @@ __device__ __forceinline__ uint32_t f8_encode4(float a, float b, float c, float 
 // Whether one of a word's codes is a NaN.
 __device__ __forceinline__ bool f8_any_nan(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
 
+// The softmax's scale (log2 domain) taken apart: its magnitude is mantissa * 2^exponent, the mantissa in [1, 2) or an infinity,
+// and q is multiplied by its sign, so that the largest product is the largest score.  Of a scale of 0 or NaN the
+// sign is 0 or NaN, which makes every score that, and the rest stands for 1.
+struct F8Scale {
+  float mantissa, sign;
+  int exponent;
+};
+__host__ __device__ __forceinline__ F8Scale f8_softmax_scale(float scale) {
+  F8Scale r = {1.f, scale, 0};
+  const float a = fabsf(scale);
+  if (a > 0.f) {
+    r.sign = scale < 0.f ? -1.f : 1.f;
+    r.mantissa = a;
+    if (a < INFINITY) {
+      r.mantissa = 2.f * frexpf(a, &r.exponent);
+      --r.exponent;
+    }
+  }
+  return r;
+}
+
 // 2^(b - 127), 0 for 0.
 __device__ __forceinline__ float f8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 

@@ -136,12 +136,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
   const int per_split = (all_tiles + p.num_splits - 1) / p.num_splits;
   const int k_begin = split * per_split, k_end = min(all_tiles, k_begin + per_split);
 
-  // The scale's sign goes into q, so that the largest product is the largest score; its exponent to the rows'.  A scale of 0
-  // becomes one that leaves every score at 0.
-  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
-  const bool whole = scale < INFINITY;
-  const int scale_exp = whole ? static_cast<int>(__float_as_uint(scale) >> 23) - 127 : 0;
-  const float mantissa = whole ? __uint_as_float((__float_as_uint(scale) & 0x7fffffu) | 0x3f800000u) : scale;
+  const F8Scale scale = f8_softmax_scale(p.scale_log2);  // its exponent goes to the rows'
+  const float mantissa = scale.mantissa;
 
   // ---- copies of a tile's codes: a thread's chunks, in the order of memory, K's, then V's ----
   struct Chunk {
@@ -326,9 +322,10 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
     }
     top = max(top, __shfl_xor_sync(kAll, top, 1));
     top = max(top, __shfl_xor_sync(kAll, top, 2));
-    int e = top >= 0x7f800000u ? 0 : min(14 - (static_cast<int>(top >> 23) - 127), 126);  // not finite: as it is
-    const float f = exp2i(e) * (p.scale_log2 < 0.f ? -1.f : 1.f);
-    if (t == 0) row_exp[r] = scale_exp - e;
+    // not finite: as it is; nor do zeros need a power
+    const int e = top >= 0x7f800000u || top == 0 || scale.sign == 0.f ? 0 : min(14 - (static_cast<int>(top >> 23) - 127), 126);
+    const float f = exp2i(e) * scale.sign;
+    if (t == 0) row_exp[r] = scale.exponent - e;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
 #pragma unroll

@@ -134,7 +134,8 @@ __device__ __forceinline__ int largest_byte(uint32_t a, uint32_t b) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_prefill_tc_kernel(const __grid_constant__ CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page) {
+    fp8_prefill_tc_kernel(const __grid_constant__ CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page,
+                          const __grid_constant__ F8Scale scale) {
   using C = TcCfg<D>;
   constexpr int kKStages = C::kKStages;
   constexpr uint32_t kIdescQK = tc::idesc_f16(128, 128, 0, false);
@@ -191,11 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int x = warp >> 2, r = threadIdx.x & 127;  // query tile, TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + x * 128 + lane_off, tO = tmem + 256 + x * 128 + lane_off;
-    const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
-    const float mantissa = scale < INFINITY ? __uint_as_float((__float_as_uint(scale) & 0x7fffffu) | 0x3f800000u) : scale;
     const int G = p.num_q_heads / p.num_kv_heads;
-    const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;  // into q, so that the largest product is the largest score
-    const int scale_exp = scale < INFINITY ? static_cast<int>(__float_as_uint(scale) >> 23) - 127 : 0;
     uint32_t sc = 0, uses = 0, tiles = 0;
     bool ok = true, odd = false;
     F8Meta meta = {0, 0, 0, 0};
@@ -227,9 +224,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint16_t most = static_cast<uint16_t>(max(top & 0xffffu, top >> 16));
       top = __float_as_uint(Elem<T>::to_float(*reinterpret_cast<const T *>(&most)));
-      // not finite: as it is; nor does a row of zeros need a power
-      const int e = top >= 0x7f800000u || top == 0 ? 0 : min(14 - (static_cast<int>(top >> 23) - 127), 126);
-      const float f = exp2i(e) * sign;
+      // not finite: as it is; nor do zeros need a power
+      const int e = top >= 0x7f800000u || top == 0 || scale.sign == 0.f ? 0 : min(14 - (static_cast<int>(top >> 23) - 127), 126);
+      const float f = exp2i(e) * scale.sign;
       uint8_t *to = smem + C::kOffQ + x * C::kTile + r * 128;
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
@@ -241,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&bar[B_QFULL + x]);
-      return scale_exp - e;
+      return scale.exponent - e;
     };
     const F8Item *it = get(0);
     int power = load_q(it);
@@ -276,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t none = *reinterpret_cast<const uint32_t *>(entry + 16);
         if (j == j0) {
           const bool normal = power >= -126 && power <= kFactorMax;
-          unit = __uint_as_float(static_cast<uint32_t>((normal ? power : 0) + 127) << 23) * mantissa;
+          unit = __uint_as_float(static_cast<uint32_t>((normal ? power : 0) + 127) << 23) * scale.mantissa;
           top_byte = normal ? kFactorMax + 127 - power : -1;
         }
         tc::tmem_wait_ld();
@@ -758,7 +755,8 @@ cudaError_t launch_tc(const CodedPrefillParams &p, cudaStream_t stream) {
   }
   const int ctas = sm_count_current();
   const FastDiv by_group(p.num_q_heads / p.num_kv_heads), by_page(p.block_size / kF8Group);
-  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(kThreads), C::kSmem, stream, p, by_group, by_page);
+  cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(kThreads), C::kSmem, stream, p, by_group, by_page,
+                             f8_softmax_scale(p.scale_log2));
   if (e == cudaSuccess)
     e = launch_pdl(fp8_prefill_tc_join_kernel<T, D>, dim3(ctas, 8), dim3(256), 0, stream, p, by_group, ctas);
   return e;

@@ -210,3 +210,33 @@ def test_prefill_scales(cuda_device, way, name, spread, scale):  # noqa: F811
     got, free, want = prefill_case(cuda_device, name, 2, 4, 128, 16, [50, 20], [70, 150], scale=scale, spread=spread)
     for x in (got, free):
         close(x, *want, PREFILL_STEP[DTYPES[name]], lost=DENSE_LOST)
+
+
+# ---------------------------------------------------------------------------
+# the softmax's scale: 0, far below any other, not a number
+# ---------------------------------------------------------------------------
+SCALES = [(246, 0.0), (230, 2.0 ** -110), (246, 2.0 ** -126), (246, -2.0 ** -127), (127, float("nan"))]
+
+
+def _softmax_scale(device, name, d, k_byte, scale, decode):
+    got, want = _range_case(device, name, d, k_byte, 0, 127, scale, decode)
+    if np.isnan(scale):
+        assert bool(torch.isnan(got).all())
+    else:
+        close(got, *want, (DECODE_STEP if decode else PREFILL_STEP)[DTYPES[name]], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("k_byte,scale", SCALES)
+def test_prefill_of_any_softmax_scale(cuda_device, way, name, d, k_byte, scale):  # noqa: F811
+    _softmax_scale(cuda_device, name, d, k_byte, scale, False)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("k_byte,scale", SCALES)
+def test_any_softmax_scale(cuda_device, name, decode, k_byte, scale):
+    _softmax_scale(cuda_device, name, 96, k_byte, scale, decode)
