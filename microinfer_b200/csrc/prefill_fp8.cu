@@ -637,19 +637,23 @@ __global__ void __launch_bounds__(kThreads, P8Cfg<T, NB>::kCtas)
 }
 
 // After the tcgen05 kernel: the sequences and kv heads in whose CTAs it met what it cannot do, over again.  Hardly ever any.
+// Their tiles are dealt out in turn, across them: short chunks have one each.
 template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, 1)
     fp8_prefill_redo_kernel(const CodedPrefillParams p, const FastDiv by_group, const FastDiv by_page, int ctas) {
   __shared__ int64_t prefix[kF8MaxSeqs + 1], scratch[32];
+  __shared__ bool met[kF8MaxCtas];
   pdl_wait();
-  const uint8_t *odd = f8_odd(p, NB * 32, ctas);
+  const uint64_t *odd = reinterpret_cast<const uint64_t *>(f8_odd(p, NB * 32, ctas));  // a byte for each warp of a CTA
   bool any = false;
-  for (int i = threadIdx.x; i < ctas * 8; i += kThreads) any |= odd[i] != 0;
+  for (int i = threadIdx.x; i < ctas; i += kThreads) any |= met[i] = odd[i] != 0;
   if (!__syncthreads_or(any)) {
     pdl_launch_dependents();
     return;
   }
   const F8Work work = f8_work(p, by_group, prefix, scratch, ctas);
+  const int grid = gridDim.x;
+  int turn = blockIdx.x;  // tiles until this CTA's next
   for (int seq = 0; seq < p.num_seqs; ++seq) {
     const int64_t cost = (prefix[seq + 1] - prefix[seq]) / p.num_kv_heads;
     if (cost == 0) continue;
@@ -659,12 +663,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t from = prefix[seq] + kvh * cost;
       const int first = static_cast<int>(from / work.share), last = static_cast<int>((from + cost - 1) / work.share);
       any = false;
-      for (int i = first * 8 + threadIdx.x; i < (last + 1) * 8; i += kThreads) any |= odd[i] != 0;
-      if (!__syncthreads_or(any)) continue;
-      for (int tile = blockIdx.x; tile < (q.rows + kRows - 1) / kRows; tile += gridDim.x) {
-        prefill_tile<T, NB>(p, by_group, by_page, seq, kvh, tile, 0);
+      for (int i = first; i <= last; ++i) any |= met[i];
+      if (!any) continue;
+      const int tiles = (q.rows + kRows - 1) / kRows;
+      for (; turn < tiles; turn += grid) {
+        prefill_tile<T, NB>(p, by_group, by_page, seq, kvh, turn, 0);
         __syncthreads();  // every warp has read what the next tile overwrites
       }
+      turn -= tiles;
     }
   }
   pdl_launch_dependents();

@@ -13,6 +13,7 @@
 namespace mi {
 
 constexpr int kF8MaxSeqs = 1024;  // of one launch (prefix sums in shared memory)
+constexpr int kF8MaxCtas = 1024;
 constexpr int kPairCost = 7, kSingleCost = 4, kUnitCost = 8;
 constexpr int kLeastShare = 28;   // of a CTA: above kUnitCost + kPairCost, so every CTA inside a unit has a tile of it
 

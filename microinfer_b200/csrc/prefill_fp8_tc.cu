@@ -771,7 +771,7 @@ cudaError_t launch_tc(const CodedPrefillParams &p, cudaStream_t stream) {
 // 4000 58 : 58, 1 x 512 on 16000 118 : 276, 4 x 1024 on 4000 194 : 655.
 bool fp8_prefill_tc_takes(int dtype, int head_dim, int64_t num_blocks, int block_size, int num_q_heads, int num_kv_heads,
                           int64_t num_seqs, int64_t max_seqlen_q, int64_t max_context, int sms) {
-  if ((dtype != MI_DTYPE_BFLOAT16 && dtype != MI_DTYPE_FLOAT16) || (head_dim != 64 && head_dim != 128) ||
+  if ((dtype != MI_DTYPE_BFLOAT16 && dtype != MI_DTYPE_FLOAT16) || (head_dim != 64 && head_dim != 128) || sms > kF8MaxCtas ||
       num_blocks >= (int64_t{1} << 31) / num_kv_heads / (block_size / kF8Group))  // places are 32 bits here
     return false;
   const int64_t rows = max_seqlen_q * (num_q_heads / num_kv_heads);

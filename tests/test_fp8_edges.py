@@ -240,3 +240,39 @@ def test_prefill_of_any_softmax_scale(cuda_device, way, name, d, k_byte, scale):
 @pytest.mark.parametrize("k_byte,scale", SCALES)
 def test_any_softmax_scale(cuda_device, name, decode, k_byte, scale):
     _softmax_scale(cuda_device, name, 96, k_byte, scale, decode)
+
+
+# ---------------------------------------------------------------------------
+# what is done over
+# ---------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("distance", [12, 13, 16, 40])
+def test_prefill_of_scales_that_fall_from_tile_to_tile(cuda_device, way, d, distance):  # noqa: F811
+    """V's scales fall by 2^distance between the first tile of keys and the next ones: the keys behind count."""
+    def edit(kp, vp, table):
+        for pos in range(0, 700, 16):
+            _set_byte(vp, table[0, pos // 16], 0, 0, 150 - (distance if pos >= 128 else 0))
+        _set_code(vp, True, _place(5, table[0]), 0, 0, 0)
+
+    got, free, want = prefill_case(cuda_device, "bf16", 1, 2, d, 16, [300, 30], [700, 30], edit=edit)
+    for x in (got, free):
+        close(x, *want, PREFILL_STEP[torch.bfloat16], lost=DENSE_LOST)
+
+
+@gpu
+@pytest.mark.parametrize("name,d", [("bf16", 64), ("f16", 128)])
+def test_prefill_of_many_sequences_with_a_nan_each(cuda_device, way, name, d):  # noqa: F811
+    rng = np.random.default_rng(d)
+    count, hkv = 260, 2
+    q_lens = rng.integers(1, 4, count)
+    ctxs = (q_lens + rng.integers(0, 30, count)).tolist()
+    nb = sum(-(-c // 16) for c in ctxs)
+    kp, vp = pages(rng, nb, 16, hkv, d)
+    tables = table_of(rng, ctxs, nb, 16)
+    for r, c in enumerate(ctxs):
+        if r % 7:
+            _set_code(vp, True, _place(int(rng.integers(0, c)), tables[r]), r % hkv, r % d, 127)
+    query = cuda(rng.standard_normal((int(q_lens.sum()), 2 * hkv, d)), cuda_device, DTYPES[name])
+    got, want = _attend(cuda_device, query, kp, vp, tables, q_lens.tolist(), ctxs, d ** -0.5)
+    _same(got, want, PREFILL_STEP[DTYPES[name]])
