@@ -313,7 +313,7 @@ struct F8Warp {
       }
       if (first) ref = max(byte[0], byte[1]) + 2;  // two binades of room
     }
-    // m follows the largest score, up to kLag binades behind it
+    // m follows the largest score, up to kLag binades behind it (by the difference: m + kLag may round to m + 4 from 2^24 on)
     float top[CT][kCols];
     bool behind = false;
 #pragma unroll
@@ -322,7 +322,7 @@ struct F8Warp {
       for (int u = 0; u < kCols; ++u) {
         top[c][u] = fmaxf(fmaxf(x[0][c][0][u], x[0][c][1][u]) * factor[0][c][u],
                           fmaxf(x[1][c][0][u], x[1][c][1][u]) * factor[1][c][u]);
-        behind |= top[c][u] > m[c][u] + kLag;
+        behind |= top[c][u] - m[c][u] > kLag;
       }
     if (__any_sync(kAll, behind)) {
 #pragma unroll

@@ -457,7 +457,7 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
       for (int u = 0; u < 2; ++u)
         top[u] = fmaxf(top[u], fmaxf(fmaxf(s[2 * i][2 * u], s[2 * i][2 * u + 1]),
                                      fmaxf(s[2 * i + 1][2 * u], s[2 * i + 1][2 * u + 1])) * factor[i][u]);
-    if (__any_sync(kAll, top[0] > m[0] + kLag || top[1] > m[1] + kLag)) {
+    if (__any_sync(kAll, top[0] - m[0] > kLag || top[1] - m[1] > kLag)) {  // m + kLag may round to m + 4 from 2^24 on
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         top[i] = fmaxf(top[i], __shfl_xor_sync(kAll, top[i], 1));

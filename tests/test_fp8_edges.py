@@ -276,3 +276,46 @@ def test_prefill_of_many_sequences_with_a_nan_each(cuda_device, way, name, d):  
     query = cuda(rng.standard_normal((int(q_lens.sum()), 2 * hkv, d)), cuda_device, DTYPES[name])
     got, want = _attend(cuda_device, query, kp, vp, tables, q_lens.tolist(), ctxs, d ** -0.5)
     _same(got, want, PREFILL_STEP[DTYPES[name]])
+
+
+# ---------------------------------------------------------------------------
+# scores of which fp32 has only every second or fourth whole number
+# ---------------------------------------------------------------------------
+def _steps_case(device, name, d, power, run, decode):
+    """Runs of keys whose largest score is in turn 2^power and a step or two of fp32 (up to 4) above it; V of the latter is 4, V's
+    reference after the first, so that p goes in as it is: within f16."""
+    ctx = 1280
+    nb = ctx // 16
+    high = np.arange(nb) * 16 // run % 2 == 1
+    k, v = np.zeros((nb, 16, 1, d)), np.ones((nb, 16, 1, d))
+    k[..., 0] = 1.0
+    k[high, 3, 0, 1] = 1.0
+    v[high] = 4.0
+    kp, vp = fo.pack(*fo.encode(k), False), fo.pack(*fo.encode(v), True)
+    rows = 1 if decode else 2
+    query = np.zeros((rows, 1, d))
+    query[:, 0, 0], query[:, 0, 1] = 1.0, 2.0 ** (2 - power)
+    # a softmax scale whose product with log2(e) in fp32 is 2^power, or a few steps above
+    scale = np.float32(2.0 ** power / np.log2(np.e))
+    while float(scale * np.float32(np.log2(np.e))) % 4 or float(scale * np.float32(np.log2(np.e))) < 2.0 ** power:
+        scale = np.nextafter(scale, np.float32(np.inf))
+    got, want = _attend(device, cuda(query, device, DTYPES[name]), kp, vp, [np.arange(nb)], [rows], [ctx], float(scale), decode)
+    # scores are off by a step, two at most: p by 2^(2^(power - 22)) against the others, the mean stays between 1 and 4
+    assert bool(torch.isfinite(got).all()) and bool((got >= 1 - 2.0 ** -7).all()) and bool((got <= 4 + 2.0 ** -5).all())
+    if power <= 23:
+        assert np.abs(got.double().cpu().numpy() - want[0]).max() < 3.0 * (2.0 ** 2.0 ** (power - 22) - 1)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("power", [18, 20, 22, 23, 24])
+@pytest.mark.parametrize("d,run,decode", [(64, 32, True), (128, 32, True), (64, 64, False), (96, 64, False)])
+def test_largest_scores_a_step_apart(cuda_device, name, power, d, run, decode):
+    _steps_case(cuda_device, name, d, power, run, decode)
+
+
+@gpu
+@pytest.mark.parametrize("d,run", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("power", [18, 20, 22, 23, 24])
+def test_prefill_of_largest_scores_a_step_apart(cuda_device, way, d, run, power):  # noqa: F811
+    _steps_case(cuda_device, "bf16", d, power, run, False)
