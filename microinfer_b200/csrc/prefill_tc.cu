@@ -90,6 +90,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
   return *reinterpret_cast<uint32_t *>(&h);
 }
 
+// A pair of p.  In fp16 the lift and m's lag bring p up to 2^15, and m rounds away up to another binade or two of scores from 2^24
+// on: the largest finite one then, not an infinity.
+__device__ __forceinline__ uint32_t pack_p(float a, float b, bool bf16) {
+  if (bf16) return pack2(a, b, true);
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -536,7 +545,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
             const float2 a2 = ffma2(make_float2(sr[q * 16 + 2 * i], sr[q * 16 + 2 * i + 1]), sc2, nb2);
             const float2 e = make_float2(fast_exp2(a2.x), fast_exp2(a2.y));
             sum2[i & 1] = fadd2(sum2[i & 1], e);
-            pk[i] = __uint_as_float(pack2(e.x, e.y, kBf16));
+            pk[i] = __uint_as_float(pack_p(e.x, e.y, kBf16));
           }
           tc::tmem_st8(tS + q * 8, pk);
         }

@@ -281,8 +281,8 @@ def test_prefill_of_many_sequences_with_a_nan_each(cuda_device, way, name, d):  
 # ---------------------------------------------------------------------------
 # scores of which fp32 has only every second or fourth whole number
 # ---------------------------------------------------------------------------
-def _steps_case(device, name, d, power, run, decode):
-    """Runs of keys whose largest score is in turn 2^power and a step or two of fp32 (up to 4) above it; V of the latter is 4, V's
+def _steps_case(device, name, d, power, run, decode, ahead=4):
+    """Runs of keys whose largest score is in turn 2^power and `ahead` above it, a few steps of fp32; V of the latter is 4, V's
     reference after the first, so that p goes in as it is: within f16."""
     ctx = 1280
     nb = ctx // 16
@@ -294,7 +294,7 @@ def _steps_case(device, name, d, power, run, decode):
     kp, vp = fo.pack(*fo.encode(k), False), fo.pack(*fo.encode(v), True)
     rows = 1 if decode else 2
     query = np.zeros((rows, 1, d))
-    query[:, 0, 0], query[:, 0, 1] = 1.0, 2.0 ** (2 - power)
+    query[:, 0, 0], query[:, 0, 1] = 1.0, ahead * 2.0 ** -power
     # a softmax scale whose product with log2(e) in fp32 is 2^power, or a few steps above
     scale = np.float32(2.0 ** power / np.log2(np.e))
     while float(scale * np.float32(np.log2(np.e))) % 4 or float(scale * np.float32(np.log2(np.e))) < 2.0 ** power:
@@ -315,7 +315,8 @@ def test_largest_scores_a_step_apart(cuda_device, name, power, d, run, decode):
 
 
 @gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
 @pytest.mark.parametrize("d,run", [(64, 64), (64, 128), (128, 64), (128, 128)])
-@pytest.mark.parametrize("power", [18, 20, 22, 23, 24])
-def test_prefill_of_largest_scores_a_step_apart(cuda_device, way, d, run, power):  # noqa: F811
-    _steps_case(cuda_device, "bf16", d, power, run, False)
+@pytest.mark.parametrize("power,ahead", [(18, 4), (20, 4), (22, 4), (23, 4), (24, 4), (24, 8), (26, 8), (27, 16), (28, 0), (31, 0)])
+def test_prefill_of_largest_scores_a_step_apart(cuda_device, way, name, d, run, power, ahead):  # noqa: F811
+    _steps_case(cuda_device, name, d, power, run, False, ahead)
