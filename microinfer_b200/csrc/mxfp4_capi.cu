@@ -16,7 +16,8 @@ int capi_varlen_prefill_lifted(void *out, const void *query, const void *keys, c
                                int64_t kv_token_stride, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                int32_t dtype, const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k,
                                int64_t num_seqs, int64_t num_tokens, int64_t num_kv_tokens, int32_t max_seqlen_q,
-                               float scale, float p_lift, int32_t *dev_status, void *stream);
+                               float scale, float p_lift, uint8_t *redo, int64_t redo_stride, int32_t *dev_status,
+                               void *stream);
 
 cudaError_t launch_mxfp4_store(const CodedStoreParams &p, int dtype, int index_dtype, bool vec,
                                cudaStream_t stream);
@@ -352,7 +353,8 @@ int mi_paged_prefill_mxfp4_gathered(void *out, const void *query, const void *ke
   const float p_lift = dtype == MI_DTYPE_FLOAT16 ? 7.f : 0.f;  // small p keep their bits, as in the kernels on the pages
   if (const int s = capi_varlen_prefill_lifted(
           out, query, keys, values, static_cast<int64_t>(num_kv_heads) * head_dim, num_q_heads, num_kv_heads, head_dim, dtype,
-          cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens, kv_rows, max_seqlen_q, scale, p_lift, dev_status, stream))
+          cu_seqlens_q, cu_seqlens_k, num_seqs, num_tokens, kv_rows, max_seqlen_q, scale, p_lift,
+          p_lift != 0.f ? redo : nullptr, groups, dev_status, stream))
     return s;
   if (redo == nullptr) return MI_OK;
   CodedPrefillParams p = {};

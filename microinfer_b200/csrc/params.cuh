@@ -73,6 +73,10 @@ struct AttnParams {
   // The tensor-core prefill kernel holds p as 2^(x - m + p_lift), m up to 8 binades behind: up to 7 in fp16, whose
   // small p otherwise lose bits from 2^-14 of the largest on.
   float p_lift;
+  // Where it notes, with the lift, the sequences and kv heads with an m past 2^20: there m is off by more than p has room
+  // for in fp16.  [seq][kv head][redo_stride], the first byte is set; null: nowhere.
+  uint8_t *redo;
+  int64_t redo_stride;
 };
 struct DecodeParams {
   void *out;

@@ -48,6 +48,8 @@ struct __align__(64) PrefillTcParams {
   int32_t paged;
   float scale_log2;
   float p_lift;  // p is 2^(x - m + p_lift)
+  uint8_t *redo;  // with the lift: where a sequence and kv head whose m is past 2^20 is noted (params.cuh), or null
+  int64_t redo_stride;
   int32_t *status;
   // Mixed batches: sequences with one query token are left to the decode kernel
   // launched right after this one, which may start once every CTA here has passed
@@ -88,15 +90,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
   }
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t *>(&h);
-}
-
-// A pair of p.  In fp16 the lift and m's lag bring p up to 2^15, and m rounds away up to another binade or two of scores from 2^24
-// on: the largest finite one then, not an infinity.
-__device__ __forceinline__ uint32_t pack_p(float a, float b, bool bf16) {
-  if (bf16) return pack2(a, b, true);
-  uint32_t r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  return r;
 }
 
 }  // namespace
@@ -545,7 +538,7 @@ __global__ void __launch_bounds__(kThreads2, 1)
             const float2 a2 = ffma2(make_float2(sr[q * 16 + 2 * i], sr[q * 16 + 2 * i + 1]), sc2, nb2);
             const float2 e = make_float2(fast_exp2(a2.x), fast_exp2(a2.y));
             sum2[i & 1] = fadd2(sum2[i & 1], e);
-            pk[i] = __uint_as_float(pack_p(e.x, e.y, kBf16));
+            pk[i] = __uint_as_float(pack2(e.x, e.y, kBf16));
           }
           tc::tmem_st8(tS + q * 8, pk);
         }
@@ -576,6 +569,8 @@ __global__ void __launch_bounds__(kThreads2, 1)
         if (!ok) break;
         tc::fence_after_sync();
       }
+      if (!kBf16 && p.redo != nullptr && rvalid && fabsf(m) > 0x1p20f && m != -INFINITY)
+        p.redo[(it.seq * p.num_kv_heads + it.kvh) * p.redo_stride] = 1;
       const float inv = l > 0.f ? 1.f / l : 0.f;
       T *orow = out + (static_cast<int64_t>(it.q_start + it.t0 + x * TQ + tok) * p.num_q_heads +
                        it.kvh * G + r % G) * 128;
@@ -705,6 +700,8 @@ cudaError_t launch_prefill_tc(const AttnParams &a, int dtype, int G, int32_t max
   // A masked score is an infinity times the scale, so a scale of 0 is one that leaves every finite score at 0.
   p.scale_log2 = a.scale_log2 == 0.f ? 1e-30f : a.scale_log2;
   p.p_lift = a.p_lift;
+  p.redo = a.redo;
+  p.redo_stride = a.redo_stride;
   p.status = a.status;
   p.skip_single = paged && a.mixed_decode ? 1 : 0;
   const int64_t n = a.num_seqs;
