@@ -108,6 +108,13 @@ __device__ __forceinline__ float fmin3(float a, float b, float c) {
   return r;
 }
 
+// The smaller of two, NaN if one is.
+__device__ __forceinline__ float fmin_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // n / d by a multiplication, n below 2^31.
 struct FastDiv {
   uint32_t mul;

@@ -53,6 +53,7 @@ namespace {
 constexpr int kQueries = 4;          // query heads of a column tile
 constexpr float kLift = 12.f;       // p is held as 2^(x - m + kLift): f16 reaches 2^-37 of the largest p
 constexpr float kLag = 3.f;         // m may be this far behind: p <= 2^15
+constexpr float kExact = 0x1p20f;   // kLift - m is off by 2^-4 at most for m up to here
 constexpr uint32_t kLowestRef = 0x20202020u;  // R_b - 255 then has a bit of 0xf8 set, like every far scale
 
 // NB blocks of 32 per head, CT column tiles of 4 query heads, SPLIT: fp32.  One tile leaves the registers for
@@ -547,13 +548,13 @@ struct MxWarp {
         mask_scales(w[j], j ? valid1 : valid0, ref);  // whatever they are: their p is zero
       }
     }
-    // m follows the largest score, up to kLag binades behind it
+    // m follows the largest score, up to kLag binades behind it (by the difference: m + kLag may round to m + 4 from 2^24 on)
     float top[CT];
     bool behind = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       top[c] = fmaxf(fmaxf(x[0][c][0], x[0][c][1]), fmaxf(x[1][c][0], x[1][c][1]));
-      behind |= top[c] > m[c] + kLag;
+      behind |= top[c] - m[c] > kLag;
     }
     if (__any_sync(kAll, behind)) {
 #pragma unroll
@@ -573,7 +574,12 @@ struct MxWarp {
     uint32_t p[2][kParts][CT][4];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const float lift = kLift - m[c];
+      float lift = kLift - m[c];
+      if (fabsf(m[c]) > kExact) {  // which m would round away: m goes at once
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i / 2][c][i % 2] -= m[c];
+        lift = kLift;
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float p0 = fast_exp2(x[j][c][0] + lift), p1 = fast_exp2(x[j][c][1] + lift);

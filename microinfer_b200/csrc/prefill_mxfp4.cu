@@ -430,6 +430,8 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         s[i][u] = fast_exp2(fmaf(s[i][u], scale, base[u >> 1]));
+        // m is off by a step of fp32, which from 2^24 on is binades: p stays within f16, in the sum as in the product
+        if constexpr (kLift > 0.f) s[i][u] = fmin_nan(s[i][u], 65504.f);
         l[u >> 1] += s[i][u];
       }
 #pragma unroll
