@@ -185,9 +185,11 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
         for (int u = 0; u < 4; ++u) x[2 * u] = f[u].x, x[2 * u + 1] = f[u].y;
       }
     }
-    if (p.scale_log2 < 0.f)
+    // q goes in with the sign of the scale, so that the largest product is the largest score; a scale of 0 or NaN makes it
+    // that, and so every score
+    if (!(p.scale_log2 > 0.f))
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = -x[u];
+      for (int u = 0; u < 8; ++u) x[u] *= p.scale_log2 < 0.f ? -1.f : p.scale_log2;
 #pragma unroll
     for (int part = 0; part < kParts; ++part) {
       *reinterpret_cast<uint4 *>(smem + part * C::kQuery + at<NB>(r, c)) =
@@ -307,9 +309,7 @@ __device__ __forceinline__ void prefill_tile(const CodedPrefillParams &p, const 
   }
   const int first_pos = static_cast<int>(prefix + by_group.div(static_cast<uint32_t>(row0) + min(warp * 16, rows - 1)));
   // m follows the largest score, up to kLag binades behind it: p <= 2^(kLift + kLag) is within f16
-  // q goes in with the sign of the scale, so that the largest product is the largest score; a scale of 0
-  // becomes one that leaves every score at 0
-  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  const float scale = fabsf(p.scale_log2) > 0.f ? fabsf(p.scale_log2) : 1.f;  // 0 and NaN are in q
   constexpr float kLift = std::is_same<E, __half>::value ? 12.f : 0.f, kLag = 3.f;
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll

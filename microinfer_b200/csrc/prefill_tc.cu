@@ -697,8 +697,9 @@ cudaError_t launch_prefill_tc(const AttnParams &a, int dtype, int G, int32_t max
   p.block_size = paged ? a.block_size : 16;
   p.num_q_heads = a.num_q_heads;
   p.paged = paged ? 1 : 0;
-  // A masked score is an infinity times the scale, so a scale of 0 is one that leaves every finite score at 0.
-  p.scale_log2 = a.scale_log2 == 0.f ? 1e-30f : a.scale_log2;
+  // A masked score is an infinity times the scale, so a scale of 0 is the smallest number, which leaves every finite score below
+  // 2^-21.
+  p.scale_log2 = a.scale_log2 == 0.f ? 0x1p-149f : a.scale_log2;
   p.p_lift = a.p_lift;
   p.redo = a.redo;
   p.redo_stride = a.redo_stride;

@@ -55,3 +55,53 @@ def test_scores_a_step_apart(cuda_device, name, d, way, rows, power, ahead, off)
     # off: scores that are no fp32 numbers
     got = _attend(cuda_device, _cuda(query, cuda_device, DTYPES[name]), kp, vp, ctx, float(scale) * off, way)
     assert bool(torch.isfinite(got).all()) and bool((got >= 1 - 2.0 ** -7).all()) and bool((got <= 4 + 2.0 ** -5).all())
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("way,rows", WAYS)
+def test_softmax_scale_of_zero_with_large_keys(cuda_device, name, d, way, rows):
+    """Every visible key weighs the same, however large its product with the query."""
+    rng = np.random.default_rng(d)
+    ctx = 1280
+    nb = ctx // 16
+    code, byte = mo.encode(rng.standard_normal((nb, 16, 1, d)))
+    power = 108 if name != "f16" or way == "decode" else 14  # prefill's K is fp16 there
+    kp = mo.pack(code, np.where(byte == 0, 0, byte + power).astype(np.uint8))
+    vp = mo.pack(*mo.encode(rng.standard_normal((nb, 16, 1, d))))
+    query = _cuda(rng.standard_normal((rows, 2, d)), cuda_device, DTYPES[name])
+    got = _attend(cuda_device, query, kp, vp, ctx, 0.0, way).double().cpu().numpy()
+    v = mo.rows(vp, np.arange(nb), ctx)[:, 0]
+    seen = np.arange(ctx - rows, ctx) + 1
+    want = np.cumsum(v, 0)[seen - 1] / seen[:, None]
+    size = np.cumsum(np.abs(v), 0)[seen - 1] / seen[:, None]
+    u = torch.finfo(DTYPES[name]).eps / 2
+    # p is 1, exact in every type; scores off by 2^-20 at most; the result is rounded once
+    assert (np.abs(got - want[:, None]) <= u * np.abs(want[:, None]) + (2.0 ** -18 + ctx * 2.0 ** -24) * size[:, None]).all()
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("way,rows", WAYS)
+def test_softmax_scale_that_is_nan(cuda_device, name, way, rows):
+    rng = np.random.default_rng(3)
+    kp, vp = (mo.pack(*mo.encode(rng.standard_normal((80, 16, 1, 128)))) for _ in range(2))
+    query = _cuda(rng.standard_normal((rows, 2, 128)), cuda_device, DTYPES[name])
+    assert bool(torch.isnan(_attend(cuda_device, query, kp, vp, 1280, float("nan"), way)).all())
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_softmax_scale_of_zero_with_large_keys_in_16_and_32_bits(cuda_device, name, d, rows):
+    rng = np.random.default_rng(d)
+    q, k, v = (torch.from_numpy(rng.standard_normal((rows, 1, d))).to(cuda_device, DTYPES[name]) for _ in range(3))
+    cu = torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+    got = mi.varlen_prefill(q, k * 2.0 ** 108, v, cu, cu, max_seqlen_q=rows, scale=0.0).double().cpu()
+    v = v.double().cpu()
+    count = torch.arange(1, rows + 1, dtype=torch.float64)[:, None, None]
+    want, size = v.cumsum(0) / count, v.abs().cumsum(0) / count
+    u = torch.finfo(DTYPES[name]).eps / 2
+    assert bool(((got - want).abs() <= u * want.abs() + (2.0 ** -18 + rows * 2.0 ** -24) * size).all())
