@@ -20,13 +20,14 @@
 //                    4600 cycles a tile with issuing and with the stalls of its waits, and everything else waits for it
 //   warp 13          walks the work list and tells the others of each item, looks up pages and scales ahead and brings the
 //                    codes of a tile by bulk copies
+//   warp 14          looks for NaN of V in groups of scale 0
 // TMEM: S_A at 0, S_B at 128, O_A at 256, O_B at 384; P (f16 pairs) goes over the first 64 columns of its S and is the A
 // operand of P V from there.  Barriers and rings stay up across items; each role counts their phases.
 // Every wait is bounded; a timeout flags MI_DEV_TIMEOUT, unwinds every role, waits for the MMAs, frees TMEM and returns.
 //
 // What it leaves to the kernel on the warp-level tensor cores, launched behind it for those sequences and heads alone ("odd"): a NaN
-// of V (0 * NaN reaches rows that do not see its key; one in a group of scale 0 is looked for by the loader), scales of V more than 14 binades apart, scores past 2^20 or
-// whose factor leaves fp32's range.  Without any it returns at once.
+// of V (0 * NaN reaches rows that do not see its key), scales of V more than 14 binades below R, which is at most 2 above the largest
+// that the item has met so far and never falls, scores past 2^20 or whose factor leaves fp32's range.  Without any it returns at once.
 //
 // Measured (cold L2): head_dim 64, 32 heads on 8: 1 x 256 rows on 16000 keys 110 us, 1 x 2048 on 6144 316 us (380 TFLOP/s; the warp-level
 // kernel 698), 4 x 1024 on 4000 320; 6 x 300 87 us; head_dim 128: 1 x 128 on 16000 95 us (194 there), 12 heads
@@ -55,7 +56,7 @@ constexpr int kVStages = 2;
 constexpr int kItems = 4;  // items ahead
 constexpr int kFactorMax = 94;             // largest exponent of a score's factor: sums of products are below 2^32
 constexpr float kLift = 11.f, kLag = 4.f;  // p is 2^(x - m + kLift), m this far behind at most: within f16
-constexpr int kSpread = 14;                // binades between V's scales that p takes in
+constexpr int kSpread = 14;                // binades below R that p takes in
 constexpr float kExact = 0x1p20f;          // m up to here is off by 2^-4 at most
 
 template <int D>
@@ -96,7 +97,7 @@ enum {
   B_INFO = 33,    // two words: what the loader says of the tile of K and of V
   B_COUNT = 34
 };
-static_assert(B_COUNT * 8 + 12 <= 288 && kItems == 4, "their place in shared memory");
+static_assert(B_COUNT * 8 + 16 <= 288 && kItems == 4, "their place in shared memory");
 constexpr uint32_t kNoMore = 1u << 31;  // of K's word: there is no tile; else bits 0-7 the groups that exist, 8-15 those whose
                                         // V is zero, 16-20 the keys of the last group that exists
 
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t *bar = reinterpret_cast<uint64_t *>(smem + C::kOffMisc);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bar + B_COUNT);
-  int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1), *nan_flag = abort_flag + 1;
+  int *abort_flag = reinterpret_cast<int *>(tmem_slot + 1), *nan_flag = abort_flag + 1, *zero_flag = nan_flag + 1;
   constexpr int kScaleRing = C::kScaleRing;
   uint8_t *scales = smem + C::kOffScales;  // ring: K's bytes of 8 groups, V's, then a bit for each whose page is none
   F8Item *item_ring = reinterpret_cast<F8Item *>(smem + C::kOffItems);
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t *prefix = reinterpret_cast<int64_t *>(smem + C::kOffK);
   const F8Work work = f8_work(p, by_group, prefix, prefix + kF8MaxSeqs + 1, gridDim.x);
   F8Walker walk;
-  if (warp == 13) walk.start(p, by_group, prefix, work, blockIdx.x);
+  if (warp == 13 || warp == 14) walk.start(p, by_group, prefix, work, blockIdx.x);
   __syncthreads();  // the prefix sums are read: the rings are free
   // Item i, or null where there is none (or something has gone wrong: !ok).
   auto item = [&](uint32_t i, bool &ok) -> const F8Item * {
@@ -421,7 +422,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       it = next;
     }
     if (!ok && lane == 0) *(volatile int *)abort_flag = 1;
-    odd |= *(volatile const int *)nan_flag != 0;  // of this CTA's tiles, which have all come by way of the loader
     const bool any = __any_sync(kAll, odd);
     if (lane == 0) f8_odd(p, D, gridDim.x)[blockIdx.x * 8 + warp] = any;
     if (threadIdx.x == 0) f8_meta(p, D, gridDim.x)[blockIdx.x] = meta;
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t *raw = smem + C::kOffRaw;
       uint32_t tiles = 0;
       uint32_t number = 0;
-      bool ok = true;
+      bool ok = true, zeros = false;  // whether there is a group of V of scale 0
       F8Item it;
       auto tell = [&] {  // the others of the item
         if (!__all_sync(kAll, mbar_wait_bounded(&bar[B_ITEMEMPTY + number % kItems], (number / kItems & 1) ^ 1, p.status) &&
@@ -620,25 +620,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t next_byte = scale_of(next);
           const unsigned exists = __ballot_sync(kAll, lane < 8 && place >= 0), none = __ballot_sync(kAll, lane < 8 && place == -2);
           const unsigned zero = __ballot_sync(kAll, lane >= 8 && lane < 16 && byte == 0) >> 8;
+          zeros |= (zero & exists) != 0;
           // keys of the last group that exists (later ones may have no page; theirs are zeros in any case)
           const int last = 31 - __clz(static_cast<int>(exists));
           const int in_last = exists ? min(kF8Group, it.keys - (j * 8 + last) * kF8Group) : 0;
-          // Groups of V of scale 0 are decoded to zeros.  What the store makes of a group without a finite element but zeros is one,
-          // with NaN codes: looked for here, where it costs the tile nothing (in the decoding warps 3 to 7 us of 75).
-          for (unsigned left = zero & exists; left; left &= left - 1) {
-            const int group = __ffs(static_cast<int>(left)) - 1;
-            const int from = __shfl_sync(kAll, place, group), tokens = group == last ? in_last : kF8Group;
-            const uint4 *codes = reinterpret_cast<const uint4 *>(p.value_pages + static_cast<int64_t>(from) * C::kGroup);
-            bool nan = false;
-#pragma unroll
-            for (int i = lane; i < D; i += 32) {
-              const uint4 w = __ldg(codes + i);
-              const int tok = i % 64 / 32 * 8 + i % 4 * 2;  // 8 dims of it and the next
-              const uint32_t keep = (tok < tokens ? 0x00ff00ffu : 0u) | (tok + 1 < tokens ? 0xff00ff00u : 0u);
-              nan |= f8_any_nan(w.x & keep) || f8_any_nan(w.y & keep) || f8_any_nan(w.z & keep) || f8_any_nan(w.w & keep);
-            }
-            if (nan) *(volatile int *)nan_flag = 1;
-          }
 #pragma unroll
           for (int o = 0; o < 2; ++o) {  // K, V
             if (!__all_sync(kAll, mbar_wait_bounded(&bar[B_RAWEMPTY + o], (tiles & 1) ^ 1, p.status) && !aborted(abort_flag))) {
@@ -679,12 +664,50 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (tiles > 0) mbar_wait_bounded(&bar[B_RAWFULL + o], (tiles - 1) & 1, p.status);
         mbar_wait_bounded(&bar[B_RAWFULL], tiles & 1, nullptr);  // the tile under way, if it was asked for
       }
+      if (lane == 0) *(volatile int *)zero_flag = zeros;
+      asm volatile("bar.sync 1, 64;" ::: "memory");  // warp 14 looks at them
+    } else {
+      // ---------------------------------------------------------- NaN of V in groups of scale 0
+      // Such groups are decoded to zeros; the store makes one with NaN codes of 16 tokens without a finite element but zeros.  Looked
+      // for at the end, where the loader has met one, beside the last tiles: in the decoding warps it took 3 to 7 us of 75 (6 x 300
+      // at head_dim 64), in the loader up to 4%.
+      asm volatile("bar.sync 1, 64;" ::: "memory");
+      const int per_page = p.block_size / kF8Group;
+      F8Item it;
+      while (*(volatile const int *)zero_flag && walk.next(p, by_group, it)) {
+        const int32_t *table = p.block_tables + it.seq * p.bt_stride;
+        const int groups = min(it.j1 * 8, (it.keys + kF8Group - 1) / kF8Group);
+        for (int g0 = it.j0 * 8; g0 < groups; g0 += 32) {
+          const int group = g0 + lane, col = static_cast<int>(by_page.div(group));
+          const int page = group < groups ? __ldg(table + col) : -1;
+          const uint8_t *codes = p.value_pages;
+          bool zero = page >= 0 && page < p.num_blocks;
+          if (zero) {
+            codes += static_cast<int64_t>((page * p.num_kv_heads + it.kvh) * per_page + group - col * per_page) * C::kGroup;
+            zero = codes[kF8Group * D] == 0;
+          }
+          for (unsigned left = __ballot_sync(kAll, zero); left; left &= left - 1) {
+            const int from = __ffs(static_cast<int>(left)) - 1, tokens = it.keys - (g0 + from) * kF8Group;
+            const uint4 *at = reinterpret_cast<const uint4 *>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(codes), from));
+            bool nan = false;
+#pragma unroll
+            for (int i = lane; i < D; i += 32) {
+              const uint4 w = __ldg(at + i);
+              const int tok = i % 64 / 32 * 8 + i % 4 * 2;  // 8 dims of it and the next
+              const uint32_t keep = (tok < tokens ? 0x00ff00ffu : 0u) | (tok + 1 < tokens ? 0xff00ff00u : 0u);
+              nan |= f8_any_nan(w.x & keep) || f8_any_nan(w.y & keep) || f8_any_nan(w.z & keep) || f8_any_nan(w.w & keep);
+            }
+            if (nan) *(volatile int *)nan_flag = 1;
+          }
+        }
+      }
     }
   }
 
   pdl_launch_dependents();
   tc::fence_before_sync();
   __syncthreads();
+  if (threadIdx.x == 0 && *(volatile const int *)nan_flag) f8_odd(p, D, gridDim.x)[blockIdx.x * 8] = 1;
   if (warp == 12) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
