@@ -580,7 +580,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t *raw = smem + C::kOffRaw;
       uint32_t tiles = 0;
       uint32_t number = 0;
-      bool ok = true, zeros = false;  // whether there is a group of V of scale 0
+      bool ok = true, told = false;
+      // To warp 14, once: there is a group of V of scale 0, or there is none.
+      auto tell_zero = [&](int is) {
+        if (told) return;
+        told = true;
+        if (lane == 0) *(volatile int *)zero_flag = is;
+        __syncwarp();
+        asm volatile("bar.arrive 1, 64;" ::: "memory");
+      };
       F8Item it;
       auto tell = [&] {  // the others of the item
         if (!__all_sync(kAll, mbar_wait_bounded(&bar[B_ITEMEMPTY + number % kItems], (number / kItems & 1) ^ 1, p.status) &&
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t next_byte = scale_of(next);
           const unsigned exists = __ballot_sync(kAll, lane < 8 && place >= 0), none = __ballot_sync(kAll, lane < 8 && place == -2);
           const unsigned zero = __ballot_sync(kAll, lane >= 8 && lane < 16 && byte == 0) >> 8;
-          zeros |= (zero & exists) != 0;
+          if (zero & exists) tell_zero(1);
           // keys of the last group that exists (later ones may have no page; theirs are zeros in any case)
           const int last = 31 - __clz(static_cast<int>(exists));
           const int in_last = exists ? min(kF8Group, it.keys - (j * 8 + last) * kF8Group) : 0;
@@ -664,13 +672,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (tiles > 0) mbar_wait_bounded(&bar[B_RAWFULL + o], (tiles - 1) & 1, p.status);
         mbar_wait_bounded(&bar[B_RAWFULL], tiles & 1, nullptr);  // the tile under way, if it was asked for
       }
-      if (lane == 0) *(volatile int *)zero_flag = zeros;
-      asm volatile("bar.sync 1, 64;" ::: "memory");  // warp 14 looks at them
+      __syncwarp();
+      tell_zero(0);
     } else {
       // ---------------------------------------------------------- NaN of V in groups of scale 0
-      // Such groups are decoded to zeros; the store makes one with NaN codes of 16 tokens without a finite element but zeros.  Looked
-      // for at the end, where the loader has met one, beside the last tiles: in the decoding warps it took 3 to 7 us of 75 (6 x 300
-      // at head_dim 64), in the loader up to 4%.
+      // Such groups are decoded to zeros; the store makes one with NaN codes of 16 tokens without a finite element but zeros.  This
+      // warp goes over the CTA's keys by itself as soon as the loader has met one: in the decoding warps the look took 3 to 7 us of 75
+      // (6 x 300 at head_dim 64, where there is none), in the loader up to 4%.
       asm volatile("bar.sync 1, 64;" ::: "memory");
       const int per_page = p.block_size / kF8Group;
       F8Item it;
@@ -686,17 +694,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             codes += static_cast<int64_t>((page * p.num_kv_heads + it.kvh) * per_page + group - col * per_page) * C::kGroup;
             zero = codes[kF8Group * D] == 0;
           }
-          for (unsigned left = __ballot_sync(kAll, zero); left; left &= left - 1) {
-            const int from = __ffs(static_cast<int>(left)) - 1, tokens = it.keys - (g0 + from) * kF8Group;
-            const uint4 *at = reinterpret_cast<const uint4 *>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(codes), from));
+          constexpr int kAtOnce = 256 / D;  // groups whose reads are on their way together
+          for (unsigned left = __ballot_sync(kAll, zero); left;) {
+            uint4 w[kAtOnce][D / 32];
+            int tokens[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+              const int from = left ? __ffs(static_cast<int>(left)) - 1 : 0;
+              const uint4 *at = reinterpret_cast<const uint4 *>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(codes), from));
+              tokens[u] = left ? it.keys - (g0 + from) * kF8Group : 0;
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) w[u][i] = tokens[u] > 0 ? __ldg(at + i * 32 + lane) : make_uint4(0u, 0u, 0u, 0u);
+              left &= left - 1;
+            }
             bool nan = false;
 #pragma unroll
-            for (int i = lane; i < D; i += 32) {
-              const uint4 w = __ldg(at + i);
-              const int tok = i % 64 / 32 * 8 + i % 4 * 2;  // 8 dims of it and the next
-              const uint32_t keep = (tok < tokens ? 0x00ff00ffu : 0u) | (tok + 1 < tokens ? 0xff00ff00u : 0u);
-              nan |= f8_any_nan(w.x & keep) || f8_any_nan(w.y & keep) || f8_any_nan(w.z & keep) || f8_any_nan(w.w & keep);
-            }
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+              for (int i = 0; i < D / 32; ++i) {
+                const int tok = (i * 32 + lane) % 64 / 32 * 8 + lane % 4 * 2;  // 8 dims of it and the next
+                const uint32_t keep = (tok < tokens[u] ? 0x00ff00ffu : 0u) | (tok + 1 < tokens[u] ? 0xff00ff00u : 0u);
+                const uint4 v = w[u][i];
+                nan |= f8_any_nan(v.x & keep) || f8_any_nan(v.y & keep) || f8_any_nan(v.z & keep) || f8_any_nan(v.w & keep);
+              }
             if (nan) *(volatile int *)nan_flag = 1;
           }
         }

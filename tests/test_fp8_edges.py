@@ -78,6 +78,29 @@ def test_prefill_of_values_that_are_nowhere_finite(cuda_device, way, name, d):  
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("where", [None, 0, 1403, 1950, 2047])
+def test_prefill_of_zeros_with_one_nan(cuda_device, way, d, where):  # noqa: F811
+    """Values that are zero throughout but for one that is NaN, or none: 128 groups of scale 0 to look through."""
+    rng = np.random.default_rng(d)
+    ctx, rows = 2048, 150
+    kp, _ = pages(rng, ctx // 16, 16, 2, d)
+    vp = np.zeros_like(kp)
+    table = rng.permutation(ctx // 16).astype(np.int32)
+    if where is not None:
+        _set_code(vp, True, _place(where, table), 1, d - 7, 127)
+    query = cuda(rng.standard_normal((rows, 4, d)), cuda_device, torch.bfloat16)
+    got, _ = _attend(cuda_device, query, kp, vp, [table], [rows], [ctx], d ** -0.5)
+    nan = torch.isnan(got)
+    if where is None:
+        assert bool((got == 0).all())
+        return
+    first = max(0, where - (ctx - rows))
+    assert bool(nan[first:, 2:, d - 7].all()) and int(nan.sum()) == 2 * (rows - first)
+    assert bool((got[~nan] == 0).all())
+
+
+@gpu
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("d", [64, 96, 128])
 @pytest.mark.parametrize("decode", [False, True])
