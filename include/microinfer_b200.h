@@ -480,8 +480,8 @@ MI_API int mi_paged_prefill_mxfp4(void *out, const void *query, const void *key_
 /*
  * The same by way of rows: K and V of the contexts (kv_rows, their sum or a bound on it; rows past it are flagged)
  * are decoded into the workspace and attended to as mi_varlen_prefill does, for chunks large enough for the tensor
- * cores' dense kernel.  Sequences with what does not go through it (a NaN of V, in f16 a block past 65504, a
- * page that is none) are then done over from the pages, so results are those of mi_paged_prefill_mxfp4; `out`
+ * cores' dense kernel.  Sequences with what does not go through it (a NaN of V, in f16 a block past 65504 or scores
+ * past 2^20, a page that is none) are then done over from the pages, so results are those of mi_paged_prefill_mxfp4; `out`
  * must not overlap the query.  In f32 above head_dim 128, which has no kernel for the pages, a page that is
  * none (MI_DEV_BAD_BLOCK) counts as zeros; elsewhere its keys are left out.  `max_context` bounds one context:
  * what a longer one has past it is treated as pages that are none.
@@ -602,7 +602,8 @@ MI_API int mi_paged_prefill_fp8(void *out, const void *query, const void *key_pa
  * The same by way of rows, for chunks large enough for the tensor cores' dense kernel and shapes that it takes
  * (MI_ERR_UNSUPPORTED otherwise): K and V of the contexts (kv_rows, their sum or a bound on it; rows past it are
  * flagged) are decoded into the workspace and attended to as mi_varlen_prefill does.  Sequences with what does not go
- * through it (a NaN of V, in f16 a value past 65504, a page that is none) are then done over from the
+ * through it (a NaN of V; in f16 a value past 65504, a K that f16 does not hold exactly or scores past 2^20; in bf16 a K
+ * beyond 2^-64 to 2^64 or a V above that; a page that is none) are then done over from the
  * pages, so results are those of mi_paged_prefill_fp8; `out` must not overlap the query.  `max_context` bounds one
  * context: what a longer one has past it is treated as pages that are none.
  */

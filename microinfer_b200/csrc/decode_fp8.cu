@@ -18,7 +18,7 @@
 //     (exact for bf16 down to 2^-28 of that element); that power, K's scale and the softmax's scale become
 //     one factor, put together from exponents so that it leaves fp32's range only where the scores do.
 // Measured: 32 x 8192, 32 heads on 8 of 128, bf16: 99 us, 5.75 TB/s (88% of a copy), ALU 39%, issue slots 38%; 128 ragged up to 6000
-// 148 us (166 with rings of 16-byte cp.async), 1 x 100001 44, 1 x 300 7.1 (10.8 as called; 14.7 with a join behind every call).
+// 147 us (166 with rings of 16-byte cp.async), 1 x 100001 44, 1 x 300 7.1 (10.8 as called; 14.7 with a join behind every call).
 #include <type_traits>
 
 #include "common.cuh"

@@ -359,8 +359,8 @@ int mi_paged_prefill_fp8_gathered(void *out, const void *query, const void *key_
   if (const int s = capi_select_device(key_pages)) return s;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   char *keys = static_cast<char *>(workspace), *values = keys + rows;
-  // The tensor-core kernel multiplies what a row does not see by zero: sequences with codes that this does not suit are
-  // noted by the gather and done over from the pages.
+  // The tensor-core kernel multiplies what a row does not see by zero, and its operands have 16 bits: sequences with codes that
+  // this does not suit are noted by the gather, in fp16 those with scores past 2^20 by that kernel, and done over from the pages.
   const int64_t groups = (max_context + kF8Group - 1) / kF8Group;
   uint8_t *redo = reinterpret_cast<uint8_t *>(values + rows);
   CodedGatherParams g = {};

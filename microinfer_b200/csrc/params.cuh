@@ -209,7 +209,7 @@ struct CodedPrefillParams {
   const int32_t *cu_seqlens_q;
   const int32_t *cu_seqlens_k;
   float *workspace;  // num_splits > 1: [split][token][q head][2 + D]
-  const uint8_t *redo;  // null, or the gather's: sequences and kv heads without a set byte are left as they are
+  const uint8_t *redo;  // null, or the gather's and the dense kernel's: sequences and kv heads without a set byte are left as they are
   int64_t redo_stride;
   int32_t redo_groups;  // that the gather has looked at, at most
   int64_t bt_stride;

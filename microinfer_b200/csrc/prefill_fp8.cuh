@@ -27,7 +27,8 @@ struct F8Meta {
 };
 
 // Workspace: [CTA][2][m, l, mean of V][256 rows], the part of a unit that began in an earlier CTA, then that of the one that
-// goes on; the CTAs' F8Meta; a byte for each softmax warp that met what is to be done over.
+// goes on; the CTAs' F8Meta; a byte for each softmax warp that met what is to be done over (the first also for
+// the warp that looks for NaN of V in groups of scale 0).
 __host__ __device__ inline size_t f8_parts_bytes(int head_dim, int ctas) {
   return static_cast<size_t>(ctas) * 2 * 256 * (head_dim + 2) * sizeof(float);
 }

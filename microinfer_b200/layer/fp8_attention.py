@@ -10,7 +10,8 @@ shape that the dense tensor-core kernel takes, each context is decoded once into
 type (twice its pages) and that kernel attends to the rows.  Elsewhere the pages are read: by a tcgen05 kernel (16-bit
 queries, head_dim 64 and 128), or by one on the warp-level tensor cores for little work and everything
 else.  All give the same result up to rounding: what the tensor-core kernels cannot do (a NaN of V,
-scales too far apart, in fp16 a value past its range) is done over by the third.  The choice goes by the shapes and the bounds
+scales too far apart, K or V at the ends of the range of 16 bits, scores past 2^20) is done over by the third.  The choice goes by
+the shapes and the bounds
 ``max_seqlen_q``, ``max_seqlen_k`` and ``total_k``, never by what the tensors hold.
 Workspaces come from torch's allocator for the length of the call, so that calls on several
 streams, and captured graphs, each have their own.

@@ -11,7 +11,7 @@ pages in 16 bits) and that kernel attends to the rows: a chunk of n tokens does 
 Hkv elements decoded, so the extra pass is a few percent of a large chunk, and most of the call
 where every request has a few tokens.  Few tiles, and shapes that kernel does not take, are computed from the
 pages.  Both give the same result up to rounding: sequences with what the dense kernel cannot do
-(a NaN or, in fp16, a block past its range; a page that is none) are done over from the pages.
+(a NaN or, in fp16, a block past its range or scores past 2^20; a page that is none) are done over from the pages.
 Workspaces come from torch's allocator for the length of the call, so that calls on several
 streams, and captured graphs, each have their own.
 """
